@@ -425,7 +425,10 @@ std::unique_ptr<Program> program_of(const py::dict& d) {
 
 }  // namespace
 
+void frnn_bind_lm(py::module& m);      // frnn_lm_host.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    frnn_bind_lm(m);
     m.def("bind", [](uintptr_t launch, uintptr_t encode, uintptr_t error) {
         g_launch = (launch_fn)launch;
         g_encode = (encode_fn)encode;

@@ -23,13 +23,18 @@ namespace {
 
 thread_local std::string g_err;
 
-int fail(int code, const char* fmt, ...) {
+int vfail(int code, const char* fmt, va_list ap) {
     char buf[1024];
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    g_err = buf;
+    return code;
+}
+
+int fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
+    vfail(code, fmt, ap);
     va_end(ap);
-    g_err = buf;
     return code;
 }
 
@@ -137,6 +142,15 @@ const char* cu_str(Driver* d, CUresult r) {
 }
 
 }  // namespace
+
+// The same for the library's other files (frnn_lm.cuh).
+int frnn_fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vfail(code, fmt, ap);
+    va_end(ap);
+    return code;
+}
 
 struct frnn_module {
     CUmodule mod = nullptr;
@@ -311,6 +325,7 @@ const char* kernel_code_text(int code) {
     switch (code) {
         case 1: return "a staged-input copy did not arrive within the wait limit";
         case 2: return "a checkpoint copy did not arrive within the wait limit";
+        case 96: return "a token is outside the vocabulary";
         default: return "unknown code";
     }
 }

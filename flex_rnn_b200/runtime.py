@@ -20,7 +20,9 @@ LIB_PATH = os.path.join(HERE, "libfrnn_b200.so")
 SYMBOLS = ["frnn_abi_version", "frnn_last_error", "frnn_compile", "frnn_free", "frnn_module_load",
            "frnn_module_unload", "frnn_launch", "frnn_kernel_attrs", "frnn_l2_flush", "frnn_fp32_peak_probe",
            "frnn_launch_static_scratch", "frnn_static_scratch_capacity", "frnn_tensor_map_encode",
-           "frnn_nvrtc_version", "frnn_status", "frnn_status_post", "frnn_status_check", "frnn_fp32_mix_probe"]
+           "frnn_nvrtc_version", "frnn_status", "frnn_status_post", "frnn_status_check", "frnn_fp32_mix_probe",
+           "frnn_embedding_forward", "frnn_embedding_backward", "frnn_embedding_backward_workspace", "frnn_layer_norm_forward",
+           "frnn_layer_norm_backward", "frnn_layer_norm_backward_workspace", "frnn_token_logprobs_forward", "frnn_token_logprobs_backward"]
 
 
 class FrnnError(RuntimeError):
@@ -69,6 +71,18 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def _status_word(device: int) -> int:
+    """Address of a device's error word (pinned host memory)."""
+    from .twopass import device_status
+    return device_status(f"cuda:{device}").word.data_ptr()
+
+
+def _status_raise(device: int):
+    """Raise what the error word of a device says, and clear it."""
+    from .twopass import device_status
+    device_status(f"cuda:{device}").check()
+
+
 _host = None
 
 
@@ -87,7 +101,10 @@ def host():
             spec = importlib.util.spec_from_file_location("_frnn_host", _build.HOST_LIB)
             m = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(m)
-            m.bind(*[ctypes.cast(f, ctypes.c_void_p).value for f in (L.frnn_launch, L.frnn_tensor_map_encode, L.frnn_last_error)])
+            address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+            m.bind(*[address(f) for f in (L.frnn_launch, L.frnn_tensor_map_encode, L.frnn_last_error)])
+            m.bind_lm({n: address(getattr(L, n)) for n in SYMBOLS if n.startswith(("frnn_embedding", "frnn_layer_norm", "frnn_token", "frnn_last"))},
+                      _status_word, _status_raise)
             _host = m
     return _host
 

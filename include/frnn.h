@@ -173,6 +173,71 @@ int frnn_launch_static_scratch(frnn_module_t m, int kernel, const unsigned grid[
 /* Size in bytes of the static scratch array behind frnn_launch_static_scratch. */
 size_t frnn_static_scratch_capacity(void);
 
+/* ---- operators of language models around the scans ----
+ *
+ * Compiled ahead of time for sm_100a, launched on `stream` (a cudaStream_t; NULL = default stream), asynchronous.  They
+ * allocate nothing: the caller passes outputs and, where a `_workspace` function says so, scratch of at least that many
+ * bytes on a 16-byte boundary, free again when the stream has passed the call.  Pointers are device addresses; element
+ * types are FRNN_F32, FRNN_BF16 or FRNN_F16, arithmetic is in 32 bits, results are rounded once.  Sums have a fixed
+ * order: the same call gives the same bits.  Tokens are int32 or int64 (`token_bytes` 4 or 8).  `err_word` is the kernel
+ * error word described above (the forward calls that read tokens write code 96 there for a token that is outside the
+ * vocabulary and not `ignore_index`).  (No counterpart in the reference, whose scope is the recurrence itself.)
+ */
+enum { FRNN_F32 = 0, FRNN_BF16 = 1, FRNN_F16 = 2 };
+
+/*
+ * out[i, :] = scale * weight[tokens[i], :] for i < n, contiguous [n, width]; weight[v, d] is at v * row_stride + d *
+ * col_stride elements, v < rows.  Zero rows for tokens equal to ignore_index and for tokens outside the vocabulary.
+ */
+int frnn_embedding_forward(int dtype, const void* weight, int64_t rows, int64_t width, int64_t row_stride, int64_t col_stride,
+                           const void* tokens, int token_bytes, int64_t n, float scale, int64_t ignore_index,
+                           void* out, int* err_word, void* stream);
+
+/* dweight[v, :] = scale * sum of dout[i, :] over the i with tokens[i] == v: contiguous [rows, width], every row written.
+ * Tokens outside the vocabulary and ignore_index add to no row. */
+size_t frnn_embedding_backward_workspace(int dtype, int64_t rows, int64_t width, int64_t n);
+int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int token_bytes, int64_t n, int64_t rows, int64_t width,
+                            float scale, int64_t ignore_index, void* dweight, void* workspace, void* stream);
+
+/* The n0 * n1 * n2 rows of a layer norm, each `width` consecutive elements: row (i0, i1, i2) starts at element
+ * i0 * x[0] + i1 * x[1] + i2 * x[2] of x, likewise of dy and dx; y and the statistics are contiguous in the order of the
+ * rows.  heads == 1: one vector of `width` weights for all rows; heads == n2 > 1: [heads, width] weights, those of i2. */
+typedef struct frnn_rows {
+    int64_t n0, n1, n2, width, heads;
+    int64_t x[3], dy[3], dx[3];
+} frnn_rows;
+
+/*
+ * y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(variance + eps) over a row's `width` elements.  weight and bias
+ * may be NULL (1, 0) and have the type of x or FRNN_F32.  stats (may be NULL): fp32 [rows][2], mean and rstd, for the
+ * backward.
+ */
+int frnn_layer_norm_forward(const frnn_rows* rows, int dtype, const void* x, int param_dtype, const void* weight, const void* bias,
+                            float eps, void* y, float* stats, void* stream);
+
+/* Gradients of x, weight and bias; each of dx, dweight and dbias may be NULL (not wanted). */
+size_t frnn_layer_norm_backward_workspace(const frnn_rows* rows);
+int frnn_layer_norm_backward(const frnn_rows* rows, int dtype, const void* dy, const void* x, int param_dtype, const void* weight,
+                             const float* stats, void* dx, void* dweight, void* dbias, void* workspace, void* stream);
+
+/*
+ * Of n rows of `vocab` logits (row_stride elements apart), with p = softmax(logits / temperature):
+ *   logprob[i]            log p[tokens[i]]; 0 where tokens[i] == ignore_index, NaN where it is outside the vocabulary
+ *   entropy[i]            -sum p log p (0 log 0 = 0)
+ *   top_logprob, top_token [n][top]: the `top` largest logits, equal ones by the lowest token; top <= FRNN_MAX_TOP
+ *   stats                 (may be NULL) fp32 [n][3] for the backward
+ * A row whose logits are all -infinity has log probabilities -infinity, entropy 0 and gradient 0.
+ */
+enum { FRNN_MAX_TOP = 32 };
+int frnn_token_logprobs_forward(int dtype, const void* logits, int64_t n, int64_t vocab, int64_t row_stride, const void* tokens, int token_bytes,
+                                int top, float temperature, int64_t ignore_index, float* logprob, float* entropy, float* top_logprob,
+                                int64_t* top_token, float* stats, int* err_word, void* stream);
+
+/* dlogits, contiguous [n, vocab], of the upstream gradients of logprob and entropy (fp32 [n]; either may be NULL: zero). */
+int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64_t vocab, int64_t row_stride, const void* tokens, int token_bytes,
+                                 float temperature, int64_t ignore_index, const float* dlogprob, const float* dentropy, const float* stats,
+                                 void* dlogits, void* stream);
+
 /* ---- helpers compiled into the library (used by the benchmark harness) ---- */
 
 /* Overwrite `bytes` bytes at `buf` (device) with a byte pattern; writing a
