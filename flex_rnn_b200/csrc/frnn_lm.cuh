@@ -5,8 +5,10 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <cstring>
 
 #include "../../include/frnn.h"
 
@@ -42,6 +44,110 @@ inline bool on_boundary(const void* p, size_t bytes) { return ((uintptr_t)p & (b
 inline int launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? FRNN_OK : frnn_fail(FRNN_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+}
+
+// E consecutive elements as one access of 16 bytes (E = 16 / size), or a single element (E = 1).
+template <class T, int E> struct Pack;
+template <class T> struct Pack<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void store(T* p) const { *p = v; }
+    __device__ __forceinline__ void zero() { v = from_float<T>(0.f); }
+    __device__ __forceinline__ void set(int, T x) { v = x; }
+    __device__ __forceinline__ T get(int) const { return v; }
+    __device__ __forceinline__ void to(float* f) const { f[0] = to_float(v); }
+    __device__ __forceinline__ void from(const float* f) { v = from_float<T>(f[0]); }
+};
+template <> struct Pack<float, 4> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *(const float4*)p; }
+    __device__ __forceinline__ void store(float* p) const { *(float4*)p = v; }
+    __device__ __forceinline__ void zero() { v = make_float4(0, 0, 0, 0); }
+    __device__ __forceinline__ void set(int i, float x) { (&v.x)[i] = x; }
+    __device__ __forceinline__ float get(int i) const { return (&v.x)[i]; }
+    __device__ __forceinline__ void to(float* f) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+    __device__ __forceinline__ void from(const float* f) { v = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <class T> struct Pack<T, 8> {           // 16-bit elements: the lower half of a word comes first
+    uint4 v;
+    __device__ __forceinline__ void load(const T* p) { v = *(const uint4*)p; }
+    __device__ __forceinline__ void store(T* p) const { *(uint4*)p = v; }
+    __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void set(int i, T x) {
+        unsigned short b;
+        memcpy(&b, &x, 2);
+        unsigned& w = (&v.x)[i / 2];
+        w = i & 1 ? (w & 0xFFFFu) | (unsigned)b << 16 : (w & 0xFFFF0000u) | b;
+    }
+    __device__ __forceinline__ T get(int i) const {
+        const unsigned short b = (unsigned short)((&v.x)[i / 2] >> (i & 1 ? 16 : 0));
+        T x;
+        memcpy(&x, &b, 2);
+        return x;
+    }
+    __device__ __forceinline__ void to(float* f) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) pair((&v.x)[i], f + 2 * i, T());
+    }
+    __device__ __forceinline__ void from(const float* f) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) (&v.x)[i] = join(f[2 * i], f[2 * i + 1], T());
+    }
+    static __device__ __forceinline__ void pair(unsigned w, float* f, __nv_bfloat16) { f[0] = __uint_as_float(w << 16); f[1] = __uint_as_float(w & 0xFFFF0000u); }
+    static __device__ __forceinline__ void pair(unsigned w, float* f, __half) {
+        __half2 h;
+        memcpy(&h, &w, 4);
+        const float2 r = __half22float2(h);
+        f[0] = r.x;
+        f[1] = r.y;
+    }
+    static __device__ __forceinline__ unsigned join(float a, float b, __nv_bfloat16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        unsigned w;
+        memcpy(&w, &h, 4);
+        return w;
+    }
+    static __device__ __forceinline__ unsigned join(float a, float b, __half) {
+        const __half2 h = __floats2half2_rn(a, b);
+        unsigned w;
+        memcpy(&w, &h, 4);
+        return w;
+    }
+};
+template <class T> constexpr int WIDE = 16 / (int)sizeof(T);
+
+// The E elements at p + at, of which those with 0 <= at + e < n are there; the others read as zero.
+template <class T, int E> __device__ __forceinline__ void load_part(Pack<T, E>& v, const T* p, int at, int n) {
+    if (at >= 0 && at + E <= n) {
+        v.load(p + at);
+    } else {
+        v.zero();
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (at + e >= 0 && at + e < n) v.set(e, p[at + e]);
+    }
+}
+template <class T, int E> __device__ __forceinline__ void store_part(const Pack<T, E>& v, T* p, int at, int n) {
+    if (at >= 0 && at + E <= n) {
+        v.store(p + at);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (at + e >= 0 && at + e < n) p[at + e] = v.get(e);
+    }
+}
+
+// Streaming multiprocessors of the current device (148 where there is none to ask).
+inline int sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 148; }
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { cudaGetLastError(); n = 148; }
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 // Token i of int32 or int64 tokens.

@@ -402,19 +402,25 @@ Tensor embedding_backward_autograd(const Tensor& grad, const Tensor& tokens, int
     return dw;
 }
 
+// Bytes of a tensor's first element behind a 16-byte boundary (its storage starts on one; a fake tensor has no address).
+int64_t behind_boundary(const Tensor& t) { return t.storage_offset() * (int64_t)t.element_size() & 15; }
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [y, stats] = layer_norm().call(x, weight, bias, eps, true);
         // the bias only says whether it has a gradient, and of which shape
         ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), stats});
+        ctx->saved_data["behind"] = behind_boundary(x);
         ctx->mark_non_differentiable({stats});
         ctx->set_materialize_grads(false);
         return {y, stats};
     }
     static variable_list backward(AutogradContext* ctx, variable_list up) {
         if (!up[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        const variable_list kept = ctx->get_saved_variables();
+        variable_list kept = ctx->get_saved_variables();
+        // a saved-tensor hook may move x off the boundary it was on; the sums have the order of aligned rows all the same
+        if (behind_boundary(kept[0]) && !ctx->saved_data["behind"].toInt()) kept[0] = kept[0].clone();
         const bool wx = ctx->needs_input_grad(0), ww = kept[1].defined() && ctx->needs_input_grad(1), wb = kept[2].defined() && ctx->needs_input_grad(kept[1].defined() ? 2 : 1);
         auto [dx, dw, db] = layer_norm_backward().call(up[0], kept[0], maybe(kept[1]), maybe(kept[2]), kept[3], wx, ww, wb);
         return {wx ? dx : Tensor(), ww ? dw : Tensor(), wb ? db : Tensor(), Tensor()};
