@@ -33,187 +33,244 @@ struct Deal {
     unsigned rows, groups, rounds;
 };
 
-// Sums over the lanes of a group: L lanes of a warp, or (L = 0) all threads of the block, by way of shared memory.  Two
-// buffers by turns: one barrier a sum.
-template <int L> struct Sums {
-    float2 (*buffer)[MOST_THREADS / 32];
-    int turn = 0;
-    __device__ __forceinline__ float2 all(float2 v) {
+// How the rows of a call's tensors lie to 16-byte boundaries, and so how they are accessed.  WIDE_ALIKE: all rows at a
+// boundary, in accesses of 16 bytes.  WIDE_APART: evenly spaced rows, those of a group at one distance behind a boundary
+// in all tensors: accesses of 16 bytes but at the ends.  ELEMENTS: one element at a time.
+enum Access { ELEMENTS, WIDE_ALIKE, WIDE_APART };
+
+// The 16 columns of a lane: access j has E consecutive ones from at[j], of which those from 0 to width are there.
+template <class T, int L, Access A> struct Columns {
+    static constexpr int E = A == ELEMENTS ? 1 : WIDE<T>, NV = PER_LANE / E;
+    int at[NV], width;
+
+    __device__ __forceinline__ Columns(int width, int lanes, int lane, int shift) : width(width) {
 #pragma unroll
-        for (int o = L ? L / 2 : 16; o; o >>= 1) {
-            v.x += __shfl_xor_sync(~0u, v.x, o);
-            v.y += __shfl_xor_sync(~0u, v.y, o);
+        for (int j = 0; j < NV; j++) at[j] = (j * lanes + lane) * E - shift;
+    }
+    // the whole of access j is there
+    __device__ __forceinline__ bool whole(int j) const { return A == WIDE_APART ? at[j] >= 0 && at[j] + E <= width : at[j] < width; }
+    __device__ __forceinline__ bool there(int j, int e) const { return A == WIDE_APART ? at[j] + e >= 0 && at[j] + e < width : at[j] < width; }
+    __device__ __forceinline__ void load(Pack<T, E>* v, const T* row) const {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (whole(j)) v[j].load(row + at[j]);
+            else if (A == WIDE_APART) load_part(v[j], row, at[j], width);
+            else v[j].zero();
         }
-        if (L) return v;
-        if ((threadIdx.x & 31) == 0) buffer[turn][threadIdx.x / 32] = v;
-        __syncthreads();
-        float2 s = make_float2(0, 0);
-        for (int i = 0; i < blockDim.x / 32; i++) {
-            s.x += buffer[turn][i].x;
-            s.y += buffer[turn][i].y;
+    }
+    __device__ __forceinline__ void store(T* row, const float2* f) const {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (A != WIDE_APART && !whole(j)) continue;
+            Pack<T, E> v;
+            v.from(&f[0].x + j * E);
+            if (whole(j)) v.store(row + at[j]);
+            else store_part(v, row, at[j], width);
         }
-        turn ^= 1;
-        return s;
+    }
+    static __device__ __forceinline__ void unpack(const Pack<T, E>* v, float2* f) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) v[j].to(&f[0].x + j * E);
+    }
+    // zeros where there is no column
+    __device__ __forceinline__ void clear(float2* f) const {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (!whole(j))
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (!there(j, e)) (&f[0].x)[j * E + e] = 0;
+    }
+    template <class P> __device__ __forceinline__ void params(const P* p, float none, float2* f) const {
+        constexpr int EP = WIDE<P> < E ? WIDE<P> : E;         // weights in 16-byte accesses where they are on a boundary, too
+        const bool even = A == WIDE_ALIKE && p && ((uintptr_t)p & 15) == 0;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (even && whole(j)) {
+#pragma unroll
+                for (int k = 0; k < E; k += EP) {
+                    Pack<P, EP> v;
+                    v.load(p + at[j] + k);
+                    v.to(&f[0].x + j * E + k);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) (&f[0].x)[j * E + e] = p && there(j, e) ? to_float(p[at[j] + e]) : none;
+            }
+        }
+    }
+    __device__ __forceinline__ int count() const {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < NV; j++) n += max(0, min(at[j] + E, width) - max(at[j], 0));
+        return n;
     }
 };
 
-// Weights of the 16 columns of a lane, as 32-bit numbers.
-template <class P, int E, int NV> __device__ __forceinline__ void load_params(const P* p, const int* at, int width, float none, float (&out)[NV * E]) {
+// A lane's place: its group and its place in it.
+template <int L> struct Seat {
+    int lanes, lane;
+    unsigned group, head;
+    __device__ __forceinline__ Seat(const frnn_rows& s) {
+        lanes = L ? L : blockDim.x;
+        lane = L ? threadIdx.x % (L ? L : 1) : threadIdx.x;
+        group = L ? blockIdx.x * (BLOCK / (L ? L : 1)) + threadIdx.x / (L ? L : 1) : blockIdx.x;
+        head = s.heads > 1 ? group % (unsigned)s.heads : 0;
+    }
+};
+
+template <int L> __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int c = at[j] + e;
-            out[j * E + e] = p && c >= 0 && c < width ? to_float(p[c]) : none;
-        }
+    for (int o = L ? L / 2 : 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    return v;
 }
 
-// y = (x - mean) rstd w + b.  The variance is that of the centred values, so that a large mean costs no digits.
-template <class T, class P, int L, int E>
+// A float2 of each warp, seen by all threads of the block; two buffers by turns, so one barrier each time is enough.
+struct Exchange {
+    float2 (*buffer)[MOST_THREADS / 32];
+    int turn = 0;
+    template <class F> __device__ __forceinline__ void operator()(float2 mine, F each) {
+        if ((threadIdx.x & 31) == 0) buffer[turn][threadIdx.x / 32] = mine;
+        __syncthreads();
+        const int warps = blockDim.x / 32;
+        const float4* all = (const float4*)buffer[turn];
+        for (int i = 0; i < warps / 2; i++) {
+            const float4 v = all[i];
+            each(2 * i, make_float2(v.x, v.y));
+            each(2 * i + 1, make_float2(v.z, v.w));
+        }
+        if (warps & 1) each(warps - 1, buffer[turn][warps - 1]);
+        turn ^= 1;
+    }
+};
+
+// y = (x - mean) rstd w + b.  The variance is that of the centred values, so that a large mean costs no digits; warps of a
+// block each centre theirs and join: sum of squares = sum over warps of theirs + count (their mean - mean)^2.
+template <class T, class P, int L, Access A>
 __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_fw(frnn_rows s, Deal deal, const T* __restrict__ x, const P* __restrict__ w, const P* __restrict__ b, float eps,
                                                                          T* __restrict__ y, float2* __restrict__ stats) {
-    constexpr int NV = PER_LANE / E;
-    __shared__ float2 buffer[2][MOST_THREADS / 32];
-    const int width = (int)s.width, lanes = L ? L : blockDim.x, lane = L ? threadIdx.x % (L ? L : 1) : threadIdx.x;
-    const unsigned g = L ? blockIdx.x * (BLOCK / (L ? L : 1)) + threadIdx.x / (L ? L : 1) : blockIdx.x;
-    const unsigned head = s.heads > 1 ? g % (unsigned)s.heads : 0;
-    Sums<L> sums{buffer};
-    const int shift = E == 1 ? 0 : (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T);
-    int at[NV];
-#pragma unroll
-    for (int j = 0; j < NV; j++) at[j] = (j * lanes + lane) * E - shift;
-    float wf[PER_LANE], bf[PER_LANE];
-    load_params<P, E, NV>(w ? w + (int64_t)head * width : w, at, width, 1.f, wf);
-    load_params<P, E, NV>(b ? b + (int64_t)head * width : b, at, width, 0.f, bf);
-    Pack<T, E> v[NV], next[NV];
-    auto fetch = [&](Pack<T, E>* to, unsigned r) {
-        const T* from = x + place(s, s.x, r);
-#pragma unroll
-        for (int j = 0; j < NV; j++) load_part(to[j], from, at[j], width);
-    };
-    if (g < deal.rows) fetch(next, g);
+    typedef Columns<T, L, A> C;
+    __shared__ __align__(16) float2 buffer[2][MOST_THREADS / 32];
+    __shared__ float counts[MOST_THREADS / 32];
+    const Seat<L> seat(s);
+    const unsigned g = seat.group;
+    const int width = (int)s.width;
+    const int shift = A == WIDE_APART ? (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T) : 0;
+    const C cols(width, seat.lanes, seat.lane, shift);
+    Exchange exchange{buffer};
+    float2 wf[PER_LANE / 2], bf[PER_LANE / 2], f[PER_LANE / 2];
+    cols.params(w ? w + (int64_t)seat.head * width : w, 1.f, wf);
+    cols.params(b ? b + (int64_t)seat.head * width : b, 0.f, bf);
+    const float per_row = 1.f / (float)width;
+    float per_warp = 0;
+    if (!L) {
+        const float mine = lanes_sum<0>((float)cols.count());
+        per_warp = mine > 0 ? 1.f / mine : 0.f;
+        if (seat.lane % 32 == 0) counts[seat.lane / 32] = mine;      // (seen by all after the first exchange's barrier)
+    }
+    Pack<T, C::E> next[C::NV];
+    if (g < deal.rows) cols.load(next, x + place(s, s.x, g));
     for (unsigned i = 0; i < deal.rounds; i++) {
         const unsigned r = i * deal.groups + g;
         const bool there = r < deal.rows;
+        C::unpack(next, f);
+        if (there && deal.rows - r > deal.groups) cols.load(next, x + place(s, s.x, r + deal.groups));
+        float2 t = f[0];
 #pragma unroll
-        for (int j = 0; j < NV; j++) v[j] = next[j];
-        if (there && deal.rows - r > deal.groups) fetch(next, r + deal.groups);
-        float sum = 0, sq = 0;
+        for (int k = 1; k < PER_LANE / 2; k++) t = add2(t, f[k]);
+        const float sum = lanes_sum<L>(t.x + t.y);
+        float mean = sum * (L ? per_row : per_warp);
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            float f[E];
-            v[j].to(f);
+        for (int k = 0; k < PER_LANE / 2; k++) f[k] = add2(f[k], both(-mean));
+        cols.clear(f);
+        t = mul2(f[0], f[0]);
 #pragma unroll
-            for (int e = 0; e < E; e++) sum += f[e];
-        }
-        const float mean = sums.all(make_float2(sum, 0)).x / (float)width;
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-            float f[E];
-            v[j].to(f);
-            const bool whole = at[j] >= 0 && at[j] + E <= width;
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float c = f[e] - mean;
-                if (whole || (at[j] + e >= 0 && at[j] + e < width)) sq += c * c;
+        for (int k = 1; k < PER_LANE / 2; k++) t = fma2(f[k], f[k], t);
+        float sq = lanes_sum<L>(t.x + t.y);
+        if (!L) {
+            const float own = mean;
+            float2 t = both(0.f);
+            exchange(make_float2(own, sq), [&](int k, float2 v) { t = fma2(v, make_float2(counts[k], 1.f), t); });
+            mean = t.x * per_row;
+            sq = t.y;
+            const float2* all = buffer[exchange.turn ^ 1];
+            for (int k = 0; k < blockDim.x / 32; k++) {
+                const float d = all[k].x - mean;
+                sq = fmaf(counts[k] * d, d, sq);
             }
+            const float2 move = both(own - mean);
+#pragma unroll
+            for (int k = 0; k < PER_LANE / 2; k++) f[k] = add2(f[k], move);
         }
-        const float rstd = rsqrtf(sums.all(make_float2(sq, 0)).x / (float)width + eps);
+        const float rstd = rsqrtf(sq * per_row + eps);
         if (!there) continue;
-        if (stats && lane == 0) stats[r] = make_float2(mean, rstd);
-        T* to = y + (int64_t)r * width;
+        if (stats && seat.lane == 0) stats[r] = make_float2(mean, rstd);
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            float f[E];
-            v[j].to(f);
-#pragma unroll
-            for (int e = 0; e < E; e++) f[e] = fmaf((f[e] - mean) * rstd, wf[j * E + e], bf[j * E + e]);
-            Pack<T, E> out;
-            out.from(f);
-            store_part(out, to, at[j], width);
-        }
+        for (int k = 0; k < PER_LANE / 2; k++) f[k] = fma2(mul2(f[k], both(rstd)), wf[k], bf[k]);
+        cols.store(y + (int64_t)r * width, f);
     }
 }
 
 // dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w, xh = (x - mean) rstd; sums over the group's rows of dy xh and dy.
 // part: [partials][2][width], one for each group, or (merge) for each warp; may be NULL, and so may dx.
-template <class T, class P, int L, int E>
+template <class T, class P, int L, Access A>
 __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_bw(frnn_rows s, Deal deal, const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ w,
                                                                          const float2* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, bool merge) {
-    constexpr int NV = PER_LANE / E;
-    __shared__ float2 buffer[2][MOST_THREADS / 32];
-    const int width = (int)s.width, lanes = L ? L : blockDim.x, lane = L ? threadIdx.x % (L ? L : 1) : threadIdx.x;
-    const unsigned g = L ? blockIdx.x * (BLOCK / (L ? L : 1)) + threadIdx.x / (L ? L : 1) : blockIdx.x;
-    const unsigned head = s.heads > 1 ? g % (unsigned)s.heads : 0;
-    Sums<L> sums{buffer};
-    const int shift = E == 1 ? 0 : (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T);
-    int at[NV];
+    typedef Columns<T, L, A> C;
+    __shared__ __align__(16) float2 buffer[2][MOST_THREADS / 32];
+    const Seat<L> seat(s);
+    const unsigned g = seat.group;
+    const int width = (int)s.width;
+    const int shift = A == WIDE_APART ? (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T) : 0;
+    const C cols(width, seat.lanes, seat.lane, shift);
+    Exchange exchange{buffer};
+    float2 wf[PER_LANE / 2], dw[PER_LANE / 2], db[PER_LANE / 2], f[PER_LANE / 2], u[PER_LANE / 2];
+    cols.params(w ? w + (int64_t)seat.head * width : w, 1.f, wf);
+    const float per_row = 1.f / (float)width;
 #pragma unroll
-    for (int j = 0; j < NV; j++) at[j] = (j * lanes + lane) * E - shift;
-    float wf[PER_LANE], dw[PER_LANE], db[PER_LANE];
-    load_params<P, E, NV>(w ? w + (int64_t)head * width : w, at, width, 1.f, wf);
-#pragma unroll
-    for (int i = 0; i < PER_LANE; i++) dw[i] = db[i] = 0;
-    Pack<T, E> xv[NV], gv[NV], xn[NV], gn[NV];
-    float2 st, sn = make_float2(0, 0);
+    for (int k = 0; k < PER_LANE / 2; k++) dw[k] = db[k] = both(0.f);
+    Pack<T, C::E> xn[C::NV], gn[C::NV];
+    float2 sn = both(0.f);
     auto fetch = [&](unsigned r) {
-        const T *px = x + place(s, s.x, r), *pg = dy + place(s, s.dy, r);
         sn = stats[r];
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-            load_part(xn[j], px, at[j], width);
-            load_part(gn[j], pg, at[j], width);
-        }
+        cols.load(xn, x + place(s, s.x, r));
+        cols.load(gn, dy + place(s, s.dy, r));
     };
 #pragma unroll
-    for (int j = 0; j < NV; j++) { xn[j].zero(); gn[j].zero(); }
+    for (int j = 0; j < C::NV; j++) { xn[j].zero(); gn[j].zero(); }
     if (g < deal.rows) fetch(g);
     for (unsigned i = 0; i < deal.rounds; i++) {
         const unsigned r = i * deal.groups + g;
         const bool there = r < deal.rows;
-        st = sn;
-#pragma unroll
-        for (int j = 0; j < NV; j++) { xv[j] = xn[j]; gv[j] = gn[j]; }
+        const float2 st = sn;
+        C::unpack(xn, f);
+        C::unpack(gn, u);
         if (there && deal.rows - r > deal.groups) fetch(r + deal.groups);
-        float2 a = make_float2(0, 0);
+        float2 a = both(0.f), c = both(0.f);
         if (there) {
 #pragma unroll
-            for (int j = 0; j < NV; j++) {
-                float f[E], u[E];
-                xv[j].to(f);
-                gv[j].to(u);
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const float xh = (f[e] - st.x) * st.y, gw = u[e] * wf[j * E + e];      // u = 0 where there is no column
-                    a.x += gw;
-                    a.y += gw * xh;
-                    dw[j * E + e] += u[e] * xh;
-                    db[j * E + e] += u[e];
-                }
+            for (int k = 0; k < PER_LANE / 2; k++) {
+                f[k] = mul2(add2(f[k], both(-st.x)), both(st.y));
+                dw[k] = fma2(u[k], f[k], dw[k]);           // u = 0 where there is no column
+                db[k] = add2(db[k], u[k]);
+                u[k] = mul2(u[k], wf[k]);
+                a = add2(a, u[k]);
+                c = fma2(u[k], f[k], c);
             }
         }
-        if (dx) {
-            a = sums.all(a);
-            a.x /= (float)width;
-            a.y /= (float)width;
-            if (there) {
-                T* to = dx + place(s, s.dx, r);
-#pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    float f[E], u[E];
-                    xv[j].to(f);
-                    gv[j].to(u);
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const float xh = (f[e] - st.x) * st.y;
-                        f[e] = st.y * (u[e] * wf[j * E + e] - a.x - xh * a.y);
-                    }
-                    Pack<T, E> out;
-                    out.from(f);
-                    store_part(out, to, at[j], width);
-                }
-            }
+        if (!dx) continue;
+        float ma = lanes_sum<L>(a.x + a.y), mc = lanes_sum<L>(c.x + c.y);
+        if (!L) {
+            float2 t = both(0.f);
+            exchange(make_float2(ma, mc), [&](int, float2 v) { t = add2(t, v); });
+            ma = t.x;
+            mc = t.y;
         }
+        if (!there) continue;
+        const float2 off = both(-st.y * (ma * per_row)), by = both(-st.y * (mc * per_row));
+#pragma unroll
+        for (int k = 0; k < PER_LANE / 2; k++) f[k] = fma2(f[k], by, fma2(u[k], both(st.y), off));
+        cols.store(dx + place(s, s.dx, r), f);
     }
     if (!part) return;
     unsigned p = g;
@@ -221,24 +278,23 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_bw(frnn_r
 #pragma unroll
         for (int o = L ? L : 32; o < 32; o *= 2)
 #pragma unroll
-            for (int i = 0; i < PER_LANE; i++) {
-                dw[i] += __shfl_xor_sync(~0u, dw[i], o);
-                db[i] += __shfl_xor_sync(~0u, db[i], o);
+            for (int k = 0; k < PER_LANE / 2; k++) {
+                dw[k] = add2(dw[k], make_float2(__shfl_xor_sync(~0u, dw[k].x, o), __shfl_xor_sync(~0u, dw[k].y, o)));
+                db[k] = add2(db[k], make_float2(__shfl_xor_sync(~0u, db[k].x, o), __shfl_xor_sync(~0u, db[k].y, o)));
             }
         p = g * (L ? L : 1) / 32;
         if (threadIdx.x % 32 >= (L ? L : 1)) return;
     }
     float* to = part + 2ll * p * width;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < C::NV; j++)
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int c = at[j] + e;
-            if (c >= 0 && c < width) {
-                to[c] = dw[j * E + e];
-                to[width + c] = db[j * E + e];
+        for (int e = 0; e < C::E; e++)
+            if (cols.there(j, e)) {
+                const int k = j * C::E + e;
+                to[cols.at[j] + e] = (&dw[0].x)[k];
+                to[width + cols.at[j] + e] = (&db[0].x)[k];
             }
-        }
 }
 
 // ---- rows that no block keeps in registers: read again for each step ---------------------------------------------------
@@ -315,22 +371,36 @@ __global__ void layer_norm_dw_long(frnn_rows s, const T* __restrict__ dy, const 
     to[s.width + d] = db;
 }
 
-// Sum of the partial sums of a head: partials head, head + heads, ..., a warp takes every eighth of them.
-template <class P>
+// Sum of the partial sums of a head (partials head, head + heads, ...): 8 lanes have V columns each, 32 slices of the
+// partials are summed side by side, so that few loads wait for one another.
+template <class P, int V>
 __global__ void __launch_bounds__(BLOCK) layer_norm_join(const float* __restrict__ part, int partials, int heads, int width, P* __restrict__ dw, P* __restrict__ db) {
-    __shared__ float share[BLOCK / 32][32];
-    const int c = blockIdx.x * 32 + threadIdx.x % 32, slice = threadIdx.x / 32, head = blockIdx.y;
+    constexpr int LANES = 8, SLICES = BLOCK / LANES;
+    __shared__ float share[SLICES][LANES * V];
+    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, head = blockIdx.y, c = (blockIdx.x * LANES + lane) * V;
     P* to = blockIdx.z ? db : dw;
     if (!to) return;
-    float sum = 0;
+    float sum[V] = {};
     if (c < width)
 #pragma unroll 8
-        for (int64_t p = head + (int64_t)slice * heads; p < partials; p += (int64_t)heads * (BLOCK / 32)) sum += part[(2 * p + blockIdx.z) * width + c];
-    share[slice][threadIdx.x % 32] = sum;
+        for (int64_t p = head + (int64_t)slice * heads; p < partials; p += (int64_t)heads * SLICES) {
+            const float* from = part + (2 * p + blockIdx.z) * width + c;
+            if constexpr (V == 4) {
+                const float4 v = *(const float4*)from;
+                sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+            } else {
+                sum[0] += *from;
+            }
+        }
+#pragma unroll
+    for (int v = 0; v < V; v++) share[slice][lane * V + v] = sum[v];
     __syncthreads();
-    if (slice || c >= width) return;
-    for (int i = 1; i < BLOCK / 32; i++) sum += share[i][threadIdx.x];
-    to[(int64_t)head * width + c] = from_float<P>(sum);
+    const int i = threadIdx.x, col = blockIdx.x * LANES * V + i;
+    if (i >= LANES * V || col >= width) return;
+    float total = 0;
+#pragma unroll
+    for (int k = 0; k < SLICES; k++) total += share[k][i];
+    to[(int64_t)head * width + col] = from_float<P>(total);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -388,10 +458,6 @@ Lie lie_of(const frnn_rows& s, const void* p, const int64_t* stride, size_t size
     return l;
 }
 
-enum Access { ELEMENTS, WIDE_ALIKE, WIDE_APART };
-
-// 16-byte accesses need rows of all tensors at the same distance behind a boundary.  WIDE_ALIKE: all rows at a boundary;
-// WIDE_APART: evenly spaced rows, each group's at one distance (groups are dealt out in multiples of 8 rows).
 Access access_of(const frnn_rows& s, const Lie* l, int count) {
     bool alike = s.width % 8 == 0, apart = s.width % 8 != 0;
     for (int i = 0; i < count; i++) {
@@ -418,11 +484,12 @@ template <class F> int with_types(int dtype, int param_dtype, F f) {
     });
 }
 
-// Calls f(integral_constant L, integral_constant E).
-template <class T, class F> int with_lanes(int lanes, Access access, F f) {
+// Calls f(integral_constant L, integral_constant A).
+template <class F> int with_lanes(int lanes, Access access, F f) {
     auto pick = [&](auto l) {
-        if (access == ELEMENTS) return f(l, std::integral_constant<int, 1>());
-        return f(l, std::integral_constant<int, WIDE<T>>());
+        if (access == ELEMENTS) return f(l, std::integral_constant<Access, ELEMENTS>());
+        if (access == WIDE_ALIKE) return f(l, std::integral_constant<Access, WIDE_ALIKE>());
+        return f(l, std::integral_constant<Access, WIDE_APART>());
     };
     switch (lanes) {
         case 2: return pick(std::integral_constant<int, 2>());
@@ -434,7 +501,7 @@ template <class T, class F> int with_lanes(int lanes, Access access, F f) {
     }
 }
 
-enum { FW_THREADS_PER_SM = 1536, BW_THREADS_PER_SM = 768 };
+enum { FW_THREADS_PER_SM = 768, BW_THREADS_PER_SM = 512 };
 
 }  // namespace
 
@@ -460,8 +527,8 @@ int frnn_layer_norm_forward(const frnn_rows* s, int dtype, const void* x, int pa
             layer_norm_fw_long<T, P><<<(unsigned)rows, BLOCK, 0, st>>>(*s, (const T*)x, (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
             return launched("frnn_layer_norm_forward");
         }
-        return with_lanes<T>(plan.lanes, access_of(*s, lies, 2), [&](auto l, auto e) {
-            layer_norm_fw<T, P, l.value, e.value><<<plan.grid, plan.threads, 0, st>>>(*s, plan.deal, (const T*)x, (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
+        return with_lanes(plan.lanes, access_of(*s, lies, 2), [&](auto l, auto a) {
+            layer_norm_fw<T, P, l.value, a.value><<<plan.grid, plan.threads, 0, st>>>(*s, plan.deal, (const T*)x, (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
             return launched("frnn_layer_norm_forward");
         });
     });
@@ -503,15 +570,19 @@ int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, cons
                 rc = launched("frnn_layer_norm_backward");
             }
         } else if (rows && (dx || sums)) {
-            rc = with_lanes<T>(plan.lanes, access, [&](auto l, auto e) {
-                layer_norm_bw<T, P, l.value, e.value><<<plan.grid, plan.threads, 0, st>>>(*s, plan.deal, (const T*)dy, (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx,
+            rc = with_lanes(plan.lanes, access, [&](auto l, auto a) {
+                layer_norm_bw<T, P, l.value, a.value><<<plan.grid, plan.threads, 0, st>>>(*s, plan.deal, (const T*)dy, (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx,
                                                                                           sums ? (float*)workspace : nullptr, merge);
                 return launched("frnn_layer_norm_backward");
             });
         }
         if (rc || !sums) return rc;
-        layer_norm_join<P><<<dim3((unsigned)((s->width + 31) / 32), (unsigned)s->heads, 2), BLOCK, 0, st>>>((const float*)workspace, partials, (int)s->heads, (int)s->width, (P*)dweight,
-                                                                                                          (P*)dbias);
+        auto join = [&](auto v) {
+            layer_norm_join<P, v.value><<<dim3((unsigned)((s->width + 8 * v.value - 1) / (8 * v.value)), (unsigned)s->heads, 2), BLOCK, 0, st>>>(
+                (const float*)workspace, partials, (int)s->heads, (int)s->width, (P*)dweight, (P*)dbias);
+        };
+        if (s->width % 4) join(std::integral_constant<int, 1>());
+        else join(std::integral_constant<int, 4>());
         return launched("frnn_layer_norm_backward");
     });
 }
