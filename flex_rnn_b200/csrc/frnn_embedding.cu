@@ -1,20 +1,69 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+// The lookup moves rows and is bound by memory.  The gradient is dense: most of its bytes are the rows of tokens that do
+// not occur.  `embedding_sort` therefore does two things side by side: one cluster of blocks sorts the tokens (places of
+// equal tokens stay in order), all other blocks write the zero rows, which only have to know which tokens occur.
+// `embedding_sums` then walks over the sorted places in chunks of one length, whatever the frequencies of the tokens (a
+// text's most frequent token has hundreds of times its average share): runs of equal tokens inside a chunk are finished
+// there, those that cross its ends leave a partial sum each, which `embedding_join` adds in order.  No sum depends on how
+// threads are scheduled.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <type_traits>
+
 #include "frnn_lm.cuh"
 
 using namespace frnn_lm;
+namespace cg = cooperative_groups;
 
 namespace {
 
-// y_i = scale * W[t_i]; a zero row where t_i is ignored or (reported) outside the vocabulary.
-template <class T>
-__global__ void embedding_fw(const T* __restrict__ w, int64_t rows, int64_t width, int64_t row_stride, int64_t col_stride, const void* __restrict__ tokens,
-                             int token_bytes, int64_t n, float scale, int64_t ignore, T* __restrict__ out, int* err) {
-    for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
-        const int64_t t = token_at(tokens, token_bytes, i);
+enum { BLOCK = 256, UNROLL = 8 };
+
+// How a block's threads stand to rows: `lanes` threads (a power of two, all of the block for wide rows) have E columns
+// each, blockIdx.y counts the parts of rows wider than that.
+struct Shape {
+    int lanes, groups;         // threads of a group, groups of a block
+    unsigned parts;            // blocks side by side over a row's columns
+};
+
+Shape shape_of(int64_t width, int each) {
+    const int64_t vectors = (width + each - 1) / each;
+    Shape s{1, 1, 1};
+    while (s.lanes < BLOCK && s.lanes < vectors) s.lanes *= 2;
+    s.groups = BLOCK / s.lanes;
+    s.parts = (unsigned)((vectors + s.lanes - 1) / s.lanes);
+    return s;
+}
+
+// y_i = scale * W[t_i]; a zero row where t_i is ignored or (reported) outside the vocabulary.  A group takes UNROLL / 2
+// rows, whose loads are all under way before the first is used.
+template <class T, int E>
+__global__ void __launch_bounds__(BLOCK) embedding_fw(const T* __restrict__ w, int64_t rows, int width, int64_t row_stride, int64_t col_stride, const void* __restrict__ tokens,
+                                                      int token_bytes, int n, float scale, int64_t ignore, T* __restrict__ out, int* err, Shape shape) {
+    constexpr int ROWS = UNROLL / 2;
+    const int lane = threadIdx.x % shape.lanes, first = (blockIdx.x * shape.groups + threadIdx.x / shape.lanes) * ROWS, c = (int)(blockIdx.y * shape.lanes + lane) * E;
+    Pack<T, E> v[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; u++) {
+        v[u].zero();
+        if (first + u >= n) continue;
+        const int64_t t = token_at(tokens, token_bytes, first + u);
         const bool there = t != ignore && t >= 0 && t < rows;
-        if (t != ignore && !there && threadIdx.x == 0) *err = CODE_TOKEN;
-        for (int64_t d = threadIdx.x; d < width; d += blockDim.x)
-            out[i * width + d] = from_float<T>(there ? scale * to_float(w[t * row_stride + d * col_stride]) : 0.f);
+        if (t != ignore && !there && c == 0) *err = CODE_TOKEN;
+        if (there && c < width) v[u].load(w + t * row_stride + (E == 1 ? c * col_stride : c));
+    }
+    if (c >= width) return;
+#pragma unroll
+    for (int u = 0; u < ROWS; u++) {
+        if (first + u >= n) return;
+        float f[E];
+        v[u].to(f);
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e] *= scale;
+        v[u].from(f);
+        v[u].store(out + (int64_t)(first + u) * width + c);
     }
 }
 
@@ -24,93 +73,259 @@ __device__ __forceinline__ unsigned key_of(const void* tokens, int bytes, int64_
     return t != ignore && t >= 0 && t < rows ? (unsigned)t : (unsigned)rows;
 }
 
-enum { SORT_THREADS = 1024, DIGIT_BITS = 8, DIGITS = 1 << DIGIT_BITS };
+enum { CLUSTER = 8, SORT_THREADS = 1024, WARPS = SORT_THREADS / 32, MOST_BITS = 9, DIGITS = 1 << MOST_BITS, FLAGS = 32768 };
 
-// Stable radix sort of (token, place) by token, one block: places of equal tokens stay in order, so the sums below do
-// not depend on how threads are scheduled.  Each warp takes a contiguous part of the places in rounds of 32.
-__global__ void __launch_bounds__(SORT_THREADS) embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, int passes,
-                                                               unsigned* key_a, unsigned* key_b, int* at_a, int* at_b) {
-    extern __shared__ unsigned count[];                        // [warps][DIGITS]
-    __shared__ unsigned total[DIGITS];
-    const int warps = SORT_THREADS / 32, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const int part = (int)(((int64_t)n + warps - 1) / warps + 31) / 32 * 32;
-    const int lo = min((int64_t)n, (int64_t)warp * part), hi = min((int64_t)n, (int64_t)lo + part);
+// Zeros into the bytes [lo, hi) of p, by the lanes of a warp; lo, hi and p are on boundaries of elements of `size` bytes.
+__device__ __forceinline__ void fill_zero(char* p, int64_t lo, int64_t hi, int size) {
+    const int lane = threadIdx.x & 31;
+    const int64_t head = min(hi, lo + (int64_t)(-(uintptr_t)(p + lo) & 15)), tail = max(head, hi - (int64_t)((uintptr_t)(p + hi) & 15));
+    for (int64_t i = head + 16 * lane; i < tail; i += 512) *(uint4*)(p + i) = make_uint4(0, 0, 0, 0);
+    if (size == 4) {
+        if (lo + 4 * lane < head) *(unsigned*)(p + lo + 4 * lane) = 0;
+        if (tail + 4 * lane < hi) *(unsigned*)(p + tail + 4 * lane) = 0;
+    } else {
+        if (lo + 2 * lane < head) *(unsigned short*)(p + lo + 2 * lane) = 0;
+        if (tail + 2 * lane < hi) *(unsigned short*)(p + tail + 2 * lane) = 0;
+    }
+}
+
+// Block 0 to CLUSTER - 1: stable radix sort of (token, place) by token, `bits` bits a pass.  Each warp takes a contiguous
+// part of the places in rounds of 32; a place's rank is what comes before it in its round, its warp, its block, its
+// cluster and among the smaller digits.  The other blocks: zero rows for the tokens that do not occur.
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SORT_THREADS, 1)
+embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, int passes, int bits, unsigned* key_a, unsigned* key_b, int* at_a,
+               int* at_b, char* dw, int64_t row_bytes, int size) {
+    extern __shared__ unsigned count[];                        // [WARPS][DIGITS]; the other blocks: a byte for each row
+    __shared__ unsigned total[DIGITS], carry[WARPS];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (blockIdx.x >= CLUSTER) {
+        unsigned char* occurs = (unsigned char*)count;
+        const int64_t blocks = gridDim.x - CLUSTER, each = (rows + blocks - 1) / blocks, from = (blockIdx.x - CLUSTER) * each, to = min(rows, from + each);
+        for (int64_t lo = from; lo < to; lo += FLAGS) {
+            const int here = (int)min((int64_t)FLAGS, to - lo);
+            __syncthreads();
+            for (int i = threadIdx.x; i < here; i += SORT_THREADS) occurs[i] = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += SORT_THREADS) {
+                const int64_t t = token_at(tokens, token_bytes, i);
+                if (t >= lo && t < lo + here && t != ignore) occurs[t - lo] = 1;
+            }
+            __syncthreads();
+            for (int i = warp; i < here; i += WARPS)
+                if (!occurs[i]) fill_zero(dw, (lo + i) * row_bytes, (lo + i + 1) * row_bytes, size);
+        }
+        return;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    const unsigned rank = blockIdx.x, mask = (1u << bits) - 1, digits = 1u << bits;
+    const int64_t part = (((int64_t)n + CLUSTER * WARPS - 1) / (CLUSTER * WARPS) + 31) / 32 * 32;
+    const int lo = (int)min((int64_t)n, (int64_t)(rank * WARPS + warp) * part), hi = (int)min((int64_t)n, lo + part);
+    unsigned* mine = count + warp * DIGITS;
     for (int pass = 0; pass < passes; pass++) {
-        const int shift = pass * DIGIT_BITS;
-        const unsigned *from = (pass & 1) ? key_b : key_a;
-        const int* from_at = (pass & 1) ? at_b : at_a;
-        unsigned* to = (pass & 1) ? key_a : key_b;
-        int* to_at = (pass & 1) ? at_a : at_b;
-        for (int i = threadIdx.x; i < warps * DIGITS; i += SORT_THREADS) count[i] = 0;
+        const int shift = pass * bits;
+        const unsigned* from = pass & 1 ? key_b : key_a;
+        const int* from_at = pass & 1 ? at_b : at_a;
+        unsigned* to = pass & 1 ? key_a : key_b;
+        int* to_at = pass & 1 ? at_a : at_b;
+        // the buffers were written by other SMs: read past this one's L1
+        auto key = [&](int i) { return pass ? __ldcg(from + i) : key_of(tokens, token_bytes, i, rows, ignore); };
+        for (int i = lane; i < digits; i += 32) mine[i] = 0;
+        __syncwarp();
+        for (int i = lo + lane; i < hi; i += 32) atomicAdd(&mine[(key(i) >> shift) & mask], 1u);
         __syncthreads();
-        for (int i = lo + lane; i < hi; i += 32)
-            atomicAdd(&count[warp * DIGITS + (((pass ? from[i] : key_of(tokens, token_bytes, i, rows, ignore)) >> shift) & (DIGITS - 1))], 1u);
-        __syncthreads();
-        for (int d = threadIdx.x; d < DIGITS; d += SORT_THREADS) {
+        unsigned all = 0, below = 0;
+        const int d = threadIdx.x;
+        if (d < digits) {
             unsigned sum = 0;
-            for (int k = 0; k < warps; k++) { const unsigned c = count[k * DIGITS + d]; count[k * DIGITS + d] = sum; sum += c; }
+#pragma unroll 8
+            for (int k = 0; k < WARPS; k++) { const unsigned c = count[k * DIGITS + d]; count[k * DIGITS + d] = sum; sum += c; }
             total[d] = sum;
         }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned sum = 0;
-            for (int d = 0; d < DIGITS; d++) { const unsigned c = total[d]; total[d] = sum; sum += c; }
+        cluster.sync();
+        if (d < digits)
+#pragma unroll
+            for (int k = 0; k < CLUSTER; k++) {
+                const unsigned c = cluster.map_shared_rank(total, k)[d];
+                if (k < rank) below += c;
+                all += c;
+            }
+        cluster.sync();                                        // everyone has read `total`; it takes the digits' bases next
+        unsigned scan = all;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const unsigned v = __shfl_up_sync(~0u, scan, o);
+            if (lane >= o) scan += v;
         }
+        if (lane == 31) carry[warp] = scan;
+        __syncthreads();
+        unsigned before = 0;
+        for (int k = 0; k < warp && k < DIGITS / 32; k++) before += carry[k];
+        if (d < digits) total[d] = before + scan - all + below;
         __syncthreads();
         for (int i0 = lo; i0 < hi; i0 += 32) {
             const int i = i0 + lane;
             const bool in = i < hi;
-            const unsigned key = !in ? 0 : pass ? from[i] : key_of(tokens, token_bytes, i, rows, ignore);
-            const unsigned digit = in ? (key >> shift) & (DIGITS - 1) : DIGITS;
-            const unsigned same = __match_any_sync(~0u, digit);
+            const unsigned k = in ? key(i) : 0, digit = in ? (k >> shift) & mask : digits;
+            const unsigned same = __match_any_sync(~0u, digit), earlier = same & ((1u << lane) - 1);
             if (in) {
-                const unsigned before = __popc(same & ((1u << lane) - 1));
-                const unsigned base = count[warp * DIGITS + digit];
-                to[total[digit] + base + before] = key;
-                to_at[total[digit] + base + before] = pass ? from_at[i] : i;
+                const unsigned p = total[digit] + mine[digit] + __popc(earlier);
+                to[p] = k;
+                to_at[p] = pass ? __ldcg(from_at + i) : i;
             }
             __syncwarp();
-            if (in && (same & ((1u << lane) - 1)) == 0) count[warp * DIGITS + digit] += __popc(same);
+            if (in && !earlier) mine[digit] += __popc(same);
             __syncwarp();
         }
-        __syncthreads();
+        cluster.sync();
     }
 }
 
-__device__ __forceinline__ int lower_bound(const unsigned* keys, int n, unsigned key) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (keys[mid] < key) lo = mid + 1; else hi = mid;
+enum : unsigned { NO_KEY = 0xFFFFFFFFu };
+
+template <class T, int E> __device__ __forceinline__ void write_row(const float* sum, float scale, T* to) {
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) f[e] = scale * sum[e];
+    Pack<T, E> v;
+    v.from(f);
+    v.store(to);
+}
+template <int E> __device__ __forceinline__ void write_part(const float* sum, float* to) {
+#pragma unroll
+    for (int e = 0; e < E; e += E < 4 ? 1 : 4) {
+        if constexpr (E >= 4) *(float4*)(to + e) = make_float4(sum[e], sum[e + 1], sum[e + 2], sum[e + 3]);
+        else to[e] = sum[e];
     }
-    return lo;
 }
 
-// dW_v = scale * sum of the upstream rows at the places of token v, in the order of the places, in 32 bits.
-template <class T>
-__global__ void embedding_bw(const T* __restrict__ dy, const unsigned* __restrict__ keys, const int* __restrict__ at, int n, int64_t rows, int64_t width,
-                             float scale, T* __restrict__ dw) {
-    for (int64_t v = blockIdx.x; v < rows; v += gridDim.x) {
-        const int lo = lower_bound(keys, n, (unsigned)v), hi = lower_bound(keys, n, (unsigned)v + 1);
-        for (int64_t d = threadIdx.x; d < width; d += blockDim.x) {
-            float sum = 0;
-            for (int j = lo; j < hi; j++) sum += to_float(dy[(int64_t)at[j] * width + d]);
-            dw[v * width + d] = from_float<T>(scale * sum);
+// A group sums a chunk of the sorted places.  part: [chunks][2][width], sums of the run that came in over the chunk's start
+// and of the one that goes on over its end.
+template <class T, int E>
+__global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy, const unsigned* __restrict__ keys, const int* __restrict__ at, int n, unsigned rows, int width,
+                                                        int chunk, float scale, T* __restrict__ dw, float* __restrict__ part, Shape shape) {
+    const int lane = threadIdx.x % shape.lanes, c = (int)(blockIdx.y * shape.lanes + lane) * E;
+    const int64_t mine = (int64_t)blockIdx.x * shape.groups + threadIdx.x / shape.lanes, from = mine * chunk;
+    if (from >= n || c >= width) return;
+    const int lo = (int)from, hi = (int)min((int64_t)n, from + chunk);
+    unsigned run = keys[lo];
+    bool came_in = lo > 0 && keys[lo - 1] == run;
+    const unsigned after = hi < n ? keys[hi] : NO_KEY;
+    float* parts = part + 2 * mine * width + c;
+    float sum[E] = {};
+    for (int j = lo; j < hi && run < rows; j += UNROLL) {
+        unsigned k[UNROLL];
+        Pack<T, E> v[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            k[u] = j + u < hi ? keys[j + u] : NO_KEY;
+            v[u].zero();
+            if (k[u] < rows) v[u].load(dy + (int64_t)at[j + u] * width + c);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            if (j + u < hi && k[u] != run) {
+                if (run < rows) {
+                    if (came_in) write_part<E>(sum, parts);
+                    else write_row<T, E>(sum, scale, dw + (int64_t)run * width + c);
+                }
+                run = k[u];
+                came_in = false;
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] = 0;
+            }
+            float f[E];
+            v[u].to(f);
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] += f[e];
         }
     }
+    if (run >= rows) return;
+    if (came_in) write_part<E>(sum, parts);
+    else if (after == run) write_part<E>(sum, parts + width);
+    else write_row<T, E>(sum, scale, dw + (int64_t)run * width + c);
 }
 
-int sort_passes(int64_t rows) {
-    int bits = 1;
-    while ((rows >> bits) != 0) bits++;          // the keys are 0 .. rows
-    return (bits + DIGIT_BITS - 1) / DIGIT_BITS;
+// The block of the chunk that a crossing run starts in adds that run's partial sums: 64 threads with V columns each, 4
+// slices of the partials side by side.
+template <class T, int V>
+__global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restrict__ keys, int n, unsigned rows, int width, int chunk, float scale, T* __restrict__ dw,
+                                                        const float* __restrict__ part) {
+    constexpr int LANES = 64, SLICES = BLOCK / LANES;
+    __shared__ float share[SLICES][LANES * V];
+    const int64_t mine = blockIdx.x, lo = mine * chunk, hi = lo + chunk;
+    if (hi >= n) return;
+    const unsigned run = keys[hi];
+    if (run >= rows || keys[hi - 1] != run || (lo > 0 && keys[lo - 1] == run)) return;
+    int64_t last = mine;                                  // the last chunk that the run reaches
+    for (;;) {
+        const int64_t q = last + 1 + threadIdx.x;
+        const int more = __syncthreads_count(q * chunk < n && keys[q * chunk] == run);      // sorted: the first `more` of them
+        last += more;
+        if (more < BLOCK) break;
+    }
+    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (int)(blockIdx.y * LANES + lane) * V;
+    float sum[V] = {};
+    if (c < width)
+#pragma unroll 8
+        for (int64_t q = mine + slice; q <= last; q += SLICES) {
+            const float* from = part + (2 * q + (q == mine)) * width + c;
+            if constexpr (V == 4) {
+                const float4 v = *(const float4*)from;
+                sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+            } else {
+                sum[0] += *from;
+            }
+        }
+#pragma unroll
+    for (int v = 0; v < V; v++) share[slice][lane * V + v] = sum[v];
+    __syncthreads();
+    for (int i = threadIdx.x; i < LANES * V; i += BLOCK) {
+        const int col = blockIdx.y * LANES * V + i;
+        if (col >= width) continue;
+        float total = 0;
+#pragma unroll
+        for (int k = 0; k < SLICES; k++) total += share[k][i];
+        dw[(int64_t)run * width + col] = from_float<T>(scale * total);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+
+struct Plan {
+    int passes, bits;          // of the sort
+    int chunk;                 // places of a chunk: 8 to 128, so that about eight blocks an SM have one
+    int64_t chunks;
+    size_t at_parts, bytes;    // of the workspace: where the partial sums are, all of it
+};
+
+Plan plan_of(int dtype, int64_t rows, int64_t width, int64_t n) {
+    Plan p;
+    int all = 1;
+    while ((rows >> all) != 0) all++;          // the keys are 0 .. rows
+    p.passes = (all + MOST_BITS - 1) / MOST_BITS;
+    p.bits = (all + p.passes - 1) / p.passes;
+    const double blocks = (double)n * width * dtype_bytes(dtype) / (16 * BLOCK);       // blocks' worth of places, with 16 bytes a thread
+    for (p.chunk = 8; p.chunk < 128 && blocks / p.chunk > 8.0 * sm_count(); p.chunk *= 2) {}
+    p.chunks = (n + p.chunk - 1) / p.chunk;
+    p.at_parts = ((size_t)n * 16 + 255) / 256 * 256;
+    p.bytes = p.at_parts + (size_t)p.chunks * 2 * width * 4;
+    return p;
 }
 
 int bad_shape(const char* what, int dtype, int64_t rows, int64_t width, int token_bytes, int64_t n) {
     if (!dtype_known(dtype) || (token_bytes != 4 && token_bytes != 8)) return frnn_fail(FRNN_E_ARG, "%s: unknown data type", what);
-    if (rows < 0 || width < 0 || n < 0 || rows >= (1ll << 31) || width >= (1ll << 31) || n >= (1ll << 31))
-        return frnn_fail(FRNN_E_ARG, "%s: sizes have to be below 2^31", what);
+    if (rows < 0 || width < 0 || n < 0 || rows >= (1ll << 31) || width >= (1ll << 21) || n >= (1ll << 30))
+        return frnn_fail(FRNN_E_ARG, "%s: the vocabulary has to be below 2^31, the width below 2^21, the number of tokens below 2^30", what);
     return FRNN_OK;
+}
+
+// Calls f(T(), integral_constant E): 16 bytes an access, or one element.
+template <class F> int with_access(int dtype, bool wide, F f) {
+    return with_dtype(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (wide) return f(t, std::integral_constant<int, WIDE<T>>());
+        return f(t, std::integral_constant<int, 1>());
+    });
 }
 
 }  // namespace
@@ -122,19 +337,22 @@ int frnn_embedding_forward(int dtype, const void* weight, int64_t rows, int64_t 
     if (int rc = bad_shape("frnn_embedding_forward", dtype, rows, width, token_bytes, n)) return rc;
     if (n == 0 || width == 0) return FRNN_OK;
     if ((!weight && rows) || !tokens || !out || !err_word) return frnn_fail(FRNN_E_ARG, "frnn_embedding_forward: bad argument");
-    if (!on_boundary(weight, dtype_bytes(dtype)) || !on_boundary(out, dtype_bytes(dtype)) || !on_boundary(tokens, token_bytes) || !on_boundary(err_word, 4))
+    const size_t size = dtype_bytes(dtype);
+    if (!on_boundary(weight, size) || !on_boundary(out, size) || !on_boundary(tokens, token_bytes) || !on_boundary(err_word, 4))
         return frnn_fail(FRNN_E_ARG, "frnn_embedding_forward: a pointer is not on a boundary of its elements");
-    return with_dtype(dtype, [&](auto t) {
+    const bool wide = col_stride == 1 && width * size % 16 == 0 && row_stride * (int64_t)size % 16 == 0 && on_boundary(weight, 16) && on_boundary(out, 16);
+    return with_access(dtype, wide, [&](auto t, auto e) {
         typedef decltype(t) T;
-        embedding_fw<T><<<(unsigned)(n < 65535 ? n : 65535), 256, 0, (cudaStream_t)stream>>>((const T*)weight, rows, width, row_stride, col_stride, tokens, token_bytes, n,
-                                                                                          scale, ignore_index, (T*)out, err_word);
+        const Shape shape = shape_of(width, e.value);
+        const int64_t each = shape.groups * (UNROLL / 2);
+        embedding_fw<T, e.value><<<dim3((unsigned)((n + each - 1) / each), shape.parts), BLOCK, 0, (cudaStream_t)stream>>>(
+            (const T*)weight, rows, (int)width, row_stride, col_stride, tokens, token_bytes, (int)n, scale, ignore_index, (T*)out, err_word, shape);
         return launched("frnn_embedding_forward");
     });
 }
 
 size_t frnn_embedding_backward_workspace(int dtype, int64_t rows, int64_t width, int64_t n) {
-    (void)dtype; (void)rows; (void)width;
-    return n <= 0 ? 0 : (size_t)n * 16;
+    return n <= 0 || rows <= 0 || width <= 0 || bad_shape("frnn_embedding_backward_workspace", dtype, rows, width, 8, n) ? 0 : plan_of(dtype, rows, width, n).bytes;
 }
 
 int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int token_bytes, int64_t n, int64_t rows, int64_t width, float scale,
@@ -142,20 +360,45 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     if (int rc = bad_shape("frnn_embedding_backward", dtype, rows, width, token_bytes, n)) return rc;
     if (rows == 0 || width == 0) return FRNN_OK;
     if (!dweight || (n && (!dout || !tokens || !workspace))) return frnn_fail(FRNN_E_ARG, "frnn_embedding_backward: bad argument");
-    if (!on_boundary(dout, dtype_bytes(dtype)) || !on_boundary(dweight, dtype_bytes(dtype)) || !on_boundary(tokens, token_bytes) || !on_boundary(workspace, 16))
+    const size_t size = dtype_bytes(dtype);
+    if (!on_boundary(dout, size) || !on_boundary(dweight, size) || !on_boundary(tokens, token_bytes) || !on_boundary(workspace, 16))
         return frnn_fail(FRNN_E_ARG, "frnn_embedding_backward: a pointer is not on a boundary of its elements (the workspace: of 16 bytes)");
+    const cudaStream_t st = (cudaStream_t)stream;
+    const Plan plan = plan_of(dtype, rows, width, n);
     unsigned* key = (unsigned*)workspace;
     int* at = (int*)(key + 2 * n);
-    const int passes = sort_passes(rows);
-    if (n) {
-        embedding_sort<<<1, SORT_THREADS, SORT_THREADS / 32 * DIGITS * 4, (cudaStream_t)stream>>>(tokens, token_bytes, (int)n, rows, ignore_index, passes, key, key + n, at, at + n);
-        if (int rc = launched("frnn_embedding_backward")) return rc;
+    float* part = n ? (float*)((char*)workspace + plan.at_parts) : nullptr;
+    // the sorting cluster, and clusters that fill: enough blocks for a quarter of a megabyte of zeros each, one an SM at most
+    const int64_t most = sm_count() / CLUSTER * CLUSTER, fill = (rows * width * (int64_t)size / (1 << 18) / CLUSTER + 1) * CLUSTER;
+    const int grid = (int)std::min<int64_t>(most, CLUSTER + fill);
+    static std::atomic<bool> raised[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    enum { SMEM = WARPS * DIGITS * 4 };
+    if (dev < 0 || dev >= 64 || !raised[dev].load(std::memory_order_relaxed)) {
+        if (cudaFuncSetAttribute(embedding_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return launched("frnn_embedding_backward");
+        if (dev >= 0 && dev < 64) raised[dev].store(true, std::memory_order_relaxed);
     }
-    const int side = passes & 1;
-    return with_dtype(dtype, [&](auto t) {
+    embedding_sort<<<grid, SORT_THREADS, SMEM, st>>>(tokens, token_bytes, (int)n, rows, ignore_index, n ? plan.passes : 0, plan.bits, key, key + n, at, at + n, (char*)dweight,
+                                                     width * (int64_t)size, (int)size);
+    if (int rc = launched("frnn_embedding_backward")) return rc;
+    if (n == 0) return FRNN_OK;
+    const int side = plan.passes & 1;
+    const unsigned* keys = key + side * n;
+    const bool wide = width * size % 16 == 0 && on_boundary(dout, 16) && on_boundary(dweight, 16);
+    return with_access(dtype, wide, [&](auto t, auto e) {
         typedef decltype(t) T;
-        embedding_bw<T><<<(unsigned)(rows < 65535 ? rows : 65535), 256, 0, (cudaStream_t)stream>>>((const T*)dout, key + side * n, at + side * n, (int)n, rows, width,
-                                                                                             scale, (T*)dweight);
+        const Shape shape = shape_of(width, e.value);
+        embedding_sums<T, e.value><<<dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st>>>(
+            (const T*)dout, keys, at + side * n, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape);
+        if (int rc = launched("frnn_embedding_backward")) return rc;
+        if (plan.chunks < 2) return (int)FRNN_OK;
+        auto join = [&](auto v) {
+            embedding_join<T, v.value><<<dim3((unsigned)plan.chunks, (unsigned)((width + 64 * v.value - 1) / (64 * v.value))), BLOCK, 0, st>>>(
+                keys, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part);
+        };
+        if (width % 4) join(std::integral_constant<int, 1>());
+        else join(std::integral_constant<int, 4>());
         return launched("frnn_embedding_backward");
     });
 }

@@ -619,13 +619,13 @@ def test_c_entries_refuse_bad_arguments():
     i64, f32, some = ctypes.c_int64, ctypes.c_float, ctypes.c_void_p(256)
     fw = lambda dtype=0, w=some, rows=4, width=8, tok=some, tb=8, n=2, out=some, err=some: L.frnn_embedding_forward(
         dtype, w, i64(rows), i64(width), i64(8), i64(1), tok, tb, i64(n), f32(1), i64(-100), out, err, None)
-    assert fw(dtype=7) == fw(tb=2) == fw(w=None) == fw(tok=None) == fw(out=None) == fw(err=None) == fw(rows=1 << 31) == fw(n=-1) == fw(width=-1) == 1
+    assert fw(dtype=7) == fw(tb=2) == fw(w=None) == fw(tok=None) == fw(out=None) == fw(err=None) == fw(rows=1 << 31) == fw(n=-1) == fw(width=-1) == fw(n=1 << 30) == 1
     assert fw(n=0) == fw(width=0) == 0
     bw = lambda dtype=1, dy=some, tok=some, n=2, rows=4, width=8, dw=some, work=some: L.frnn_embedding_backward(
         dtype, dy, tok, 8, i64(n), i64(rows), i64(width), f32(1), i64(-100), dw, work, None)
     assert bw(dtype=3) == bw(dy=None) == bw(tok=None) == bw(dw=None) == bw(work=None) == bw(n=1 << 31) == 1
     assert bw(rows=0) == bw(width=0) == 0
-    assert b"2^31" in (bw(n=1 << 31), L.frnn_last_error())[1]
+    assert b"2^30" in (bw(n=1 << 31), L.frnn_last_error())[1]
 
     class Rows(ctypes.Structure):
         _fields_ = [("n", i64 * 3), ("width", i64), ("heads", i64), ("x", i64 * 3), ("dy", i64 * 3), ("dx", i64 * 3)]
