@@ -640,7 +640,7 @@ def test_c_entries_refuse_bad_arguments():
     lp = lambda dtype=0, x=some, n=2, V=8, tok=some, tb=4, top=0, T=1.0, out=some, tl=some, err=some: L.frnn_token_logprobs_forward(
         dtype, x, i64(n), i64(V), i64(V), tok, tb, top, f32(T), i64(-100), out, out, tl, some, None, err, None)
     assert lp(dtype=5) == lp(tb=1) == lp(V=0) == lp(top=33) == lp(top=9) == lp(top=-1) == lp(T=0) == lp(T=math.nan) == lp(T=math.inf) == lp(x=None) == lp(tok=None) == 1
-    assert lp(out=None) == lp(top=2, tl=None) == lp(err=None) == lp(n=1 << 31) == 1
+    assert lp(out=None) == lp(top=2, tl=None) == lp(err=None) == lp(n=1 << 31) == lp(V=1 << 30) == 1
     assert lp(n=0) == 0
     odd = ctypes.c_void_p(257)                      # no pointer off the boundary of its elements gets as far as a kernel
     assert fw(w=odd) == fw(tok=odd) == fw(out=odd) == fw(err=odd) == bw(dy=odd) == bw(dw=odd) == bw(work=odd) == ln(x=odd) == ln(y=odd) == lb(st=ctypes.c_void_p(260)) == lb(dx=odd) == 1
