@@ -20,7 +20,11 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-enum { THREADS = 256, WARPS = THREADS / 32, LOADS = 4, GROUPS = 64, MOST_CANDIDATES = 1024, MOST_CLUSTER = 8 };
+enum { LOADS = 4, MOST_CLUSTER = 8 };
+// A row, or a cluster block's part of it, belongs to a block of 256 threads, or of 32 where rows are short.
+template <int N> struct Block {
+    static constexpr int THREADS = N, WARPS = N / 32, GROUPS = N < 64 ? N : 64, MOST = N < 256 ? 512 : 1024;      // MOST: candidates
+};
 constexpr float NIL = -512.f;      // 2^NIL is 0 in 32 bits; finite, so that 0 * log 0 is 0
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -36,10 +40,25 @@ __device__ __forceinline__ float exp2_fast(float x) {              // 2 units in
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float exp2_small(float x) {             // the same, down to the smallest numbers
-    float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
+
+// The largest of several accesses' logits, NaN if one is: in pairs for 16-bit types.
+template <int N> __device__ __forceinline__ float largest(const Pack<float, 4> (&v)[N]) {
+    float m = v[0].v.x;
+#pragma unroll
+    for (int i = 0; i < N; i++) m = max_nan(max_nan(max_nan(m, v[i].v.x), max_nan(v[i].v.y, v[i].v.z)), v[i].v.w);
+    return m;
+}
+template <class T, int N> __device__ __forceinline__ float largest(const Pack<T, 8> (&v)[N]) {
+    typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type T2;
+    auto two = [](unsigned w) {
+        T2 r;
+        memcpy(&r, &w, 4);
+        return r;
+    };
+    T2 m = two(v[0].v.x);
+#pragma unroll
+    for (int i = 0; i < N; i++) m = __hmax2_nan(__hmax2_nan(__hmax2_nan(m, two(v[i].v.x)), __hmax2_nan(two(v[i].v.y), two(v[i].v.z))), two(v[i].v.w));
+    return max_nan(to_float(m.x), to_float(m.y));
 }
 
 // Orders floats as unsigned numbers; every NaN above +infinity, -0 with +0.
@@ -48,6 +67,7 @@ __device__ __forceinline__ unsigned ordered(float x) {
     const unsigned b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
 __device__ __forceinline__ Key key_of(float x, int64_t token) { return (Key)ordered(x) << 32 | (0xFFFFFFFFu - (unsigned)token); }
 __device__ __forceinline__ int64_t token_of(Key k) { return 0xFFFFFFFFu - (unsigned)k; }
 
@@ -65,14 +85,12 @@ template <class T, int E> struct Row {
     __device__ __forceinline__ bool whole(int access) const { return at(access) >= 0 && at(access) <= vocab - E; }
     __device__ __forceinline__ bool there(int access, int e) const { return at(access) + e >= 0 && at(access) + e < vocab; }
     // logits of an access; -inf, which adds nothing, where there are none
-    __device__ __forceinline__ void get(int access, float* f) const {
+    __device__ __forceinline__ void get(int access, Pack<T, E>& v) const {
         if (access < end && whole(access)) {
-            Pack<T, E> v;
             v.load(x + at(access));
-            v.to(f);
         } else {
 #pragma unroll
-            for (int e = 0; e < E; e++) f[e] = access < end && there(access, e) ? to_float(x[at(access) + e]) : -INFINITY;
+            for (int e = 0; e < E; e++) v.set(e, access < end && there(access, e) ? x[at(access) + e] : from_float<T>(-INFINITY));
         }
     }
 };
@@ -88,7 +106,8 @@ __device__ __forceinline__ Part move_to(Part p, float m, float c) {
     return Part{m, p.s * r, (p.t + d * p.s) * r};
 }
 
-__device__ __forceinline__ Part block_join(Part p, float c) {
+template <int N> __device__ __forceinline__ Part block_join(Part p, float c) {
+    constexpr int WARPS = Block<N>::WARPS;
     __shared__ float largest[WARPS];
     __shared__ float2 sums[WARPS];
     float m = p.m;
@@ -117,61 +136,47 @@ __device__ __forceinline__ Part block_join(Part p, float c) {
 
 // ---- alternatives ----------------------------------------------------------------------------------------------------------
 
-struct Candidates {
-    Key key[MOST_CANDIDATES];
+template <int N> struct Candidates {
+    Key key[Block<N>::MOST];
     int count;
 };
 
-// Adds the keys of the lanes that have one, as long as there is room; counts all of them.
-__device__ __forceinline__ void push(Candidates& c, bool has, Key key, unsigned lanes) {
-    const unsigned who = __ballot_sync(lanes, has);
-    if (!who) return;
-    const int lane = threadIdx.x & 31, leader = __ffs(who) - 1;
-    int base = 0;
-    if (lane == leader) base = atomicAdd(&c.count, __popc(who));
-    base = __shfl_sync(lanes, base, leader);
-    const int slot = base + __popc(who & ((1u << lane) - 1));
-    if (has && slot < MOST_CANDIDATES) c.key[slot] = key;
-}
-
-// Candidates of the logits that are at least (strictly: above) `bound`, from the threads whose largest logit is.
-template <class T, int E> __device__ void collect(const Row<T, E>& row, Candidates& c, unsigned largest, unsigned bound, bool strictly) {
+// Candidates among the logits that are at least (strictly: above) `bound`, from the threads that have seen one.  More
+// than there is room for: the count says so, and what is kept is of no use.
+template <class T, int E, int N> __device__ void collect(const Row<T, E>& row, Candidates<N>& c, bool mine, float bound, bool strictly) {
     __syncthreads();                                       // (everyone has read the last count)
     if (threadIdx.x == 0) c.count = 0;
     __syncthreads();
-    const bool mine = strictly ? largest > bound : largest >= bound;
-    if (__any_sync(~0u, mine)) {
-        for (int a0 = row.first + (threadIdx.x & ~31); a0 < row.end; a0 += LOADS * THREADS) {
-            float f[LOADS][E];
+    const unsigned least = ordered(bound);
+    if (mine)
+        for (int a0 = row.first + threadIdx.x; a0 < row.end && *(volatile int*)&c.count <= Block<N>::MOST; a0 += LOADS * N) {
+            Pack<T, E> v[LOADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) row.get(a0 + u * N, v[u]);
 #pragma unroll
             for (int u = 0; u < LOADS; u++) {
-                const int a = a0 + (threadIdx.x & 31) + u * THREADS;
-                if (mine && a < row.end) row.get(a, f[u]);
-            }
+                const Pack<T, E> one[1] = {v[u]};
+                if (largest(one) < bound) continue;        // (a NaN is not)
+                const int a = a0 + u * N;
+                float f[E];
+                v[u].to(f);
 #pragma unroll
-            for (int u = 0; u < LOADS; u++) {
-                const int a = a0 + (threadIdx.x & 31) + u * THREADS;
-                unsigned hits = 0;
-                if (mine && a < row.end)
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const unsigned o = ordered(f[u][e]);
-                        if (row.there(a, e) && (strictly ? o > bound : o >= bound)) hits |= 1u << e;
-                    }
-                if (!__any_sync(~0u, hits)) continue;
-#pragma unroll
-                for (int e = 0; e < E; e++) push(c, hits >> e & 1, key_of(f[u][e], row.at(a) + e), ~0u);
+                for (int e = 0; e < E; e++) {
+                    const unsigned o = ordered(f[e]);
+                    if (a >= row.end || !row.there(a, e) || (strictly ? o <= least : o < least)) continue;
+                    const int slot = atomicAdd(&c.count, 1);
+                    if (slot < Block<N>::MOST) c.key[slot] = key_of(f[e], row.at(a) + e);
+                }
             }
         }
-    }
     __syncthreads();
 }
 
-// The first `want` candidates by (logit, lowest token) of `n` in best[0 ...]; zeros behind them.
-__device__ void rank(const Key* key, int n, int want, Key* best) {
-    for (int i = threadIdx.x; i < FRNN_MAX_TOP; i += THREADS) best[i] = 0;
+// The first `want` of `n` keys in best[0 ...], zeros behind them: a key's place is the number of larger ones.
+template <int N> __device__ void rank(const Key* key, int n, int want, Key* best) {
+    for (int i = threadIdx.x; i < FRNN_MAX_TOP; i += N) best[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += THREADS) {
+    for (int i = threadIdx.x; i < n; i += N) {
         const Key k = key[i];
         int before = 0;
         for (int j = 0; j < n; j++) before += key[j] > k;
@@ -180,52 +185,53 @@ __device__ void rank(const Key* key, int n, int want, Key* best) {
     __syncthreads();
 }
 
-// The `top` best logits of a block's part of the row, in best[]; `largest`: the largest logit that this thread has seen.
-template <class T, int E> __device__ void block_top(const Row<T, E>& row, float largest, int top, Candidates& c, Key* best) {
-    __shared__ unsigned group[GROUPS];
-    __shared__ unsigned found;
+// The `top` best logits of a block's part of the row, in best[]; `seen`: the largest logit that this thread has seen.
+template <class T, int E, int N> __device__ void block_top(const Row<T, E>& row, float seen, int top, Candidates<N>& c, Key* best) {
+    constexpr int WARPS = Block<N>::WARPS, GROUPS = Block<N>::GROUPS, EACH = N / GROUPS, MOST = Block<N>::MOST;
+    __shared__ unsigned group[GROUPS], found;
     __shared__ int before[WARPS];
     __shared__ Key leader[WARPS];
-    constexpr int EACH = THREADS / GROUPS;
-    const unsigned mine = ordered(largest);
-    unsigned g = mine;
+    float g = seen;
 #pragma unroll
-    for (int o = 1; o < EACH; o *= 2) g = max(g, __shfl_xor_sync(~0u, g, o));
-    if (threadIdx.x % EACH == 0) group[threadIdx.x / EACH] = g;
+    for (int o = 1; o < EACH; o *= 2) g = max_nan(g, __shfl_xor_sync(~0u, g, o));
+    if (threadIdx.x % EACH == 0) group[threadIdx.x / EACH] = ordered(g);
     __syncthreads();
     if (threadIdx.x < GROUPS) {
-        const unsigned v = group[threadIdx.x];
+        const unsigned o = group[threadIdx.x];
         int larger = 0;
-        for (int i = 0; i < GROUPS; i++) larger += group[i] > v || (group[i] == v && i < threadIdx.x);
-        if (larger == top - 1) found = v;
+#pragma unroll 8
+        for (int i = 0; i < GROUPS; i++) larger += group[i] > o || (group[i] == o && i < threadIdx.x);
+        if (larger == top - 1) found = o;
     }
     __syncthreads();
-    const unsigned bound = found;
-    // a bound of -inf says that fewer than `top` groups hold any token that may follow: all of those, then the first others
-    bool many = bound <= ordered(-INFINITY) && (int64_t)(row.end - row.first) * E > MOST_CANDIDATES;
+    // a bound of -inf says that fewer than `top` groups hold a token that may follow: all of those, then the first others
+    const float bound = value_of(found);
+    bool many = bound == -INFINITY && (int64_t)(row.end - row.first) * E > MOST;
     if (!many) {
-        collect(row, c, mine, bound, false);
-        many = c.count > MOST_CANDIDATES;
+        collect<T, E, N>(row, c, !(seen < bound), bound, false);
+        many = c.count > MOST;
     }
     if (many) {                            // many logits equal to the bound: those above it, then the equal ones in order
-        collect(row, c, mine, bound, true);
+        collect<T, E, N>(row, c, !(seen <= bound), bound, true);
         const int above = c.count;
         __syncthreads();
-        if (above <= MOST_CANDIDATES - FRNN_MAX_TOP) {
+        if (above <= MOST - FRNN_MAX_TOP) {
             int have = 0;
-            for (int a0 = row.first; a0 < row.end && have < top; a0 += THREADS) {
+            for (int a0 = row.first; a0 < row.end && have < top; a0 += N) {
                 const int a = a0 + threadIdx.x;
+                Pack<T, E> v;
                 float f[E];
-                row.get(a, f);
+                row.get(a, v);
+                v.to(f);
                 unsigned hits = 0;
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (a < row.end && row.there(a, e) && ordered(f[e]) == bound) hits |= 1u << e;
+                    if (a < row.end && row.there(a, e) && ordered(f[e]) == ordered(bound)) hits |= 1u << e;
                 int upto = __popc(hits);
 #pragma unroll
                 for (int o = 1; o < 32; o *= 2) {
-                    const int v = __shfl_up_sync(~0u, upto, o);
-                    if ((threadIdx.x & 31) >= o) upto += v;
+                    const int w = __shfl_up_sync(~0u, upto, o);
+                    if ((threadIdx.x & 31) >= o) upto += w;
                 }
                 if ((threadIdx.x & 31) == 31) before[threadIdx.x / 32] = upto;
                 __syncthreads();
@@ -245,14 +251,16 @@ template <class T, int E> __device__ void block_top(const Row<T, E>& row, float 
             }
             if (threadIdx.x == 0) c.count = above + have;
             __syncthreads();
-        } else {                           // more than the buffer holds: one alternative after the other
+        } else {                           // more than there is room for: one alternative after the other
             Key last = ~0ull;
-            if (threadIdx.x < FRNN_MAX_TOP) best[threadIdx.x] = 0;
+            for (int i = threadIdx.x; i < FRNN_MAX_TOP; i += N) best[i] = 0;
             for (int k = 0; k < top; k++) {
                 Key b = 0;
-                for (int a = row.first + threadIdx.x; a < row.end; a += THREADS) {
+                for (int a = row.first + threadIdx.x; a < row.end; a += N) {
+                    Pack<T, E> v;
                     float f[E];
-                    row.get(a, f);
+                    row.get(a, v);
+                    v.to(f);
 #pragma unroll
                     for (int e = 0; e < E; e++) {
                         const Key key = key_of(f[e], row.at(a) + e);
@@ -272,7 +280,7 @@ template <class T, int E> __device__ void block_top(const Row<T, E>& row, float 
             return;
         }
     }
-    rank(c.key, c.count, top, best);
+    rank<N>(c.key, c.count, top, best);
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
@@ -283,12 +291,12 @@ struct Share {
     Key best[FRNN_MAX_TOP];
 };
 
-template <class T, int E>
-__global__ void __launch_bounds__(THREADS, 4) logprobs_fw(const T* __restrict__ logits, int vocab, int64_t row_stride, const void* __restrict__ tokens, int token_bytes, float inv_t,
-                                                          int64_t ignore, int top, int blocks, float* logprob, float* entropy, float* top_logprob, int64_t* top_token, float* stats,
-                                                          int* err) {
+template <class T, int E, int N>
+__global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __restrict__ logits, int vocab, int64_t row_stride, const void* __restrict__ tokens, int token_bytes,
+                                                                   float inv_t, int64_t ignore, int top, int blocks, float* logprob, float* entropy, float* top_logprob,
+                                                                   int64_t* top_token, float* stats, int* err) {
     __shared__ Share share;
-    __shared__ Candidates candidates;
+    __shared__ Candidates<N> candidates;
     const int rank_ = blockIdx.x % blocks;
     const int64_t row = blockIdx.x / blocks;
     const T* x = logits + row * row_stride;
@@ -297,15 +305,19 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_fw(const T* __restrict__ 
     float m = -INFINITY, m0 = 0;                          // m0: m, but 0 before there is any finite logit
     float2 s = both(0.f), t = both(0.f);
     const float2 c2 = both(c);
-    for (int a = part.first + threadIdx.x; a < part.end; a += LOADS * THREADS) {
-        constexpr int N = LOADS * E;
-        float2 f[(N + 1) / 2];
-        float* f1 = &f[0].x;
+    Pack<T, E> next[LOADS];
+    int a = part.first + threadIdx.x;
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) part.get(a + u * THREADS, f1 + u * E);
-        float b = f1[0];
+    for (int u = 0; u < LOADS; u++) part.get(a + u * N, next[u]);
+    while (a < part.end) {
+        Pack<T, E> v[LOADS];
 #pragma unroll
-        for (int i = 1; i < N; i++) b = max_nan(b, f1[i]);
+        for (int u = 0; u < LOADS; u++) v[u] = next[u];
+        a += LOADS * N;
+        if (a < part.end)                                  // the next round's loads are under way during this one
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) part.get(a + u * N, next[u]);
+        const float b = largest(v);
         if (!(b <= m)) {
             const float d = max_nan((m - b) * c, NIL), r = exp2_fast(d);
             t = mul2(fma2(s, both(d), t), both(r));
@@ -315,17 +327,22 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_fw(const T* __restrict__ 
         }
         const float2 from = both(-m0);
 #pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            float2 u = mul2(add2(f[i], from), c2);
-            u.x = max_nan(u.x, NIL);
-            u.y = max_nan(u.y, NIL);
-            const float2 e = make_float2(exp2_fast(u.x), exp2_fast(u.y));
-            s = add2(s, e);
-            t = fma2(e, u, t);
+        for (int u = 0; u < LOADS; u++) {
+            float2 f[E / 2];
+            v[u].to(&f[0].x);
+#pragma unroll
+            for (int i = 0; i < E / 2; i++) {
+                float2 w = mul2(add2(f[i], from), c2);
+                w.x = max_nan(w.x, NIL);
+                w.y = max_nan(w.y, NIL);
+                const float2 e = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+                s = add2(s, e);
+                t = fma2(e, w, t);
+            }
         }
     }
-    Part all = block_join(Part{m, s.x + s.y, t.x + t.y}, c);
-    if (top) block_top(part, m, top, candidates, share.best);
+    Part all = block_join<N>(Part{m, s.x + s.y, t.x + t.y}, c);
+    if (top) block_top<T, E, N>(part, m, top, candidates, share.best);
     if (blocks > 1) {
         cg::cluster_group cluster = cg::this_cluster();
         if (threadIdx.x == 0) share.part = all;
@@ -340,11 +357,11 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_fw(const T* __restrict__ 
                 all.t += p.t;
             }
             if (top)
-                for (int i = threadIdx.x; i < blocks * top; i += THREADS) candidates.key[i] = cluster.map_shared_rank(&share, i / top)->best[i % top];
+                for (int i = threadIdx.x; i < blocks * top; i += N) candidates.key[i] = cluster.map_shared_rank(&share, i / top)->best[i % top];
         }
         cluster.sync();                                    // the others' shared memory has been read
         if (rank_) return;
-        if (top) rank(candidates.key, blocks * top, top, share.best);
+        if (top) rank<N>(candidates.key, blocks * top, top, share.best);
     }
     const bool empty = all.m == -INFINITY;                 // nothing may follow here
     const float l2s = log2f(all.s), h = empty ? 0.f : LN2 * (l2s - all.t / all.s);
@@ -365,56 +382,68 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_fw(const T* __restrict__ 
             stats[3 * row + 2] = h;
         }
     }
-    if (threadIdx.x < top) {
-        const int64_t j = token_of(share.best[threadIdx.x]);
-        top_token[row * top + threadIdx.x] = j;
-        top_logprob[row * top + threadIdx.x] = logp(to_float(x[j]));
+    for (int k = threadIdx.x; k < top; k += N) {
+        const int64_t j = token_of(share.best[k]);
+        top_token[row * top + k] = j;
+        top_logprob[row * top + k] = logp(to_float(x[j]));
     }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
 
 // d logits_j = 1/T [ g (1[j = token] - p_j) - h p_j (ln p_j + H) ], g and h the upstream gradients of log probability and
-// entropy: p_j times a linear function of log2 p_j, and the token's own term.  A block has LOADS * THREADS accesses of a row.
+// entropy: p_j times a linear function of log2 p_j, and the token's own term.  p is the square of 2^(log2 p / 2): a gradient
+// is p times some tens and may be seen where p itself is below the smallest number that the exponential gives.
+// `lanes` threads have a row's tile of LOADS * lanes accesses.
 template <class T, int E>
-__global__ void __launch_bounds__(THREADS) logprobs_bw(const T* __restrict__ logits, int vocab, int64_t row_stride, const void* __restrict__ tokens, int token_bytes, float inv_t,
-                                                       int64_t ignore, const float* __restrict__ glp, const float* __restrict__ gent, const float* __restrict__ stats,
-                                                       T* __restrict__ dlogits, unsigned tiles) {
-    const unsigned row = blockIdx.x / tiles, tile = blockIdx.x - row * tiles;
+__global__ void __launch_bounds__(256) logprobs_bw(const T* __restrict__ logits, unsigned n, int vocab, int64_t row_stride, const void* __restrict__ tokens, int token_bytes,
+                                                   float inv_t, int64_t ignore, const float* __restrict__ glp, const float* __restrict__ gent, const float* __restrict__ stats,
+                                                   T* __restrict__ dlogits, unsigned tiles, int lanes) {
+    const unsigned unit = blockIdx.x * (256u / lanes) + threadIdx.x / lanes, row = unit / tiles, tile = unit - row * tiles;
+    if (row >= n) return;
     const Row<T, E> part(logits + row * row_stride, vocab, 0, 1);
     T* d = dlogits + (int64_t)row * vocab;
-    const int first = (int)(tile * (LOADS * THREADS) + threadIdx.x);
-    float f[LOADS][E];
+    const int first = (int)(tile * (LOADS * lanes) + threadIdx.x % lanes);
+    Pack<T, E> v[LOADS];
 #pragma unroll
-    for (int u = 0; u < LOADS; u++) part.get(first + u * THREADS, f[u]);
-    const float m = stats[3ll * row], l2s = stats[3ll * row + 1], H = stats[3ll * row + 2], c = LOG2E * inv_t;
+    for (int u = 0; u < LOADS; u++) part.get(first + u * lanes, v[u]);
+    const float m = stats[3ll * row], l2s = stats[3ll * row + 1], H = stats[3ll * row + 2];
     const int64_t tok = token_at(tokens, token_bytes, row);
     const float g = glp && tok != ignore ? glp[row] : 0.f, h = gent ? gent[row] : 0.f;
     const bool empty = m == -INFINITY;
-    const float slope = empty ? 0.f : -inv_t * LN2 * h, level = empty ? 0.f : -inv_t * fmaf(h, H, g), own = empty ? 0.f : inv_t * g;
-    const float m0 = empty ? 0.f : m, l0 = empty ? 0.f : l2s;
+    const float half_c = 0.5f * LOG2E * inv_t;
+    const float2 by = both(half_c), from = both(empty ? 0.f : -m), less = both(empty ? 0.f : -0.5f * l2s);
+    const float2 slope = both(empty ? 0.f : -2.f * inv_t * LN2 * h), level = both(empty ? 0.f : -inv_t * fmaf(h, H, g));
+    const float own = empty ? 0.f : inv_t * g;
 #pragma unroll
     for (int u = 0; u < LOADS; u++) {
-        const int a = first + u * THREADS;
+        const int a = first + u * lanes;
         if (a >= part.end) return;
+        float2 f[(E + 1) / 2];
+        float* f1 = &f[0].x;
+        if (E == 1) f1[1] = 0;
+        v[u].to(f1);
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const float l = max_nan(fmaf(f[u][e] - m0, c, -l0), NIL);
-            f[u][e] = exp2_small(l) * fmaf(l, slope, level);      // (a gradient is p times some tens: it may be seen where p is not)
+        for (int i = 0; i < (E + 1) / 2; i++) {
+            float2 l = fma2(add2(f[i], from), by, less);       // log2 p / 2
+            l.x = max_nan(l.x, NIL);
+            l.y = max_nan(l.y, NIL);
+            const float2 q = make_float2(exp2_fast(l.x), exp2_fast(l.y));
+            f[i] = mul2(mul2(fma2(l, slope, level), q), q);
         }
         const int64_t k = tok - part.at(a);
         if (k >= 0 && k < E)
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (k == e) f[u][e] += own;
+                if (k == e) f1[e] += own;
+        Pack<T, E> out;
+        out.from(f1);
         if (part.whole(a)) {
-            Pack<T, E> v;
-            v.from(f[u]);
-            v.store(d + part.at(a));
+            out.store(d + part.at(a));
         } else {
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (part.there(a, e)) d[part.at(a) + e] = from_float<T>(f[u][e]);
+                if (part.there(a, e)) d[part.at(a) + e] = out.get(e);
         }
     }
 }
@@ -428,10 +457,12 @@ int bad_shape(const char* what, int dtype, int64_t n, int64_t vocab, int token_b
     return FRNN_OK;
 }
 
+enum { SHORT_ROW = 8192 };       // bytes of a row that a block of one warp takes, where there are rows enough for eight of them on each SM
+
 // Blocks that share a row: as many as it takes for two on each SM, as long as each thread has one round of loads.
 int blocks_of(int64_t n, int64_t vocab, size_t size) {
     int blocks = 1;
-    while (blocks < MOST_CLUSTER && n * blocks < 2 * sm_count() && vocab * (int64_t)size >= 2 * blocks * THREADS * LOADS * 16) blocks *= 2;
+    while (blocks < MOST_CLUSTER && n * blocks < 2 * sm_count() && vocab * (int64_t)size >= 2 * blocks * 256 * LOADS * 16) blocks *= 2;
     return blocks;
 }
 
@@ -458,12 +489,13 @@ int frnn_token_logprobs_forward(int dtype, const void* logits, int64_t n, int64_
     if (!on_boundary(logits, dtype_bytes(dtype)) || !on_boundary(tokens, token_bytes) || !on_boundary(logprob, 4) || !on_boundary(entropy, 4) || !on_boundary(top_logprob, 4) ||
         !on_boundary(top_token, 8) || !on_boundary(stats, 4) || !on_boundary(err_word, 4))
         return frnn_fail(FRNN_E_ARG, "frnn_token_logprobs_forward: a pointer is not on a boundary of its elements");
-    int blocks = blocks_of(n, vocab, dtype_bytes(dtype));
+    const int blocks = blocks_of(n, vocab, dtype_bytes(dtype));
+    const bool is_short = vocab * (int64_t)dtype_bytes(dtype) <= SHORT_ROW && n > 8 * sm_count();
     return with_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3((unsigned)(n * blocks));
-        config.blockDim = dim3(THREADS);
+        config.blockDim = dim3(is_short ? 32 : 256);
         config.stream = (cudaStream_t)stream;
         cudaLaunchAttribute cluster;
         cluster.id = cudaLaunchAttributeClusterDimension;
@@ -471,8 +503,8 @@ int frnn_token_logprobs_forward(int dtype, const void* logits, int64_t n, int64_
         cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
         config.attrs = &cluster;
         config.numAttrs = blocks > 1;
-        cudaLaunchKernelEx(&config, logprobs_fw<T, WIDE<T>>, (const T*)logits, (int)vocab, row_stride, tokens, token_bytes, 1.f / temperature, ignore_index, top, blocks, logprob, entropy,
-                           top_logprob, top_token, stats, err_word);
+        cudaLaunchKernelEx(&config, is_short ? logprobs_fw<T, WIDE<T>, 32> : logprobs_fw<T, WIDE<T>, 256>, (const T*)logits, (int)vocab, row_stride, tokens, token_bytes,
+                           1.f / temperature, ignore_index, top, blocks, logprob, entropy, top_logprob, top_token, stats, err_word);
         return launched("frnn_token_logprobs_forward");
     });
 }
@@ -490,10 +522,14 @@ int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64
     const bool wide = (((uintptr_t)logits ^ (uintptr_t)dlogits) & 15) == 0 && (n == 1 || (row_stride - vocab) * size % 16 == 0);
     return with_access(dtype, wide, [&](auto t, auto e) {
         typedef decltype(t) T;
-        const int64_t each = LOADS * THREADS * e.value, tiles = (vocab + e.value - 1 + each - 1) / each;
-        if (n * tiles >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "frnn_token_logprobs_backward: too many logits");
-        logprobs_bw<T, e.value><<<(unsigned)(n * tiles), THREADS, 0, (cudaStream_t)stream>>>((const T*)logits, (int)vocab, row_stride, tokens, token_bytes, 1.f / temperature, ignore_index,
-                                                                                             dlogprob, dentropy, stats, (T*)dlogits, (unsigned)tiles);
+        const int64_t accesses = (vocab + e.value - 1 + e.value - 1) / e.value;      // with up to E - 1 elements before a row's first
+        const int lanes = accesses <= 32 * LOADS ? 32 : 256;                          // a warp has short rows to itself
+        const int64_t tiles = (accesses + LOADS * lanes - 1) / (LOADS * lanes), units = n * tiles;
+        if (units >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "frnn_token_logprobs_backward: too many logits");
+        const int in_block = 256 / lanes;
+        logprobs_bw<T, e.value><<<(unsigned)((units + in_block - 1) / in_block), 256, 0, (cudaStream_t)stream>>>((const T*)logits, (unsigned)n, (int)vocab, row_stride, tokens, token_bytes,
+                                                                                                               1.f / temperature, ignore_index, dlogprob, dentropy, stats, (T*)dlogits,
+                                                                                                               (unsigned)tiles, lanes);
         return launched("frnn_token_logprobs_backward");
     });
 }
