@@ -136,39 +136,51 @@ template <int N> __device__ __forceinline__ Part block_join(Part p, float c) {
 
 // ---- alternatives ----------------------------------------------------------------------------------------------------------
 
+enum { SLOTS = 16 };
 template <int N> struct Candidates {
     Key key[Block<N>::MOST];
-    int count;
+    unsigned short where[Block<N>::MOST];     // slots to look into: slot * N + thread
+    int count, places;
+    float seen[SLOTS][N];          // the largest logit of a thread in each `rounds` rounds of its loads
+    int rounds;
 };
 
-// Candidates among the logits that are at least (strictly: above) `bound`, from the threads that have seen one.  More
-// than there is room for: the count says so, and what is kept is of no use.
-template <class T, int E, int N> __device__ void collect(const Row<T, E>& row, Candidates<N>& c, bool mine, float bound, bool strictly) {
+// Candidates among the logits that are at least (strictly: above) `bound`.  The slots that have one are listed first, then
+// their loads are dealt out to all threads, so that they wait for memory once.  More than there is room for: the count says
+// so, and what is kept is of no use.
+template <class T, int E, int N> __device__ void collect(const Row<T, E>& row, Candidates<N>& c, float bound, bool strictly) {
+    constexpr int MOST = Block<N>::MOST;
     __syncthreads();                                       // (everyone has read the last count)
-    if (threadIdx.x == 0) c.count = 0;
+    if (threadIdx.x == 0) c.count = c.places = 0;
     __syncthreads();
     const unsigned least = ordered(bound);
-    if (mine)
-        for (int a0 = row.first + threadIdx.x; a0 < row.end && *(volatile int*)&c.count <= Block<N>::MOST; a0 += LOADS * N) {
-            Pack<T, E> v[LOADS];
+    const int each = LOADS * c.rounds;
+    for (int slot = 0; row.first + (int)threadIdx.x + slot * each * N < row.end; slot++) {
+        const float seen = c.seen[slot][threadIdx.x];
+        if (strictly ? seen <= bound : seen < bound) continue;      // (a NaN is not)
+        const int i = atomicAdd(&c.places, 1);
+        if (i < MOST) c.where[i] = (unsigned short)(slot * N + threadIdx.x);
+    }
+    __syncthreads();
+    const int places = c.places;
+    for (int i = threadIdx.x; i < min(places, MOST) * each; i += N) {
+        const int where = c.where[i / each], a = row.first + where % N + (where / N * each + i % each) * N;
+        if (a >= row.end) continue;
+        Pack<T, E> v[1];
+        row.get(a, v[0]);
+        if (largest(v) < bound) continue;
+        float f[E];
+        v[0].to(f);
 #pragma unroll
-            for (int u = 0; u < LOADS; u++) row.get(a0 + u * N, v[u]);
-#pragma unroll
-            for (int u = 0; u < LOADS; u++) {
-                const Pack<T, E> one[1] = {v[u]};
-                if (largest(one) < bound) continue;        // (a NaN is not)
-                const int a = a0 + u * N;
-                float f[E];
-                v[u].to(f);
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const unsigned o = ordered(f[e]);
-                    if (a >= row.end || !row.there(a, e) || (strictly ? o <= least : o < least)) continue;
-                    const int slot = atomicAdd(&c.count, 1);
-                    if (slot < Block<N>::MOST) c.key[slot] = key_of(f[e], row.at(a) + e);
-                }
-            }
+        for (int e = 0; e < E; e++) {
+            const unsigned o = ordered(f[e]);
+            if (!row.there(a, e) || (strictly ? o <= least : o < least)) continue;
+            const int at = atomicAdd(&c.count, 1);
+            if (at < MOST) c.key[at] = key_of(f[e], row.at(a) + e);
         }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && places > MOST) c.count = MOST + 1;
     __syncthreads();
 }
 
@@ -208,11 +220,11 @@ template <class T, int E, int N> __device__ void block_top(const Row<T, E>& row,
     const float bound = value_of(found);
     bool many = bound == -INFINITY && (int64_t)(row.end - row.first) * E > MOST;
     if (!many) {
-        collect<T, E, N>(row, c, !(seen < bound), bound, false);
+        collect<T, E, N>(row, c, bound, false);
         many = c.count > MOST;
     }
     if (many) {                            // many logits equal to the bound: those above it, then the equal ones in order
-        collect<T, E, N>(row, c, !(seen <= bound), bound, true);
+        collect<T, E, N>(row, c, bound, true);
         const int above = c.count;
         __syncthreads();
         if (above <= MOST - FRNN_MAX_TOP) {
@@ -306,9 +318,16 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
     float2 s = both(0.f), t = both(0.f);
     const float2 c2 = both(c);
     Pack<T, E> next[LOADS];
+    const int64_t tok = token_at(tokens, token_bytes, row);
+    const int rounds = (part.end - part.first + SLOTS * LOADS * N - 1) / (SLOTS * LOADS * N);      // of a slot
+    float slot_max = -INFINITY;
+    int slot = 0, left = rounds;
     int a = part.first + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < LOADS; u++) part.get(a + u * N, next[u]);
+    // the token's logit is on its way behind the first round's
+    const bool in = tok >= 0 && tok < vocab;
+    const float own = rank_ == 0 && threadIdx.x == 0 && tok != ignore && in ? to_float(x[tok]) : 0.f;
     while (a < part.end) {
         Pack<T, E> v[LOADS];
 #pragma unroll
@@ -318,6 +337,15 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
 #pragma unroll
             for (int u = 0; u < LOADS; u++) part.get(a + u * N, next[u]);
         const float b = largest(v);
+        if (top) {
+            slot_max = max_nan(slot_max, b);
+            candidates.seen[slot][threadIdx.x] = slot_max;
+            if (--left == 0) {
+                slot++;
+                left = rounds;
+                slot_max = -INFINITY;
+            }
+        }
         if (!(b <= m)) {
             const float d = max_nan((m - b) * c, NIL), r = exp2_fast(d);
             t = mul2(fma2(s, both(d), t), both(r));
@@ -342,6 +370,7 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
         }
     }
     Part all = block_join<N>(Part{m, s.x + s.y, t.x + t.y}, c);
+    if (top && threadIdx.x == 0) candidates.rounds = rounds;
     if (top) block_top<T, E, N>(part, m, top, candidates, share.best);
     if (blocks > 1) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -367,14 +396,8 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
     const float l2s = log2f(all.s), h = empty ? 0.f : LN2 * (l2s - all.t / all.s);
     auto logp = [&](float v) { return empty ? -INFINITY : (v - all.m) * inv_t - LN2 * l2s; };
     if (threadIdx.x == 0) {
-        const int64_t tok = token_at(tokens, token_bytes, row);
-        float lp = 0;
-        if (tok != ignore) {
-            const bool in = tok >= 0 && tok < vocab;
-            if (!in) *err = CODE_TOKEN;
-            lp = in ? logp(to_float(x[tok])) : NAN;
-        }
-        logprob[row] = lp;
+        if (tok != ignore && !in) *err = CODE_TOKEN;
+        logprob[row] = tok == ignore ? 0.f : in ? logp(own) : NAN;
         entropy[row] = h;
         if (stats) {
             stats[3 * row] = all.m;
@@ -383,9 +406,8 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
         }
     }
     for (int k = threadIdx.x; k < top; k += N) {
-        const int64_t j = token_of(share.best[k]);
-        top_token[row * top + k] = j;
-        top_logprob[row * top + k] = logp(to_float(x[j]));
+        top_token[row * top + k] = token_of(share.best[k]);
+        top_logprob[row * top + k] = logp(value_of((unsigned)(share.best[k] >> 32)));
     }
 }
 
