@@ -212,15 +212,26 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
     const unsigned after = hi < n ? keys[hi] : NO_KEY;
     float* parts = part + 2 * mine * width + c;
     float sum[E] = {};
+    unsigned next[UNROLL];
+    int place[UNROLL];
+    auto look = [&](int j) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            next[u] = j + u < hi ? keys[j + u] : NO_KEY;
+            place[u] = j + u < hi ? at[j + u] : 0;
+        }
+    };
+    look(lo);
     for (int j = lo; j < hi && run < rows; j += UNROLL) {
         unsigned k[UNROLL];
         Pack<T, E> v[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            k[u] = j + u < hi ? keys[j + u] : NO_KEY;
+            k[u] = next[u];
             v[u].zero();
-            if (k[u] < rows) v[u].load(dy + (int64_t)at[j + u] * width + c);
+            if (k[u] < rows) v[u].load(dy + (int64_t)place[u] * width + c);
         }
+        look(j + UNROLL);                                 // the next round's places, while these rows are on their way
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             if (j + u < hi && k[u] != run) {
@@ -245,47 +256,61 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
     else write_row<T, E>(sum, scale, dw + (int64_t)run * width + c);
 }
 
-// The block of the chunk that a crossing run starts in adds that run's partial sums: 64 threads with V columns each, 4
-// slices of the partials side by side.
+// Sums of the runs that cross ends of chunks, each in the order of its partial sums.  A block looks at JOINED chunks for
+// runs that start there and go on, and adds those runs' partial sums: 64 threads with V columns each, 4 slices side by side.
+enum { JOINED = 8 };
 template <class T, int V>
 __global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restrict__ keys, int n, unsigned rows, int width, int chunk, float scale, T* __restrict__ dw,
                                                         const float* __restrict__ part) {
     constexpr int LANES = 64, SLICES = BLOCK / LANES;
     __shared__ float share[SLICES][LANES * V];
-    const int64_t mine = blockIdx.x, lo = mine * chunk, hi = lo + chunk;
-    if (hi >= n) return;
-    const unsigned run = keys[hi];
-    if (run >= rows || keys[hi - 1] != run || (lo > 0 && keys[lo - 1] == run)) return;
-    int64_t last = mine;                                  // the last chunk that the run reaches
-    for (;;) {
-        const int64_t q = last + 1 + threadIdx.x;
-        const int more = __syncthreads_count(q * chunk < n && keys[q * chunk] == run);      // sorted: the first `more` of them
-        last += more;
-        if (more < BLOCK) break;
-    }
-    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (int)(blockIdx.y * LANES + lane) * V;
-    float sum[V] = {};
-    if (c < width)
-#pragma unroll 8
-        for (int64_t q = mine + slice; q <= last; q += SLICES) {
-            const float* from = part + (2 * q + (q == mine)) * width + c;
-            if constexpr (V == 4) {
-                const float4 v = *(const float4*)from;
-                sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
-            } else {
-                sum[0] += *from;
-            }
+    __shared__ unsigned runs[JOINED];
+    if (threadIdx.x < JOINED) {
+        const int64_t q = (int64_t)blockIdx.x * JOINED + threadIdx.x, lo = q * chunk, hi = lo + chunk;
+        unsigned run = NO_KEY;
+        if (hi < n) {
+            const unsigned over = keys[hi], last = keys[hi - 1], before = lo > 0 ? keys[lo - 1] : NO_KEY;
+            if (over < rows && last == over && before != over) run = over;
         }
-#pragma unroll
-    for (int v = 0; v < V; v++) share[slice][lane * V + v] = sum[v];
+        runs[threadIdx.x] = run;
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < LANES * V; i += BLOCK) {
-        const int col = blockIdx.y * LANES * V + i;
-        if (col >= width) continue;
-        float total = 0;
+    for (int r = 0; r < JOINED; r++) {
+        const unsigned run = runs[r];
+        if (run == NO_KEY) continue;
+        const int64_t mine = (int64_t)blockIdx.x * JOINED + r;
+        int64_t last = mine;                              // the last chunk that the run reaches
+        for (;;) {
+            const int64_t q = last + 1 + threadIdx.x;
+            const int more = __syncthreads_count(q * chunk < n && keys[q * chunk] == run);      // sorted: the first `more` of them
+            last += more;
+            if (more < BLOCK) break;
+        }
+        const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (int)(blockIdx.y * LANES + lane) * V;
+        float sum[V] = {};
+        if (c < width)
+#pragma unroll 8
+            for (int64_t q = mine + slice; q <= last; q += SLICES) {
+                const float* from = part + (2 * q + (q == mine)) * width + c;
+                if constexpr (V == 4) {
+                    const float4 v = *(const float4*)from;
+                    sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+                } else {
+                    sum[0] += *from;
+                }
+            }
 #pragma unroll
-        for (int k = 0; k < SLICES; k++) total += share[k][i];
-        dw[(int64_t)run * width + col] = from_float<T>(scale * total);
+        for (int v = 0; v < V; v++) share[slice][lane * V + v] = sum[v];
+        __syncthreads();
+        for (int i = threadIdx.x; i < LANES * V; i += BLOCK) {
+            const int col = blockIdx.y * LANES * V + i;
+            if (col >= width) continue;
+            float total = 0;
+#pragma unroll
+            for (int k = 0; k < SLICES; k++) total += share[k][i];
+            dw[(int64_t)run * width + col] = from_float<T>(scale * total);
+        }
+        __syncthreads();
     }
 }
 
@@ -317,6 +342,26 @@ int bad_shape(const char* what, int dtype, int64_t rows, int64_t width, int toke
     if (rows < 0 || width < 0 || n < 0 || rows >= (1ll << 31) || width >= (1ll << 21) || n >= (1ll << 30))
         return frnn_fail(FRNN_E_ARG, "%s: the vocabulary has to be below 2^31, the width below 2^21, the number of tokens below 2^30", what);
     return FRNN_OK;
+}
+
+enum { SORT_SHARED = WARPS * DIGITS * 4 };
+
+// Clusters of `embedding_sort` that run at once (those that do not would fill in a second round: 131 us for 0.5 GB with 18
+// clusters where 16 run at once); asked for once a device.
+int clusters_of() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+    if (cudaFuncSetAttribute(embedding_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SHARED) != cudaSuccess) return 0;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(CLUSTER);
+    config.blockDim = dim3(SORT_THREADS);
+    config.dynamicSmemBytes = SORT_SHARED;
+    if (cudaOccupancyMaxActiveClusters(&n, embedding_sort, &config) != cudaSuccess) return 0;
+    known[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 // Calls f(T(), integral_constant E): 16 bytes an access, or one element.
@@ -368,18 +413,12 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     unsigned* key = (unsigned*)workspace;
     int* at = (int*)(key + 2 * n);
     float* part = n ? (float*)((char*)workspace + plan.at_parts) : nullptr;
-    // the sorting cluster, and clusters that fill: enough blocks for a quarter of a megabyte of zeros each, one an SM at most
-    const int64_t most = sm_count() / CLUSTER * CLUSTER, fill = (rows * width * (int64_t)size / (1 << 18) / CLUSTER + 1) * CLUSTER;
-    const int grid = (int)std::min<int64_t>(most, CLUSTER + fill);
-    static std::atomic<bool> raised[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    enum { SMEM = WARPS * DIGITS * 4 };
-    if (dev < 0 || dev >= 64 || !raised[dev].load(std::memory_order_relaxed)) {
-        if (cudaFuncSetAttribute(embedding_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return launched("frnn_embedding_backward");
-        if (dev >= 0 && dev < 64) raised[dev].store(true, std::memory_order_relaxed);
-    }
-    embedding_sort<<<grid, SORT_THREADS, SMEM, st>>>(tokens, token_bytes, (int)n, rows, ignore_index, n ? plan.passes : 0, plan.bits, key, key + n, at, at + n, (char*)dweight,
+    const int clusters = clusters_of();
+    if (clusters < 2) return frnn_fail(FRNN_E_LAUNCH, "frnn_embedding_backward: the device takes no two clusters of %d blocks at once", (int)CLUSTER);
+    // the sorting cluster, and others that fill: a quarter of a megabyte of zeros for each of their blocks, at most as many as run at once
+    const int64_t fill = rows * width * (int64_t)size / (CLUSTER << 18) + 1;
+    const int grid = (int)(1 + std::min<int64_t>(clusters - 1, fill)) * CLUSTER;
+    embedding_sort<<<grid, SORT_THREADS, SORT_SHARED, st>>>(tokens, token_bytes, (int)n, rows, ignore_index, n ? plan.passes : 0, plan.bits, key, key + n, at, at + n, (char*)dweight,
                                                      width * (int64_t)size, (int)size);
     if (int rc = launched("frnn_embedding_backward")) return rc;
     if (n == 0) return FRNN_OK;
@@ -394,7 +433,7 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
         if (int rc = launched("frnn_embedding_backward")) return rc;
         if (plan.chunks < 2) return (int)FRNN_OK;
         auto join = [&](auto v) {
-            embedding_join<T, v.value><<<dim3((unsigned)plan.chunks, (unsigned)((width + 64 * v.value - 1) / (64 * v.value))), BLOCK, 0, st>>>(
+            embedding_join<T, v.value><<<dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 64 * v.value - 1) / (64 * v.value))), BLOCK, 0, st>>>(
                 keys, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part);
         };
         if (width % 4) join(std::integral_constant<int, 1>());
