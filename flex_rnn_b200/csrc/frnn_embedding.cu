@@ -1,9 +1,9 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens.
 //
 // The lookup moves rows and is bound by memory.  The gradient is dense: most of its bytes are the rows of tokens that do
-// not occur.  `embedding_sort` therefore does two things side by side: one cluster of blocks sorts the tokens (places of
-// equal tokens stay in order), all other blocks write the zero rows, which only have to know which tokens occur.
-// `embedding_sums` then walks over the sorted places in chunks of one length, whatever the frequencies of the tokens (a
+// not occur.  Two kernels run side by side, therefore: in `embedding_sort` one cluster of blocks sorts the tokens (places
+// of equal tokens stay in order), and `embedding_fill` writes the zero rows, for which it only has to know which tokens
+// occur.  `embedding_sums` then walks over the sorted places in chunks of one length, whatever the frequencies of the tokens (a
 // text's most frequent token has hundreds of times its average share): runs of equal tokens inside a chunk are finished
 // there, those that cross its ends leave a partial sum each, which `embedding_join` adds in order.  No sum depends on how
 // threads are scheduled.
@@ -73,7 +73,7 @@ __device__ __forceinline__ unsigned key_of(const void* tokens, int bytes, int64_
     return t != ignore && t >= 0 && t < rows ? (unsigned)t : (unsigned)rows;
 }
 
-enum { CLUSTER = 8, SORT_THREADS = 1024, WARPS = SORT_THREADS / 32, MOST_BITS = 9, DIGITS = 1 << MOST_BITS, FLAGS = 32768 };
+enum { CLUSTER = 8, SORT_THREADS = 1024, WARPS = SORT_THREADS / 32, MOST_BITS = 9, DIGITS = 1 << MOST_BITS, ROUNDS = 4, FLAGS = 32768 };
 
 // Zeros into the bytes [lo, hi) of p, by the lanes of a warp; lo, hi and p are on boundaries of elements of `size` bytes.
 __device__ __forceinline__ void fill_zero(char* p, int64_t lo, int64_t hi, int size) {
@@ -89,33 +89,39 @@ __device__ __forceinline__ void fill_zero(char* p, int64_t lo, int64_t hi, int s
     }
 }
 
-// Block 0 to CLUSTER - 1: stable radix sort of (token, place) by token, `bits` bits a pass.  Each warp takes a contiguous
-// part of the places in rounds of 32; a place's rank is what comes before it in its round, its warp, its block, its
-// cluster and among the smaller digits.  The other blocks: zero rows for the tokens that do not occur.
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SORT_THREADS, 1)
-embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, int passes, int bits, unsigned* key_a, unsigned* key_b, int* at_a,
-               int* at_b, char* dw, int64_t row_bytes, int size) {
-    extern __shared__ unsigned count[];                        // [WARPS][DIGITS]; the other blocks: a byte for each row
+// Zero rows for the tokens that do not occur: each block has a range of rows and looks through all tokens for it.
+__global__ void __launch_bounds__(SORT_THREADS, 1)
+embedding_fill(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, char* dw, int64_t row_bytes, int size) {
+    extern __shared__ unsigned char occurs[];                  // of FLAGS rows
+    const int warp = threadIdx.x / 32;
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int64_t each = (rows + gridDim.x - 1) / gridDim.x, from = blockIdx.x * each, to = min(rows, from + each);
+    for (int64_t lo = from; lo < to; lo += FLAGS) {
+        const int here = (int)min((int64_t)FLAGS, to - lo);
+        __syncthreads();
+        for (int i = threadIdx.x; i < here; i += SORT_THREADS) occurs[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += SORT_THREADS) {
+            const int64_t t = token_at(tokens, token_bytes, i);
+            if (t >= lo && t < lo + here && t != ignore) occurs[t - lo] = 1;
+        }
+        __syncthreads();
+        for (int i = warp; i < here; i += WARPS)
+            if (!occurs[i]) fill_zero(dw, (lo + i) * row_bytes, (lo + i + 1) * row_bytes, size);
+    }
+    cudaGridDependencySynchronize();                           // not done before the sort is: the next kernel waits for this one
+}
+
+// One cluster: stable radix sort of (token, place) by token, `bits` bits a pass.  Each warp takes a contiguous part of the
+// places, 32 a round; a place's rank is what comes before it in its round, its warp, its block, its cluster and among the
+// smaller digits.
+__global__ void __launch_bounds__(SORT_THREADS, 1)
+embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, int passes, int bits, unsigned* key_a, unsigned* key_b, int* at_a, int* at_b) {
+    extern __shared__ unsigned count[];                        // [WARPS][DIGITS]
     __shared__ unsigned total[DIGITS], carry[WARPS];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    if (blockIdx.x >= CLUSTER) {
-        unsigned char* occurs = (unsigned char*)count;
-        const int64_t blocks = gridDim.x - CLUSTER, each = (rows + blocks - 1) / blocks, from = (blockIdx.x - CLUSTER) * each, to = min(rows, from + each);
-        for (int64_t lo = from; lo < to; lo += FLAGS) {
-            const int here = (int)min((int64_t)FLAGS, to - lo);
-            __syncthreads();
-            for (int i = threadIdx.x; i < here; i += SORT_THREADS) occurs[i] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < n; i += SORT_THREADS) {
-                const int64_t t = token_at(tokens, token_bytes, i);
-                if (t >= lo && t < lo + here && t != ignore) occurs[t - lo] = 1;
-            }
-            __syncthreads();
-            for (int i = warp; i < here; i += WARPS)
-                if (!occurs[i]) fill_zero(dw, (lo + i) * row_bytes, (lo + i + 1) * row_bytes, size);
-        }
-        return;
-    }
+    cudaTriggerProgrammaticLaunchCompletion();                 // `embedding_fill` needs nothing from here
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned rank = blockIdx.x, mask = (1u << bits) - 1, digits = 1u << bits;
     const int64_t part = (((int64_t)n + CLUSTER * WARPS - 1) / (CLUSTER * WARPS) + 31) / 32 * 32;
@@ -131,7 +137,14 @@ embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
         auto key = [&](int i) { return pass ? __ldcg(from + i) : key_of(tokens, token_bytes, i, rows, ignore); };
         for (int i = lane; i < digits; i += 32) mine[i] = 0;
         __syncwarp();
-        for (int i = lo + lane; i < hi; i += 32) atomicAdd(&mine[(key(i) >> shift) & mask], 1u);
+        for (int i0 = lo + lane; i0 < hi; i0 += 32 * ROUNDS) {
+            unsigned k[ROUNDS];
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) k[u] = i0 + 32 * u < hi ? key(i0 + 32 * u) : 0;
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++)
+                if (i0 + 32 * u < hi) atomicAdd(&mine[(k[u] >> shift) & mask], 1u);
+        }
         __syncthreads();
         unsigned all = 0, below = 0;
         const int d = threadIdx.x;
@@ -159,22 +172,34 @@ embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
         if (lane == 31) carry[warp] = scan;
         __syncthreads();
         unsigned before = 0;
-        for (int k = 0; k < warp && k < DIGITS / 32; k++) before += carry[k];
+#pragma unroll
+        for (int k = 0; k < DIGITS / 32; k++) before += k < warp ? carry[k] : 0;
         if (d < digits) total[d] = before + scan - all + below;
         __syncthreads();
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            const bool in = i < hi;
-            const unsigned k = in ? key(i) : 0, digit = in ? (k >> shift) & mask : digits;
-            const unsigned same = __match_any_sync(~0u, digit), earlier = same & ((1u << lane) - 1);
-            if (in) {
-                const unsigned p = total[digit] + mine[digit] + __popc(earlier);
-                to[p] = k;
-                to_at[p] = pass ? __ldcg(from_at + i) : i;
+        for (int i0 = lo + lane; i0 < hi + lane; i0 += 32 * ROUNDS) {
+            unsigned k[ROUNDS];
+            int at[ROUNDS];
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                const int i = i0 + 32 * u;
+                k[u] = i < hi ? key(i) : 0;
+                at[u] = i < hi && pass ? __ldcg(from_at + i) : i;
             }
-            __syncwarp();
-            if (in && !earlier) mine[digit] += __popc(same);
-            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < ROUNDS; u++) {
+                if (i0 - lane + 32 * u >= hi) break;
+                const bool in = i0 + 32 * u < hi;
+                const unsigned digit = in ? (k[u] >> shift) & mask : digits;
+                const unsigned same = __match_any_sync(~0u, digit), earlier = same & ((1u << lane) - 1);
+                if (in) {
+                    const unsigned p = total[digit] + mine[digit] + __popc(earlier);
+                    to[p] = k[u];
+                    to_at[p] = at[u];
+                }
+                __syncwarp();
+                if (in && !earlier) mine[digit] += __popc(same);
+                __syncwarp();
+            }
         }
         cluster.sync();
     }
@@ -205,6 +230,8 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
                                                         int chunk, float scale, T* __restrict__ dw, float* __restrict__ part, Shape shape) {
     const int lane = threadIdx.x % shape.lanes, c = (int)(blockIdx.y * shape.lanes + lane) * E;
     const int64_t mine = (int64_t)blockIdx.x * shape.groups + threadIdx.x / shape.lanes, from = mine * chunk;
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     if (from >= n || c >= width) return;
     const int lo = (int)from, hi = (int)min((int64_t)n, from + chunk);
     unsigned run = keys[lo];
@@ -258,34 +285,40 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
 
 // Sums of the runs that cross ends of chunks, each in the order of its partial sums.  A block looks at JOINED chunks for
 // runs that start there and go on, and adds those runs' partial sums: 64 threads with V columns each, 4 slices side by side.
-enum { JOINED = 8 };
+enum { JOINED = BLOCK / 32 };
 template <class T, int V>
 __global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restrict__ keys, int n, unsigned rows, int width, int chunk, float scale, T* __restrict__ dw,
                                                         const float* __restrict__ part) {
     constexpr int LANES = 64, SLICES = BLOCK / LANES;
     __shared__ float share[SLICES][LANES * V];
     __shared__ unsigned runs[JOINED];
-    if (threadIdx.x < JOINED) {
-        const int64_t q = (int64_t)blockIdx.x * JOINED + threadIdx.x, lo = q * chunk, hi = lo + chunk;
+    __shared__ int64_t ends[JOINED];                      // the last chunk that the run reaches
+    cudaGridDependencySynchronize();
+    {
+        const int r = threadIdx.x / 32, lane = threadIdx.x & 31;
+        const int64_t q = (int64_t)blockIdx.x * JOINED + r, lo = q * chunk, hi = lo + chunk;
         unsigned run = NO_KEY;
         if (hi < n) {
             const unsigned over = keys[hi], last = keys[hi - 1], before = lo > 0 ? keys[lo - 1] : NO_KEY;
             if (over < rows && last == over && before != over) run = over;
         }
-        runs[threadIdx.x] = run;
+        int64_t last = q;
+        while (run != NO_KEY) {
+            const int64_t next = last + 1 + lane;
+            const int more = __popc(__ballot_sync(~0u, next * chunk < n && keys[next * chunk] == run));      // sorted: the first `more` of them
+            last += more;
+            if (more < 32) break;
+        }
+        if (lane == 0) {
+            runs[r] = run;
+            ends[r] = last;
+        }
     }
     __syncthreads();
     for (int r = 0; r < JOINED; r++) {
         const unsigned run = runs[r];
         if (run == NO_KEY) continue;
-        const int64_t mine = (int64_t)blockIdx.x * JOINED + r;
-        int64_t last = mine;                              // the last chunk that the run reaches
-        for (;;) {
-            const int64_t q = last + 1 + threadIdx.x;
-            const int more = __syncthreads_count(q * chunk < n && keys[q * chunk] == run);      // sorted: the first `more` of them
-            last += more;
-            if (more < BLOCK) break;
-        }
+        const int64_t mine = (int64_t)blockIdx.x * JOINED + r, last = ends[r];
         const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (int)(blockIdx.y * LANES + lane) * V;
         float sum[V] = {};
         if (c < width)
@@ -344,24 +377,17 @@ int bad_shape(const char* what, int dtype, int64_t rows, int64_t width, int toke
     return FRNN_OK;
 }
 
-enum { SORT_SHARED = WARPS * DIGITS * 4 };
+enum { SORT_SHARED = WARPS * DIGITS * 4, FILL_BLOCKS = 128 };
 
-// Clusters of `embedding_sort` that run at once (those that do not would fill in a second round: 131 us for 0.5 GB with 18
-// clusters where 16 run at once); asked for once a device.
-int clusters_of() {
-    static std::atomic<int> known[64];
+// The sort's shared memory has to be allowed once a device.
+bool allow_shared() {
+    static std::atomic<bool> done[64];
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    int n = known[dev].load(std::memory_order_relaxed);
-    if (n) return n;
-    if (cudaFuncSetAttribute(embedding_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SHARED) != cudaSuccess) return 0;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(CLUSTER);
-    config.blockDim = dim3(SORT_THREADS);
-    config.dynamicSmemBytes = SORT_SHARED;
-    if (cudaOccupancyMaxActiveClusters(&n, embedding_sort, &config) != cudaSuccess) return 0;
-    known[dev].store(n, std::memory_order_relaxed);
-    return n;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(embedding_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SHARED) != cudaSuccess) return false;
+    done[dev].store(true, std::memory_order_relaxed);
+    return true;
 }
 
 // Calls f(T(), integral_constant E): 16 bytes an access, or one element.
@@ -413,14 +439,18 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     unsigned* key = (unsigned*)workspace;
     int* at = (int*)(key + 2 * n);
     float* part = n ? (float*)((char*)workspace + plan.at_parts) : nullptr;
-    const int clusters = clusters_of();
-    if (clusters < 2) return frnn_fail(FRNN_E_LAUNCH, "frnn_embedding_backward: the device takes no two clusters of %d blocks at once", (int)CLUSTER);
-    // the sorting cluster, and others that fill: a quarter of a megabyte of zeros for each of their blocks, at most as many as run at once
-    const int64_t fill = rows * width * (int64_t)size / (CLUSTER << 18) + 1;
-    const int grid = (int)(1 + std::min<int64_t>(clusters - 1, fill)) * CLUSTER;
-    embedding_sort<<<grid, SORT_THREADS, SORT_SHARED, st>>>(tokens, token_bytes, (int)n, rows, ignore_index, n ? plan.passes : 0, plan.bits, key, key + n, at, at + n, (char*)dweight,
-                                                     width * (int64_t)size, (int)size);
-    if (int rc = launched("frnn_embedding_backward")) return rc;
+    if (n) {
+        // 8 blocks: 16 sort 32768 tokens 5 us faster, but then fewer blocks fill (0.5 GB of zeros and 8192 tokens: 116 us, with 16 blocks 128)
+        if (!allow_shared()) return launched("frnn_embedding_backward");
+        if (int rc = launch("frnn_embedding_backward", embedding_sort, dim3(CLUSTER), SORT_THREADS, SORT_SHARED, st, false, CLUSTER, tokens, token_bytes, (int)n, rows, ignore_index,
+                            plan.passes, plan.bits, key, key + n, at, at + n))
+            return rc;
+    }
+    // 64 KB of zeros for each block, and at most 128 blocks: with more, the same bytes took longer (0.5 GB: 78 us, with 136 to 296 blocks 89)
+    const int64_t fill = rows * width * (int64_t)size / (1 << 16) + 1;
+    if (int rc = launch("frnn_embedding_backward", embedding_fill, dim3((unsigned)std::min<int64_t>(fill, FILL_BLOCKS)), SORT_THREADS, FLAGS, st, n > 0, 1, tokens, token_bytes, (int)n,
+                        rows, ignore_index, (char*)dweight, width * (int64_t)size, (int)size))
+        return rc;
     if (n == 0) return FRNN_OK;
     const int side = plan.passes & 1;
     const unsigned* keys = key + side * n;
@@ -428,17 +458,16 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     return with_access(dtype, wide, [&](auto t, auto e) {
         typedef decltype(t) T;
         const Shape shape = shape_of(width, e.value);
-        embedding_sums<T, e.value><<<dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st>>>(
-            (const T*)dout, keys, at + side * n, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape);
-        if (int rc = launched("frnn_embedding_backward")) return rc;
+        if (int rc = launch("frnn_embedding_backward", embedding_sums<T, e.value>, dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st, true, 1,
+                            (const T*)dout, keys, at + side * n, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape))
+            return rc;
         if (plan.chunks < 2) return (int)FRNN_OK;
         auto join = [&](auto v) {
-            embedding_join<T, v.value><<<dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 64 * v.value - 1) / (64 * v.value))), BLOCK, 0, st>>>(
-                keys, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part);
+            return launch("frnn_embedding_backward", embedding_join<T, v.value>,
+                          dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 64 * v.value - 1) / (64 * v.value))), BLOCK, 0, st, true, 1, keys, (int)n, (unsigned)rows,
+                          (int)width, plan.chunk, scale, (T*)dweight, (const float*)part);
         };
-        if (width % 4) join(std::integral_constant<int, 1>());
-        else join(std::integral_constant<int, 4>());
-        return launched("frnn_embedding_backward");
+        return width % 4 ? join(std::integral_constant<int, 1>()) : join(std::integral_constant<int, 4>());
     });
 }
 

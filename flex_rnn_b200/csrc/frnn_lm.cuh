@@ -156,6 +156,31 @@ template <class T, int E> __device__ __forceinline__ void store_part(const Pack<
     }
 }
 
+// Launches a kernel; `early`: it may start while the one before it in the stream still runs, and itself waits where it needs
+// that one's results (cudaGridDependencySynchronize).  `cluster` > 1: blocks of a cluster.
+template <class... P, class... A> inline int launch(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, bool early, int cluster, A... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    config.attrs = attrs;
+    if (early) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[config.numAttrs].val.clusterDim.x = cluster;
+        attrs[config.numAttrs].val.clusterDim.y = attrs[config.numAttrs].val.clusterDim.z = 1;
+        config.numAttrs++;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, P(args)...);
+    cudaGetLastError();
+    return e == cudaSuccess ? (int)FRNN_OK : frnn_fail(FRNN_E_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+}
+
 // Streaming multiprocessors of the current device (148 where there is none to ask).
 inline int sm_count() {
     static std::atomic<int> known[64];
