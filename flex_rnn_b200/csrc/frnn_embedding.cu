@@ -379,17 +379,6 @@ int bad_shape(const char* what, int dtype, int64_t rows, int64_t width, int toke
 
 enum { SORT_SHARED = WARPS * DIGITS * 4, FILL_BLOCKS = 128 };
 
-// The sort's shared memory has to be allowed once a device.
-bool allow_shared() {
-    static std::atomic<bool> done[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    if (done[dev].load(std::memory_order_relaxed)) return true;
-    if (cudaFuncSetAttribute(embedding_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SHARED) != cudaSuccess) return false;
-    done[dev].store(true, std::memory_order_relaxed);
-    return true;
-}
-
 // Calls f(T(), integral_constant E): 16 bytes an access, or one element.
 template <class F> int with_access(int dtype, bool wide, F f) {
     return with_dtype(dtype, [&](auto t) {
@@ -441,7 +430,7 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     float* part = n ? (float*)((char*)workspace + plan.at_parts) : nullptr;
     if (n) {
         // 8 blocks: 16 sort 32768 tokens 5 us faster, but then fewer blocks fill (0.5 GB of zeros and 8192 tokens: 116 us, with 16 blocks 128)
-        if (!allow_shared()) return launched("frnn_embedding_backward");
+        if (!allow_shared<embedding_sort>(SORT_SHARED)) return launched("frnn_embedding_backward");
         if (int rc = launch("frnn_embedding_backward", embedding_sort, dim3(CLUSTER), SORT_THREADS, SORT_SHARED, st, false, CLUSTER, tokens, token_bytes, (int)n, rows, ignore_index,
                             plan.passes, plan.bits, key, key + n, at, at + n))
             return rc;

@@ -16,6 +16,7 @@ using namespace frnn_lm;
 namespace {
 
 enum { PER_LANE = 16, BLOCK = 256, MOST_THREADS = 512 };
+template <class T> constexpr int STAGES = sizeof(T) == 4 ? 3 : 4;      // rows under way in a ring: two blocks of 256 threads share an SM in the backward
 
 // A row's place in a tensor: row r of `frnn_rows` is (r / (n1 n2), r / n2 mod n1, r mod n2).
 __device__ __forceinline__ int64_t place(const frnn_rows& s, const int64_t* stride, unsigned r) {
@@ -28,9 +29,29 @@ __device__ __forceinline__ int64_t place(const frnn_rows& s, const int64_t* stri
 }
 
 // How rows are dealt out: `groups` groups in all, group g takes rows g, g + groups, ... ; groups is a multiple of the number
-// of heads (a group's rows have one head) and of 8 (its rows lie alike to 16-byte boundaries whatever the width).
+// of heads (a group's rows have one head) and of 8 (its rows lie alike to 16-byte boundaries whatever the width), and, if
+// that is not too many, of n2: a group's rows then are `step` elements apart (0: not).
 struct Deal {
     unsigned rows, groups, rounds;
+    int64_t x, dy, dx;          // steps
+    bool even;                  // the steps hold
+};
+
+// The rows of a group in a tensor, one after the other: by steps for groups of lanes of a warp, whose rows are short and a
+// place's two divisions dear (32 heads of 128: backward 57 us, by steps 50); blocks, whose registers are short, work each
+// place out.
+template <class T, bool STEPS> struct Walk {
+    T *base, *now;
+    __device__ __forceinline__ Walk(T* base, const frnn_rows& s, const int64_t* stride, unsigned r, unsigned rows) : base(base) {
+        if (STEPS) now = base + (r < rows ? place(s, stride, r) : 0);
+    }
+    __device__ __forceinline__ T* at(const frnn_rows& s, const int64_t* stride, unsigned r) const { return STEPS ? now : base + place(s, stride, r); }
+    // on to row r
+    __device__ __forceinline__ void next(const frnn_rows& s, const int64_t* stride, const Deal& d, int64_t step, unsigned r) {
+        if (!STEPS) return;
+        if (d.even) now += step;
+        else if (r < d.rows) now = base + place(s, stride, r);
+    }
 };
 
 // How the rows of a call's tensors lie to 16-byte boundaries, and so how they are accessed.  WIDE_ALIKE: all rows at a
@@ -39,7 +60,7 @@ struct Deal {
 enum Access { ELEMENTS, WIDE_ALIKE, WIDE_APART };
 
 // The 16 columns of a lane: access j has E consecutive ones from at[j], of which those from 0 to width are there.
-template <class T, int L, Access A> struct Columns {
+template <class T, Access A> struct Columns {
     static constexpr int E = A == ELEMENTS ? 1 : WIDE<T>, NV = PER_LANE / E;
     int at[NV], width;
 
@@ -55,6 +76,18 @@ template <class T, int L, Access A> struct Columns {
         for (int j = 0; j < NV; j++) {
             if (whole(j)) v[j].load(row + at[j]);
             else if (A == WIDE_APART) load_part(v[j], row, at[j], width);
+            else v[j].zero();
+        }
+    }
+    template <class R> __device__ __forceinline__ void copy(const R& ring, int first, const T* row) const {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (whole(j)) ring.copy(first + j, row + at[j]);
+    }
+    template <class R> __device__ __forceinline__ void take(const R& ring, int first, Pack<T, E>* v) const {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (whole(j)) ring.take(first + j, v[j]);
             else v[j].zero();
         }
     }
@@ -119,6 +152,27 @@ template <int L> struct Seat {
     }
 };
 
+// Rows on their way to a thread, a few rounds ahead: each thread has slots of its own in shared memory for its accesses,
+// filled by asynchronous copies, so no registers and no barriers are spent on them.  (With the next row in registers 32 KB
+// an SM were under way: 8192 x 4096 bf16 backward 52 us.)
+template <class T, int N, int ROUNDS> struct Ring {
+    static constexpr int E = WIDE<T>;
+    char* slot;                  // this thread's first 16 bytes; its next ones follow at distances of 16 bytes a thread
+    int stage = 0;
+    __device__ __forceinline__ Ring(char* shared) : slot(shared + 16 * threadIdx.x) {}
+    __device__ __forceinline__ char* place(int i) const { return slot + 16 * (stage * N + i) * blockDim.x; }
+    __device__ __forceinline__ void copy(int i, const T* from) const {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(place(i))), "l"(from) : "memory");
+    }
+    __device__ __forceinline__ void commit() {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        stage = stage + 1 == ROUNDS ? 0 : stage + 1;
+    }
+    // the oldest round is there
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(ROUNDS - 1) : "memory"); }
+    __device__ __forceinline__ void take(int i, Pack<T, E>& v) const { v.load((const T*)place(i)); }
+};
+
 template <int L> __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
     for (int o = L ? L / 2 : 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
@@ -132,24 +186,29 @@ struct Exchange {
     template <class F> __device__ __forceinline__ void operator()(float2 mine, F each) {
         if ((threadIdx.x & 31) == 0) buffer[turn][threadIdx.x / 32] = mine;
         __syncthreads();
+        turn ^= 1;
+        again(each);
+    }
+    // the last ones once more
+    template <class F> __device__ __forceinline__ void again(F each) const {
+        const float4* all = (const float4*)buffer[turn ^ 1];
         const int warps = blockDim.x / 32;
-        const float4* all = (const float4*)buffer[turn];
-        for (int i = 0; i < warps / 2; i++) {
+#pragma unroll
+        for (int i = 0; i < MOST_THREADS / 64; i++) {
+            if (2 * i >= warps) break;
             const float4 v = all[i];
             each(2 * i, make_float2(v.x, v.y));
-            each(2 * i + 1, make_float2(v.z, v.w));
+            if (2 * i + 1 < warps) each(2 * i + 1, make_float2(v.z, v.w));
         }
-        if (warps & 1) each(warps - 1, buffer[turn][warps - 1]);
-        turn ^= 1;
     }
 };
 
 // y = (x - mean) rstd w + b.  The variance is that of the centred values, so that a large mean costs no digits; warps of a
 // block each centre theirs and join: sum of squares = sum over warps of theirs + count (their mean - mean)^2.
 template <class T, class P, int L, Access A>
-__global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_fw(frnn_rows s, Deal deal, const T* __restrict__ x, const P* __restrict__ w, const P* __restrict__ b, float eps,
+__global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_norm_fw(frnn_rows s, Deal deal, const T* __restrict__ x, const P* __restrict__ w, const P* __restrict__ b, float eps,
                                                                          T* __restrict__ y, float2* __restrict__ stats) {
-    typedef Columns<T, L, A> C;
+    typedef Columns<T, A> C;
     __shared__ __align__(16) float2 buffer[2][MOST_THREADS / 32];
     __shared__ float counts[MOST_THREADS / 32];
     const Seat<L> seat(s);
@@ -168,13 +227,35 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_fw(frnn_r
         per_warp = mine > 0 ? 1.f / mine : 0.f;
         if (seat.lane % 32 == 0) counts[seat.lane / 32] = mine;      // (seen by all after the first exchange's barrier)
     }
+    constexpr bool RING = A == WIDE_ALIKE;
+    extern __shared__ __align__(16) char shared[];
     Pack<T, C::E> next[C::NV];
-    if (g < deal.rows) cols.load(next, x + place(s, s.x, g));
+    Ring<T, RING ? C::NV : 0, RING ? STAGES<T> : 1> ring(shared);
+    // rows are on their way AHEAD rounds before they are used
+    Walk<const T, (L > 0)> wx(x, s, s.x, g, deal.rows);
+    unsigned left = g < deal.rows ? (deal.rows - g + deal.groups - 1) / deal.groups : 0;      // rows that are still to be fetched
+    auto fetch = [&](unsigned r) {
+        if (left) {
+            const T* px = wx.at(s, s.x, r);
+            if constexpr (RING) cols.copy(ring, 0, px);
+            else cols.load(next, px);
+            left--;
+            wx.next(s, s.x, deal, deal.x, r + deal.groups);
+        }
+        if constexpr (RING) ring.commit();
+    };
+    constexpr int AHEAD = RING ? STAGES<T> : 1;
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) fetch(g + i * deal.groups);
     for (unsigned i = 0; i < deal.rounds; i++) {
         const unsigned r = i * deal.groups + g;
         const bool there = r < deal.rows;
+        if constexpr (RING) {
+            ring.wait();
+            cols.take(ring, 0, next);
+        }
         C::unpack(next, f);
-        if (there && deal.rows - r > deal.groups) cols.load(next, x + place(s, s.x, r + deal.groups));
+        fetch(r + AHEAD * deal.groups);
         float2 t = f[0];
 #pragma unroll
         for (int k = 1; k < PER_LANE / 2; k++) t = add2(t, f[k]);
@@ -193,11 +274,10 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_fw(frnn_r
             exchange(make_float2(own, sq), [&](int k, float2 v) { t = fma2(v, make_float2(counts[k], 1.f), t); });
             mean = t.x * per_row;
             sq = t.y;
-            const float2* all = buffer[exchange.turn ^ 1];
-            for (int k = 0; k < blockDim.x / 32; k++) {
-                const float d = all[k].x - mean;
+            exchange.again([&](int k, float2 v) {
+                const float d = v.x - mean;
                 sq = fmaf(counts[k] * d, d, sq);
-            }
+            });
             const float2 move = both(own - mean);
 #pragma unroll
             for (int k = 0; k < PER_LANE / 2; k++) f[k] = add2(f[k], move);
@@ -214,9 +294,9 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_fw(frnn_r
 // dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w, xh = (x - mean) rstd; sums over the group's rows of dy xh and dy.
 // part: [partials][2][width], one for each group, or (merge) for each warp; may be NULL, and so may dx.
 template <class T, class P, int L, Access A>
-__global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_bw(frnn_rows s, Deal deal, const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ w,
+__global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_norm_bw(frnn_rows s, Deal deal, const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ w,
                                                                          const float2* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, bool merge) {
-    typedef Columns<T, L, A> C;
+    typedef Columns<T, A> C;
     __shared__ __align__(16) float2 buffer[2][MOST_THREADS / 32];
     const Seat<L> seat(s);
     const unsigned g = seat.group;
@@ -224,28 +304,55 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_bw(frnn_r
     const int shift = A == WIDE_APART ? (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T) : 0;
     const C cols(width, seat.lanes, seat.lane, shift);
     Exchange exchange{buffer};
+    cudaTriggerProgrammaticLaunchCompletion();
     float2 wf[PER_LANE / 2], dw[PER_LANE / 2], db[PER_LANE / 2], f[PER_LANE / 2], u[PER_LANE / 2];
     cols.params(w ? w + (int64_t)seat.head * width : w, 1.f, wf);
     const float per_row = 1.f / (float)width;
 #pragma unroll
     for (int k = 0; k < PER_LANE / 2; k++) dw[k] = db[k] = both(0.f);
+    constexpr bool RING = A == WIDE_ALIKE;
+    extern __shared__ __align__(16) char shared[];
     Pack<T, C::E> xn[C::NV], gn[C::NV];
+    Ring<T, RING ? 2 * C::NV : 0, RING ? STAGES<T> : 1> ring(shared);
     float2 sn = both(0.f);
-    auto fetch = [&](unsigned r) {
-        sn = stats[r];
-        cols.load(xn, x + place(s, s.x, r));
-        cols.load(gn, dy + place(s, s.dy, r));
-    };
 #pragma unroll
     for (int j = 0; j < C::NV; j++) { xn[j].zero(); gn[j].zero(); }
-    if (g < deal.rows) fetch(g);
+    Walk<const T, (L > 0)> wx(x, s, s.x, g, deal.rows), wg(dy, s, s.dy, g, deal.rows);
+    Walk<T, (L > 0)> wd(dx, s, s.dx, g, deal.rows);
+    unsigned left = g < deal.rows ? (deal.rows - g + deal.groups - 1) / deal.groups : 0;      // rows that are still to be fetched
+    auto fetch = [&](unsigned r) {
+        if (left) {
+            const T *px = wx.at(s, s.x, r), *pg = wg.at(s, s.dy, r);
+            if constexpr (RING) {
+                cols.copy(ring, 0, px);
+                cols.copy(ring, C::NV, pg);
+            } else {
+                cols.load(xn, px);
+                cols.load(gn, pg);
+            }
+            left--;
+            wx.next(s, s.x, deal, deal.x, r + deal.groups);
+            wg.next(s, s.dy, deal, deal.dy, r + deal.groups);
+        }
+        if constexpr (RING) ring.commit();
+    };
+    constexpr int AHEAD = RING ? STAGES<T> : 1;
+    if (g < deal.rows) sn = stats[g];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) fetch(g + i * deal.groups);
     for (unsigned i = 0; i < deal.rounds; i++) {
         const unsigned r = i * deal.groups + g;
         const bool there = r < deal.rows;
         const float2 st = sn;
+        if constexpr (RING) {
+            ring.wait();
+            cols.take(ring, 0, xn);
+            cols.take(ring, C::NV, gn);
+        }
         C::unpack(xn, f);
         C::unpack(gn, u);
-        if (there && deal.rows - r > deal.groups) fetch(r + deal.groups);
+        if (there && deal.rows - r > deal.groups) sn = stats[r + deal.groups];
+        fetch(r + AHEAD * deal.groups);
         float2 a = both(0.f), c = both(0.f);
         if (there) {
 #pragma unroll
@@ -270,7 +377,8 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS) layer_norm_bw(frnn_r
         const float2 off = both(-st.y * (ma * per_row)), by = both(-st.y * (mc * per_row));
 #pragma unroll
         for (int k = 0; k < PER_LANE / 2; k++) f[k] = fma2(f[k], by, fma2(u[k], both(st.y), off));
-        cols.store(dx + place(s, s.dx, r), f);
+        cols.store(wd.at(s, s.dx, r), f);
+        wd.next(s, s.dx, deal, deal.dx, r + deal.groups);
     }
     if (!part) return;
     unsigned p = g;
@@ -379,6 +487,7 @@ __global__ void __launch_bounds__(BLOCK) layer_norm_join(const float* __restrict
     __shared__ float share[SLICES][LANES * V];
     const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, head = blockIdx.y, c = (blockIdx.x * LANES + lane) * V;
     P* to = blockIdx.z ? db : dw;
+    cudaGridDependencySynchronize();
     if (!to) return;
     float sum[V] = {};
     if (c < width)
@@ -426,14 +535,23 @@ Plan plan_of(const frnn_rows& s, int threads_per_sm) {
     for (p.lanes = 2; p.lanes <= 32 && p.lanes * PER_LANE < need; p.lanes *= 2) {}
     if (p.lanes > 32) p.lanes = 0;
     p.threads = p.lanes ? BLOCK : (int)((need + PER_LANE * 32 - 1) / (PER_LANE * 32) * 32);
-    const int64_t in_block = p.lanes ? BLOCK / p.lanes : 1, unit = std::lcm<int64_t>(s.heads, 8);
-    const int64_t step = unit / std::gcd(unit, in_block);                 // blocks by which the number of groups stays a multiple of `unit`
+    const int64_t in_block = p.lanes ? BLOCK / p.lanes : 1;
+    int64_t unit = std::lcm<int64_t>(s.heads, 8);
+    if (s.n2 <= 128) unit = std::lcm<int64_t>(unit, std::max<int64_t>(1, s.n2));
+    const int64_t by = unit / std::gcd(unit, in_block);                   // blocks by which the number of groups stays a multiple of `unit`
     const int64_t full = (int64_t)sm_count() * std::max(1, threads_per_sm / p.threads), want = std::max<int64_t>(1, std::min((rows + in_block - 1) / in_block, full));
-    const int64_t down = want / step * step;
-    p.grid = (int)(down && (rows + in_block - 1) / in_block > full ? down : (want + step - 1) / step * step);
+    const int64_t down = want / by * by;
+    p.grid = (int)(down && (rows + in_block - 1) / in_block > full ? down : (want + by - 1) / by * by);
     p.deal.rows = (unsigned)rows;
     p.deal.groups = (unsigned)(p.grid * in_block);
     p.deal.rounds = (unsigned)((rows + p.deal.groups - 1) / p.deal.groups);
+    // rows (i0, i1, i2) and `groups` rows on: the same i2, and i1 further on by a fixed number as long as there is no i0
+    const int64_t down1 = p.deal.groups / std::max<int64_t>(1, s.n2);
+    p.deal.even = s.n1 * s.n2 == 1 || (s.n0 == 1 && p.deal.groups % std::max<int64_t>(1, s.n2) == 0);
+    auto step = [&](const int64_t* stride) { return s.n1 * s.n2 == 1 ? p.deal.groups * stride[0] : down1 * stride[1]; };
+    p.deal.x = step(s.x);
+    p.deal.dy = step(s.dy);
+    p.deal.dx = step(s.dx);
     return p;
 }
 
@@ -501,7 +619,7 @@ template <class F> int with_lanes(int lanes, Access access, F f) {
     }
 }
 
-enum { FW_THREADS_PER_SM = 768, BW_THREADS_PER_SM = 512 };
+enum { FW_THREADS_PER_SM = 512, BW_THREADS_PER_SM = 512 };
 
 }  // namespace
 
@@ -527,9 +645,12 @@ int frnn_layer_norm_forward(const frnn_rows* s, int dtype, const void* x, int pa
             layer_norm_fw_long<T, P><<<(unsigned)rows, BLOCK, 0, st>>>(*s, (const T*)x, (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
             return launched("frnn_layer_norm_forward");
         }
-        return with_lanes(plan.lanes, access_of(*s, lies, 2), [&](auto l, auto a) {
-            layer_norm_fw<T, P, l.value, a.value><<<plan.grid, plan.threads, 0, st>>>(*s, plan.deal, (const T*)x, (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
-            return launched("frnn_layer_norm_forward");
+        const Access access = access_of(*s, lies, 2);
+        return with_lanes(plan.lanes, access, [&](auto l, auto a) {
+            const size_t shared = a.value == WIDE_ALIKE ? (size_t)plan.threads * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
+            if (!allow_shared<layer_norm_fw<T, P, l.value, a.value>>(shared)) return launched("frnn_layer_norm_forward");
+            return launch("frnn_layer_norm_forward", layer_norm_fw<T, P, l.value, a.value>, dim3(plan.grid), plan.threads, shared, st, false, 1, *s, plan.deal, (const T*)x,
+                          (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
         });
     });
 }
@@ -571,19 +692,18 @@ int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, cons
             }
         } else if (rows && (dx || sums)) {
             rc = with_lanes(plan.lanes, access, [&](auto l, auto a) {
-                layer_norm_bw<T, P, l.value, a.value><<<plan.grid, plan.threads, 0, st>>>(*s, plan.deal, (const T*)dy, (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx,
-                                                                                          sums ? (float*)workspace : nullptr, merge);
-                return launched("frnn_layer_norm_backward");
+                const size_t shared = a.value == WIDE_ALIKE ? (size_t)plan.threads * 2 * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
+                if (!allow_shared<layer_norm_bw<T, P, l.value, a.value>>(shared)) return launched("frnn_layer_norm_backward");
+                return launch("frnn_layer_norm_backward", layer_norm_bw<T, P, l.value, a.value>, dim3(plan.grid), plan.threads, shared, st, false, 1, *s, plan.deal, (const T*)dy,
+                              (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx, sums ? (float*)workspace : (float*)nullptr, merge);
             });
         }
         if (rc || !sums) return rc;
         auto join = [&](auto v) {
-            layer_norm_join<P, v.value><<<dim3((unsigned)((s->width + 8 * v.value - 1) / (8 * v.value)), (unsigned)s->heads, 2), BLOCK, 0, st>>>(
-                (const float*)workspace, partials, (int)s->heads, (int)s->width, (P*)dweight, (P*)dbias);
+            return launch("frnn_layer_norm_backward", layer_norm_join<P, v.value>, dim3((unsigned)((s->width + 8 * v.value - 1) / (8 * v.value)), (unsigned)s->heads, 2), BLOCK, 0, st,
+                          rows > 0, 1, (const float*)workspace, partials, (int)s->heads, (int)s->width, (P*)dweight, (P*)dbias);
         };
-        if (s->width % 4) join(std::integral_constant<int, 1>());
-        else join(std::integral_constant<int, 4>());
-        return launched("frnn_layer_norm_backward");
+        return s->width % 4 ? join(std::integral_constant<int, 1>()) : join(std::integral_constant<int, 4>());
     });
 }
 

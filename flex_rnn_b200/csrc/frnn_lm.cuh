@@ -117,22 +117,9 @@ template <class T> struct Pack<T, 8> {           // 16-bit elements: the lower h
 template <class T> constexpr int WIDE = 16 / (int)sizeof(T);
 
 // Two 32-bit numbers at a time (add, mul, fma.rn.f32x2): half the instructions, the roundings of the single ones.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 r, a, b;\n\tmov.b64 {%0, %1}, r;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 r, a, b;\n\tmov.b64 {%0, %1}, r;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // The E elements at p + at, of which those with 0 <= at + e < n are there; the others read as zero.
@@ -192,6 +179,18 @@ inline int sm_count() {
         known[dev].store(n, std::memory_order_relaxed);
     }
     return n;
+}
+
+// Shared memory beyond 48 KB has to be allowed for a kernel, once a device.
+template <auto KERNEL> inline bool allow_shared(size_t bytes) {
+    static std::atomic<size_t> allowed[64];
+    int dev = 0;
+    if (bytes <= 40 * 1024) return true;             // (with what the kernel has besides)
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+    allowed[dev].store(bytes, std::memory_order_relaxed);
+    return true;
 }
 
 // Token i of int32 or int64 tokens.
