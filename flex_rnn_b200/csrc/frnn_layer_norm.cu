@@ -3,8 +3,10 @@
 // Both directions are bound by memory: a pass over x (and dy) that keeps a row in registers between its reductions and its
 // results, so each element is read and written once.  A row belongs to a group of lanes, 16 elements a lane: 2 to 32
 // lanes of a warp up to 512 columns, a block of up to 512 threads up to 8192; longer rows are read again (``*_long``).
-// A group walks over rows of one head, so its weights and the sums of its weight gradients stay in registers; the sums go
-// to the workspace once and `layer_norm_join` adds them in a fixed order.
+// A group walks over rows of one head, so its weights and the sums of its weight gradients stay in registers.  At the end
+// each block (with weights for each head: each group) writes one partial sum to the workspace, and `layer_norm_join` adds
+// those, all in a fixed order.  (Clusters that add theirs first through each other's shared memory gained nothing with 2
+// blocks, 8192 x 4096 bf16 backward 55 us, and with 4 not all of them ran at once: 75 us.)
 #include <algorithm>
 #include <numeric>
 #include <type_traits>
@@ -292,10 +294,10 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
 }
 
 // dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w, xh = (x - mean) rstd; sums over the group's rows of dy xh and dy.
-// part: [partials][2][width], one for each group, or (merge) for each warp; may be NULL, and so may dx.
+// part: [blocks][2][width] where groups of lanes of a warp have one head, else [groups][2][width]; may be NULL, and so may dx.
 template <class T, class P, int L, Access A>
 __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_norm_bw(frnn_rows s, Deal deal, const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ w,
-                                                                         const float2* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, bool merge) {
+                                                                         const float2* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part) {
     typedef Columns<T, A> C;
     __shared__ __align__(16) float2 buffer[2][MOST_THREADS / 32];
     const Seat<L> seat(s);
@@ -381,28 +383,55 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
         wd.next(s, s.dx, deal, deal.dx, r + deal.groups);
     }
     if (!part) return;
-    unsigned p = g;
-    if (L && L < 32 && merge) {           // the groups of a warp hold the same columns of the same head
+    const bool merged = L && s.heads == 1;
+    float* to = part + 2ll * g * width;
+    int places = BLOCK / (L ? L : 1);
+    bool write = true;
+    if (merged) {
+        int place = threadIdx.x / (L ? L : 1);
+        if (L < 32 && A != WIDE_APART) {                   // the groups of a warp hold the same columns
 #pragma unroll
-        for (int o = L ? L : 32; o < 32; o *= 2)
+            for (int o = L ? L : 32; o < 32; o *= 2)
 #pragma unroll
-            for (int k = 0; k < PER_LANE / 2; k++) {
-                dw[k] = add2(dw[k], make_float2(__shfl_xor_sync(~0u, dw[k].x, o), __shfl_xor_sync(~0u, dw[k].y, o)));
-                db[k] = add2(db[k], make_float2(__shfl_xor_sync(~0u, db[k].x, o), __shfl_xor_sync(~0u, db[k].y, o)));
-            }
-        p = g * (L ? L : 1) / 32;
-        if (threadIdx.x % 32 >= (L ? L : 1)) return;
+                for (int k = 0; k < PER_LANE / 2; k++) {
+                    dw[k] = add2(dw[k], make_float2(__shfl_xor_sync(~0u, dw[k].x, o), __shfl_xor_sync(~0u, dw[k].y, o)));
+                    db[k] = add2(db[k], make_float2(__shfl_xor_sync(~0u, db[k].x, o), __shfl_xor_sync(~0u, db[k].y, o)));
+                }
+            place = threadIdx.x / 32;
+            places = BLOCK / 32;
+            write = threadIdx.x % 32 < (L ? L : 1);
+        }
+        __syncthreads();                                   // the rows' shared memory takes the sums
+        to = (float*)shared + 2 * place * width;
     }
-    float* to = part + 2ll * p * width;
+    if (write)
 #pragma unroll
-    for (int j = 0; j < C::NV; j++)
+        for (int j = 0; j < C::NV; j++) {
+            const float *pw = &dw[0].x + j * C::E, *pb = &db[0].x + j * C::E;
+            if (A == WIDE_ALIKE) {                         // (widths of multiples of 8)
+                if (cols.whole(j))
 #pragma unroll
-        for (int e = 0; e < C::E; e++)
-            if (cols.there(j, e)) {
-                const int k = j * C::E + e;
-                to[cols.at[j] + e] = (&dw[0].x)[k];
-                to[width + cols.at[j] + e] = (&db[0].x)[k];
+                    for (int e = 0; e < C::E; e += 4) {
+                        *(float4*)(to + cols.at[j] + e) = make_float4(pw[e], pw[e + 1], pw[e + 2], pw[e + 3]);
+                        *(float4*)(to + width + cols.at[j] + e) = make_float4(pb[e], pb[e + 1], pb[e + 2], pb[e + 3]);
+                    }
+                continue;
             }
+#pragma unroll
+            for (int e = 0; e < C::E; e++)
+                if (cols.there(j, e)) {
+                    to[cols.at[j] + e] = pw[e];
+                    to[width + cols.at[j] + e] = pb[e];
+                }
+        }
+    if (!merged) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * width; i += BLOCK) {
+        float sum = 0;
+#pragma unroll 8
+        for (int k = 0; k < places; k++) sum += ((const float*)shared)[2 * k * width + i];
+        part[2ll * blockIdx.x * width + i] = sum;
+    }
 }
 
 // ---- rows that no block keeps in registers: read again for each step ---------------------------------------------------
@@ -519,7 +548,9 @@ __global__ void __launch_bounds__(BLOCK) layer_norm_join(const float* __restrict
 struct Plan {
     int lanes = 0, threads = 0, grid = 0;
     bool is_long = false;
+    bool merged = false;       // partial sums of weight gradients: one for a block, or one for a group
     Deal deal{};
+    int64_t partials() const { return merged ? grid : deal.groups; }
 };
 
 Plan plan_of(const frnn_rows& s, int threads_per_sm) {
@@ -539,6 +570,7 @@ Plan plan_of(const frnn_rows& s, int threads_per_sm) {
     int64_t unit = std::lcm<int64_t>(s.heads, 8);
     if (s.n2 <= 128) unit = std::lcm<int64_t>(unit, std::max<int64_t>(1, s.n2));
     const int64_t by = unit / std::gcd(unit, in_block);                   // blocks by which the number of groups stays a multiple of `unit`
+    p.merged = p.lanes && s.heads == 1;
     const int64_t full = (int64_t)sm_count() * std::max(1, threads_per_sm / p.threads), want = std::max<int64_t>(1, std::min((rows + in_block - 1) / in_block, full));
     const int64_t down = want / by * by;
     p.grid = (int)(down && (rows + in_block - 1) / in_block > full ? down : (want + by - 1) / by * by);
@@ -656,7 +688,7 @@ int frnn_layer_norm_forward(const frnn_rows* s, int dtype, const void* x, int pa
 }
 
 size_t frnn_layer_norm_backward_workspace(const frnn_rows* s) {
-    return s && s->heads >= 1 && s->width > 0 ? (size_t)plan_of(*s, BW_THREADS_PER_SM).deal.groups * 2 * s->width * 4 : 0;
+    return s && s->heads >= 1 && s->width > 0 ? (size_t)plan_of(*s, BW_THREADS_PER_SM).partials() * 2 * s->width * 4 : 0;
 }
 
 int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, const void* x, int param_dtype, const void* weight, const float* stats, void* dx,
@@ -674,8 +706,7 @@ int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, cons
     const size_t size = dtype_bytes(dtype);
     const Lie lies[3] = {lie_of(*s, x, s->x, size), lie_of(*s, dy, s->dy, size), lie_of(*s, dx, s->dx, size)};
     const Access access = access_of(*s, lies, dx ? 3 : 2);
-    const bool merge = s->heads == 1 && access != WIDE_APART && plan.lanes && plan.lanes < 32;
-    const int partials = (int)(rows == 0 ? 0 : merge ? plan.deal.groups * plan.lanes / 32 : plan.deal.groups);
+    const int partials = rows ? (int)plan.partials() : 0;
     return with_types(dtype, param_dtype, [&](auto t, auto p) {
         typedef decltype(t) T;
         typedef decltype(p) P;
@@ -692,10 +723,11 @@ int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, cons
             }
         } else if (rows && (dx || sums)) {
             rc = with_lanes(plan.lanes, access, [&](auto l, auto a) {
-                const size_t shared = a.value == WIDE_ALIKE ? (size_t)plan.threads * 2 * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
+                const size_t ring = a.value == WIDE_ALIKE ? (size_t)plan.threads * 2 * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
+                const size_t shared = std::max(ring, sums && plan.merged ? (size_t)plan.threads * PER_LANE * 2 * 4 : 0);
                 if (!allow_shared<layer_norm_bw<T, P, l.value, a.value>>(shared)) return launched("frnn_layer_norm_backward");
                 return launch("frnn_layer_norm_backward", layer_norm_bw<T, P, l.value, a.value>, dim3(plan.grid), plan.threads, shared, st, false, 1, *s, plan.deal, (const T*)dy,
-                              (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx, sums ? (float*)workspace : (float*)nullptr, merge);
+                              (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx, sums ? (float*)workspace : (float*)nullptr);
             });
         }
         if (rc || !sums) return rc;
