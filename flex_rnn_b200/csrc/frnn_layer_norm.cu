@@ -1,8 +1,8 @@
 // Layer norm over the last dimension, forward and backward, with weights for each column or for each head and column.
 //
 // Both directions are bound by memory: a pass over x (and dy) that keeps a row in registers between its reductions and its
-// results, so each element is read and written once.  A row belongs to a group of lanes, 16 elements a lane: 2 to 32
-// lanes of a warp up to 512 columns, a block of up to 512 threads up to 8192; longer rows are read again (``*_long``).
+// results, so each element is read and written once.  A row belongs to a group of lanes, 16 elements a lane: 2 to 64
+// lanes up to 1024 columns, a block of up to 512 threads up to 8192; longer rows are read again (``*_long``).
 // A group walks over rows of one head, so its weights and the sums of its weight gradients stay in registers.  At the end
 // each block (with weights for each head: each group) writes one partial sum to the workspace, and `layer_norm_join` adds
 // those, all in a fixed order.  (Clusters that add theirs first through each other's shared memory gained nothing with 2
@@ -81,17 +81,30 @@ template <class T, Access A> struct Columns {
             else v[j].zero();
         }
     }
-    template <class R> __device__ __forceinline__ void copy(const R& ring, int first, const T* row) const {
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (whole(j)) ring.copy(first + j, row + at[j]);
-    }
-    template <class R> __device__ __forceinline__ void take(const R& ring, int first, Pack<T, E>* v) const {
+    // Row's accesses on their way; `begin`: the tensor's first element.  An access that begins before its row begins in the
+    // row before (or the gap between them), one that ends behind it stops there; what is not the row's is cleared later.
+    template <class R> __device__ __forceinline__ void copy(const R& ring, int first, const T* row, const T* begin) const {
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            if (whole(j)) ring.take(first + j, v[j]);
-            else v[j].zero();
+            if (whole(j)) {
+                ring.copy(first + j, row + at[j], 16);
+            } else if (A == WIDE_APART && at[j] < width && at[j] > -E) {
+                const int upto = min(E, width - at[j]);
+                if (row + at[j] >= begin) ring.copy(first + j, row + at[j], upto * (int)sizeof(T));
+                else
+                    for (int e = max(0, -at[j]); e < upto; e++) ring.put(first + j, e, row[at[j] + e]);
+            }
         }
+    }
+    template <class R> __device__ __forceinline__ void take(const R& ring, int first, float2* f) const {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            Pack<T, E> v;
+            if (whole(j) || A == WIDE_APART) ring.take(first + j, v);
+            else v.zero();
+            v.to(&f[0].x + j * E);
+        }
+        if (A == WIDE_APART) clear(f);
     }
     __device__ __forceinline__ void store(T* row, const float2* f) const {
 #pragma unroll
@@ -144,12 +157,13 @@ template <class T, Access A> struct Columns {
 
 // A lane's place: its group and its place in it.
 template <int L> struct Seat {
-    int lanes, lane;
+    int lanes, lane, place;      // place: of the group in its block
     unsigned group, head;
     __device__ __forceinline__ Seat(const frnn_rows& s) {
         lanes = L ? L : blockDim.x;
+        place = L ? threadIdx.x / (L ? L : 1) : 0;
         lane = L ? threadIdx.x % (L ? L : 1) : threadIdx.x;
-        group = L ? blockIdx.x * (BLOCK / (L ? L : 1)) + threadIdx.x / (L ? L : 1) : blockIdx.x;
+        group = blockIdx.x * (L ? BLOCK / (L ? L : 1) : 1) + place;
         head = s.heads > 1 ? group % (unsigned)s.heads : 0;
     }
 };
@@ -163,9 +177,11 @@ template <class T, int N, int ROUNDS> struct Ring {
     int stage = 0;
     __device__ __forceinline__ Ring(char* shared) : slot(shared + 16 * threadIdx.x) {}
     __device__ __forceinline__ char* place(int i) const { return slot + 16 * (stage * N + i) * blockDim.x; }
-    __device__ __forceinline__ void copy(int i, const T* from) const {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(place(i))), "l"(from) : "memory");
+    // the first `bytes` of 16, and zeros behind them
+    __device__ __forceinline__ void copy(int i, const T* from, int bytes) const {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(place(i))), "l"(from), "r"(bytes) : "memory");
     }
+    __device__ __forceinline__ void put(int i, int e, T x) const { ((T*)place(i))[e] = x; }
     __device__ __forceinline__ void commit() {
         asm volatile("cp.async.commit_group;" ::: "memory");
         stage = stage + 1 == ROUNDS ? 0 : stage + 1;
@@ -177,26 +193,29 @@ template <class T, int N, int ROUNDS> struct Ring {
 
 template <int L> __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int o = L ? L / 2 : 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    for (int o = L && L < 32 ? L / 2 : 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     return v;
 }
 
-// A float2 of each warp, seen by all threads of the block; two buffers by turns, so one barrier each time is enough.
-struct Exchange {
+// A float2 of each warp of a group of several warps (a block, L = 0, or L lanes), seen by all its threads; two buffers by
+// turns, so one barrier of the group each time is enough.
+template <int L> struct Exchange {
     float2 (*buffer)[MOST_THREADS / 32];
     int turn = 0;
+    static __device__ __forceinline__ int first() { return L ? threadIdx.x / (L ? L : 1) * (L / 32) : 0; }      // the group's first warp
     template <class F> __device__ __forceinline__ void operator()(float2 mine, F each) {
         if ((threadIdx.x & 31) == 0) buffer[turn][threadIdx.x / 32] = mine;
-        __syncthreads();
+        if (L) asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / (L ? L : 1)), "n"(L ? L : 32) : "memory");
+        else __syncthreads();
         turn ^= 1;
         again(each);
     }
     // the last ones once more
     template <class F> __device__ __forceinline__ void again(F each) const {
-        const float4* all = (const float4*)buffer[turn ^ 1];
-        const int warps = blockDim.x / 32;
+        const float4* all = (const float4*)(buffer[turn ^ 1] + first());
+        const int warps = L ? L / 32 : blockDim.x / 32;
 #pragma unroll
-        for (int i = 0; i < MOST_THREADS / 64; i++) {
+        for (int i = 0; i < (L ? L : MOST_THREADS) / 64; i++) {
             if (2 * i >= warps) break;
             const float4 v = all[i];
             each(2 * i, make_float2(v.x, v.y));
@@ -218,18 +237,19 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
     const int width = (int)s.width;
     const int shift = A == WIDE_APART ? (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T) : 0;
     const C cols(width, seat.lanes, seat.lane, shift);
-    Exchange exchange{buffer};
+    Exchange<L> exchange{buffer};
+    constexpr bool CROSS = L == 0 || L > 32;               // a group is several warps
     float2 wf[PER_LANE / 2], bf[PER_LANE / 2], f[PER_LANE / 2];
     cols.params(w ? w + (int64_t)seat.head * width : w, 1.f, wf);
     cols.params(b ? b + (int64_t)seat.head * width : b, 0.f, bf);
     const float per_row = 1.f / (float)width;
     float per_warp = 0;
-    if (!L) {
+    if (CROSS) {
         const float mine = lanes_sum<0>((float)cols.count());
         per_warp = mine > 0 ? 1.f / mine : 0.f;
-        if (seat.lane % 32 == 0) counts[seat.lane / 32] = mine;      // (seen by all after the first exchange's barrier)
+        if (seat.lane % 32 == 0) counts[threadIdx.x / 32] = mine;      // (seen by the group after the first exchange's barrier)
     }
-    constexpr bool RING = A == WIDE_ALIKE;
+    constexpr bool RING = A != ELEMENTS;
     extern __shared__ __align__(16) char shared[];
     Pack<T, C::E> next[C::NV];
     Ring<T, RING ? C::NV : 0, RING ? STAGES<T> : 1> ring(shared);
@@ -239,7 +259,7 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
     auto fetch = [&](unsigned r) {
         if (left) {
             const T* px = wx.at(s, s.x, r);
-            if constexpr (RING) cols.copy(ring, 0, px);
+            if constexpr (RING) cols.copy(ring, 0, px, x);
             else cols.load(next, px);
             left--;
             wx.next(s, s.x, deal, deal.x, r + deal.groups);
@@ -254,15 +274,16 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
         const bool there = r < deal.rows;
         if constexpr (RING) {
             ring.wait();
-            cols.take(ring, 0, next);
+            cols.take(ring, 0, f);
+        } else {
+            C::unpack(next, f);
         }
-        C::unpack(next, f);
         fetch(r + AHEAD * deal.groups);
         float2 t = f[0];
 #pragma unroll
         for (int k = 1; k < PER_LANE / 2; k++) t = add2(t, f[k]);
         const float sum = lanes_sum<L>(t.x + t.y);
-        float mean = sum * (L ? per_row : per_warp);
+        float mean = sum * (CROSS ? per_warp : per_row);
 #pragma unroll
         for (int k = 0; k < PER_LANE / 2; k++) f[k] = add2(f[k], both(-mean));
         cols.clear(f);
@@ -270,15 +291,15 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
 #pragma unroll
         for (int k = 1; k < PER_LANE / 2; k++) t = fma2(f[k], f[k], t);
         float sq = lanes_sum<L>(t.x + t.y);
-        if (!L) {
+        if (CROSS) {
             const float own = mean;
             float2 t = both(0.f);
-            exchange(make_float2(own, sq), [&](int k, float2 v) { t = fma2(v, make_float2(counts[k], 1.f), t); });
+            exchange(make_float2(own, sq), [&](int k, float2 v) { t = fma2(v, make_float2(counts[exchange.first() + k], 1.f), t); });
             mean = t.x * per_row;
             sq = t.y;
             exchange.again([&](int k, float2 v) {
                 const float d = v.x - mean;
-                sq = fmaf(counts[k] * d, d, sq);
+                sq = fmaf(counts[exchange.first() + k] * d, d, sq);
             });
             const float2 move = both(own - mean);
 #pragma unroll
@@ -294,7 +315,8 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
 }
 
 // dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w, xh = (x - mean) rstd; sums over the group's rows of dy xh and dy.
-// part: [blocks][2][width] where groups of lanes of a warp have one head, else [groups][2][width]; may be NULL, and so may dx.
+// part: [blocks][2][pitch] where blocks have several groups of one head, else [groups][2][pitch], pitch the next multiple
+// of 4 of the width; may be NULL, and so may dx.
 template <class T, class P, int L, Access A>
 __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_norm_bw(frnn_rows s, Deal deal, const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ w,
                                                                          const float2* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part) {
@@ -305,14 +327,15 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
     const int width = (int)s.width;
     const int shift = A == WIDE_APART ? (int)((uintptr_t)(x + (g < deal.rows ? place(s, s.x, g) : 0)) & 15) / (int)sizeof(T) : 0;
     const C cols(width, seat.lanes, seat.lane, shift);
-    Exchange exchange{buffer};
+    Exchange<L> exchange{buffer};
+    constexpr bool CROSS = L == 0 || L > 32;               // a group is several warps
     cudaTriggerProgrammaticLaunchCompletion();
     float2 wf[PER_LANE / 2], dw[PER_LANE / 2], db[PER_LANE / 2], f[PER_LANE / 2], u[PER_LANE / 2];
     cols.params(w ? w + (int64_t)seat.head * width : w, 1.f, wf);
     const float per_row = 1.f / (float)width;
 #pragma unroll
     for (int k = 0; k < PER_LANE / 2; k++) dw[k] = db[k] = both(0.f);
-    constexpr bool RING = A == WIDE_ALIKE;
+    constexpr bool RING = A != ELEMENTS;
     extern __shared__ __align__(16) char shared[];
     Pack<T, C::E> xn[C::NV], gn[C::NV];
     Ring<T, RING ? 2 * C::NV : 0, RING ? STAGES<T> : 1> ring(shared);
@@ -326,8 +349,8 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
         if (left) {
             const T *px = wx.at(s, s.x, r), *pg = wg.at(s, s.dy, r);
             if constexpr (RING) {
-                cols.copy(ring, 0, px);
-                cols.copy(ring, C::NV, pg);
+                cols.copy(ring, 0, px, x);
+                cols.copy(ring, C::NV, pg, dy);
             } else {
                 cols.load(xn, px);
                 cols.load(gn, pg);
@@ -348,11 +371,12 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
         const float2 st = sn;
         if constexpr (RING) {
             ring.wait();
-            cols.take(ring, 0, xn);
-            cols.take(ring, C::NV, gn);
+            cols.take(ring, 0, f);
+            cols.take(ring, C::NV, u);
+        } else {
+            C::unpack(xn, f);
+            C::unpack(gn, u);
         }
-        C::unpack(xn, f);
-        C::unpack(gn, u);
         if (there && deal.rows - r > deal.groups) sn = stats[r + deal.groups];
         fetch(r + AHEAD * deal.groups);
         float2 a = both(0.f), c = both(0.f);
@@ -369,7 +393,7 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
         }
         if (!dx) continue;
         float ma = lanes_sum<L>(a.x + a.y), mc = lanes_sum<L>(c.x + c.y);
-        if (!L) {
+        if (CROSS) {
             float2 t = both(0.f);
             exchange(make_float2(ma, mc), [&](int, float2 v) { t = add2(t, v); });
             ma = t.x;
@@ -383,13 +407,17 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
         wd.next(s, s.dx, deal, deal.dx, r + deal.groups);
     }
     if (!part) return;
+    const int pitch = (width + 3) & ~3;
+    // by way of shared memory where groups of a block have one head (their sums are added there), and where columns are not
+    // in runs of 16 bytes (single ones would be written 32 bytes apart)
+    int places = L ? BLOCK / (L ? L : 1) : 1;
     const bool merged = L && s.heads == 1;
-    float* to = part + 2ll * g * width;
-    int places = BLOCK / (L ? L : 1);
+    const bool staged = merged || A != WIDE_ALIKE;
+    float* to = part + 2ll * g * pitch;
     bool write = true;
-    if (merged) {
-        int place = threadIdx.x / (L ? L : 1);
-        if (L < 32 && A != WIDE_APART) {                   // the groups of a warp hold the same columns
+    if (staged) {
+        int place = seat.place;
+        if (merged && L && L < 32 && A != WIDE_APART) {         // the groups of a warp hold the same columns
 #pragma unroll
             for (int o = L ? L : 32; o < 32; o *= 2)
 #pragma unroll
@@ -402,7 +430,7 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
             write = threadIdx.x % 32 < (L ? L : 1);
         }
         __syncthreads();                                   // the rows' shared memory takes the sums
-        to = (float*)shared + 2 * place * width;
+        to = (float*)shared + 2 * place * pitch;
     }
     if (write)
 #pragma unroll
@@ -413,7 +441,7 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
 #pragma unroll
                     for (int e = 0; e < C::E; e += 4) {
                         *(float4*)(to + cols.at[j] + e) = make_float4(pw[e], pw[e + 1], pw[e + 2], pw[e + 3]);
-                        *(float4*)(to + width + cols.at[j] + e) = make_float4(pb[e], pb[e + 1], pb[e + 2], pb[e + 3]);
+                        *(float4*)(to + pitch + cols.at[j] + e) = make_float4(pb[e], pb[e + 1], pb[e + 2], pb[e + 3]);
                     }
                 continue;
             }
@@ -421,16 +449,21 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
             for (int e = 0; e < C::E; e++)
                 if (cols.there(j, e)) {
                     to[cols.at[j] + e] = pw[e];
-                    to[width + cols.at[j] + e] = pb[e];
+                    to[pitch + cols.at[j] + e] = pb[e];
                 }
         }
-    if (!merged) return;
+    if (!staged) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * width; i += BLOCK) {
-        float sum = 0;
+    if (merged) {
+        for (int i = threadIdx.x; i < 2 * pitch; i += blockDim.x) {
+            float sum = 0;
 #pragma unroll 8
-        for (int k = 0; k < places; k++) sum += ((const float*)shared)[2 * k * width + i];
-        part[2ll * blockIdx.x * width + i] = sum;
+            for (int k = 0; k < places; k++) sum += ((const float*)shared)[2 * k * pitch + i];
+            part[2ll * blockIdx.x * pitch + i] = sum;
+        }
+    } else {
+        float4* out = (float4*)(part + 2ll * blockIdx.x * places * pitch);
+        for (int i = threadIdx.x; i < places * pitch / 2; i += blockDim.x) out[i] = ((const float4*)shared)[i];
     }
 }
 
@@ -503,41 +536,36 @@ __global__ void layer_norm_dw_long(frnn_rows s, const T* __restrict__ dy, const 
         dw += g * ((to_float(x[place(s, s.x, (unsigned)r) + d]) - st.x) * st.y);
         db += g;
     }
-    float* to = part + 2 * ((int64_t)blockIdx.z * heads + head) * s.width;
+    const int64_t pitch = (s.width + 3) & ~3ll;
+    float* to = part + 2 * ((int64_t)blockIdx.z * heads + head) * pitch;
     to[d] = dw;
-    to[s.width + d] = db;
+    to[pitch + d] = db;
 }
 
-// Sum of the partial sums of a head (partials head, head + heads, ...): 8 lanes have V columns each, 32 slices of the
+// Sum of the partial sums of a head (partials head, head + heads, ...): 8 lanes have 4 columns each, 32 slices of the
 // partials are summed side by side, so that few loads wait for one another.
-template <class P, int V>
+template <class P>
 __global__ void __launch_bounds__(BLOCK) layer_norm_join(const float* __restrict__ part, int partials, int heads, int width, P* __restrict__ dw, P* __restrict__ db) {
     constexpr int LANES = 8, SLICES = BLOCK / LANES;
-    __shared__ float share[SLICES][LANES * V];
-    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, head = blockIdx.y, c = (blockIdx.x * LANES + lane) * V;
+    __shared__ float4 share[SLICES][LANES];
+    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, head = blockIdx.y, c = (blockIdx.x * LANES + lane) * 4, pitch = (width + 3) & ~3;
     P* to = blockIdx.z ? db : dw;
     cudaGridDependencySynchronize();
     if (!to) return;
-    float sum[V] = {};
+    float4 sum = make_float4(0, 0, 0, 0);
     if (c < width)
 #pragma unroll 8
         for (int64_t p = head + (int64_t)slice * heads; p < partials; p += (int64_t)heads * SLICES) {
-            const float* from = part + (2 * p + blockIdx.z) * width + c;
-            if constexpr (V == 4) {
-                const float4 v = *(const float4*)from;
-                sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
-            } else {
-                sum[0] += *from;
-            }
+            const float4 v = *(const float4*)(part + (2 * p + blockIdx.z) * pitch + c);      // (columns behind the width are read and dropped)
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
-#pragma unroll
-    for (int v = 0; v < V; v++) share[slice][lane * V + v] = sum[v];
+    share[slice][lane] = sum;
     __syncthreads();
-    const int i = threadIdx.x, col = blockIdx.x * LANES * V + i;
-    if (i >= LANES * V || col >= width) return;
+    const int i = threadIdx.x, col = blockIdx.x * LANES * 4 + i;
+    if (i >= LANES * 4 || col >= width) return;
     float total = 0;
 #pragma unroll
-    for (int k = 0; k < SLICES; k++) total += share[k][i];
+    for (int k = 0; k < SLICES; k++) total += ((const float*)share[k])[i];
     to[(int64_t)head * width + col] = from_float<P>(total);
 }
 
@@ -563,15 +591,16 @@ Plan plan_of(const frnn_rows& s, int threads_per_sm) {
         p.deal.groups = (unsigned)(slabs * s.heads);
         return p;
     }
-    for (p.lanes = 2; p.lanes <= 32 && p.lanes * PER_LANE < need; p.lanes *= 2) {}
-    if (p.lanes > 32) p.lanes = 0;
+    for (p.lanes = 2; p.lanes <= 64 && p.lanes * PER_LANE < need; p.lanes *= 2) {}
+    if (p.lanes > 64) p.lanes = 0;
     p.threads = p.lanes ? BLOCK : (int)((need + PER_LANE * 32 - 1) / (PER_LANE * 32) * 32);
     const int64_t in_block = p.lanes ? BLOCK / p.lanes : 1;
     int64_t unit = std::lcm<int64_t>(s.heads, 8);
     if (s.n2 <= 128) unit = std::lcm<int64_t>(unit, std::max<int64_t>(1, s.n2));
     const int64_t by = unit / std::gcd(unit, in_block);                   // blocks by which the number of groups stays a multiple of `unit`
     p.merged = p.lanes && s.heads == 1;
-    const int64_t full = (int64_t)sm_count() * std::max(1, threads_per_sm / p.threads), want = std::max<int64_t>(1, std::min((rows + in_block - 1) / in_block, full));
+    const int64_t full = (int64_t)sm_count() * std::max(1, threads_per_sm / p.threads);
+    const int64_t want = std::max<int64_t>(1, std::min((rows + in_block - 1) / in_block, full));
     const int64_t down = want / by * by;
     p.grid = (int)(down && (rows + in_block - 1) / in_block > full ? down : (want + by - 1) / by * by);
     p.deal.rows = (unsigned)rows;
@@ -647,6 +676,7 @@ template <class F> int with_lanes(int lanes, Access access, F f) {
         case 8: return pick(std::integral_constant<int, 8>());
         case 16: return pick(std::integral_constant<int, 16>());
         case 32: return pick(std::integral_constant<int, 32>());
+        case 64: return pick(std::integral_constant<int, 64>());
         default: return pick(std::integral_constant<int, 0>());
     }
 }
@@ -679,7 +709,7 @@ int frnn_layer_norm_forward(const frnn_rows* s, int dtype, const void* x, int pa
         }
         const Access access = access_of(*s, lies, 2);
         return with_lanes(plan.lanes, access, [&](auto l, auto a) {
-            const size_t shared = a.value == WIDE_ALIKE ? (size_t)plan.threads * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
+            const size_t shared = a.value != ELEMENTS ? (size_t)plan.threads * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
             if (!allow_shared<layer_norm_fw<T, P, l.value, a.value>>(shared)) return launched("frnn_layer_norm_forward");
             return launch("frnn_layer_norm_forward", layer_norm_fw<T, P, l.value, a.value>, dim3(plan.grid), plan.threads, shared, st, false, 1, *s, plan.deal, (const T*)x,
                           (const P*)weight, (const P*)bias, eps, (T*)y, (float2*)stats);
@@ -688,7 +718,7 @@ int frnn_layer_norm_forward(const frnn_rows* s, int dtype, const void* x, int pa
 }
 
 size_t frnn_layer_norm_backward_workspace(const frnn_rows* s) {
-    return s && s->heads >= 1 && s->width > 0 ? (size_t)plan_of(*s, BW_THREADS_PER_SM).partials() * 2 * s->width * 4 : 0;
+    return s && s->heads >= 1 && s->width > 0 ? (size_t)plan_of(*s, BW_THREADS_PER_SM).partials() * 2 * ((s->width + 3) & ~3ll) * 4 : 0;
 }
 
 int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, const void* x, int param_dtype, const void* weight, const float* stats, void* dx,
@@ -723,19 +753,16 @@ int frnn_layer_norm_backward(const frnn_rows* s, int dtype, const void* dy, cons
             }
         } else if (rows && (dx || sums)) {
             rc = with_lanes(plan.lanes, access, [&](auto l, auto a) {
-                const size_t ring = a.value == WIDE_ALIKE ? (size_t)plan.threads * 2 * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
-                const size_t shared = std::max(ring, sums && plan.merged ? (size_t)plan.threads * PER_LANE * 2 * 4 : 0);
+                const size_t ring = a.value != ELEMENTS ? (size_t)plan.threads * 2 * (PER_LANE / WIDE<T>) * STAGES<T> * 16 : 0;
+                const size_t shared = std::max(ring, sums && (plan.merged || a.value != WIDE_ALIKE) ? (size_t)plan.threads * (PER_LANE + 2) * 2 * 4 : 0);      // (pitch: up to 3 floats more than a group's columns)
                 if (!allow_shared<layer_norm_bw<T, P, l.value, a.value>>(shared)) return launched("frnn_layer_norm_backward");
                 return launch("frnn_layer_norm_backward", layer_norm_bw<T, P, l.value, a.value>, dim3(plan.grid), plan.threads, shared, st, false, 1, *s, plan.deal, (const T*)dy,
                               (const T*)x, (const P*)weight, (const float2*)stats, (T*)dx, sums ? (float*)workspace : (float*)nullptr);
             });
         }
         if (rc || !sums) return rc;
-        auto join = [&](auto v) {
-            return launch("frnn_layer_norm_backward", layer_norm_join<P, v.value>, dim3((unsigned)((s->width + 8 * v.value - 1) / (8 * v.value)), (unsigned)s->heads, 2), BLOCK, 0, st,
-                          rows > 0, 1, (const float*)workspace, partials, (int)s->heads, (int)s->width, (P*)dweight, (P*)dbias);
-        };
-        return s->width % 4 ? join(std::integral_constant<int, 1>()) : join(std::integral_constant<int, 4>());
+        return launch("frnn_layer_norm_backward", layer_norm_join<P>, dim3((unsigned)((s->width + 31) / 32), (unsigned)s->heads, 2), BLOCK, 0, st, rows > 0, 1, (const float*)workspace, partials,
+                      (int)s->heads, (int)s->width, (P*)dweight, (P*)dbias);
     });
 }
 
