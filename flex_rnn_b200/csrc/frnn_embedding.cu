@@ -21,6 +21,13 @@ namespace {
 
 enum { BLOCK = 256, UNROLL = 8 };
 
+// How rows are accessed.  ALIKE: all of them at 16-byte boundaries, in accesses of 16 bytes.  APART: rows at any distances
+// behind boundaries; a thread's columns follow the boundaries of the row that is written, the row that is read comes in
+// two accesses and shifts.  ELEMENTS: one element at a time (columns that are not consecutive).
+enum Access { ALIKE, APART, ELEMENTS };
+
+template <class T, Access A> constexpr int EACH = A == ELEMENTS ? 1 : WIDE<T>;
+
 // How a block's threads stand to rows: `lanes` threads (a power of two, all of the block for wide rows) have E columns
 // each, blockIdx.y counts the parts of rows wider than that.
 struct Shape {
@@ -28,8 +35,9 @@ struct Shape {
     unsigned parts;            // blocks side by side over a row's columns
 };
 
-Shape shape_of(int64_t width, int each) {
-    const int64_t vectors = (width + each - 1) / each;
+template <class T, Access A> Shape shape_of(int64_t width) {
+    constexpr int E = EACH<T, A>;
+    const int64_t vectors = (width + (A == APART ? E - 1 : 0) + E - 1) / E;
     Shape s{1, 1, 1};
     while (s.lanes < BLOCK && s.lanes < vectors) s.lanes *= 2;
     s.groups = BLOCK / s.lanes;
@@ -37,24 +45,49 @@ Shape shape_of(int64_t width, int each) {
     return s;
 }
 
+// First of a thread's columns of a row that is written at `row`, thread `t` along the row.
+template <class T, Access A> __device__ __forceinline__ int column(const T* row, unsigned t) {
+    return (int)t * EACH<T, A> - (A == APART ? (int)((uintptr_t)row & 15) / (int)sizeof(T) : 0);
+}
+
+template <class T, Access A> __device__ __forceinline__ void write_columns(const Pack<T, EACH<T, A>>& v, T* row, int c, int width) {
+    if (A != APART) {
+        if (c < width) v.store(row + c);
+    } else {
+        store_part(v, row, c, width);
+    }
+}
+
 // y_i = scale * W[t_i]; a zero row where t_i is ignored or (reported) outside the vocabulary.  A group takes UNROLL / 2
 // rows, whose loads are all under way before the first is used.
-template <class T, int E>
+template <class T, Access A>
 __global__ void __launch_bounds__(BLOCK) embedding_fw(const T* __restrict__ w, int64_t rows, int width, int64_t row_stride, int64_t col_stride, const void* __restrict__ tokens,
                                                       int token_bytes, int n, float scale, int64_t ignore, T* __restrict__ out, int* err, Shape shape) {
-    constexpr int ROWS = UNROLL / 2;
-    const int lane = threadIdx.x % shape.lanes, first = (blockIdx.x * shape.groups + threadIdx.x / shape.lanes) * ROWS, c = (int)(blockIdx.y * shape.lanes + lane) * E;
+    constexpr int ROWS = UNROLL / 2, E = EACH<T, A>;
+    const unsigned t = blockIdx.y * shape.lanes + threadIdx.x % shape.lanes;
+    const int first = (blockIdx.x * shape.groups + threadIdx.x / shape.lanes) * ROWS;
+    const T* end = w + (rows - 1) * row_stride + width;
     Pack<T, E> v[ROWS];
 #pragma unroll
     for (int u = 0; u < ROWS; u++) {
         v[u].zero();
         if (first + u >= n) continue;
-        const int64_t t = token_at(tokens, token_bytes, first + u);
-        const bool there = t != ignore && t >= 0 && t < rows;
-        if (t != ignore && !there && c == 0) *err = CODE_TOKEN;
-        if (there && c < width) v[u].load(w + t * row_stride + (E == 1 ? c * col_stride : c));
+        const int64_t k = token_at(tokens, token_bytes, first + u);
+        const bool there = k != ignore && k >= 0 && k < rows;
+        if (k != ignore && !there && t == 0) *err = CODE_TOKEN;
+        if (!there) continue;
+        const T* row = w + k * row_stride;
+        const int c = column<T, A>(out + (int64_t)(first + u) * width, t);
+        if constexpr (A == APART) {
+            if (c >= 0 && c + E <= width) load_anywhere(v[u], row + c, w, end);
+            else
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (c + e >= 0 && c + e < width) v[u].set(e, row[c + e]);
+        } else if (c < width) {
+            v[u].load(row + (A == ELEMENTS ? c * col_stride : c));
+        }
     }
-    if (c >= width) return;
 #pragma unroll
     for (int u = 0; u < ROWS; u++) {
         if (first + u >= n) return;
@@ -63,7 +96,8 @@ __global__ void __launch_bounds__(BLOCK) embedding_fw(const T* __restrict__ w, i
 #pragma unroll
         for (int e = 0; e < E; e++) f[e] *= scale;
         v[u].from(f);
-        v[u].store(out + (int64_t)(first + u) * width + c);
+        T* to = out + (int64_t)(first + u) * width;
+        write_columns<T, A>(v[u], to, column<T, A>(to, t), width);
     }
 }
 
@@ -207,90 +241,136 @@ embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
 
 enum : unsigned { NO_KEY = 0xFFFFFFFFu };
 
-template <class T, int E> __device__ __forceinline__ void write_row(const float* sum, float scale, T* to) {
-    float f[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) f[e] = scale * sum[e];
+// The E columns from c on of a row of `width`, zeros where there are none: `fetch` starts the loads, `get` waits for them,
+// so that those of several rows are under way at once.  [begin, end): the tensor.  APART reads the 32 aligned bytes around
+// its columns, which may hold other rows' elements but nothing outside of the tensor: there, one element at a time.
+template <class T, Access A> struct Reader {
+    static constexpr int E = EACH<T, A>;
     Pack<T, E> v;
-    v.from(f);
-    v.store(to);
-}
-template <int E> __device__ __forceinline__ void write_part(const float* sum, float* to) {
-#pragma unroll
-    for (int e = 0; e < E; e += E < 4 ? 1 : 4) {
-        if constexpr (E >= 4) *(float4*)(to + e) = make_float4(sum[e], sum[e + 1], sum[e + 2], sum[e + 3]);
-        else to[e] = sum[e];
+    __device__ __forceinline__ void fetch(const T* row, int c, int width, const T*, const T*, bool there) {
+        v.zero();
+        if (there && c < width) v.load(row + c);
     }
-}
-
-// A group sums a chunk of the sorted places.  part: [chunks][2][width], sums of the run that came in over the chunk's start
-// and of the one that goes on over its end.
-template <class T, int E>
+    __device__ __forceinline__ void get(Pack<T, E>& to) const { to = v; }
+};
+template <class T> struct Reader<T, APART> {
+    static constexpr int E = WIDE<T>;
+    uint4 low, high;
+    const T* row;
+    int c, width;             // width: 0 where there is no row
+    bool wide;
+    __device__ __forceinline__ void fetch(const T* row_, int c_, int width_, const T* begin, const T* end, bool there) {
+        row = row_;
+        c = c_;
+        width = there ? width_ : 0;
+        const T* from = row + c - ((uintptr_t)(row + c) & 15) / sizeof(T);
+        wide = there && c < width && from >= begin && from + 2 * E <= end;
+        if (wide) {
+            low = *(const uint4*)from;
+            high = *(const uint4*)(from + E);
+        }
+    }
+    __device__ __forceinline__ void get(Pack<T, E>& to) const {
+        if (!wide) {
+#pragma unroll
+            for (int e = 0; e < E; e++) to.set(e, c + e >= 0 && c + e < width ? row[c + e] : from_float<T>(0.f));
+            return;
+        }
+        shift_out(to, low, high, (unsigned)((uintptr_t)(row + c) & 15) / (unsigned)sizeof(T));
+        if (c < 0 || c + E > width)
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (c + e < 0 || c + e >= width) to.set(e, from_float<T>(0.f));
+    }
+};
+// A group sums a chunk of the sorted places.  part: [chunks][2][pitch] (pitch: the width's next multiple of 4), sums of the
+// run that came in over the chunk's start and of the one that goes on over its end.
+template <class T, Access A>
 __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy, const unsigned* __restrict__ keys, const int* __restrict__ at, int n, unsigned rows, int width,
                                                         int chunk, float scale, T* __restrict__ dw, float* __restrict__ part, Shape shape) {
-    const int lane = threadIdx.x % shape.lanes, c = (int)(blockIdx.y * shape.lanes + lane) * E;
+    constexpr int E = EACH<T, A>;
+    const unsigned t = blockIdx.y * shape.lanes + threadIdx.x % shape.lanes;
     const int64_t mine = (int64_t)blockIdx.x * shape.groups + threadIdx.x / shape.lanes, from = mine * chunk;
     cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();
-    if (from >= n || c >= width) return;
-    const int lo = (int)from, hi = (int)min((int64_t)n, from + chunk);
+    if (from >= n || (int)t * E >= width + (A == APART ? E - 1 : 0)) return;
+    const int lo = (int)from, hi = (int)min((int64_t)n, from + chunk), pitch = (width + 3) & ~3;
+    const T* end = dy + (int64_t)n * width;
     unsigned run = keys[lo];
     bool came_in = lo > 0 && keys[lo - 1] == run;
     const unsigned after = hi < n ? keys[hi] : NO_KEY;
-    float* parts = part + 2 * mine * width + c;
     float sum[E] = {};
-    unsigned next[UNROLL];
-    int place[UNROLL];
+    auto finish = [&](bool goes_on) {
+        T* row = dw + (int64_t)run * width;
+        const int c = column<T, A>(row, t);
+        if (came_in || goes_on) {
+            float* to = part + (2 * mine + !came_in) * pitch;
+            if (A == ALIKE) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) *(float4*)(to + c + e) = make_float4(sum[e], sum[e + 1], sum[e + 2], sum[e + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (c + e >= 0 && c + e < width) to[c + e] = sum[e];
+            }
+            return;
+        }
+        float f[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e] = scale * sum[e];
+        Pack<T, E> v;
+        v.from(f);
+        write_columns<T, A>(v, row, c, width);
+    };
+    constexpr int ROUND = A == APART ? UNROLL / 2 : UNROLL;       // rows under way at once
+    unsigned next[ROUND];
+    int place[ROUND];
     auto look = [&](int j) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
+        for (int u = 0; u < ROUND; u++) {
             next[u] = j + u < hi ? keys[j + u] : NO_KEY;
             place[u] = j + u < hi ? at[j + u] : 0;
         }
     };
     look(lo);
-    for (int j = lo; j < hi && run < rows; j += UNROLL) {
-        unsigned k[UNROLL];
-        Pack<T, E> v[UNROLL];
+    for (int j = lo; j < hi && run < rows; j += ROUND) {
+        unsigned k[ROUND];
+        Reader<T, A> in[ROUND];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
+        for (int u = 0; u < ROUND; u++) {
             k[u] = next[u];
-            v[u].zero();
-            if (k[u] < rows) v[u].load(dy + (int64_t)place[u] * width + c);
+            const bool there = k[u] < rows;
+            in[u].fetch(dy + (int64_t)place[u] * width, column<T, A>(dw + (int64_t)(there ? k[u] : 0) * width, t), width, dy, end, there);
         }
-        look(j + UNROLL);                                 // the next round's places, while these rows are on their way
+        look(j + ROUND);                                  // the next round's places, while these rows are on their way
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
+        for (int u = 0; u < ROUND; u++) {
             if (j + u < hi && k[u] != run) {
-                if (run < rows) {
-                    if (came_in) write_part<E>(sum, parts);
-                    else write_row<T, E>(sum, scale, dw + (int64_t)run * width + c);
-                }
+                if (run < rows) finish(false);
                 run = k[u];
                 came_in = false;
 #pragma unroll
                 for (int e = 0; e < E; e++) sum[e] = 0;
             }
+            Pack<T, E> v;
             float f[E];
-            v[u].to(f);
+            in[u].get(v);
+            v.to(f);
 #pragma unroll
             for (int e = 0; e < E; e++) sum[e] += f[e];
         }
     }
-    if (run >= rows) return;
-    if (came_in) write_part<E>(sum, parts);
-    else if (after == run) write_part<E>(sum, parts + width);
-    else write_row<T, E>(sum, scale, dw + (int64_t)run * width + c);
+    if (run < rows) finish(after == run);
 }
 
 // Sums of the runs that cross ends of chunks, each in the order of its partial sums.  A block looks at JOINED chunks for
-// runs that start there and go on, and adds those runs' partial sums: 64 threads with V columns each, 4 slices side by side.
+// runs that start there and go on, and adds those runs' partial sums: 64 threads with 4 columns each, 4 slices side by side.
 enum { JOINED = BLOCK / 32 };
-template <class T, int V>
+template <class T>
 __global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restrict__ keys, int n, unsigned rows, int width, int chunk, float scale, T* __restrict__ dw,
                                                         const float* __restrict__ part) {
     constexpr int LANES = 64, SLICES = BLOCK / LANES;
-    __shared__ float share[SLICES][LANES * V];
+    __shared__ float4 share[SLICES][LANES];
     __shared__ unsigned runs[JOINED];
     __shared__ int64_t ends[JOINED];                      // the last chunk that the run reaches
     cudaGridDependencySynchronize();
@@ -319,28 +399,21 @@ __global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restri
         const unsigned run = runs[r];
         if (run == NO_KEY) continue;
         const int64_t mine = (int64_t)blockIdx.x * JOINED + r, last = ends[r];
-        const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (int)(blockIdx.y * LANES + lane) * V;
-        float sum[V] = {};
+        const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES, c = (int)(blockIdx.y * LANES + lane) * 4, pitch = (width + 3) & ~3;
+        float4 sum = make_float4(0, 0, 0, 0);
         if (c < width)
 #pragma unroll 8
             for (int64_t q = mine + slice; q <= last; q += SLICES) {
-                const float* from = part + (2 * q + (q == mine)) * width + c;
-                if constexpr (V == 4) {
-                    const float4 v = *(const float4*)from;
-                    sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
-                } else {
-                    sum[0] += *from;
-                }
+                const float4 v = *(const float4*)(part + (2 * q + (q == mine)) * pitch + c);      // (columns behind the width are read and dropped)
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
             }
-#pragma unroll
-        for (int v = 0; v < V; v++) share[slice][lane * V + v] = sum[v];
+        share[slice][lane] = sum;
         __syncthreads();
-        for (int i = threadIdx.x; i < LANES * V; i += BLOCK) {
-            const int col = blockIdx.y * LANES * V + i;
-            if (col >= width) continue;
+        const int col = blockIdx.y * LANES * 4 + threadIdx.x;
+        if (col < width) {
             float total = 0;
 #pragma unroll
-            for (int k = 0; k < SLICES; k++) total += share[k][i];
+            for (int k = 0; k < SLICES; k++) total += ((const float*)share[k])[threadIdx.x];
             dw[(int64_t)run * width + col] = from_float<T>(scale * total);
         }
         __syncthreads();
@@ -366,7 +439,7 @@ Plan plan_of(int dtype, int64_t rows, int64_t width, int64_t n) {
     for (p.chunk = 8; p.chunk < 128 && blocks / p.chunk > 8.0 * sm_count(); p.chunk *= 2) {}
     p.chunks = (n + p.chunk - 1) / p.chunk;
     p.at_parts = ((size_t)n * 16 + 255) / 256 * 256;
-    p.bytes = p.at_parts + (size_t)p.chunks * 2 * width * 4;
+    p.bytes = p.at_parts + (size_t)p.chunks * 2 * ((width + 3) & ~3ll) * 4;
     return p;
 }
 
@@ -379,12 +452,14 @@ int bad_shape(const char* what, int dtype, int64_t rows, int64_t width, int toke
 
 enum { SORT_SHARED = WARPS * DIGITS * 4, FILL_BLOCKS = 128 };
 
-// Calls f(T(), integral_constant E): 16 bytes an access, or one element.
-template <class F> int with_access(int dtype, bool wide, F f) {
+// Calls f(T(), integral_constant A).
+template <class F> int with_access(int dtype, Access access, F f) {
     return with_dtype(dtype, [&](auto t) {
-        typedef decltype(t) T;
-        if (wide) return f(t, std::integral_constant<int, WIDE<T>>());
-        return f(t, std::integral_constant<int, 1>());
+        switch (access) {
+            case ALIKE: return f(t, std::integral_constant<Access, ALIKE>());
+            case APART: return f(t, std::integral_constant<Access, APART>());
+            default: return f(t, std::integral_constant<Access, ELEMENTS>());
+        }
     });
 }
 
@@ -400,12 +475,12 @@ int frnn_embedding_forward(int dtype, const void* weight, int64_t rows, int64_t 
     const size_t size = dtype_bytes(dtype);
     if (!on_boundary(weight, size) || !on_boundary(out, size) || !on_boundary(tokens, token_bytes) || !on_boundary(err_word, 4))
         return frnn_fail(FRNN_E_ARG, "frnn_embedding_forward: a pointer is not on a boundary of its elements");
-    const bool wide = col_stride == 1 && width * size % 16 == 0 && row_stride * (int64_t)size % 16 == 0 && on_boundary(weight, 16) && on_boundary(out, 16);
-    return with_access(dtype, wide, [&](auto t, auto e) {
+    const bool alike = width * size % 16 == 0 && row_stride * (int64_t)size % 16 == 0 && on_boundary(weight, 16) && on_boundary(out, 16);
+    return with_access(dtype, col_stride != 1 ? ELEMENTS : alike ? ALIKE : APART, [&](auto t, auto a) {
         typedef decltype(t) T;
-        const Shape shape = shape_of(width, e.value);
+        const Shape shape = shape_of<T, a.value>(width);
         const int64_t each = shape.groups * (UNROLL / 2);
-        embedding_fw<T, e.value><<<dim3((unsigned)((n + each - 1) / each), shape.parts), BLOCK, 0, (cudaStream_t)stream>>>(
+        embedding_fw<T, a.value><<<dim3((unsigned)((n + each - 1) / each), shape.parts), BLOCK, 0, (cudaStream_t)stream>>>(
             (const T*)weight, rows, (int)width, row_stride, col_stride, tokens, token_bytes, (int)n, scale, ignore_index, (T*)out, err_word, shape);
         return launched("frnn_embedding_forward");
     });
@@ -443,20 +518,20 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     if (n == 0) return FRNN_OK;
     const int side = plan.passes & 1;
     const unsigned* keys = key + side * n;
-    const bool wide = width * size % 16 == 0 && on_boundary(dout, 16) && on_boundary(dweight, 16);
-    return with_access(dtype, wide, [&](auto t, auto e) {
+    const bool alike = width * size % 16 == 0 && on_boundary(dout, 16) && on_boundary(dweight, 16);
+    return with_access(dtype, alike ? ALIKE : APART, [&](auto t, auto a) {
         typedef decltype(t) T;
-        const Shape shape = shape_of(width, e.value);
-        if (int rc = launch("frnn_embedding_backward", embedding_sums<T, e.value>, dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st, true, 1,
-                            (const T*)dout, keys, at + side * n, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape))
-            return rc;
-        if (plan.chunks < 2) return (int)FRNN_OK;
-        auto join = [&](auto v) {
-            return launch("frnn_embedding_backward", embedding_join<T, v.value>,
-                          dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 64 * v.value - 1) / (64 * v.value))), BLOCK, 0, st, true, 1, keys, (int)n, (unsigned)rows,
-                          (int)width, plan.chunk, scale, (T*)dweight, (const float*)part);
-        };
-        return width % 4 ? join(std::integral_constant<int, 1>()) : join(std::integral_constant<int, 4>());
+        if constexpr (a.value == ELEMENTS) {
+            return (int)FRNN_E_ARG;                        // (no call comes here)
+        } else {
+            const Shape shape = shape_of<T, a.value>(width);
+            if (int rc = launch("frnn_embedding_backward", embedding_sums<T, a.value>, dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st, true, 1,
+                                (const T*)dout, keys, at + side * n, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape))
+                return rc;
+            if (plan.chunks < 2) return (int)FRNN_OK;
+            return launch("frnn_embedding_backward", embedding_join<T>, dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 255) / 256)), BLOCK, 0, st, true, 1, keys,
+                          (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, (const float*)part);
+        }
     });
 }
 

@@ -143,6 +143,32 @@ template <class T, int E> __device__ __forceinline__ void store_part(const Pack<
     }
 }
 
+// E elements out of 32 aligned bytes, from the one numbered `off` on.
+template <class T, int E> __device__ __forceinline__ void shift_out(Pack<T, E>& v, const uint4& low, const uint4& high, unsigned off) {
+    const unsigned words = off * (unsigned)sizeof(T) / 4, bits = sizeof(T) == 2 ? (off & 1) * 16 : 0;
+    unsigned w[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = words & 2 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = words & 1 ? w[i + 1] : w[i];
+    const uint4 r = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    memcpy(&v.v, &r, 16);
+}
+
+// E elements from p, which may lie anywhere between 16-byte boundaries, by two accesses of 16 bytes and shifts.  These may
+// hold other elements of the tensor [begin, end), but nothing outside of it: there, one element at a time.
+template <class T, int E> __device__ __forceinline__ void load_anywhere(Pack<T, E>& v, const T* p, const T* begin, const T* end) {
+    const unsigned off = (unsigned)((uintptr_t)p & 15) / (unsigned)sizeof(T);
+    if (off == 0) {
+        v.load(p);
+    } else if (p - off >= begin && p - off + 2 * E <= end) {
+        shift_out(v, *(const uint4*)(p - off), *(const uint4*)(p - off + E), off);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) v.set(e, p[e]);
+    }
+}
+
 // Launches a kernel; `early`: it may start while the one before it in the stream still runs, and itself waits where it needs
 // that one's results (cudaGridDependencySynchronize).  `cluster` > 1: blocks of a cluster.
 template <class... P, class... A> inline int launch(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream, bool early, int cluster, A... args) {
