@@ -151,7 +151,7 @@ embedding_fill(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
 // places, 32 a round; a place's rank is what comes before it in its round, its warp, its block, its cluster and among the
 // smaller digits.
 __global__ void __launch_bounds__(SORT_THREADS, 1)
-embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, int passes, int bits, unsigned* key_a, unsigned* key_b, int* at_a, int* at_b) {
+embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t rows, int64_t ignore, int passes, int bits, uint2* a, uint2* b) {
     extern __shared__ unsigned count[];                        // [WARPS][DIGITS]
     __shared__ unsigned total[DIGITS], carry[WARPS];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -163,18 +163,16 @@ embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
     unsigned* mine = count + warp * DIGITS;
     for (int pass = 0; pass < passes; pass++) {
         const int shift = pass * bits;
-        const unsigned* from = pass & 1 ? key_b : key_a;
-        const int* from_at = pass & 1 ? at_b : at_a;
-        unsigned* to = pass & 1 ? key_a : key_b;
-        int* to_at = pass & 1 ? at_a : at_b;
+        const uint2* from = pass & 1 ? b : a;
+        uint2* to = pass & 1 ? a : b;                          // a token and its place together: one scattered store, not two
         // the buffers were written by other SMs: read past this one's L1
-        auto key = [&](int i) { return pass ? __ldcg(from + i) : key_of(tokens, token_bytes, i, rows, ignore); };
+        auto pair = [&](int i) { return pass ? __ldcg(from + i) : make_uint2(key_of(tokens, token_bytes, i, rows, ignore), (unsigned)i); };
         for (int i = lane; i < digits; i += 32) mine[i] = 0;
         __syncwarp();
         for (int i0 = lo + lane; i0 < hi; i0 += 32 * ROUNDS) {
             unsigned k[ROUNDS];
 #pragma unroll
-            for (int u = 0; u < ROUNDS; u++) k[u] = i0 + 32 * u < hi ? key(i0 + 32 * u) : 0;
+            for (int u = 0; u < ROUNDS; u++) k[u] = i0 + 32 * u < hi ? pair(i0 + 32 * u).x : 0;
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++)
                 if (i0 + 32 * u < hi) atomicAdd(&mine[(k[u] >> shift) & mask], 1u);
@@ -211,25 +209,16 @@ embedding_sort(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
         if (d < digits) total[d] = before + scan - all + below;
         __syncthreads();
         for (int i0 = lo + lane; i0 < hi + lane; i0 += 32 * ROUNDS) {
-            unsigned k[ROUNDS];
-            int at[ROUNDS];
+            uint2 k[ROUNDS];
 #pragma unroll
-            for (int u = 0; u < ROUNDS; u++) {
-                const int i = i0 + 32 * u;
-                k[u] = i < hi ? key(i) : 0;
-                at[u] = i < hi && pass ? __ldcg(from_at + i) : i;
-            }
+            for (int u = 0; u < ROUNDS; u++) k[u] = i0 + 32 * u < hi ? pair(i0 + 32 * u) : make_uint2(0, 0);
 #pragma unroll
             for (int u = 0; u < ROUNDS; u++) {
                 if (i0 - lane + 32 * u >= hi) break;
                 const bool in = i0 + 32 * u < hi;
-                const unsigned digit = in ? (k[u] >> shift) & mask : digits;
+                const unsigned digit = in ? (k[u].x >> shift) & mask : digits;
                 const unsigned same = __match_any_sync(~0u, digit), earlier = same & ((1u << lane) - 1);
-                if (in) {
-                    const unsigned p = total[digit] + mine[digit] + __popc(earlier);
-                    to[p] = k[u];
-                    to_at[p] = at[u];
-                }
+                if (in) to[total[digit] + mine[digit] + __popc(earlier)] = k[u];
                 __syncwarp();
                 if (in && !earlier) mine[digit] += __popc(same);
                 __syncwarp();
@@ -286,7 +275,7 @@ template <class T> struct Reader<T, APART> {
 // A group sums a chunk of the sorted places.  part: [chunks][2][pitch] (pitch: the width's next multiple of 4), sums of the
 // run that came in over the chunk's start and of the one that goes on over its end.
 template <class T, Access A>
-__global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy, const unsigned* __restrict__ keys, const int* __restrict__ at, int n, unsigned rows, int width,
+__global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy, const uint2* __restrict__ sorted, int n, unsigned rows, int width,
                                                         int chunk, float scale, T* __restrict__ dw, float* __restrict__ part, Shape shape) {
     constexpr int E = EACH<T, A>;
     const unsigned t = blockIdx.y * shape.lanes + threadIdx.x % shape.lanes;
@@ -296,9 +285,9 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
     if (from >= n || (int)t * E >= width + (A == APART ? E - 1 : 0)) return;
     const int lo = (int)from, hi = (int)min((int64_t)n, from + chunk), pitch = (width + 3) & ~3;
     const T* end = dy + (int64_t)n * width;
-    unsigned run = keys[lo];
-    bool came_in = lo > 0 && keys[lo - 1] == run;
-    const unsigned after = hi < n ? keys[hi] : NO_KEY;
+    unsigned run = sorted[lo].x;
+    bool came_in = lo > 0 && sorted[lo - 1].x == run;
+    const unsigned after = hi < n ? sorted[hi].x : NO_KEY;
     float sum[E] = {};
     auto finish = [&](bool goes_on) {
         T* row = dw + (int64_t)run * width;
@@ -323,14 +312,10 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
         write_columns<T, A>(v, row, c, width);
     };
     constexpr int ROUND = A == APART ? UNROLL / 2 : UNROLL;       // rows under way at once
-    unsigned next[ROUND];
-    int place[ROUND];
+    uint2 next[ROUND];
     auto look = [&](int j) {
 #pragma unroll
-        for (int u = 0; u < ROUND; u++) {
-            next[u] = j + u < hi ? keys[j + u] : NO_KEY;
-            place[u] = j + u < hi ? at[j + u] : 0;
-        }
+        for (int u = 0; u < ROUND; u++) next[u] = j + u < hi ? sorted[j + u] : make_uint2(NO_KEY, 0);
     };
     look(lo);
     for (int j = lo; j < hi && run < rows; j += ROUND) {
@@ -338,9 +323,9 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
         Reader<T, A> in[ROUND];
 #pragma unroll
         for (int u = 0; u < ROUND; u++) {
-            k[u] = next[u];
+            k[u] = next[u].x;
             const bool there = k[u] < rows;
-            in[u].fetch(dy + (int64_t)place[u] * width, column<T, A>(dw + (int64_t)(there ? k[u] : 0) * width, t), width, dy, end, there);
+            in[u].fetch(dy + (int64_t)next[u].y * width, column<T, A>(dw + (int64_t)(there ? k[u] : 0) * width, t), width, dy, end, there);
         }
         look(j + ROUND);                                  // the next round's places, while these rows are on their way
 #pragma unroll
@@ -364,10 +349,11 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
 }
 
 // Sums of the runs that cross ends of chunks, each in the order of its partial sums.  A block looks at JOINED chunks for
-// runs that start there and go on, and adds those runs' partial sums: 64 threads with 4 columns each, 4 slices side by side.
-enum { JOINED = BLOCK / 32 };
+// runs that start there and go on.  A run of few partial sums is added by one warp, all of them side by side; a longer one
+// by the block, 64 threads with 4 columns each and 4 slices of the partial sums.
+enum { JOINED = BLOCK / 32, FEW = 16 };
 template <class T>
-__global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restrict__ keys, int n, unsigned rows, int width, int chunk, float scale, T* __restrict__ dw,
+__global__ void __launch_bounds__(BLOCK) embedding_join(const uint2* __restrict__ sorted, int n, unsigned rows, int width, int chunk, float scale, T* __restrict__ dw,
                                                         const float* __restrict__ part) {
     constexpr int LANES = 64, SLICES = BLOCK / LANES;
     __shared__ float4 share[SLICES][LANES];
@@ -379,20 +365,37 @@ __global__ void __launch_bounds__(BLOCK) embedding_join(const unsigned* __restri
         const int64_t q = (int64_t)blockIdx.x * JOINED + r, lo = q * chunk, hi = lo + chunk;
         unsigned run = NO_KEY;
         if (hi < n) {
-            const unsigned over = keys[hi], last = keys[hi - 1], before = lo > 0 ? keys[lo - 1] : NO_KEY;
+            const unsigned over = sorted[hi].x, last = sorted[hi - 1].x, before = lo > 0 ? sorted[lo - 1].x : NO_KEY;
             if (over < rows && last == over && before != over) run = over;
         }
         int64_t last = q;
         while (run != NO_KEY) {
             const int64_t next = last + 1 + lane;
-            const int more = __popc(__ballot_sync(~0u, next * chunk < n && keys[next * chunk] == run));      // sorted: the first `more` of them
+            const int more = __popc(__ballot_sync(~0u, next * chunk < n && sorted[next * chunk].x == run));      // sorted: the first `more` of them
             last += more;
             if (more < 32) break;
         }
+        const bool few = run != NO_KEY && last - q < FEW;
         if (lane == 0) {
-            runs[r] = run;
+            runs[r] = few ? NO_KEY : run;
             ends[r] = last;
         }
+        if (few)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int c = (int)(blockIdx.y * 64 + half * 32 + lane) * 4, pitch = (width + 3) & ~3;
+                if (c >= width) continue;
+                float4 sum = *(const float4*)(part + (2 * q + 1) * pitch + c);      // (columns behind the width are read and dropped)
+#pragma unroll 8
+                for (int64_t k = q + 1; k <= last; k++) {
+                    const float4 v = *(const float4*)(part + 2 * k * pitch + c);
+                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                }
+                T* to = dw + (int64_t)run * width + c;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (c + e < width) to[e] = from_float<T>(scale * (&sum.x)[e]);
+            }
     }
     __syncthreads();
     for (int r = 0; r < JOINED; r++) {
@@ -500,14 +503,13 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
         return frnn_fail(FRNN_E_ARG, "frnn_embedding_backward: a pointer is not on a boundary of its elements (the workspace: of 16 bytes)");
     const cudaStream_t st = (cudaStream_t)stream;
     const Plan plan = plan_of(dtype, rows, width, n);
-    unsigned* key = (unsigned*)workspace;
-    int* at = (int*)(key + 2 * n);
+    uint2* pairs = (uint2*)workspace;
     float* part = n ? (float*)((char*)workspace + plan.at_parts) : nullptr;
     if (n) {
         // 8 blocks: 16 sort 32768 tokens 5 us faster, but then fewer blocks fill (0.5 GB of zeros and 8192 tokens: 116 us, with 16 blocks 128)
         if (!allow_shared<embedding_sort>(SORT_SHARED)) return launched("frnn_embedding_backward");
         if (int rc = launch("frnn_embedding_backward", embedding_sort, dim3(CLUSTER), SORT_THREADS, SORT_SHARED, st, false, CLUSTER, tokens, token_bytes, (int)n, rows, ignore_index,
-                            plan.passes, plan.bits, key, key + n, at, at + n))
+                            plan.passes, plan.bits, pairs, pairs + n))
             return rc;
     }
     // 64 KB of zeros for each block, and at most 128 blocks: with more, the same bytes took longer (0.5 GB: 78 us, with 136 to 296 blocks 89)
@@ -516,8 +518,7 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
                         rows, ignore_index, (char*)dweight, width * (int64_t)size, (int)size))
         return rc;
     if (n == 0) return FRNN_OK;
-    const int side = plan.passes & 1;
-    const unsigned* keys = key + side * n;
+    const uint2* sorted = pairs + (plan.passes & 1) * n;
     const bool alike = width * size % 16 == 0 && on_boundary(dout, 16) && on_boundary(dweight, 16);
     return with_access(dtype, alike ? ALIKE : APART, [&](auto t, auto a) {
         typedef decltype(t) T;
@@ -526,10 +527,10 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
         } else {
             const Shape shape = shape_of<T, a.value>(width);
             if (int rc = launch("frnn_embedding_backward", embedding_sums<T, a.value>, dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st, true, 1,
-                                (const T*)dout, keys, at + side * n, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape))
+                                (const T*)dout, sorted, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape))
                 return rc;
             if (plan.chunks < 2) return (int)FRNN_OK;
-            return launch("frnn_embedding_backward", embedding_join<T>, dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 255) / 256)), BLOCK, 0, st, true, 1, keys,
+            return launch("frnn_embedding_backward", embedding_join<T>, dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 255) / 256)), BLOCK, 0, st, true, 1, sorted,
                           (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, (const float*)part);
         }
     });
