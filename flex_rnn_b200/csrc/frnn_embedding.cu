@@ -141,8 +141,16 @@ embedding_fill(const void* __restrict__ tokens, int token_bytes, int n, int64_t 
             if (t >= lo && t < lo + here && t != ignore) occurs[t - lo] = 1;
         }
         __syncthreads();
-        for (int i = warp; i < here; i += WARPS)
-            if (!occurs[i]) fill_zero(dw, (lo + i) * row_bytes, (lo + i + 1) * row_bytes, size);
+        // a warp takes 32 rows and fills each run of them in one go
+        for (int i = 32 * warp; i < here; i += 32 * WARPS) {
+            const int lane = threadIdx.x & 31;
+            unsigned absent = __ballot_sync(~0u, i + lane < here && !occurs[i + lane]);
+            while (absent) {
+                const int first = __ffs(absent) - 1, ones = __ffs(~(absent >> first)) - 1, last = ones < 0 ? 32 : first + ones;      // (ones: 32 of them have no end)
+                fill_zero(dw, (lo + i + first) * row_bytes, (lo + i + last) * row_bytes, size);
+                absent = last >= 32 ? 0 : absent & (~0u << last);
+            }
+        }
     }
     cudaGridDependencySynchronize();                           // not done before the sort is: the next kernel waits for this one
 }

@@ -591,8 +591,9 @@ Plan plan_of(const frnn_rows& s, int threads_per_sm) {
         p.deal.groups = (unsigned)(slabs * s.heads);
         return p;
     }
-    for (p.lanes = 2; p.lanes <= 64 && p.lanes * PER_LANE < need; p.lanes *= 2) {}
-    if (p.lanes > 64) p.lanes = 0;
+    for (p.lanes = 2; p.lanes <= BLOCK && p.lanes * PER_LANE < need; p.lanes *= 2) {}
+    // a block of just the threads that a wide row needs where a group of a power of two would leave many without columns
+    if (p.lanes > BLOCK || (p.lanes > 64 && 5 * need < 4 * p.lanes * PER_LANE)) p.lanes = 0;
     p.threads = p.lanes ? BLOCK : (int)((need + PER_LANE * 32 - 1) / (PER_LANE * 32) * 32);
     const int64_t in_block = p.lanes ? BLOCK / p.lanes : 1;
     int64_t unit = std::lcm<int64_t>(s.heads, 8);
@@ -677,6 +678,8 @@ template <class F> int with_lanes(int lanes, Access access, F f) {
         case 16: return pick(std::integral_constant<int, 16>());
         case 32: return pick(std::integral_constant<int, 32>());
         case 64: return pick(std::integral_constant<int, 64>());
+        case 128: return pick(std::integral_constant<int, 128>());
+        case 256: return pick(std::integral_constant<int, 256>());
         default: return pick(std::integral_constant<int, 0>());
     }
 }
