@@ -11,6 +11,8 @@
 #include <torch/library.h>
 
 #include <atomic>
+#include <cstdlib>
+#include <cstring>
 #include <map>
 #include <string>
 
@@ -51,8 +53,27 @@ template <class F> auto with_python(F f) {
     }
 }
 
-// The error word of a device, after raising what kernels of earlier calls left there.
+// FRNN_GUARD=1: every buffer that kernels write lies between two bands of a byte pattern, which are looked at after the
+// call; FRNN_CHECK=1: each call waits and raises what its kernels reported.  Debugging only: both wait for the GPU.
+enum { BAND = 4096, FILL = 0xA5 };
+struct Guarded {
+    const char* what;
+    Tensor raw;
+    int64_t bytes;
+};
+thread_local bool t_guard = false, t_check = false;
+thread_local std::vector<Guarded> t_guarded;
+
+bool asked(const char* name) {
+    const char* e = getenv(name);
+    return e && *e && strcmp(e, "0");
+}
+
+// The error word of a device, after raising what kernels of earlier calls left there.  A call begins with it.
 int* error_word(c10::DeviceIndex device) {
+    t_guard = asked("FRNN_GUARD");
+    t_check = asked("FRNN_CHECK");
+    t_guarded.clear();
     TORCH_CHECK(device >= 0 && device < MAX_DEVICES, "flex_rnn_b200: device index ", (int)device);
     int* w = g_word[device].load(std::memory_order_acquire);
     if (!w) {
@@ -63,9 +84,24 @@ int* error_word(c10::DeviceIndex device) {
     return w;
 }
 
-void ran(int rc) { TORCH_CHECK(rc == FRNN_OK, "flex_rnn_b200: ", g_last_error()); }
-
 void* stream_of(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// The end of a call: its return code, and what the debugging switches ask for.
+void ran(int rc, const Tensor& like) {
+    TORCH_CHECK(rc == FRNN_OK, "flex_rnn_b200: ", g_last_error());
+    if (t_guard || t_check) c10::cuda::getCurrentCUDAStream(like.device().index()).synchronize();
+    std::vector<Guarded> guarded;
+    guarded.swap(t_guarded);
+    for (const Guarded& g : guarded) {
+        const int64_t lo = g.raw.narrow(0, 0, BAND).ne(FILL).sum().item<int64_t>(), hi = g.raw.narrow(0, BAND + g.bytes, g.raw.numel() - BAND - g.bytes).ne(FILL).sum().item<int64_t>();
+        TORCH_CHECK(!lo && !hi, "flex_rnn_b200: a kernel wrote ", lo + hi, " byte(s) outside ", g.what, " (", lo ? "before" : "after", " the buffer)");
+    }
+    if (t_check) {
+        const bool guard = t_guard;
+        error_word(like.device().index());
+        t_guard = guard;
+    }
+}
 
 int dtype_of(const char* op, const char* what, const Tensor& t) {
     switch (t.scalar_type()) {
@@ -92,11 +128,22 @@ Tensor check_tokens(const char* op, const Tensor& tokens, const Tensor& first) {
     return tokens.contiguous();
 }
 
-Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+Tensor make_strided(const char* what, at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType type, const Tensor& like) {
+    if (!t_guard) return at::detail::empty_strided_cuda(sizes, strides, type, like.device());
+    int64_t extent = 1;
+    for (size_t d = 0; d < sizes.size(); d++) extent = sizes[d] == 0 ? 0 : extent ? extent + (sizes[d] - 1) * strides[d] : 0;
+    const int64_t bytes = extent * (int64_t)c10::elementSize(type);
+    Tensor raw = at::detail::empty_strided_cuda({2 * BAND + (bytes + 255) / 256 * 256}, {1}, at::kByte, like.device());
+    raw.fill_(FILL);
+    t_guarded.push_back({what, raw, bytes});
+    return raw.narrow(0, BAND, bytes).view(type).as_strided(sizes, strides);
+}
+
+Tensor make(const char* what, at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
     std::vector<int64_t> strides(sizes.size());
     int64_t s = 1;
     for (size_t d = sizes.size(); d--;) { strides[d] = s; s *= std::max<int64_t>(1, sizes[d]); }
-    return at::detail::empty_strided_cuda(sizes, strides, type, like.device());
+    return make_strided(what, sizes, strides, type, like);
 }
 
 // What a forward saved, contiguous and on a 16-byte boundary, whatever a saved-tensor hook made of it.
@@ -105,7 +152,7 @@ Tensor saved(const Tensor& t) {
     return (uintptr_t)c.data_ptr() & 15 ? c.clone() : c;
 }
 
-Tensor workspace(size_t bytes, const Tensor& like) { return bytes ? make({(int64_t)bytes}, at::kByte, like) : Tensor(); }
+Tensor workspace(size_t bytes, const Tensor& like) { return bytes ? make("the workspace", {(int64_t)bytes}, at::kByte, like) : Tensor(); }
 template <class T = void> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
 template <class T = void> T* ptr(const optional<Tensor>& t) { return t.has_value() && t->defined() ? (T*)t->data_ptr() : nullptr; }
 
@@ -121,9 +168,9 @@ Tensor embedding_cuda(const Tensor& tokens, const Tensor& weight, double scale, 
     int* err = error_word(weight.device().index());
     auto sizes = tokens.sizes().vec();
     sizes.push_back(weight.size(1));
-    Tensor out = make(sizes, weight.scalar_type(), weight);
+    Tensor out = make("the output", sizes, weight.scalar_type(), weight);
     ran(g_embedding_forward(dtype, weight.data_ptr(), weight.size(0), weight.size(1), weight.stride(0), weight.stride(1), tok.data_ptr(), (int)tok.element_size(),
-                            tok.numel(), (float)scale, ignore_index, out.data_ptr(), err, stream_of(weight)));
+                            tok.numel(), (float)scale, ignore_index, out.data_ptr(), err, stream_of(weight)), weight);
     return out;
 }
 
@@ -138,8 +185,8 @@ Tensor embedding_backward_cuda(const Tensor& grad, const Tensor& tokens, int64_t
     error_word(grad.device().index());
     const int64_t width = grad.size(-1), n = tok.numel();
     const Tensor g = grad.contiguous(), work = workspace(g_embedding_backward_workspace(dtype, rows, width, n), grad);
-    Tensor dw = make({rows, width}, grad.scalar_type(), grad);
-    ran(g_embedding_backward(dtype, g.data_ptr(), tok.data_ptr(), (int)tok.element_size(), n, rows, width, (float)scale, ignore_index, dw.data_ptr(), ptr(work), stream_of(grad)));
+    Tensor dw = make("the weight's gradient", {rows, width}, grad.scalar_type(), grad);
+    ran(g_embedding_backward(dtype, g.data_ptr(), tok.data_ptr(), (int)tok.element_size(), n, rows, width, (float)scale, ignore_index, dw.data_ptr(), ptr(work), stream_of(grad)), grad);
     return dw;
 }
 
@@ -223,11 +270,11 @@ std::tuple<Tensor, Tensor> layer_norm_cuda(const Tensor& x, const optional<Tenso
         from = x.contiguous();
         TORCH_INTERNAL_ASSERT(rows_of(ts, 1, heads, r));
     }
-    Tensor y = make(x.sizes(), x.scalar_type(), x);
+    Tensor y = make("the output", x.sizes(), x.scalar_type(), x);
     const int64_t rows = x.numel() ? x.numel() / x.size(-1) : 0;
-    Tensor stats = make({save ? rows : 0, 2}, at::kFloat, x);
+    Tensor stats = make("the statistics", {save ? rows : 0, 2}, at::kFloat, x);
     const optional<Tensor> w = dense(weight), b = dense(bias);
-    if (x.numel()) ran(g_layer_norm_forward(&r, dtype, from.data_ptr(), ptype, ptr(w), ptr(b), (float)eps, y.data_ptr(), save ? stats.data_ptr<float>() : nullptr, stream_of(x)));
+    if (x.numel()) ran(g_layer_norm_forward(&r, dtype, from.data_ptr(), ptype, ptr(w), ptr(b), (float)eps, y.data_ptr(), save ? stats.data_ptr<float>() : nullptr, stream_of(x)), x);
     return {y, stats};
 }
 
@@ -245,27 +292,31 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_cuda(const Tensor& grad, 
     TORCH_CHECK(stats.dim() == 2 && stats.size(0) == rows && stats.size(1) == 2 && stats.scalar_type() == at::kFloat, "flex_rnn_b200: layer_norm_backward: the statistics have to be those of the forward");
     c10::cuda::CUDAGuard guard(x.device());
     error_word(x.device().index());
-    Tensor dx = want_x ? at::empty_like(x) : Tensor();
-    Tensor from = rows_dense(x) ? x : x.contiguous(), g = rows_dense(grad) ? grad : grad.contiguous(), to = want_x && rows_dense(dx) ? dx : make(x.sizes(), x.scalar_type(), x);
+    Tensor dx = want_x && !t_guard ? at::empty_like(x) : Tensor();
+    if (want_x && t_guard) {
+        const Tensor shape = at::empty_like(x, x.options().device(at::kMeta));      // (the same layout)
+        dx = make_strided("x's gradient", shape.sizes(), shape.strides(), x.scalar_type(), x);
+    }
+    Tensor from = rows_dense(x) ? x : x.contiguous(), g = rows_dense(grad) ? grad : grad.contiguous(), to = want_x && rows_dense(dx) ? dx : make("x's gradient", x.sizes(), x.scalar_type(), x);
     frnn_rows r;
     const Tensor* ts[3] = {&from, &g, &to};
     if (!rows_of(ts, 3, heads, r)) {
         from = x.contiguous();
         g = grad.contiguous();
-        to = make(x.sizes(), x.scalar_type(), x);
+        to = make("x's gradient", x.sizes(), x.scalar_type(), x);
         TORCH_INTERNAL_ASSERT(rows_of(ts, 3, heads, r));
     }
     const optional<Tensor> w = dense(weight);
     const Tensor st = saved(stats);
-    auto param = [&](bool want, const optional<Tensor>& p) { return want && p.has_value() && p->defined() ? make(p->sizes(), p->scalar_type(), x) : Tensor(); };
+    auto param = [&](bool want, const optional<Tensor>& p) { return want && p.has_value() && p->defined() ? make("a weight's gradient", p->sizes(), p->scalar_type(), x) : Tensor(); };
     Tensor dw = param(want_weight, weight), db = param(want_bias, bias);
     if (x.size(-1)) {
         const Tensor work = dw.defined() || db.defined() ? workspace(g_layer_norm_backward_workspace(&r), x) : Tensor();
         ran(g_layer_norm_backward(&r, dtype, g.data_ptr(), from.data_ptr(), ptype, ptr(w), st.data_ptr<float>(), want_x ? to.data_ptr() : nullptr, ptr(dw), ptr(db), ptr(work),
-                                  stream_of(x)));
+                                  stream_of(x)), x);
     }
     if (want_x && !to.is_same(dx)) dx.copy_(to);
-    auto some = [&](const Tensor& t) { return t.defined() ? t : make({0}, x.scalar_type(), x); };
+    auto some = [&](const Tensor& t) { return t.defined() ? t : make("nothing", {0}, x.scalar_type(), x); };
     return {some(dx), some(dw), some(db)};
 }
 
@@ -298,12 +349,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_cuda(const Ten
     int* err = error_word(logits.device().index());
     const Tensor x = n ? as_rows(logits) : logits;
     auto sizes = tokens.sizes().vec();
-    Tensor lp = make(sizes, at::kFloat, logits), ent = make(sizes, at::kFloat, logits), stats = make({save ? n : 0, 3}, at::kFloat, logits);
+    Tensor lp = make("the log probabilities", sizes, at::kFloat, logits), ent = make("the entropies", sizes, at::kFloat, logits), stats = make("the statistics", {save ? n : 0, 3}, at::kFloat, logits);
     sizes.push_back(top);
-    Tensor top_lp = make(sizes, at::kFloat, logits), top_tok = make(sizes, at::kLong, logits);
+    Tensor top_lp = make("the alternatives' log probabilities", sizes, at::kFloat, logits), top_tok = make("the alternatives", sizes, at::kLong, logits);
     if (n)
         ran(g_token_logprobs_forward(dtype, x.data_ptr(), n, vocab, x.stride(0), tok.data_ptr(), (int)tok.element_size(), (int)top, (float)temperature, ignore_index, lp.data_ptr<float>(),
-                                     ent.data_ptr<float>(), top_lp.data_ptr<float>(), top_tok.data_ptr<int64_t>(), save ? stats.data_ptr<float>() : nullptr, err, stream_of(logits)));
+                                     ent.data_ptr<float>(), top_lp.data_ptr<float>(), top_tok.data_ptr<int64_t>(), save ? stats.data_ptr<float>() : nullptr, err, stream_of(logits)), logits);
     return {lp, ent, top_lp, top_tok, stats};
 }
 
@@ -325,10 +376,10 @@ Tensor token_logprobs_backward_cuda(const optional<Tensor>& dlogprob, const opti
     c10::cuda::CUDAGuard guard(logits.device());
     error_word(logits.device().index());
     const Tensor glp = upstream(dlogprob), gent = upstream(dentropy), st = saved(stats), x = n ? as_rows(logits) : logits;
-    Tensor dx = make(logits.sizes(), logits.scalar_type(), logits);
+    Tensor dx = make("the logits' gradient", logits.sizes(), logits.scalar_type(), logits);
     if (n)
         ran(g_token_logprobs_backward(dtype, x.data_ptr(), n, vocab, x.stride(0), tok.data_ptr(), (int)tok.element_size(), (float)temperature, ignore_index, ptr<float>(glp),
-                                      ptr<float>(gent), st.data_ptr<float>(), dx.data_ptr(), stream_of(logits)));
+                                      ptr<float>(gent), st.data_ptr<float>(), dx.data_ptr(), stream_of(logits)), logits);
     return dx;
 }
 

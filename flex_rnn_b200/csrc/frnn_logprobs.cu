@@ -297,6 +297,10 @@ template <class T, int E, int N> __device__ void block_top(const Row<T, E>& row,
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
 
+// 8192 x 65536 bf16: 189 us, 5.7 TB/s of the copy's 6.5 (the exponentials' unit is 63 % busy, issue slots 76 %); with 5
+// alternatives 235 us, with 20 250; 2000 x 50003 fp32: 73 and with 5 alternatives 89.  One row: 6 us, of which the launch is
+// most.  The next round's loads go out before this round's arithmetic (without that 325 us).
+
 // What the blocks of a cluster tell each other.
 struct Share {
     Part part;
@@ -416,6 +420,7 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
 // d logits_j = 1/T [ g (1[j = token] - p_j) - h p_j (ln p_j + H) ], g and h the upstream gradients of log probability and
 // entropy: p_j times a linear function of log2 p_j, and the token's own term.  p is the square of 2^(log2 p / 2): a gradient
 // is p times some tens and may be seen where p itself is below the smallest number that the exponential gives.
+// 8192 x 65536 bf16: 371 us for 2 GB (5.8 TB/s; a copy of as much 334); 2000 x 50003 fp32: 123 us, the copy's rate.
 // `lanes` threads have a row's tile of LOADS * lanes accesses.
 template <class T, int E>
 __global__ void __launch_bounds__(256) logprobs_bw(const T* __restrict__ logits, unsigned n, int vocab, int64_t row_stride, const void* __restrict__ tokens, int token_bytes,

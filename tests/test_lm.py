@@ -567,6 +567,28 @@ def test_graph_semantics(name):
 
 
 @pytest.mark.gpu
+def test_guard_bands_and_checked_calls(monkeypatch):
+    """With FRNN_GUARD=1 no kernel writes outside of its buffers, at sizes that end inside of accesses, tiles and chunks;
+    with FRNN_CHECK=1 a call raises what its own kernels reported."""
+    monkeypatch.setenv("FRNN_GUARD", "1")
+    for dtype in DTYPES:
+        for n, V, D in [(1, 3, 1), (37, 100, 64), (301, 50, 77), (700, 2003, 515), (3000, 70, 1030), (5000, 300, 33)]:
+            embedding_check(*embedding_case(n, V, D, dtype, pad=n % 2 == 1, same=n == 5000))
+        for rows, H, D in [(1, 1, 1), (5, 1, 31), (40, 3, 77), (33, 5, 128), (130, 1, 1001), (61, 1, 2047), (9, 1, 4096), (5, 1, 8200)]:
+            x, dy = rand(rows, H, D).to(dtype), rand(rows, H, D, seed=2).to(dtype)
+            layer_norm_check(x, *params("heads" if H > 1 else "vector", H, D, dtype), dy)
+            layer_norm_check(rand(rows, H, D + 3, seed=4).to(dtype)[..., 3:], *params("vector", H, D, torch.float32), dy)
+        for n, V, top in [(1, 1, 1), (3, 33, 32), (16, 65536, 20), (1300, 313, 5), (70, 3001, 3), (2, 131073, 32)]:
+            logprobs_check(*logits_of(n, V, dtype), top=top)
+    monkeypatch.setenv("FRNN_GUARD", "0")
+    monkeypatch.setenv("FRNN_CHECK", "1")
+    w = rand(11, 16)
+    with pytest.raises(runtime.FrnnError, match="outside the vocabulary"):
+        fr.embedding(torch.tensor([3, 11], device="cuda"), w)
+    assert torch.equal(fr.embedding(torch.tensor([3], device="cuda"), w)[0], w[3])
+
+
+@pytest.mark.gpu
 def test_inputs_without_gradients():
     f, (x, g, b), (up,) = calls()["layer_norm"]
     want = both(f, [x, g, b], [up])
