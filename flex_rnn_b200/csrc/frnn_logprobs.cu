@@ -93,6 +93,17 @@ template <class T, int E> struct Row {
             for (int e = 0; e < E; e++) v.set(e, access < end && there(access, e) ? x[at(access) + e] : from_float<T>(-INFINITY));
         }
     }
+    // LOADS accesses, `step` apart: the checks of all of them at once where none is at an end
+    __device__ __forceinline__ void get_round(int access, int step, Pack<T, E> (&v)[LOADS]) const {
+        if (access + (LOADS - 1) * step < end && at(access) >= 0 && at(access + (LOADS - 1) * step) <= vocab - E) {
+            const T* from = x + at(access);
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) v[u].load(from + u * step * E);
+        } else {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) get(access + u * step, v[u]);
+        }
+    }
 };
 
 // m, s, t of a part of a row.  Without any finite logit: m = -inf, s = t = 0.
@@ -297,9 +308,10 @@ template <class T, int E, int N> __device__ void block_top(const Row<T, E>& row,
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
 
-// 8192 x 65536 bf16: 189 us, 5.7 TB/s of the copy's 6.5 (the exponentials' unit is 63 % busy, issue slots 76 %); with 5
-// alternatives 235 us, with 20 250; 2000 x 50003 fp32: 73 and with 5 alternatives 89.  One row: 6 us, of which the launch is
-// most.  The next round's loads go out before this round's arithmetic (without that 325 us).
+// 8192 x 65536 bf16: 173 us, 6.2 TB/s of the copy's 6.5 (the exponentials' unit is two thirds busy, issue slots three
+// quarters); with 5 alternatives 223 us, with 20 236; 2000 x 50003 fp32: 70 and with 5 alternatives 87.  One row: 6 us, of
+// which the launch is most.  The next round's loads go out before this round's arithmetic (without that 325 us), and a round
+// is checked for the row's ends once (each access by itself: 189 us).
 
 // What the blocks of a cluster tell each other.
 struct Share {
@@ -327,8 +339,7 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
     float slot_max = -INFINITY;
     int slot = 0, left = rounds;
     int a = part.first + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < LOADS; u++) part.get(a + u * N, next[u]);
+    part.get_round(a, N, next);
     // the token's logit is on its way behind the first round's
     const bool in = tok >= 0 && tok < vocab;
     const float own = rank_ == 0 && threadIdx.x == 0 && tok != ignore && in ? to_float(x[tok]) : 0.f;
@@ -337,9 +348,7 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
 #pragma unroll
         for (int u = 0; u < LOADS; u++) v[u] = next[u];
         a += LOADS * N;
-        if (a < part.end)                                  // the next round's loads are under way during this one
-#pragma unroll
-            for (int u = 0; u < LOADS; u++) part.get(a + u * N, next[u]);
+        if (a < part.end) part.get_round(a, N, next);      // the next round's loads are under way during this one
         const float b = largest(v);
         if (top) {
             slot_max = max_nan(slot_max, b);
@@ -420,20 +429,19 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
 // d logits_j = 1/T [ g (1[j = token] - p_j) - h p_j (ln p_j + H) ], g and h the upstream gradients of log probability and
 // entropy: p_j times a linear function of log2 p_j, and the token's own term.  p is the square of 2^(log2 p / 2): a gradient
 // is p times some tens and may be seen where p itself is below the smallest number that the exponential gives.
-// 8192 x 65536 bf16: 371 us for 2 GB (5.8 TB/s; a copy of as much 334); 2000 x 50003 fp32: 123 us, the copy's rate.
-// `lanes` threads have a row's tile of LOADS * lanes accesses.
+// 8192 x 65536 bf16: 326 us for 2 GB, 2000 x 50003 fp32: 122 us, both a copy's rate.
+// `lanes` threads have `tiles` tiles of a row, of LOADS * lanes accesses each.
 template <class T, int E>
 __global__ void __launch_bounds__(256) logprobs_bw(const T* __restrict__ logits, unsigned n, int vocab, int64_t row_stride, const void* __restrict__ tokens, int token_bytes,
                                                    float inv_t, int64_t ignore, const float* __restrict__ glp, const float* __restrict__ gent, const float* __restrict__ stats,
-                                                   T* __restrict__ dlogits, unsigned tiles, int lanes) {
-    const unsigned unit = blockIdx.x * (256u / lanes) + threadIdx.x / lanes, row = unit / tiles, tile = unit - row * tiles;
+                                                   T* __restrict__ dlogits, unsigned spans, int tiles, int lanes) {
+    const unsigned unit = blockIdx.x * (256u / lanes) + threadIdx.x / lanes, row = unit / spans, span = unit - row * spans;
     if (row >= n) return;
     const Row<T, E> part(logits + row * row_stride, vocab, 0, 1);
     T* d = dlogits + (int64_t)row * vocab;
-    const int first = (int)(tile * (LOADS * lanes) + threadIdx.x % lanes);
+    int a = (int)(span * (tiles * LOADS * lanes) + threadIdx.x % lanes);
     Pack<T, E> v[LOADS];
-#pragma unroll
-    for (int u = 0; u < LOADS; u++) part.get(first + u * lanes, v[u]);
+    part.get_round(a, lanes, v);
     const float m = stats[3ll * row], l2s = stats[3ll * row + 1], H = stats[3ll * row + 2];
     const int64_t tok = token_at(tokens, token_bytes, row);
     const float g = glp && tok != ignore ? glp[row] : 0.f, h = gent ? gent[row] : 0.f;
@@ -442,36 +450,40 @@ __global__ void __launch_bounds__(256) logprobs_bw(const T* __restrict__ logits,
     const float2 by = both(half_c), from = both(empty ? 0.f : -m), less = both(empty ? 0.f : -0.5f * l2s);
     const float2 slope = both(empty ? 0.f : -2.f * inv_t * LN2 * h), level = both(empty ? 0.f : -inv_t * fmaf(h, H, g));
     const float own = empty ? 0.f : inv_t * g;
+    const int hit = tok >= 0 && tok < vocab ? (int)tok : -E;             // (-E: in no access that is written)
+    for (int tile = 0; tile < tiles && a < part.end; tile++) {
+        if (tile) part.get_round(a, lanes, v);
+        const bool inner = part.at(a) >= 0 && part.at(a + (LOADS - 1) * lanes) <= vocab - E;
 #pragma unroll
-    for (int u = 0; u < LOADS; u++) {
-        const int a = first + u * lanes;
-        if (a >= part.end) return;
-        float2 f[(E + 1) / 2];
-        float* f1 = &f[0].x;
-        if (E == 1) f1[1] = 0;
-        v[u].to(f1);
+        for (int u = 0; u < LOADS; u++) {
+            if (!inner && a + u * lanes >= part.end) break;
+            const int at = part.at(a + u * lanes);
+            float2 f[(E + 1) / 2];
+            float* f1 = &f[0].x;
+            if (E == 1) f1[1] = 0;
+            v[u].to(f1);
 #pragma unroll
-        for (int i = 0; i < (E + 1) / 2; i++) {
-            float2 l = fma2(add2(f[i], from), by, less);       // log2 p / 2
-            l.x = max_nan(l.x, NIL);
-            l.y = max_nan(l.y, NIL);
-            const float2 q = make_float2(exp2_fast(l.x), exp2_fast(l.y));
-            f[i] = mul2(mul2(fma2(l, slope, level), q), q);
+            for (int i = 0; i < (E + 1) / 2; i++) {
+                float2 l = fma2(add2(f[i], from), by, less);       // log2 p / 2
+                l.x = max_nan(l.x, NIL);
+                l.y = max_nan(l.y, NIL);
+                const float2 q = make_float2(exp2_fast(l.x), exp2_fast(l.y));
+                f[i] = mul2(mul2(fma2(l, slope, level), q), q);
+            }
+            if ((unsigned)(hit - at) < (unsigned)E)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (hit - at == e) f1[e] += own;
+            v[u].from(f1);
+            if (inner) v[u].store(d + at);
         }
-        const int64_t k = tok - part.at(a);
-        if (k >= 0 && k < E)
+        if (!inner)
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                if (k == e) f1[e] += own;
-        Pack<T, E> out;
-        out.from(f1);
-        if (part.whole(a)) {
-            out.store(d + part.at(a));
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                if (part.there(a, e)) d[part.at(a) + e] = out.get(e);
-        }
+            for (int u = 0; u < LOADS; u++) {
+                const int access = a + u * lanes, at = part.at(access);
+                if (access < part.end) store_part(v[u], d, at, vocab);
+            }
+        a += LOADS * lanes;
     }
 }
 
@@ -550,13 +562,16 @@ int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64
     return with_access(dtype, wide, [&](auto t, auto e) {
         typedef decltype(t) T;
         const int64_t accesses = (vocab + e.value - 1 + e.value - 1) / e.value;      // with up to E - 1 elements before a row's first
-        const int lanes = accesses <= 32 * LOADS ? 32 : 256;                          // a warp has short rows to itself
-        const int64_t tiles = (accesses + LOADS * lanes - 1) / (LOADS * lanes), units = n * tiles;
+        int lanes = 32;                                    // as few as cover a short row, a block for others
+        while (lanes < 256 && lanes * LOADS < accesses) lanes *= 2;
+        // four tiles for what a thread needs besides (8192 x 65536 bf16: 326 us, one 367, eight 340), but rather one each for eight blocks an SM
+        const int tiles = n * ((accesses + 4 * LOADS * lanes - 1) / (4 * LOADS * lanes)) >= 8 * sm_count() ? 4 : 1;
+        const int64_t spans = (accesses + tiles * LOADS * lanes - 1) / (tiles * LOADS * lanes), units = n * spans;
         if (units >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "frnn_token_logprobs_backward: too many logits");
         const int in_block = 256 / lanes;
         logprobs_bw<T, e.value><<<(unsigned)((units + in_block - 1) / in_block), 256, 0, (cudaStream_t)stream>>>((const T*)logits, (unsigned)n, (int)vocab, row_stride, tokens, token_bytes,
                                                                                                                1.f / temperature, ignore_index, dlogprob, dentropy, stats, (T*)dlogits,
-                                                                                                               (unsigned)tiles, lanes);
+                                                                                                               (unsigned)spans, tiles, lanes);
         return launched("frnn_token_logprobs_backward");
     });
 }
