@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 #include <torch/library.h>
 
@@ -21,7 +22,6 @@
 namespace py = pybind11;
 using at::Tensor;
 using std::optional;
-using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 namespace {
@@ -421,26 +421,63 @@ FRNN_OP(token_logprobs_backward, token_logprobs_backward_cuda)
 bool needs(const optional<Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
 
-struct Embedding : torch::autograd::Function<Embedding> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& weight, double scale, int64_t ignore_index) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        ctx->save_for_backward({tokens});
-        ctx->saved_data["rows"] = weight.size(0);
-        ctx->saved_data["scale"] = scale;
-        ctx->saved_data["ignore"] = ignore_index;
-        return embedding().call(tokens, weight, scale, ignore_index);
+// A node of the autograd graph: what a call saved, until it has been used.  (torch::autograd::Function does the same with
+// more on the way; a training call of small tensors is all host time.)
+struct Saving : torch::autograd::Node {
+    std::vector<torch::autograd::SavedVariable> saved;
+    bool released = false;
+    explicit Saving(torch::autograd::edge_list&& e) : Node(std::move(e)) {}
+    void save(const Tensor& t) { saved.emplace_back(t, false); }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (auto& v : saved) v.reset_data();
+        released = true;
     }
-    static variable_list backward(AutogradContext* ctx, variable_list up) {
-        if (!up[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        return {Tensor(), embedding_backward().call(up[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
-                                                    ctx->saved_data["ignore"].toInt()), Tensor(), Tensor()};
+    variable_list unpack() {
+        std::lock_guard<std::mutex> lock(mutex_);
+        TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+        variable_list kept;
+        kept.reserve(saved.size());
+        for (auto& v : saved) kept.push_back(v.unpack(shared_from_this()));
+        return kept;
+    }
+};
+
+template <class N, class... T> std::shared_ptr<N> make_node(const T&... inputs) {
+    return std::shared_ptr<N>(new N(torch::autograd::collect_next_edges(inputs...)), torch::autograd::deleteNode);
+}
+
+void no_tangent(const optional<Tensor>& t) {
+    TORCH_CHECK(!t.has_value() || !t->defined() || !t->_fw_grad(0).defined(), "flex_rnn_b200: forward-mode derivatives of this operator are not built");
+}
+
+struct EmbeddingBackward : Saving {
+    using Saving::Saving;
+    int64_t rows, ignore_index;
+    double scale;
+    std::string name() const override { return "EmbeddingBackward"; }
+    variable_list apply(variable_list&& up) override {
+        if (!up[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+        return {embedding_backward().call(up[0], unpack()[0], rows, scale, ignore_index)};
     }
 };
 
 Tensor embedding_autograd(const Tensor& tokens, const Tensor& weight, double scale, int64_t ignore_index) {
-    if (at::GradMode::is_enabled() && needs(weight)) return Embedding::apply(tokens, weight, scale, ignore_index);
-    at::AutoDispatchBelowADInplaceOrView below;
-    return embedding().call(tokens, weight, scale, ignore_index);
+    no_tangent(weight);
+    Tensor y;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = embedding().call(tokens, weight, scale, ignore_index);
+    }
+    if (at::GradMode::is_enabled() && needs(weight)) {
+        auto node = make_node<EmbeddingBackward>(weight);
+        node->rows = weight.size(0);
+        node->scale = scale;
+        node->ignore_index = ignore_index;
+        node->save(tokens);
+        torch::autograd::create_gradient_edge(y, node);
+    }
+    return y;
 }
 
 Tensor embedding_backward_autograd(const Tensor& grad, const Tensor& tokens, int64_t rows, double scale, int64_t ignore_index) {
@@ -456,35 +493,39 @@ Tensor embedding_backward_autograd(const Tensor& grad, const Tensor& tokens, int
 // Bytes of a tensor's first element behind a 16-byte boundary (its storage starts on one; a fake tensor has no address).
 int64_t behind_boundary(const Tensor& t) { return t.storage_offset() * (int64_t)t.element_size() & 15; }
 
-struct LayerNorm : torch::autograd::Function<LayerNorm> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        auto [y, stats] = layer_norm().call(x, weight, bias, eps, true);
-        // the bias only says whether it has a gradient, and of which shape
-        ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), stats});
-        ctx->saved_data["behind"] = behind_boundary(x);
-        ctx->mark_non_differentiable({stats});
-        ctx->set_materialize_grads(false);
-        return {y, stats};
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list up) {
-        if (!up[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        variable_list kept = ctx->get_saved_variables();
+struct LayerNormBackward : Saving {
+    using Saving::Saving;
+    int64_t behind;
+    std::string name() const override { return "LayerNormBackward"; }
+    variable_list apply(variable_list&& up) override {
+        if (!up[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        variable_list kept = unpack();          // x, weight, bias (says only whether there is one, and of which shape), statistics
         // a saved-tensor hook may move x off the boundary it was on; the sums have the order of aligned rows all the same
-        if (behind_boundary(kept[0]) && !ctx->saved_data["behind"].toInt()) kept[0] = kept[0].clone();
-        const bool wx = ctx->needs_input_grad(0), ww = kept[1].defined() && ctx->needs_input_grad(1), wb = kept[2].defined() && ctx->needs_input_grad(kept[1].defined() ? 2 : 1);
+        if (behind_boundary(kept[0]) && !behind) kept[0] = kept[0].clone();
+        const bool wx = task_should_compute_output(0), ww = kept[1].defined() && task_should_compute_output(1), wb = kept[2].defined() && task_should_compute_output(2);
         auto [dx, dw, db] = layer_norm_backward().call(up[0], kept[0], maybe(kept[1]), maybe(kept[2]), kept[3], wx, ww, wb);
-        return {wx ? dx : Tensor(), ww ? dw : Tensor(), wb ? db : Tensor(), Tensor()};
+        return {wx ? dx : Tensor(), ww ? dw : Tensor(), wb ? db : Tensor()};
     }
 };
 
 std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps, bool save) {
-    if (at::GradMode::is_enabled() && (needs(x) || needs(weight) || needs(bias))) {
-        variable_list r = LayerNorm::apply(x, weight, bias, eps);
-        return {r[0], r[1]};
+    no_tangent(x);
+    no_tangent(weight);
+    no_tangent(bias);
+    const bool grad = at::GradMode::is_enabled() && (needs(x) || needs(weight) || needs(bias));
+    std::tuple<Tensor, Tensor> r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        r = layer_norm().call(x, weight, bias, eps, save || grad);
     }
-    at::AutoDispatchBelowADInplaceOrView below;
-    return layer_norm().call(x, weight, bias, eps, save);
+    if (grad) {
+        const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+        auto node = make_node<LayerNormBackward>(x, w, b);
+        node->behind = behind_boundary(x);
+        for (const Tensor& t : {x, w, b, std::get<1>(r)}) node->save(t);
+        torch::autograd::create_gradient_edge(std::get<0>(r), node);
+    }
+    return r;
 }
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& grad, const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, const Tensor& stats,
@@ -498,34 +539,35 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& gr
     return r;
 }
 
-struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top, double temperature, int64_t ignore_index) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        auto [lp, ent, top_lp, top_tok, stats] = token_logprobs().call(logits, tokens, top, temperature, ignore_index, true);
-        ctx->save_for_backward({logits, tokens, stats});
-        ctx->saved_data["temperature"] = temperature;
-        ctx->saved_data["ignore"] = ignore_index;
-        ctx->mark_non_differentiable({top_lp, top_tok, stats});
-        ctx->set_materialize_grads(false);
-        return {lp, ent, top_lp, top_tok, stats};
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list up) {
-        Tensor dx;
-        if (up[0].defined() || up[1].defined()) {
-            const variable_list kept = ctx->get_saved_variables();
-            dx = token_logprobs_backward().call(maybe(up[0]), maybe(up[1]), kept[0], kept[1], kept[2], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt());
-        }
-        return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+struct TokenLogprobsBackward : Saving {
+    using Saving::Saving;
+    double temperature;
+    int64_t ignore_index;
+    std::string name() const override { return "TokenLogprobsBackward"; }
+    variable_list apply(variable_list&& up) override {
+        if ((!up[0].defined() && !up[1].defined()) || !task_should_compute_output(0)) return {Tensor()};
+        const variable_list kept = unpack();
+        return {token_logprobs_backward().call(maybe(up[0]), maybe(up[1]), kept[0], kept[1], kept[2], temperature, ignore_index)};
     }
 };
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const Tensor& tokens, int64_t top, double temperature, int64_t ignore_index, bool save) {
-    if (at::GradMode::is_enabled() && needs(logits)) {
-        variable_list r = TokenLogprobs::apply(logits, tokens, top, temperature, ignore_index);
-        return {r[0], r[1], r[2], r[3], r[4]};
+    no_tangent(logits);
+    const bool grad = at::GradMode::is_enabled() && needs(logits);
+    std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> r;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        r = token_logprobs().call(logits, tokens, top, temperature, ignore_index, save || grad);
     }
-    at::AutoDispatchBelowADInplaceOrView below;
-    return token_logprobs().call(logits, tokens, top, temperature, ignore_index, save);
+    if (grad) {
+        auto node = make_node<TokenLogprobsBackward>(logits);
+        node->temperature = temperature;
+        node->ignore_index = ignore_index;
+        for (const Tensor& t : {logits, tokens, std::get<4>(r)}) node->save(t);
+        torch::autograd::create_gradient_edge(std::get<0>(r), node);
+        torch::autograd::create_gradient_edge(std::get<1>(r), node);
+    }
+    return r;
 }
 
 Tensor token_logprobs_backward_autograd(const optional<Tensor>& dlogprob, const optional<Tensor>& dentropy, const Tensor& logits, const Tensor& tokens, const Tensor& stats,
