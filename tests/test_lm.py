@@ -622,6 +622,9 @@ def test_refusals():
             (lambda: fr.token_logprobs(x, t.cpu()), "one CUDA device"), (lambda: fr.token_logprobs(x.to(torch.float8_e4m3fn), t), "float32, bfloat16 or float16")]:
         with pytest.raises(RuntimeError, match=why):
             call()
+    import torch.autograd.forward_ad as ad
+    with ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        fr.layer_norm(ad.make_dual(x, torch.ones_like(x)))
     with pytest.raises(RuntimeError, match="storage"):
         cut = rand(6, 8)
         cut.untyped_storage().resize_(64)
