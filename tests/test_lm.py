@@ -195,6 +195,18 @@ def test_layer_norm_of_heads(B, T, H, D, kind, io, par):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("io,par", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("rows,H,D", [(700, 1, 601), (90, 3, 1016), (350, 1, 1801), (30, 2, 2040), (310, 1, 3601), (20, 2, 4088), (9, 3, 1100), (300, 1, 2561), (5, 2, 6001)])
+def test_layer_norm_of_several_warps(rows, H, D, io, par):
+    """Rows of more than one warp: whole blocks and groups of 64, 128 and 256 lanes, even, odd and sliced, more rows than groups."""
+    w, b = params("heads" if H > 1 else "vector", H, D, par)
+    x, dy = (0.5 + rand(rows, H, D)).to(io), rand(rows, H, D, seed=2).to(io)
+    layer_norm_check(x, w, b, dy)
+    layer_norm_check((rand(rows, H, D + 5, seed=6) - 0.5).to(io)[..., 5:], w, b, dy)
+    layer_norm_check(x.view(rows * H, D), *params("vector", 1, D, par), dy.view(rows * H, D))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["heads", "vector"])
 def test_layer_norm_layouts(kind):
     B, T, H, D = 2, 6, 3, 64
