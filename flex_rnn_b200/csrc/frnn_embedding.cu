@@ -534,11 +534,9 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
     if (n == 0) return FRNN_OK;
     const uint2* sorted = pairs + (plan.passes & 1) * n;
     const bool alike = width * size % 16 == 0 && on_boundary(dout, 16) && on_boundary(dweight, 16);
-    return with_access(dtype, alike ? ALIKE : APART, [&](auto t, auto a) {
+    return with_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
-        if constexpr (a.value == ELEMENTS) {
-            return (int)FRNN_E_ARG;                        // (no call comes here)
-        } else {
+        auto run = [&](auto a) {
             const Shape shape = shape_of<T, a.value>(width);
             if (int rc = launch("frnn_embedding_backward", embedding_sums<T, a.value>, dim3((unsigned)((plan.chunks + shape.groups - 1) / shape.groups), shape.parts), BLOCK, 0, st, true, 1,
                                 (const T*)dout, sorted, (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, part, shape))
@@ -546,7 +544,8 @@ int frnn_embedding_backward(int dtype, const void* dout, const void* tokens, int
             if (plan.chunks < 2) return (int)FRNN_OK;
             return launch("frnn_embedding_backward", embedding_join<T>, dim3((unsigned)((plan.chunks + JOINED - 1) / JOINED), (unsigned)((width + 255) / 256)), BLOCK, 0, st, true, 1, sorted,
                           (int)n, (unsigned)rows, (int)width, plan.chunk, scale, (T*)dweight, (const float*)part);
-        }
+        };
+        return alike ? run(std::integral_constant<Access, ALIKE>()) : run(std::integral_constant<Access, APART>());
     });
 }
 

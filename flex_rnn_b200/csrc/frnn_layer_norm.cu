@@ -73,11 +73,11 @@ template <class T, Access A> struct Columns {
     // the whole of access j is there
     __device__ __forceinline__ bool whole(int j) const { return A == WIDE_APART ? at[j] >= 0 && at[j] + E <= width : at[j] < width; }
     __device__ __forceinline__ bool there(int j, int e) const { return A == WIDE_APART ? at[j] + e >= 0 && at[j] + e < width : at[j] < width; }
+    // (single elements: nothing else is loaded without a ring)
     __device__ __forceinline__ void load(Pack<T, E>* v, const T* row) const {
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             if (whole(j)) v[j].load(row + at[j]);
-            else if (A == WIDE_APART) load_part(v[j], row, at[j], width);
             else v[j].zero();
         }
     }
@@ -423,17 +423,19 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
     bool write = true;
     if (staged) {
         int place = seat.place;
-        if (merged && L && L < 32 && A != WIDE_APART) {         // the groups of a warp hold the same columns
+        if constexpr (L && L < 32 && A != WIDE_APART) {
+            if (merged) {                                  // the groups of a warp hold the same columns
 #pragma unroll
-            for (int o = L ? L : 32; o < 32; o *= 2)
+                for (int o = L; o < 32; o *= 2)
 #pragma unroll
-                for (int k = 0; k < PER_LANE / 2; k++) {
-                    dw[k] = add2(dw[k], make_float2(__shfl_xor_sync(~0u, dw[k].x, o), __shfl_xor_sync(~0u, dw[k].y, o)));
-                    db[k] = add2(db[k], make_float2(__shfl_xor_sync(~0u, db[k].x, o), __shfl_xor_sync(~0u, db[k].y, o)));
-                }
-            place = threadIdx.x / 32;
-            places = BLOCK / 32;
-            write = threadIdx.x % 32 < (L ? L : 1);
+                    for (int k = 0; k < PER_LANE / 2; k++) {
+                        dw[k] = add2(dw[k], make_float2(__shfl_xor_sync(~0u, dw[k].x, o), __shfl_xor_sync(~0u, dw[k].y, o)));
+                        db[k] = add2(db[k], make_float2(__shfl_xor_sync(~0u, db[k].x, o), __shfl_xor_sync(~0u, db[k].y, o)));
+                    }
+                place = threadIdx.x / 32;
+                places = BLOCK / 32;
+                write = threadIdx.x % 32 < L;
+            }
         }
         __syncthreads();                                   // the rows' shared memory takes the sums
         to = (float*)shared + 2 * place * pitch;
@@ -442,21 +444,21 @@ __global__ void __launch_bounds__(L ? BLOCK : MOST_THREADS, L ? 2 : 1) layer_nor
 #pragma unroll
         for (int j = 0; j < C::NV; j++) {
             const float *pw = &dw[0].x + j * C::E, *pb = &db[0].x + j * C::E;
-            if (A == WIDE_ALIKE) {                         // (widths of multiples of 8)
+            if constexpr (A == WIDE_ALIKE) {               // (widths of multiples of 8)
                 if (cols.whole(j))
 #pragma unroll
                     for (int e = 0; e < C::E; e += 4) {
                         *(float4*)(to + cols.at[j] + e) = make_float4(pw[e], pw[e + 1], pw[e + 2], pw[e + 3]);
                         *(float4*)(to + pitch + cols.at[j] + e) = make_float4(pb[e], pb[e + 1], pb[e + 2], pb[e + 3]);
                     }
-                continue;
-            }
+            } else {
 #pragma unroll
-            for (int e = 0; e < C::E; e++)
-                if (cols.there(j, e)) {
-                    to[cols.at[j] + e] = pw[e];
-                    to[pitch + cols.at[j] + e] = pb[e];
-                }
+                for (int e = 0; e < C::E; e++)
+                    if (cols.there(j, e)) {
+                        to[cols.at[j] + e] = pw[e];
+                        to[pitch + cols.at[j] + e] = pb[e];
+                    }
+            }
         }
     if (!staged) return;
     __syncthreads();

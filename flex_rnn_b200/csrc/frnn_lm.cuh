@@ -122,17 +122,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// The E elements at p + at, of which those with 0 <= at + e < n are there; the others read as zero.
-template <class T, int E> __device__ __forceinline__ void load_part(Pack<T, E>& v, const T* p, int at, int n) {
-    if (at >= 0 && at + E <= n) {
-        v.load(p + at);
-    } else {
-        v.zero();
-#pragma unroll
-        for (int e = 0; e < E; e++)
-            if (at + e >= 0 && at + e < n) v.set(e, p[at + e]);
-    }
-}
+// Stores of the E elements at p + at those with 0 <= at + e < n.
 template <class T, int E> __device__ __forceinline__ void store_part(const Pack<T, E>& v, T* p, int at, int n) {
     if (at >= 0 && at + E <= n) {
         v.store(p + at);

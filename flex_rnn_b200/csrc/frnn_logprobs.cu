@@ -23,7 +23,7 @@ namespace {
 enum { LOADS = 4, MOST_CLUSTER = 8 };
 // A row, or a cluster block's part of it, belongs to a block of 256 threads, or of 32 where rows are short.
 template <int N> struct Block {
-    static constexpr int THREADS = N, WARPS = N / 32, GROUPS = N < 64 ? N : 64, MOST = N < 256 ? 512 : 1024;      // MOST: candidates
+    static constexpr int WARPS = N / 32, GROUPS = N < 64 ? N : 64, MOST = N < 256 ? 512 : 1024;      // MOST: candidates
 };
 constexpr float NIL = -512.f;      // 2^NIL is 0 in 32 bits; finite, so that 0 * log 0 is 0
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
