@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(N, N < 256 ? 32 : 4) logprobs_fw(const T* __re
             const float d = max_nan((m - b) * c, NIL), r = exp2_fast(d);
             t = mul2(fma2(s, both(d), t), both(r));
             s = mul2(s, both(r));
-            m = b;
-            m0 = b == -INFINITY ? 0.f : b;
+            m = max_nan(m, b);                             // (a NaN stays, whatever comes after it)
+            m0 = m == -INFINITY ? 0.f : m;
         }
         const float2 from = both(-m0);
 #pragma unroll
