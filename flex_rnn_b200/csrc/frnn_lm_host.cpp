@@ -447,6 +447,7 @@ template <class N, class... T> std::shared_ptr<N> make_node(const T&... inputs) 
     return std::shared_ptr<N>(new N(torch::autograd::collect_next_edges(inputs...)), torch::autograd::deleteNode);
 }
 
+// Forward and backward refuse what would otherwise be dropped without a word: a tangent may come on an upstream gradient alone.
 void no_tangent(const optional<Tensor>& t) {
     TORCH_CHECK(!t.has_value() || !t->defined() || !t->_fw_grad(0).defined(), "flex_rnn_b200: forward-mode derivatives of this operator are not built");
 }
@@ -481,6 +482,7 @@ Tensor embedding_autograd(const Tensor& tokens, const Tensor& weight, double sca
 }
 
 Tensor embedding_backward_autograd(const Tensor& grad, const Tensor& tokens, int64_t rows, double scale, int64_t ignore_index) {
+    no_tangent(grad);
     Tensor dw;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -530,6 +532,9 @@ std::tuple<Tensor, Tensor> layer_norm_autograd(const Tensor& x, const optional<T
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& grad, const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, const Tensor& stats,
                                                                 bool want_x, bool want_weight, bool want_bias) {
+    no_tangent(grad);
+    no_tangent(x);
+    no_tangent(weight);
     std::tuple<Tensor, Tensor, Tensor> r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -572,6 +577,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autograd(const
 
 Tensor token_logprobs_backward_autograd(const optional<Tensor>& dlogprob, const optional<Tensor>& dentropy, const Tensor& logits, const Tensor& tokens, const Tensor& stats,
                                         double temperature, int64_t ignore_index) {
+    no_tangent(dlogprob);
+    no_tangent(dentropy);
+    no_tangent(logits);
     Tensor dx;
     {
         at::AutoDispatchBelowADInplaceOrView below;

@@ -3,8 +3,10 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as ad
 
 import flex_rnn_b200 as fr
+from flex_rnn_b200 import lm
 from test_lm import DTYPES
 
 
@@ -38,3 +40,32 @@ def test_nan_among_masked_logits(n, V, dtype):
     assert torch.equal(r.top_logprob.isnan().all(1), bad) and torch.equal(g.isnan().all(1), bad)
     assert (r.logprob[~bad] == -math.inf).all() and not r.entropy[~bad].any() and not g[~bad].any()
     assert r.top_token[0].tolist() == [3, 0, 1, 2] and r.top_token[1].tolist() == [0, 7, 1, 2] and r.top_token[2].tolist() == [0, 1, 2, 3]
+
+
+# ---- forward-mode derivatives ------------------------------------------------------------------------------------------------
+
+def on_meta(name):
+    """(function of its leaf, the leaf, shapes of its differentiable results) without a GPU"""
+    lm._operators()
+    t, x = torch.zeros(3, dtype=torch.int64, device="meta"), torch.empty(3, 8, device="meta")
+    return {"embedding": (lambda w: (fr.embedding(t, w),), torch.empty(5, 8, device="meta"), [(3, 8)]), "layer_norm": (lambda x: (fr.layer_norm(x),), x, [(3, 8)]),
+            "token_logprobs": (lambda x: fr.token_logprobs(x, t)[:2], x, [(3,), (3,)])}[name]
+
+
+@pytest.mark.parametrize("name", ["embedding", "layer_norm", "token_logprobs"])
+def test_tangent_on_an_upstream_gradient(name):
+    """Refused, not dropped; dual levels and functional transforms without one go through."""
+    f, leaf, shapes = on_meta(name)
+    for k in range(len(shapes)):
+        with ad.dual_level():
+            x = leaf.clone().requires_grad_()
+            up = [torch.empty(s, device="meta") for s in shapes]
+            assert torch.autograd.grad(f(x), x, up)[0].shape == leaf.shape
+            up[k] = ad.make_dual(up[k], torch.empty_like(up[k]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(f(x), x, up)
+    h = torch.empty(shapes[0], device="meta")
+    gradient = lambda h: torch.func.grad(lambda x: (f(x)[0] * h).sum())(leaf)
+    assert gradient(h).shape == leaf.shape
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(gradient, (h,), (torch.empty_like(h),))
