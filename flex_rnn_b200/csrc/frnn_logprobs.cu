@@ -275,7 +275,7 @@ template <class T, int E, int N> __device__ void block_top(const Row<T, E>& row,
             if (threadIdx.x == 0) c.count = above + have;
             __syncthreads();
         } else {                           // more than there is room for: one alternative after the other
-            Key last = ~0ull;
+            Key last = 0;                  // (none before the first: a NaN of token 0 has the largest key that there is)
             for (int i = threadIdx.x; i < FRNN_MAX_TOP; i += N) best[i] = 0;
             for (int k = 0; k < top; k++) {
                 Key b = 0;
@@ -287,7 +287,7 @@ template <class T, int E, int N> __device__ void block_top(const Row<T, E>& row,
 #pragma unroll
                     for (int e = 0; e < E; e++) {
                         const Key key = key_of(f[e], row.at(a) + e);
-                        if (row.there(a, e) && key < last && key > b) b = key;
+                        if (row.there(a, e) && (k == 0 || key < last) && key > b) b = key;
                     }
                 }
 #pragma unroll

@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as ad
 
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm
-from test_lm import DTYPES
+from test_lm import DTYPES, logits_of, logprobs_check
 
 
 # ---- log probabilities: NaN --------------------------------------------------------------------------------------------------
@@ -40,6 +40,40 @@ def test_nan_among_masked_logits(n, V, dtype):
     assert torch.equal(r.top_logprob.isnan().all(1), bad) and torch.equal(g.isnan().all(1), bad)
     assert (r.logprob[~bad] == -math.inf).all() and not r.entropy[~bad].any() and not g[~bad].any()
     assert r.top_token[0].tolist() == [3, 0, 1, 2] and r.top_token[1].tolist() == [0, 7, 1, 2] and r.top_token[2].tolist() == [0, 1, 2, 3]
+
+
+def few_threads(n, V, dtype, threads, block, seed=0):
+    """Logits of which only the accesses (16 bytes) of a few of a block's threads are large, so that next to no group of
+    threads holds a large one and the bound for candidates lets most of theirs through."""
+    x, t = logits_of(n, V, dtype, seed=seed)
+    access = torch.arange(V, device="cuda") // (128 // torch.finfo(dtype).bits)
+    return torch.where(access % block < threads, x + 40.0, x - 40.0).to(dtype), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_of_few_threads(dtype):
+    """More candidates than there is room for, all of them distinct in rank: one block, a cluster, one warp a row."""
+    logprobs_check(*few_threads(300, 40000, dtype, 16, 256), top=8)
+    logprobs_check(*few_threads(3, 200000, dtype, 16, 256), top=8)
+    logprobs_check(*few_threads(1300, short_row(dtype), dtype, 9, 32), top=12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_of_nan(dtype):
+    """NaN comes before every number and by the lowest token, token 0 among them, also where candidates are too many."""
+    for (n, V, threads, block, top) in [(300, 40000, 16, 256, 8), (3, 200000, 16, 256, 8), (1300, short_row(dtype), 9, 32, 12), (3, 900, 9, 256, 12)]:
+        x, t = few_threads(n, V, dtype, threads, block)
+        best = x[0].sort(descending=True, stable=True).indices[:top].tolist()
+        x[0, 0] = math.nan
+        x[1] = math.nan
+        x[2, 5], x[2, V - 2] = math.nan, math.nan
+        r = fr.token_logprobs(x, t, top=top)
+        assert r.top_token[0].tolist() == ([0] + [i for i in best if i != 0])[:top]
+        assert r.top_token[1].tolist() == list(range(top))
+        assert r.top_token[2, :2].tolist() == [5, V - 2]
+        assert r.top_logprob[:3].isnan().all() and r.top_logprob[3:].isfinite().all()
 
 
 # ---- forward-mode derivatives ------------------------------------------------------------------------------------------------
