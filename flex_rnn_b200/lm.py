@@ -16,22 +16,24 @@ import torch as th
 #: The most alternatives that ``token_logprobs`` returns for a row (FRNN_MAX_TOP of include/frnn.h).
 MAX_TOP = 32
 
-_ops = None
+_ops = th.ops.flex_rnn_b200
+_loaded = False
 _lock = threading.Lock()
 
 
+# (under torch.compile this runs while a call is traced and counts as a constant: the first use of an operator may be a
+# compiled one, and a tracer can neither enter the lock nor load a library)
+@th.compiler.assume_constant_result
 def _operators():
-    """The operators of the native host library, loaded on first use."""
-    global _ops
-    from . import runtime
-    with _lock:
-        if _ops is not None:
-            return _ops
-        runtime.host()
-        _register_fakes()
-        ops = th.ops.flex_rnn_b200
-        _ops = (ops.embedding.default, ops.layer_norm.default, ops.token_logprobs.default)
-        return _ops
+    """Load the operators of the native host library, once."""
+    global _loaded
+    if not _loaded:
+        from . import runtime
+        with _lock:
+            if not _loaded:
+                runtime.host()
+                _register_fakes()
+                _loaded = True
 
 
 class TokenLogprobs(NamedTuple):
@@ -48,7 +50,8 @@ def embedding(tokens: th.Tensor, weight: th.Tensor, scale: float = 1.0, ignore_i
     vocabulary gives zeros too and is reported: the next call on that GPU raises ``FrnnError`` (no call waits for the GPU
     to look).  The gradient of ``weight`` is dense and sums each token's rows in the order of their places in 32 bits, so
     it is the same in every run."""
-    return (_ops or _operators())[0](tokens, weight, scale, ignore_index)
+    _operators()
+    return _ops.embedding.default(tokens, weight, scale, ignore_index)
 
 
 def layer_norm(x: th.Tensor, weight: Optional[th.Tensor] = None, bias: Optional[th.Tensor] = None, eps: float = 1e-5) -> th.Tensor:
@@ -57,7 +60,8 @@ def layer_norm(x: th.Tensor, weight: Optional[th.Tensor] = None, bias: Optional[
     ``weight`` and ``bias`` are [width], or [heads, width] for ``x`` [..., heads, width] (a norm of each head, as on the
     output [B,T,H,M] of a scan), of the type of ``x`` or fp32.  ``x`` may have any strides; layouts whose rows are not
     runs of consecutive elements, or that need more than three strides between rows, are copied first."""
-    return (_ops or _operators())[1](x, weight, bias, eps, False)[0]
+    _operators()
+    return _ops.layer_norm.default(x, weight, bias, eps, False)[0]
 
 
 def token_logprobs(logits: th.Tensor, tokens: th.Tensor, top: int = 0, temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
@@ -69,7 +73,8 @@ def token_logprobs(logits: th.Tensor, tokens: th.Tensor, top: int = 0, temperatu
     probability 0 and no gradient through it; tokens outside the vocabulary have NaN, and the next call on that GPU raises
     ``FrnnError``.  ``logprob`` and ``entropy`` are differentiable; the alternatives carry no gradient.  A NaN logit, or
     +inf, makes its row's results NaN."""
-    return TokenLogprobs(*(_ops or _operators())[2](logits, tokens, top, temperature, ignore_index, False)[:4])
+    _operators()
+    return TokenLogprobs(*_ops.token_logprobs.default(logits, tokens, top, temperature, ignore_index, False)[:4])
 
 
 # ---- definitions ---------------------------------------------------------------------------------------------------------

@@ -1,5 +1,7 @@
 """Calls of the operators around the scans (flex_rnn_b200.lm) at their edges; tolerances are those of test_lm."""
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -7,6 +9,7 @@ import torch.autograd.forward_ad as ad
 
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm
+from conftest import ROOT
 from test_lm import DTYPES, logits_of, logprobs_check
 
 
@@ -103,3 +106,30 @@ def test_tangent_on_an_upstream_gradient(name):
     assert gradient(h).shape == leaf.shape
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(gradient, (h,), (torch.empty_like(h),))
+
+
+# ---- torch.compile -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("name", ["embedding", "layer_norm", "token_logprobs"])
+def test_first_use_is_a_compiled_one(name):
+    """A process whose first use of an operator is traced whole gets as far as the operator itself, which refuses the CPU;
+    on meta tensors the compiled call gives a result, and again without another compilation."""
+    program = f"""
+import torch, flex_rnn_b200 as fr
+def make(device):
+    t, w, x = torch.zeros(2, 3, dtype=torch.int64, device=device), torch.zeros(5, 8, device=device), torch.zeros(2, 3, 8, device=device)
+    return dict(embedding=(t, w), layer_norm=(x,), token_logprobs=(x, t))["{name}"]
+graphs = []
+compiled = torch.compile(lambda *a: fr.{name}(*a), fullgraph=True, backend=lambda g, _: graphs.append(g) or g)
+try:
+    compiled(*make("cpu"))
+except RuntimeError as e:
+    print("refused" if "CUDA tensors" in str(e) else e)
+graphs.clear()           # (the CPU call's)
+for _ in range(2):
+    r = compiled(*make("meta"))
+print(tuple(r.shape) if torch.is_tensor(r) else tuple(r.logprob.shape), len(graphs))
+"""
+    r = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, cwd=ROOT, timeout=600)
+    shape = {"embedding": (2, 3, 8), "layer_norm": (2, 3, 8), "token_logprobs": (2, 3)}[name]
+    assert r.stdout.splitlines() == ["refused", f"{shape} 1"], r.stdout + r.stderr[-2000:]
