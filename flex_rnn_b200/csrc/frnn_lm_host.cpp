@@ -492,8 +492,9 @@ Tensor embedding_backward_autograd(const Tensor& grad, const Tensor& tokens, int
     return dw;
 }
 
-// Bytes of a tensor's first element behind a 16-byte boundary (its storage starts on one; a fake tensor has no address).
-int64_t behind_boundary(const Tensor& t) { return t.storage_offset() * (int64_t)t.element_size() & 15; }
+// Bytes of a tensor's first element behind a 16-byte boundary (its storage starts on one; a fake tensor has no address, and
+// an offset that is symbolic while a call is traced does not matter: no hook moves what is saved there).
+int64_t behind_boundary(const Tensor& t) { return t.sym_storage_offset().maybe_as_int().value_or(0) * (int64_t)t.element_size() & 15; }
 
 struct LayerNormBackward : Saving {
     using Saving::Saving;

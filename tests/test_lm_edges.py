@@ -10,7 +10,7 @@ import torch.autograd.forward_ad as ad
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm
 from conftest import ROOT
-from test_lm import DTYPES, logits_of, logprobs_check
+from test_lm import DTYPES, both, logits_of, logprobs_check
 
 
 # ---- log probabilities: NaN --------------------------------------------------------------------------------------------------
@@ -133,3 +133,38 @@ print(tuple(r.shape) if torch.is_tensor(r) else tuple(r.logprob.shape), len(grap
     r = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, cwd=ROOT, timeout=600)
     shape = {"embedding": (2, 3, 8), "layer_norm": (2, 3, 8), "token_logprobs": (2, 3)}[name]
     assert r.stdout.splitlines() == ["refused", f"{shape} 1"], r.stdout + r.stderr[-2000:]
+
+
+def of_batch(name, b, device):
+    """(function, its leaves, upstream gradients) for a batch of b"""
+    t = (torch.arange(7 * b, device=device) * 5 % 11).view(b, 7)
+    one = lambda *s: torch.linspace(-2, 3, math.prod(s), device=device).sin().view(s)
+    leaf = lambda *s: one(*s).requires_grad_()
+    return {"embedding": (lambda w: (fr.embedding(t, w),), [leaf(11, 24)], [one(b, 7, 24)]),
+            "layer_norm": (lambda x, w: (fr.layer_norm(x, w),), [leaf(b, 7, 24), leaf(24)], [one(b, 7, 24)]),
+            "sliced layer_norm": (lambda x: (fr.layer_norm(x[1:, :, 3:]),), [leaf(b, 7, 24)], [one(b - 1, 7, 21)]),
+            "token_logprobs": (lambda x: fr.token_logprobs(x, t, top=2)[:2], [leaf(b, 7, 11)], [one(b, 7), one(b, 7)])}[name]
+
+
+OF_BATCH = ["embedding", "layer_norm", "sliced layer_norm", "token_logprobs"]
+
+
+@pytest.mark.parametrize("name", OF_BATCH)
+def test_symbolic_sizes(name):
+    """Traced with symbolic sizes, with gradients, whole and sliced layouts."""
+    lm._operators()
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda f, a: f(*a), fullgraph=True, backend="aot_eager", dynamic=True)
+    for b in (6, 7, 9):
+        f, leaves, up = of_batch(name, b, "meta")
+        assert [g.shape for g in torch.autograd.grad(compiled(f, leaves), leaves, up)] == [v.shape for v in leaves]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", OF_BATCH)
+def test_compiled_for_any_batch(name):
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda f, a: f(*a), fullgraph=True, dynamic=True)
+    for b in (6, 7, 9):
+        f, leaves, up = of_batch(name, b, "cuda")
+        assert all(torch.equal(a, g) for a, g in zip(both(lambda *a: compiled(f, a), leaves, up), both(f, leaves, up)))
