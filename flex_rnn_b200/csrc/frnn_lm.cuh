@@ -9,6 +9,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <cstring>
+#include <mutex>
 
 #include "../../include/frnn.h"
 
@@ -197,15 +198,19 @@ inline int sm_count() {
     return n;
 }
 
-// Shared memory beyond 48 KB has to be allowed for a kernel, once a device.
+// Shared memory beyond 48 KB has to be allowed for a kernel, once a device.  Sizes differ from launch to launch: the lock
+// keeps a thread that asks for less from setting the attribute back after one that asks for more.
 template <auto KERNEL> inline bool allow_shared(size_t bytes) {
     static std::atomic<size_t> allowed[64];
+    static std::mutex setting;
     int dev = 0;
     if (bytes <= 40 * 1024) return true;             // (with what the kernel has besides)
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (allowed[dev].load(std::memory_order_acquire) >= bytes) return true;
+    std::lock_guard<std::mutex> lock(setting);
     if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return true;
     if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
-    allowed[dev].store(bytes, std::memory_order_relaxed);
+    allowed[dev].store(bytes, std::memory_order_release);
     return true;
 }
 

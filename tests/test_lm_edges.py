@@ -1,5 +1,6 @@
 """Calls of the operators around the scans (flex_rnn_b200.lm) at their edges; tolerances are those of test_lm."""
 import math
+import os
 import subprocess
 import sys
 
@@ -8,9 +9,9 @@ import torch
 import torch.autograd.forward_ad as ad
 
 import flex_rnn_b200 as fr
-from flex_rnn_b200 import lm
+from flex_rnn_b200 import build, lm
 from conftest import ROOT
-from test_lm import DTYPES, both, logits_of, logprobs_check
+from test_lm import DTYPES, both, calls, logits_of, logprobs_check
 
 
 # ---- log probabilities: NaN --------------------------------------------------------------------------------------------------
@@ -168,3 +169,90 @@ def test_compiled_for_any_batch(name):
     for b in (6, 7, 9):
         f, leaves, up = of_batch(name, b, "cuda")
         assert all(torch.equal(a, g) for a, g in zip(both(lambda *a: compiled(f, a), leaves, up), both(f, leaves, up)))
+
+
+# ---- shared memory beyond 48 KB ------------------------------------------------------------------------------------------------
+
+ALLOW_SHARED = r"""
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <chrono>
+#include <cstdio>
+#include <thread>
+
+static std::atomic<size_t> permitted{0};        // what the kernel's attribute says
+static cudaError_t set_attribute(size_t bytes, bool slow) {
+    permitted = bytes;
+    if (slow) std::this_thread::sleep_for(std::chrono::milliseconds(400));
+    return cudaSuccess;
+}
+#define cudaGetDevice(d) (*(d) = 0, cudaSuccess)
+#define cudaFuncSetAttribute(kernel, which, bytes) set_attribute(bytes, (bytes) > 100000)
+#include "frnn_lm.cuh"
+
+__global__ void kernel() {}
+int frnn_fail(int code, const char*, ...) { return code; }
+
+int main() {
+    std::thread large([] { frnn_lm::allow_shared<kernel>(200000); });
+    std::this_thread::sleep_for(std::chrono::milliseconds(100));
+    std::thread small([] { frnn_lm::allow_shared<kernel>(90000); });
+    large.join();
+    small.join();
+    const bool ok = frnn_lm::allow_shared<kernel>(200000);
+    printf("%d %d\n", ok, permitted >= 200000);
+}
+"""
+
+
+def test_shared_memory_of_two_threads(tmp_path):
+    """A kernel is launched with sizes that differ: a thread that asks for less while another asks for more leaves the kernel
+    with what the record says.  The runtime's two calls are stand-ins, so no device is needed."""
+    source, program = tmp_path / "allow.cu", tmp_path / "allow"
+    source.write_text(ALLOW_SHARED)
+    subprocess.run([build.nvcc_path(), "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I", os.path.join(ROOT, "flex_rnn_b200", "csrc"), "-o", str(program), str(source)], check=True)
+    assert subprocess.run([str(program)], capture_output=True, text=True, check=True).stdout.split() == ["1", "1"]
+
+
+# ---- all of them --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["embedding", "layer_norm", "token_logprobs"])
+def test_threads(name):
+    """Calls from several threads, each on a stream of its own, give what one thread gives."""
+    import threading
+    f, leaves, up = calls()[name]
+    want = both(f, leaves, up)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        try:
+            mine, side = [v.detach().clone().requires_grad_() for v in leaves], torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(20):
+                    got = both(f, mine, up)
+                    side.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                        wrong.append("other results")
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+def test_repeated_alternatives_give_the_same_bits():
+    """Candidates are listed in whatever order threads come; their ranks, and joins of a cluster, do not show it."""
+    for n, V in [(2, 200001), (400, 32003), (1300, 1000)]:
+        x, t = logits_of(n, V, torch.bfloat16)
+        want = fr.token_logprobs(x, t, top=32)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(fr.token_logprobs(x, t, top=32), want))
