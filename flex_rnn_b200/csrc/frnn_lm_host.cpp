@@ -310,7 +310,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_cuda(const Tensor& grad, 
     const Tensor st = saved(stats);
     auto param = [&](bool want, const optional<Tensor>& p) { return want && p.has_value() && p->defined() ? make("a weight's gradient", p->sizes(), p->scalar_type(), x) : Tensor(); };
     Tensor dw = param(want_weight, weight), db = param(want_bias, bias);
-    if (x.size(-1)) {
+    if (x.size(-1) && r.heads) {                           // (without a head the weights have no element either)
         const Tensor work = dw.defined() || db.defined() ? workspace(g_layer_norm_backward_workspace(&r), x) : Tensor();
         ran(g_layer_norm_backward(&r, dtype, g.data_ptr(), from.data_ptr(), ptype, ptr(w), st.data_ptr<float>(), want_x ? to.data_ptr() : nullptr, ptr(dw), ptr(db), ptr(work),
                                   stream_of(x)), x);

@@ -80,6 +80,20 @@ def test_alternatives_of_nan(dtype):
         assert r.top_logprob[:3].isnan().all() and r.top_logprob[3:].isfinite().all()
 
 
+# ---- layer norm: no heads --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("guard", ["0", "1"])
+def test_layer_norm_of_no_heads(guard, monkeypatch):
+    """x [B,T,0,D] with weights [0,D], forward and backward; FRNN_GUARD=1 looks for writes into buffers of no element."""
+    monkeypatch.setenv("FRNN_GUARD", guard)
+    x = torch.empty(2, 3, 0, 16, device="cuda", requires_grad=True)
+    w, b = (torch.empty(0, 16, device="cuda", requires_grad=True) for _ in range(2))
+    y = fr.layer_norm(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert y.shape == gx.shape == x.shape and gw.shape == gb.shape == w.shape
+
+
 # ---- forward-mode derivatives ------------------------------------------------------------------------------------------------
 
 def on_meta(name):
