@@ -1,4 +1,5 @@
 """Calls of the operators around the scans (flex_rnn_b200.lm) at their edges; tolerances are those of test_lm."""
+import ctypes
 import math
 import os
 import subprocess
@@ -9,9 +10,9 @@ import torch
 import torch.autograd.forward_ad as ad
 
 import flex_rnn_b200 as fr
-from flex_rnn_b200 import build, lm
+from flex_rnn_b200 import build, lm, runtime
 from conftest import ROOT
-from test_lm import DTYPES, both, calls, logits_of, logprobs_check
+from test_lm import DTYPES, both, calls, layer_norm_check, logits_of, logprobs_check, params, rand
 
 
 # ---- log probabilities: NaN --------------------------------------------------------------------------------------------------
@@ -78,6 +79,36 @@ def test_alternatives_of_nan(dtype):
         assert r.top_token[1].tolist() == list(range(top))
         assert r.top_token[2, :2].tolist() == [5, V - 2]
         assert r.top_logprob[:3].isnan().all() and r.top_logprob[3:].isfinite().all()
+
+
+# ---- layer norm: few rows ------------------------------------------------------------------------------------------------------
+
+def test_layer_norm_workspace_follows_the_rows():
+    """Partial sums of weight gradients: no more than one for each row (with weights for each head: for each group of a block
+    that has a row), however the rows are divided."""
+    L, i64 = runtime.lib(), ctypes.c_int64
+    L.frnn_layer_norm_backward_workspace.restype = ctypes.c_size_t
+
+    def partials(n, width, heads):
+        rows = (i64 * 14)(*n, width, heads, *[0] * 9)
+        return L.frnn_layer_norm_backward_workspace(rows) // (8 * ((width + 3) // 4 * 4))
+
+    for width in (16, 77, 128, 601, 1001, 2047, 4096, 8192):
+        for rows in (*range(1, 300, 2), 1000, 3001):
+            assert partials((1, 1, rows), width, 1) <= rows and partials((rows, 1, 1), width, 1) <= rows
+            for n2 in (3, 32, 101, 127):
+                assert partials((1, rows, n2), width, 1) <= rows * n2 and partials((1, rows, n2), width, n2) <= rows * n2 + 127
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,D", [(1, 127, 4096), (3, 101, 4001), (5, 127, 1025), (11, 101, 72), (2, 1, 4096), (77, 1, 4096), (127, 1, 2047), (100, 1, 640), (7, 125, 77)])
+def test_layer_norm_of_few_rows(T, H, D, dtype):
+    """Fewer rows than groups run at once, or hardly more, and numbers of heads that share no factor with a block's groups."""
+    x, dy = (0.3 + rand(T, H, D)).to(dtype), rand(T, H, D, seed=2).to(dtype)
+    for kind in ("heads", "vector"):
+        layer_norm_check(x, *params(kind, H, D, dtype), dy)
+    layer_norm_check(rand(T, 3, H, D, seed=5).to(dtype)[:, 1], *params("vector", H, D, dtype), dy)
 
 
 # ---- layer norm: no heads --------------------------------------------------------------------------------------------------------
