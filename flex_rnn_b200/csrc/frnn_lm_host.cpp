@@ -218,9 +218,10 @@ bool rows_of(const Tensor* const* t, int count, bool heads, frnn_rows& r) {
     int64_t* size[3] = {&r.n0, &r.n1, &r.n2};
     for (int k = 0; k < 3; k++)
         for (int i = 0; i < 3; i++) to[i][k] = 0;
+    const size_t first = n.size() == 1 && !heads ? 0 : 3 - n.size();      // (one run alone is n0: kernels step through it; n2 is for heads)
     for (size_t k = 0; k < n.size(); k++) {
-        *size[3 - n.size() + k] = n[k];
-        for (int i = 0; i < count; i++) to[i][3 - n.size() + k] = s[i][k];
+        *size[first + k] = n[k];
+        for (int i = 0; i < count; i++) to[i][first + k] = s[i][k];
     }
     r.width = x.size(-1);
     r.heads = heads ? x.size(-2) : 1;

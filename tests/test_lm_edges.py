@@ -111,6 +111,41 @@ def test_layer_norm_of_few_rows(T, H, D, dtype):
     layer_norm_check(rand(T, 3, H, D, seed=5).to(dtype)[:, 1], *params("vector", H, D, dtype), dy)
 
 
+@pytest.mark.gpu
+def test_layer_norm_rows_that_kernels_get():
+    """How rows are handed over: one run of rows as n0, through which kernels step, heads with weights of their own as n2."""
+    class Rows(ctypes.Structure):
+        _fields_ = [(k, ctypes.c_int64) for k in ("n0", "n1", "n2", "width", "heads")] + [(k, ctypes.c_int64 * 3) for k in ("x", "dy", "dx")]
+
+    seen = []
+
+    def forward(rows, *rest):
+        r = rows.contents
+        seen.append((r.n0, r.n1, r.n2, r.width, r.heads, *r.x))
+        return 0
+
+    vp, ci = ctypes.c_void_p, ctypes.c_int
+    callback = ctypes.CFUNCTYPE(ci, ctypes.POINTER(Rows), ci, vp, ci, vp, vp, ctypes.c_float, vp, vp, vp)(forward)
+    host, L = runtime.host(), runtime.lib()
+    address = lambda f: ctypes.cast(f, vp).value
+    entries = {n: address(getattr(L, n)) for n in runtime.SYMBOLS if n.startswith(("frnn_embedding", "frnn_layer_norm", "frnn_token", "frnn_last"))}
+    bind = lambda **other: host.bind_lm({**entries, **other}, runtime._status_word, runtime._status_raise)
+    x, w, h = rand(4, 30, 64), rand(64), rand(5, 64)
+    bind(frnn_layer_norm_forward=address(callback))
+    try:
+        fr.layer_norm(x, w)
+        fr.layer_norm(x[..., 32:])
+        fr.layer_norm(h, w)
+        fr.layer_norm(h, h)
+        fr.layer_norm(x.view(4, 6, 5, 64), h)
+        fr.layer_norm(x[:, 3:])
+        fr.layer_norm(w, w)
+    finally:
+        bind()
+    assert seen == [(120, 1, 1, 64, 1, 64, 0, 0), (120, 1, 1, 32, 1, 64, 0, 0), (5, 1, 1, 64, 1, 64, 0, 0), (1, 1, 5, 64, 5, 0, 0, 64), (1, 24, 5, 64, 5, 0, 320, 64),
+                    (1, 4, 27, 64, 1, 0, 1920, 64), (1, 1, 1, 64, 1, 0, 0, 0)]
+
+
 # ---- layer norm: no heads --------------------------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
