@@ -5,8 +5,8 @@
 // of equal tokens stay in order), and `embedding_fill` writes the zero rows, for which it only has to know which tokens
 // occur.  `embedding_sums` then walks over the sorted places in chunks of one length, whatever the frequencies of the tokens (a
 // text's most frequent token has hundreds of times its average share): runs of equal tokens inside a chunk are finished
-// there, those that cross its ends leave a partial sum each, which `embedding_join` adds in order.  No sum depends on how
-// threads are scheduled.
+// there, those that cross its ends leave a partial sum each, which `embedding_join` adds.  The order of a sum follows from
+// where its token stands and from the chunks' length (sizes, number of SMs), never from how threads are scheduled.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -361,9 +361,9 @@ __global__ void __launch_bounds__(BLOCK) embedding_sums(const T* __restrict__ dy
     if (run < rows) finish(after == run);
 }
 
-// Sums of the runs that cross ends of chunks, each in the order of its partial sums.  A block looks at JOINED chunks for
-// runs that start there and go on.  A run of few partial sums is added by one warp, all of them side by side; a longer one
-// by the block, 64 threads with 4 columns each and 4 slices of the partial sums.  Bound by latency: 10 us for 512 chunks of
+// Sums of the runs that cross ends of chunks.  A block looks at JOINED chunks for runs that start there and go on.  A run of
+// few partial sums is added in their order by one warp, several runs side by side; a longer one by the block, 64 threads with
+// 4 columns each and 4 slices of the partial sums (every fourth one), which are added last.  Bound by latency: 10 us for 512 chunks of
 // 4096 columns, most of it three loads that wait for one another.
 enum { JOINED = BLOCK / 32, FEW = 16 };
 template <class T>

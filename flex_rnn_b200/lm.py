@@ -48,8 +48,8 @@ def embedding(tokens: th.Tensor, weight: th.Tensor, scale: float = 1.0, ignore_i
 
     ``tokens`` are int64 or int32.  Places with ``ignore_index`` give zeros and add to no gradient.  A token outside the
     vocabulary gives zeros too and is reported: the next call on that GPU raises ``FrnnError`` (no call waits for the GPU
-    to look).  The gradient of ``weight`` is dense and sums each token's rows in the order of their places in 32 bits, so
-    it is the same in every run."""
+    to look).  The gradient of ``weight`` is dense and sums each token's rows in 32 bits, in an order that the
+    tokens' places, the sizes and the GPU's number of SMs fix, so it is the same in every run."""
     _operators()
     return _ops.embedding.default(tokens, weight, scale, ignore_index)
 
