@@ -9,11 +9,12 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libfrnn_b200.so")
-SRCS = [os.path.join(HERE, "csrc", f) for f in ("frnn_shim.cu", "frnn_embedding.cu", "frnn_layer_norm.cu", "frnn_logprobs.cu")]
-DEPS = [*SRCS, os.path.join(HERE, "csrc", "frnn_lm.cuh"), os.path.join(HERE, "..", "include", "frnn.h")]
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("frnn_shim.cu", "frnn_embedding.cu", "frnn_layer_norm.cu", "frnn_logprobs.cu", "frnn_gated_mlp.cu", "frnn_linear_logprobs.cu", "frnn_rotary.cu")]
+DEPS = [*SRCS, *[os.path.join(HERE, "csrc", f) for f in ("frnn_lm.cuh", "frnn_product.cuh", "frnn_device.cuh", "frnn_chunk.cuh")],
+        os.path.join(HERE, "..", "include", "frnn.h")]
 HOST_LIB = os.path.join(HERE, "_frnn_host.so")
-HOST_SRCS = [os.path.join(HERE, "csrc", f) for f in ("frnn_host.cpp", "frnn_lm_host.cpp")]
-HOST_DEPS = [*HOST_SRCS, os.path.join(HERE, "..", "include", "frnn.h")]
+HOST_SRCS = [os.path.join(HERE, "csrc", f) for f in ("frnn_host.cpp", "frnn_lm_host.cpp", "frnn_block_host.cpp")]
+HOST_DEPS = [*HOST_SRCS, os.path.join(HERE, "csrc", "frnn_lm_host.h"), os.path.join(HERE, "..", "include", "frnn.h")]
 
 
 def nvcc_path() -> str:

@@ -1,0 +1,847 @@
+// Matrix products on the tensor cores (tcgen05) with what follows them done on the tile that leaves Tensor Memory: the products
+// of frnn_gated_mlp.cu and frnn_linear_logprobs.cu.
+//
+//   C[m, n] = sum over segments g and k of A[plane_a(g)][m, k] B_g[plane_b(g)][n, k]
+//
+// Operands are 16-bit (bf16 or fp16), accumulators 32-bit.  fp32 operands are three bf16 planes hi + mid + lo (each the rest of
+// the one before, rounded to nearest: 24 bits, exactly), a product of them six segments, the terms above 2^-24: lo hi, hi lo,
+// mid mid, mid hi, hi mid, hi hi, the small ones first.  A sum of two products (da Wg + db Wu) is segments too.
+//
+// Layout.  A block computes 128 rows.  Operands come by TMA, 64 values of k a stage, swizzled over 128 bytes.  An operand whose
+// rows run along k lies in shared memory as rows of 128 bytes (8 rows and 1024 bytes an atom); one that runs along m or n as
+// 64 rows of k, each 64 values of m, in parts of 8 KB: the tensor cores take both, nothing is transposed.  Beyond a matrix'
+// edges TMA fills in zeros, so that sizes need not be multiples of anything; rows have to start on 16-byte boundaries.
+//
+// Roles: one thread issues copies (6 stages of 32 KB under way), one the products, 8 warps take finished accumulators out of
+// Tensor Memory (which holds two sets, so that the next tile's products run meanwhile).  Blocks stay for several tiles.  CG = 2:
+// a pair of blocks computes 256 rows, each holds half of B's rows, so that a byte of B in shared memory serves 256 rows; without
+// pairs (CG = 1, tiles of 128 x 128) small products spread over more multiprocessors, and k is split where that is not enough.
+#pragma once
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "frnn_lm.cuh"
+
+#include "frnn_device.cuh"
+#include "frnn_chunk.cuh"
+
+// defined in frnn_shim.cu: a tensor map of a [planes][rows][cols] matrix of 16-bit elements, swizzled over 128 bytes
+int frnn_tensor_map_swizzled(void* out_map, const void* base, uint64_t cols, uint64_t rows, uint64_t planes, uint64_t row_bytes, uint64_t plane_bytes, uint32_t box_cols, uint32_t box_rows);
+
+namespace frnn_lm {
+
+enum { BK = 64, STAGES = 6, STAGE_BYTES = 32768, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
+// Registers of the warps that copy and issue, and of the epilogue's: 128 x 56 + 256 x 224 = 384 x 168, what a block starts with.
+enum { CONTROL_REGISTERS = 56, EPILOGUE_REGISTERS = 224, START_REGISTERS = 168 };
+enum { PRODUCT_SHARED = STAGES * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };
+enum { CODE_PRODUCT = 97 };       // error word: a wait inside a matrix product ran out
+
+// What becomes of a tile.
+enum { STORE = 0, GLU_FORWARD = 1, GLU_BACKWARD = 2, LOGPROB_STATS = 3, LOGPROB_GRAD = 4 };
+
+// A 16-bit operand of a later product as an epilogue writes it: bf16 or fp16, or for fp32 three bf16 planes.
+struct Planes {
+    void* p;
+    int64_t ld, plane;          // elements between rows, between planes
+};
+
+struct alignas(64) ProductArgs {
+    CUtensorMap a, b[2];
+    int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
+    int ksteps, segments;       // steps of 64 along k in a segment
+    int tiles_m, tiles_n, slices, group;
+    int dual;                   // a tile's columns are half of B0's rows and half of B1's
+    unsigned idesc;
+    int* err;
+    unsigned char plane_a[MAX_SEGMENTS], map_b[MAX_SEGMENTS], plane_b[MAX_SEGMENTS];
+    // STORE
+    void* out;
+    int64_t out_ld, out_slice;  // out_slice: elements between the partial sums of two slices of k
+    int out_dtype, out_wide;    // wide: rows start on 16-byte boundaries
+    const float* add;           // fp32 [M][add_ld] to add, or NULL
+    int64_t add_ld;
+    const float* alpha;         // a factor on the device, or NULL
+    // GLU_*
+    int io, activation;
+    void *save_a, *save_b;      // the two products, [M][save_ld] of the type of io; written forward (NULL: not), read backward
+    int64_t save_ld;
+    Planes h, da, db;
+    // LOGPROB_*
+    float c2;                   // log2(e) / temperature
+    float inv_t;
+    const void* tokens;
+    int token_bytes;
+    int64_t ignore_index, first;      // first: token of column 0
+    float* partial;             // STATS: [block of columns][max, sum, sum of products][M]
+    float* target;              // STATS: [M] of u at the row's token
+    const float *stats, *dlogprob, *dentropy;      // GRAD: [M][2] log2 of the sum, entropy
+    const float* scale;         // GRAD: a power of two that brings fp16 gradients into range, or NULL
+    Planes grad;
+};
+
+// ---- instructions -----------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ u32 cluster_rank() {
+    u32 r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of the same variable in block `rank` of the cluster
+__device__ __forceinline__ u32 in_block(const void* p, u32 rank) {
+    u32 r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(frnn_smem_addr(p)), "r"(rank));
+    return r;
+}
+template <int CG> __device__ __forceinline__ void tma_load(u32 dst, const CUtensorMap* map, int x, int y, int z, u32 bar) {
+    if constexpr (CG == 2)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((u64)map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((u64)map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+template <int CG> __device__ __forceinline__ void mma_f16(u32 d, u64 a, u64 b, u32 idesc, bool accumulate) {
+    if constexpr (CG == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((u32)accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((u32)accumulate) : "memory");
+}
+// An arrival on `bar` (of both blocks of a pair) when the products issued so far are done.
+template <int CG> __device__ __forceinline__ void mma_commit(u64* bar) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(frnn_smem_addr(bar)), "h"((unsigned short)3) : "memory");
+    else
+        frnn_mma_commit(bar);
+}
+template <int CG> __device__ __forceinline__ void tmem_alloc(u32* at, u32 columns) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(frnn_smem_addr(at)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        frnn_tmem_alloc(at, columns);
+    }
+}
+template <int CG> __device__ __forceinline__ void tmem_free(u32 at, u32 columns) {
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+    else frnn_tmem_dealloc(at, columns);
+}
+// Shared-memory operand swizzled over 128 bytes: 1024 bytes between groups of 8 rows; `parts` bytes between parts of 64 values
+// of m or n (only where rows run along m or n).
+__device__ __forceinline__ u64 operand_desc(u32 smem, u32 parts) {
+    return (u64)((smem & 0x3ffffu) >> 4) | ((u64)(parts >> 4) << 16) | ((u64)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// ---- rows of 32 values --------------------------------------------------------------------------------------------------------
+
+// Each lane has 32 consecutive values of its row; they go to dst (rows ld elements apart) by way of shared memory, so that
+// neighbouring lanes write neighbouring bytes.  Of the warp's 32 rows `rows` exist, of the 32 columns `cols`.
+template <class T> __device__ __forceinline__ void put_rows(unsigned char* staging, int lane, const float* v, T* dst, int64_t ld, int rows, int cols, bool wide) {
+    constexpr int W = WIDE<T>, CHUNKS = 32 / W, ROW = 32 * (int)sizeof(T);       // 4 chunks of 8, or 8 of 4
+    auto slot = [](int r, int c) { return r * ROW + ((c ^ (sizeof(T) == 2 ? (r >> 1) & 3 : r & 7)) * 16); };
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+        Pack<T, W> x;
+        x.from(v + c * W);
+        x.store((T*)(staging + slot(lane, c)));
+    }
+    __syncwarp();
+    if (wide && cols == 32) {
+        constexpr int AT_ONCE = 32 / CHUNKS;      // rows
+        const int c = lane % CHUNKS;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+            const int r = r0 + lane / CHUNKS;
+            Pack<T, W> x;
+            x.load((const T*)(staging + slot(r, c)));
+            if (r < rows) x.store(dst + r * ld + c * W);
+        }
+    } else if (lane < cols) {
+        for (int r = 0; r < rows; r++) dst[r * ld + lane] = *(const T*)(staging + slot(r, lane / W) + lane % W * sizeof(T));
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ void put_rows_as(int dtype, unsigned char* staging, int lane, const float* v, void* dst, int64_t at, int64_t ld, int rows, int cols, bool wide) {
+    if (dtype == FRNN_F32) put_rows(staging, lane, v, (float*)dst + at, ld, rows, cols, wide);
+    else if (dtype == FRNN_BF16) put_rows(staging, lane, v, (__nv_bfloat16*)dst + at, ld, rows, cols, wide);
+    else put_rows(staging, lane, v, (__half*)dst + at, ld, rows, cols, wide);
+}
+// x = hi + mid + lo in bf16, exactly (values above the largest bf16 are cut off first; what is not finite stays in hi alone).
+__device__ __forceinline__ void split3(float x, float& hi, float& mid, float& lo) {
+    hi = __bfloat162float(__float2bfloat16_rn(x));
+    if (fabsf(hi) == INFINITY && fabsf(x) != INFINITY) hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    const float rest = x - hi;
+    const bool whole = fabsf(hi) < INFINITY;
+    mid = whole ? __bfloat162float(__float2bfloat16_rn(rest)) : 0.f;
+    lo = whole ? rest - mid : 0.f;
+}
+__device__ __forceinline__ void put_planes(int io, unsigned char* staging, int lane, float* v, const Planes& to, int64_t row, int col, int rows, int cols) {
+    const int64_t at = row * to.ld + col;
+    if (io == FRNN_F16) {
+        put_rows(staging, lane, v, (__half*)to.p + at, to.ld, rows, cols, true);
+    } else if (io == FRNN_BF16) {
+        put_rows(staging, lane, v, (__nv_bfloat16*)to.p + at, to.ld, rows, cols, true);
+    } else {
+#pragma unroll 1
+        for (int plane = 0; plane < 3; plane++) {          // each round leaves the rest of the one before
+            float part[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                float mid, lo;
+                split3(v[j], part[j], mid, lo);
+                v[j] = fabsf(part[j]) < INFINITY ? v[j] - part[j] : 0.f;
+            }
+            put_rows(staging, lane, part, (__nv_bfloat16*)to.p + plane * to.plane + at, to.ld, rows, cols, true);
+        }
+    }
+}
+// 32 values of a lane's row (aligned rows; zeros beyond `cols`)
+template <class T> __device__ __forceinline__ void get_row(const T* p, int cols, float* v) {
+    constexpr int W = WIDE<T>;
+#pragma unroll
+    for (int c = 0; c < 32 / W; c++) {
+        if ((c + 1) * W <= cols) {
+            Pack<T, W> x;
+            x.load(p + c * W);
+            x.to(v + c * W);
+        } else {
+#pragma unroll
+            for (int e = 0; e < W; e++) v[c * W + e] = c * W + e < cols ? to_float(p[c * W + e]) : 0.f;
+        }
+    }
+}
+__device__ __forceinline__ void get_row_as(int dtype, const void* p, int64_t at, int cols, float* v) {
+    if (dtype == FRNN_F32) get_row((const float*)p + at, cols, v);
+    else if (dtype == FRNN_BF16) get_row((const __nv_bfloat16*)p + at, cols, v);
+    else get_row((const __half*)p + at, cols, v);
+}
+
+// ---- activations -----------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float logistic(float a) { return 1.f / (1.f + __expf(-a)); }
+__device__ __forceinline__ float activate(int kind, float a) {
+    switch (kind) {
+        case FRNN_SILU: return a * logistic(a);
+        case FRNN_GELU: return a * (0.5f * erfcf(-0.70710678118654752f * a));
+        case FRNN_RELU: return a > 0.f || a != a ? a : 0.f;
+        default: return logistic(a);
+    }
+}
+__device__ __forceinline__ float slope(int kind, float a) {
+    switch (kind) {
+        case FRNN_SILU: { const float s = logistic(a); return s * (1.f + a * (1.f - s)); }
+        case FRNN_GELU: return 0.5f * erfcf(-0.70710678118654752f * a) + a * (0.39894228040143268f * __expf(-0.5f * a * a));
+        case FRNN_RELU: return a > 0.f ? 1.f : 0.f;
+        default: { const float s = logistic(a); return s * (1.f - s); }
+    }
+}
+
+// ---- epilogues ---------------------------------------------------------------------------------------------------------------
+
+// The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last
+// bit, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096, 2e-5 at 8192 in six segments, where 32-bit
+// sums rounded to nearest lose some 3e-7).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
+// instead, from parts of FLUSH steps, in registers, half of a tile's columns a warp.
+enum { FLUSH = 4 };
+
+// Column of accumulators that a warp's i-th value lies in: its half of the tile's columns, or of both products' columns.
+template <int EPI, int BN> __device__ __forceinline__ int column_of(int half, int i) {
+    if (EPI == GLU_FORWARD) return i < BN / 4 ? half * (BN / 4) + i : BN / 2 + half * (BN / 4) + i - BN / 4;
+    return half * (BN / 2) + i;
+}
+
+template <int EPI, int BN, bool PROMOTE>
+__device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, const float* sum, int64_t row0, int tn, int slice, int half, int lane, unsigned char* staging) {
+    constexpr int ROUNDS = PROMOTE ? BN / 64 : 1;      // (registers are not indexed: unrolled)
+    auto take = [&](int i, float* v) {
+        if constexpr (PROMOTE) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = sum[i + j];
+        } else {
+            frnn_tmem_ld<32>(acc + column_of<EPI, BN>(half, i), v);
+            frnn_tmem_wait_ld();
+        }
+    };
+    const int rows = (int)min((int64_t)32, max((int64_t)0, p.M - row0));
+    const int64_t row = row0 + lane;
+    if constexpr (EPI == STORE) {
+        const float alpha = p.alpha ? *p.alpha : 1.f;
+#pragma unroll ROUNDS
+        for (int i = 0; i < BN / 2; i += 32) {
+            const int c = half * (BN / 2) + i;
+            float v[32];
+            take(i, v);
+            const int col = p.dual ? tn * (BN / 2) + c % (BN / 2) : tn * BN + c;
+            const int cols = min(32, p.N - col);
+            if (rows <= 0 || cols <= 0) continue;
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] *= alpha;
+            if (p.add && lane < rows) {
+                float o[32];
+                get_row(p.add + row * p.add_ld + col, cols, o);
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] += o[j];
+            }
+            const int64_t at = slice * p.out_slice + row0 * p.out_ld + col + (p.dual && c >= BN / 2 ? p.out_ld / 2 : 0);
+            put_rows_as(p.out_dtype, staging, lane, v, p.out, at, p.out_ld, rows, cols, p.out_wide);
+        }
+    } else if constexpr (EPI == GLU_FORWARD) {
+#pragma unroll ROUNDS
+        for (int i = 0; i < BN / 4; i += 32) {
+            const int c = half * (BN / 4) + i;
+            float a[32], b[32];
+            take(i, a);
+            take(BN / 4 + i, b);
+            const int col = tn * (BN / 2) + c, cols = min(32, p.N - col);
+            if (rows <= 0 || cols <= 0) continue;
+            if (p.save_a) {
+                const int64_t at = row0 * p.save_ld + col;
+                put_rows_as(p.io, staging, lane, a, p.save_a, at, p.save_ld, rows, cols, true);
+                put_rows_as(p.io, staging, lane, b, p.save_b, at, p.save_ld, rows, cols, true);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) a[j] = activate(p.activation, a[j]) * b[j];
+            put_planes(p.io, staging, lane, a, p.h, row0, col, rows, cols);
+        }
+    } else if constexpr (EPI == GLU_BACKWARD) {
+#pragma unroll ROUNDS
+        for (int i = 0; i < BN / 2; i += 32) {
+            const int c = half * (BN / 2) + i;
+            float d[32], a[32], b[32];
+            take(i, d);
+            const int col = tn * BN + c, cols = min(32, p.N - col);
+            if (rows <= 0 || cols <= 0) continue;
+            const int64_t at = row * p.save_ld + col;
+#pragma unroll
+            for (int j = 0; j < 32; j++) a[j] = b[j] = 0.f;
+            if (lane < rows) {
+                get_row_as(p.io, p.save_a, at, cols, a);
+                get_row_as(p.io, p.save_b, at, cols, b);
+            }
+            if (p.da.p) {
+                float t[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) t[j] = d[j] * b[j] * slope(p.activation, a[j]);
+                put_planes(p.io, staging, lane, t, p.da, row0, col, rows, cols);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float s = activate(p.activation, a[j]);
+                a[j] = d[j] * s;
+                b[j] *= s;
+            }
+            if (p.db.p) put_planes(p.io, staging, lane, a, p.db, row0, col, rows, cols);
+            if (p.h.p) put_planes(p.io, staging, lane, b, p.h, row0, col, rows, cols);
+        }
+    } else if constexpr (EPI == LOGPROB_STATS) {
+        int64_t token = -1;
+        if (lane < rows) token = token_at(p.tokens, p.token_bytes, row);
+        float m = -3.4028235e38f, s = 0.f, t = 0.f;
+#pragma unroll ROUNDS
+        for (int i = 0; i < BN / 2; i += 32) {
+            const int c = half * (BN / 2) + i;
+            float v[32];
+            take(i, v);
+            const int col = tn * BN + c, cols = min(32, p.N - col);
+            if (cols <= 0) continue;
+            float top = m;
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                v[j] = j < cols ? v[j] * p.c2 : -INFINITY;
+                top = fmaxf(top, v[j]);
+            }
+            const int64_t hit = token - p.first - col;
+            if (hit >= 0 && hit < cols && lane < rows) {
+#pragma unroll 1
+                for (int j = 0; j < 32; j++) {
+                    float x = v[0];
+#pragma unroll
+                    for (int i = 1; i < 32; i++) x = i == j ? v[i] : x;
+                    if (j == (int)hit) p.target[row] = x;
+                }
+            }
+            const float down = exp2_fast(m - top);
+            t = s == 0.f ? 0.f : down * (t + s * (m - top));
+            s *= down;
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float u = v[j] - top, e = exp2_fast(u);
+                s += e;
+                t = fmaf(e, fmaxf(u, -1e30f), t);
+            }
+            m = top;
+        }
+        if (lane < rows) {
+            float* to = p.partial + (int64_t)(tn * 2 + half) * 3 * p.M + row;
+            to[0] = m;
+            to[p.M] = s;
+            to[2 * (int64_t)p.M] = t;
+        }
+    } else {
+        int64_t token = -1;
+        float lse2 = 0.f, entropy = 0.f, g = 0.f, h = 0.f;
+        bool empty = false;
+        if (lane < rows) {
+            token = token_at(p.tokens, p.token_bytes, row);
+            lse2 = p.stats[2 * row];
+            entropy = p.stats[2 * row + 1];
+            g = p.dlogprob && token != p.ignore_index ? p.dlogprob[row] : 0.f;
+            h = p.dentropy ? p.dentropy[row] : 0.f;
+            empty = lse2 == -INFINITY;
+        }
+        const float k = p.inv_t * (p.scale ? *p.scale : 1.f);
+#pragma unroll ROUNDS
+        for (int i = 0; i < BN / 2; i += 32) {
+            const int c = half * (BN / 2) + i;
+            float v[32];
+            take(i, v);
+            const int col = tn * BN + c, cols = min(32, p.N - col);
+            if (rows <= 0 || cols <= 0) continue;
+            const int64_t hit = token - p.first - col;
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float u = fmaf(v[j], p.c2, -lse2), e = exp2_fast(u);
+                float d = -e * fmaf(h, fmaf(fmaxf(u, -1e30f), 0.69314718055994531f, entropy), g);
+                if (hit == j) d += g;
+                v[j] = empty ? 0.f : d * k;
+            }
+            put_planes(p.io, staging, lane, v, p.grad, row0, col, rows, cols);
+        }
+    }
+}
+
+// ---- the kernel ---------------------------------------------------------------------------------------------------------------
+
+struct Unit { int tm, tn, slice, from, to; };      // a tile and a range of its steps along k
+
+// Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
+__device__ __forceinline__ Unit unit_of(const ProductArgs& p, int u) {
+    Unit r;
+    r.slice = u % p.slices;
+    const int tile = u / p.slices, a_group = p.group * p.tiles_n, g = tile / a_group, in = tile % a_group, high = min(p.group, p.tiles_m - g * p.group);
+    r.tm = g * p.group + in % high;
+    r.tn = in / high;
+    const int64_t steps = (int64_t)p.ksteps * p.segments;
+    r.from = (int)(steps * r.slice / p.slices);
+    r.to = (int)(steps * (r.slice + 1) / p.slices);
+    return r;
+}
+
+// AT, BT: the operand's rows run along m (n) instead of k.
+template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
+    constexpr int NB = BN / CG;                        // B's rows in this block
+    constexpr u32 A_BYTES = 128 * BK * 2, B_BYTES = NB * BK * 2, COLUMNS = 2 * BN;
+    static_assert(A_BYTES + B_BYTES <= STAGE_BYTES && COLUMNS <= 512, "a stage or Tensor Memory is too small");
+    extern __shared__ unsigned char raw[];
+    __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+    __shared__ u32 tmem;
+    unsigned char* const smem = raw + (1024 - (frnn_smem_addr(raw) & 1023)) % 1024;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const u32 rank = CG == 2 ? cluster_rank() : 0;
+    const int units = p.tiles_m * p.tiles_n * p.slices, first = blockIdx.x / CG, stride = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            frnn_mbar_init(&full[s], 1);
+            frnn_mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            frnn_mbar_init(&acc_full[b], 1);
+            frnn_mbar_init(&acc_empty[b], EPILOGUE_WARPS * CG);
+        }
+        frnn_mbar_init_fence();
+    }
+    __syncwarp();
+    if (warp == 2) tmem_alloc<CG>(&tmem, COLUMNS);
+    frnn_tmem_fence_before_sync();
+    if constexpr (CG == 2) cluster_sync();
+    __syncthreads();
+    frnn_tmem_fence_after_sync();
+
+    if (warp < 4) {
+        frnn_regs_release<CONTROL_REGISTERS>();
+        if (warp == 0) {
+            if (frnn_elect()) {
+                u32 it = 0;
+                bool ok = true;
+                for (int u = first; ok && u < units; u += stride) {
+                    const Unit w = unit_of(p, u);
+                    const int m = (w.tm * CG + (int)rank) * 128, n = p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)rank * NB;
+                    int g = w.from / p.ksteps, k = w.from % p.ksteps;
+                    for (int i = w.from; i < w.to; i++, it++) {
+                        const int s = it % STAGES;
+                        if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
+                        if (rank == 0) frnn_mbar_expect_tx(&full[s], (A_BYTES + B_BYTES) * CG);
+                        const u32 bar = CG == 2 ? in_block(&full[s], 0) : frnn_smem_addr(&full[s]), at = frnn_smem_addr(smem + s * STAGE_BYTES);
+                        const int pa = p.plane_a[g], pb = p.plane_b[g];
+                        if constexpr (AT) {
+                            tma_load<CG>(at, &p.a, m, k * BK, pa, bar);
+                            tma_load<CG>(at + A_BYTES / 2, &p.a, m + 64, k * BK, pa, bar);
+                        } else {
+                            tma_load<CG>(at, &p.a, k * BK, m, pa, bar);
+                        }
+                        if constexpr (BT) {
+    #pragma unroll
+                            for (int part = 0; part < NB / 64; part++) tma_load<CG>(at + A_BYTES + part * 8192, &p.b[p.map_b[g]], n + part * 64, k * BK, pb, bar);
+                        } else if (!p.dual) {
+                            tma_load<CG>(at + A_BYTES, &p.b[p.map_b[g]], k * BK, n, pb, bar);
+                            static_assert(BT || NB == 128, "a copy is 128 rows high");
+                        } else if (CG == 2) {      // one block has B0's rows, the other B1's
+                            tma_load<CG>(at + A_BYTES, &p.b[rank], k * BK, n, pb, bar);
+                        } else {                   // (copies of 64 rows)
+                            tma_load<CG>(at + A_BYTES, &p.b[0], k * BK, n, pb, bar);
+                            tma_load<CG>(at + A_BYTES + B_BYTES / 2, &p.b[1], k * BK, n, pb, bar);
+                        }
+                        if (++k == p.ksteps) { k = 0; g++; }
+                    }
+                }
+                // every copy has been used, and every arrival has come, before the block leaves
+                for (u32 i = it > STAGES ? it - STAGES : 0; i < it; i++)
+                    if (!frnn_mbar_wait(&empty[i % STAGES], i / STAGES & 1, p.err, CODE_PRODUCT)) break;
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            if (rank == 0 && frnn_elect()) {
+                u32 it = 0, t = 0;
+                bool ok = true;
+                for (int u = first; ok && u < units; u += stride) {
+                    const Unit w = unit_of(p, u);
+                    for (int from = w.from; ok && from < w.to; t++) {
+                        const int to = PROMOTE ? min(from + FLUSH, w.to) : w.to;
+                        const u32 buf = t & 1, d = tmem + buf * BN;
+                        if (!(ok = frnn_mbar_wait(&acc_empty[buf], (t / 2 & 1) ^ 1, p.err, CODE_PRODUCT))) break;
+                        frnn_tmem_fence_after_sync();
+                        for (int i = from; i < to; i++, it++) {
+                            const int s = it % STAGES;
+                            if (!(ok = frnn_mbar_wait(&full[s], it / STAGES & 1, p.err, CODE_PRODUCT))) break;
+                            frnn_tmem_fence_after_sync();
+                            const u32 at = frnn_smem_addr(smem + s * STAGE_BYTES);
+                            const u64 a = operand_desc(at, 8192), b = operand_desc(at + A_BYTES, 8192);
+    #pragma unroll
+                            for (int k = 0; k < BK / 16; k++)      // 16 values of k: 32 bytes of a row, or 16 rows
+                                mma_f16<CG>(d, a + k * (AT ? 2048 / 16 : 32 / 16), b + k * (BT ? 2048 / 16 : 32 / 16), p.idesc, i > from || k > 0);
+                            mma_commit<CG>(&empty[s]);
+                        }
+                        mma_commit<CG>(&acc_full[buf]);
+                        from = to;
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        frnn_regs_acquire<EPILOGUE_REGISTERS>();
+        const int quarter = warp % 4, half = (warp - 4) / 4;
+        unsigned char* const staging = smem + STAGES * STAGE_BYTES + (warp - 4) * STAGING_BYTES;
+        u32 t = 0;
+        bool ok = true;
+        auto filled = [&] {            // waits for accumulators; their address
+            ok = __all_sync(0xffffffffu, frnn_mbar_wait(&acc_full[t & 1], t / 2 & 1, p.err, CODE_PRODUCT));
+            frnn_tmem_fence_after_sync();
+            return tmem + (t & 1) * BN + frnn_tmem_lane_base(quarter);
+        };
+        auto emptied = [&] {           // this warp has taken what it needs
+            frnn_tmem_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_block(&acc_empty[t & 1], 0)) : "memory");
+                else frnn_mbar_arrive(&acc_empty[t & 1]);
+            }
+            t++;
+        };
+        for (int u = first; ok && u < units; u += stride) {
+            const Unit w = unit_of(p, u);
+            const int64_t row0 = (int64_t)(w.tm * CG + (int)rank) * 128 + quarter * 32;
+            if constexpr (PROMOTE) {
+                float sum[BN / 2];
+                for (int from = w.from; from < w.to; from += FLUSH) {
+                    const u32 acc = filled();
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < BN / 2; i += 32) {
+                        float v[32];
+                        frnn_tmem_ld<32>(acc + column_of<EPI, BN>(half, i), v);
+                        frnn_tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) sum[i + j] = from == w.from ? v[j] : sum[i + j] + v[j];
+                    }
+                    emptied();
+                }
+                if (ok) epilogue<EPI, BN, true>(p, 0, sum, row0, w.tn, w.slice, half, lane, staging);
+            } else {
+                const u32 acc = filled();
+                if (!ok) break;
+                epilogue<EPI, BN, false>(p, acc, nullptr, row0, w.tn, w.slice, half, lane, staging);
+                emptied();
+            }
+        }
+    }
+    frnn_tmem_fence_before_sync();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    frnn_tmem_fence_after_sync();
+    if (warp == 2) tmem_free<CG>(tmem, COLUMNS);
+}
+
+// ---- the rest of a product whose k was split: partial sums added in the order of the slices ----------------------------------------
+
+__device__ __forceinline__ void store_as(int dtype, void* p, int64_t at, float v) {
+    if (dtype == FRNN_F32) ((float*)p)[at] = v;
+    else if (dtype == FRNN_BF16) ((__nv_bfloat16*)p)[at] = from_float<__nv_bfloat16>(v);
+    else ((__half*)p)[at] = from_float<__half>(v);
+}
+__device__ __forceinline__ float load_as(int dtype, const void* p, int64_t at) {
+    return dtype == FRNN_F32 ? ((const float*)p)[at] : dtype == FRNN_BF16 ? to_float(((const __nv_bfloat16*)p)[at]) : to_float(((const __half*)p)[at]);
+}
+__device__ __forceinline__ void store_planes(int io, const Planes& to, int64_t row, int64_t col, float v) {
+    const int64_t at = row * to.ld + col;
+    if (io != FRNN_F32) {
+        store_as(io, to.p, at, v);
+    } else {
+        float hi, mid, lo;
+        split3(v, hi, mid, lo);
+        store_as(FRNN_BF16, to.p, at, hi);
+        store_as(FRNN_BF16, to.p, at + to.plane, mid);
+        store_as(FRNN_BF16, to.p, at + 2 * to.plane, lo);
+    }
+}
+
+// p.out: partial sums of p.slices slices as STORE left them; to / to_dtype / to_ld: where STORE's own result goes.
+template <int EPI> __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ ProductArgs p, void* to, int to_dtype, int64_t to_ld) {
+    const int quads = (p.N + 3) / 4;
+    const float alpha = EPI == STORE && p.alpha ? *p.alpha : 1.f;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < (int64_t)p.M * quads; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / quads;
+        const int col = (int)(i % quads) * 4;
+        const float* from = (const float*)p.out + row * p.out_ld + col;
+        float4 v = make_float4(0, 0, 0, 0), w = v;
+        for (int s = 0; s < p.slices; s++) {
+            const float4 x = *(const float4*)(from + s * p.out_slice);
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            if constexpr (EPI == GLU_FORWARD) {
+                const float4 y = *(const float4*)(from + s * p.out_slice + p.out_ld / 2);
+                w.x += y.x; w.y += y.y; w.z += y.z; w.w += y.w;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (col + e >= p.N) break;
+            float x = (&v.x)[e];
+            const float y = (&w.x)[e];
+            if constexpr (EPI == STORE) {
+                x *= alpha;
+                if (p.add) x += p.add[row * p.add_ld + col + e];
+                store_as(to_dtype, to, row * to_ld + col + e, x);
+            } else if constexpr (EPI == GLU_FORWARD) {
+                if (p.save_a) {
+                    store_as(p.io, p.save_a, row * p.save_ld + col + e, x);
+                    store_as(p.io, p.save_b, row * p.save_ld + col + e, y);
+                }
+                store_planes(p.io, p.h, row, col + e, activate(p.activation, x) * y);
+            } else {
+                const float a = load_as(p.io, p.save_a, row * p.save_ld + col + e), b = load_as(p.io, p.save_b, row * p.save_ld + col + e), s = activate(p.activation, a);
+                if (p.da.p) store_planes(p.io, p.da, row, col + e, x * b * slope(p.activation, a));
+                if (p.db.p) store_planes(p.io, p.db, row, col + e, x * s);
+                if (p.h.p) store_planes(p.io, p.h, row, col + e, b * s);
+            }
+        }
+    }
+}
+
+// ---- operands -------------------------------------------------------------------------------------------------------------------
+
+// Rows of any type and stride as a 16-bit operand: rows on 16-byte boundaries, fp32 as three planes.
+template <class T> __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, Planes to, int io) {
+    const int64_t quads = (cols + 3) / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / quads, col = i % quads * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (col + e < cols) store_planes(io, to, row, col + e, to_float(x[row * stride + col + e]));
+    }
+}
+
+// Scratch handed out piece by piece; without memory behind it, the sum of what is asked for.
+struct Scratch {
+    char* base;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        void* const p = base ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+inline int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+inline int planes_of(int dtype) { return dtype == FRNN_F32 ? 3 : 1; }
+
+struct Operand {                  // a [rows][cols] matrix in 16 bits
+    const void* p = nullptr;
+    int64_t rows = 0, cols = 0, ld = 0, plane = 0;
+    int planes = 1;
+    Planes writable() const { return {const_cast<void*>(p), ld, plane}; }
+    Operand from_row(int64_t r, int64_t n) const {
+        Operand o = *this;
+        o.p = (const char*)p + r * ld * 2;
+        o.rows = n;
+        return o;
+    }
+};
+inline Operand new_operand(Scratch& s, int dtype, int64_t rows, int64_t cols, int copies = 1) {
+    Operand o;
+    o.rows = rows;
+    o.cols = cols;
+    o.ld = padded(cols);
+    o.plane = o.ld * rows;
+    o.planes = planes_of(dtype) * copies;
+    o.p = s.take((size_t)o.plane * o.planes * 2);
+    return o;
+}
+// The caller's matrix itself where the tensor cores can read it as it is, else a copy.
+inline int as_operand(Scratch& s, int dtype, const void* x, int64_t rows, int64_t cols, int64_t stride, Operand& o, cudaStream_t stream) {
+    if (rows == 1) stride = padded(cols);
+    if (dtype != FRNN_F32 && on_boundary(x, 16) && stride % 8 == 0 && stride >= cols) {
+        o.p = x;
+        o.rows = rows;
+        o.cols = cols;
+        o.ld = stride;
+        o.plane = rows * stride;
+        o.planes = 1;
+        return FRNN_OK;
+    }
+    o = new_operand(s, dtype, rows, cols);
+    if (!s.base) return FRNN_OK;
+    const int64_t blocks = std::min<int64_t>((rows * ((cols + 3) / 4) + 255) / 256, (int64_t)sm_count() * 16);
+    return with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        pack_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>((const T*)x, rows, cols, stride, o.writable(), dtype);
+        return launched("matrix product: operand");
+    });
+}
+
+// ---- products --------------------------------------------------------------------------------------------------------------------
+
+struct Product {
+    ProductArgs args = {};
+    int dtype;                                    // of the operands: FRNN_F32 means planes
+    Operand a, b[2];
+    bool at = false, bt = false;                  // stored [k][m], [k][n]
+    int64_t m, n, k;
+    int pairs = 1;                                // products that are added up: planes of a, b[0], b[1]
+    void* out = nullptr;                          // STORE
+    int out_dtype = 0;
+    int64_t out_ld = 0;
+};
+
+struct ProductPlan {
+    bool pair;
+    int slices;
+    int64_t tiles_m, tiles_n, ld;
+    size_t bytes;                                 // partial sums
+};
+
+// Which kernel, and into how many slices k is split.  Cycles of a step of 64 along k in a block: 512 of 128 x 256 (pairs), and
+// for 128 x 128 the 256 of the products, but 340 with its copies; what a tile or slice costs besides, and a second kernel for
+// the partial sums, as measured.  A split takes whole-wave shapes: the fewest cycles of the busiest multiprocessor.
+inline ProductPlan plan_product(const Product& q, bool may_split) {
+    const int sms = sm_count();
+    const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    ProductPlan best = {true, 1, up(q.m, 256), up(q.n * width, 256), 0, 0};
+    if (q.args.dual) best.tiles_n = up(q.n, 128);
+    double cost = (double)up(best.tiles_m * best.tiles_n, sms / 2) * (steps * 512 + 1000) + 4000;
+    const int64_t tm = up(q.m, 128), tn = q.args.dual ? up(q.n, 64) : up(q.n, 128), ld = padded(q.n) * width;
+    for (int s = 1; s <= (may_split ? 16 : 1) && s <= steps; s++) {
+        const size_t bytes = s > 1 ? (size_t)s * q.m * ld * 4 : 0;
+        if (bytes > ((size_t)64 << 20)) break;
+        const double c = (double)up(tm * tn * s, sms) * ((double)up(steps, s) * 340 + 1000) + 4000 + (s > 1 ? 5000 + bytes / 2000.0 : 0);
+        if (c < cost) {
+            cost = c;
+            best = {false, s, tm, tn, ld, bytes};
+        }
+    }
+    return best;
+}
+
+template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_product(const char* what, const ProductArgs& p, cudaStream_t stream) {
+    constexpr auto kernel = product_kernel<CG, BN, AT, BT, EPI, PROMOTE>;
+    // (the warps would wait for registers that the block does not have)
+    static const bool enough = [] {
+        cudaFuncAttributes a = {};
+        const bool ok = cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs >= START_REGISTERS;
+        cudaGetLastError();
+        return ok;
+    }();
+    if (!enough) return frnn_fail(FRNN_E_LAUNCH, "%s: the kernel was not built for %d registers a thread, or there is no GPU to run it", what, (int)START_REGISTERS);
+    if (!allow_shared<kernel>(PRODUCT_SHARED)) { cudaGetLastError(); return frnn_fail(FRNN_E_LAUNCH, "%s: no room in shared memory", what); }
+    const int64_t units = (int64_t)p.tiles_m * p.tiles_n * p.slices;
+    return launch(what, kernel, dim3((unsigned)(std::min<int64_t>(units, sm_count() / CG) * CG)), PRODUCT_THREADS, PRODUCT_SHARED, stream, false, CG, p);
+}
+
+// One product.  Without memory behind `s` only its scratch is counted.
+template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Product& q, Scratch& s, cudaStream_t stream) {
+    constexpr bool MAY_SPLIT = EPI != LOGPROB_STATS && EPI != LOGPROB_GRAD;
+    ProductArgs& p = q.args;
+    const ProductPlan plan = plan_product(q, MAY_SPLIT);
+    void* const partial = plan.slices > 1 ? s.take(plan.bytes) : nullptr;
+    if (!s.base) return FRNN_OK;
+    if (plan.tiles_m * plan.tiles_n * plan.slices >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "%s: too many tiles", what);
+    p.M = (int)q.m;
+    p.N = (int)q.n;
+    p.ksteps = (int)((q.k + BK - 1) / BK);
+    p.tiles_m = (int)plan.tiles_m;
+    p.tiles_n = (int)plan.tiles_n;
+    p.slices = plan.slices;
+    p.group = plan.pair ? 16 : 32;
+    const unsigned type = q.dtype == FRNN_F16 ? 0 : 1, bn = plan.pair ? 256 : 128, bm = plan.pair ? 256 : 128;
+    p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((unsigned)AT << 15) | ((unsigned)BT << 16) | ((bn >> 3) << 17) | ((bm >> 4) << 24);
+    static const unsigned char first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};      // planes of a and b, small terms first
+    const int terms = q.dtype == FRNN_F32 ? 6 : 1;
+    p.segments = 0;
+    for (int t = 0; t < terms; t++)
+        for (int pair = 0; pair < q.pairs; pair++, p.segments++) {
+            p.plane_a[p.segments] = (unsigned char)((terms == 6 ? first[t] : 0) + pair * planes_of(q.dtype));
+            p.plane_b[p.segments] = terms == 6 ? second[t] : 0;
+            p.map_b[p.segments] = (unsigned char)(q.pairs > 1 ? pair : 0);
+        }
+    auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
+        return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);
+    };
+    int rc = encode(p.a, q.a, AT, 128);
+    for (int i = 0; i < 2 && rc == FRNN_OK; i++) rc = encode(p.b[i], q.b[i].p ? q.b[i] : q.b[0], BT, p.dual && !plan.pair ? 64 : 128);
+    if (rc != FRNN_OK) return rc;
+    if (plan.slices > 1) {
+        if constexpr (MAY_SPLIT) {
+            ProductArgs part = p;
+            part.out = partial;
+            part.out_ld = plan.ld;
+            part.out_slice = q.m * plan.ld;
+            part.out_dtype = FRNN_F32;
+            part.out_wide = 1;
+            part.add = part.alpha = nullptr;
+            rc = q.dtype == FRNN_F32 ? launch_product<1, 128, AT, BT, STORE, true>(what, part, stream) : launch_product<1, 128, AT, BT, STORE, false>(what, part, stream);
+            if (rc != FRNN_OK) return rc;
+            part.add = p.add;
+            part.alpha = p.alpha;
+            const int64_t blocks = std::min<int64_t>((q.m * ((q.n + 3) / 4) + 255) / 256, (int64_t)sm_count() * 8);
+            finish_kernel<EPI><<<(unsigned)blocks, 256, 0, stream>>>(part, q.out, q.out_dtype, q.out_ld);
+            return launched(what);
+        }
+    }
+    p.out = q.out;
+    p.out_dtype = q.out_dtype;
+    p.out_ld = q.out_ld;
+    p.out_wide = on_boundary(q.out, 16) && q.out_ld * (int64_t)dtype_bytes(q.out_dtype) % 16 == 0;
+    if (q.dtype == FRNN_F32) return plan.pair ? launch_product<2, 256, AT, BT, EPI, true>(what, p, stream) : launch_product<1, 128, AT, BT, EPI, true>(what, p, stream);
+    constexpr bool EXACT = EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
+    return plan.pair ? launch_product<2, 256, AT, BT, EPI, EXACT>(what, p, stream) : launch_product<1, 128, AT, BT, EPI, EXACT>(what, p, stream);
+}
+
+}  // namespace frnn_lm

@@ -318,6 +318,24 @@ int frnn_kernel_attrs(frnn_module_t m, int kernel, int* regs, int* static_smem, 
 
 }  // extern "C"
 
+// For the matrix products compiled into this library (frnn_product.cuh): a [planes][rows][cols] matrix of 16-bit elements,
+// boxes swizzled over 128 bytes.
+int frnn_tensor_map_swizzled(void* out_map, const void* base, uint64_t cols, uint64_t rows, uint64_t planes, uint64_t row_bytes, uint64_t plane_bytes, uint32_t box_cols, uint32_t box_rows) {
+    Driver* d = driver();
+    if (!d) return fail(FRNN_E_DRIVER, "CUDA driver is not available");
+    const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {row_bytes, plane_bytes};
+    const cuuint32_t box[3] = {box_cols, box_rows, 1}, steps[3] = {1, 1, 1};
+    auto encode = [&] {
+        return d->TensorMapEncodeTiled((CUtensorMap*)out_map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, (void*)base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    int dev = 0;
+    // (a thread that has made no call of the runtime, autograd's for instance, has no context yet)
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+    return r == CUDA_SUCCESS ? (int)FRNN_OK : fail(FRNN_E_DRIVER, "cuTensorMapEncodeTiled: %s", cu_str(d, r));
+}
+
 // ---- kernel error word ---------------------------------------------------------
 
 namespace {
@@ -326,6 +344,7 @@ const char* kernel_code_text(int code) {
         case 1: return "a staged-input copy did not arrive within the wait limit";
         case 2: return "a checkpoint copy did not arrive within the wait limit";
         case 96: return "a token is outside the vocabulary";
+        case 97: return "a wait inside a matrix product ran out";
         default: return "unknown code";
     }
 }

@@ -22,7 +22,10 @@ SYMBOLS = ["frnn_abi_version", "frnn_last_error", "frnn_compile", "frnn_free", "
            "frnn_launch_static_scratch", "frnn_static_scratch_capacity", "frnn_tensor_map_encode",
            "frnn_nvrtc_version", "frnn_status", "frnn_status_post", "frnn_status_check", "frnn_fp32_mix_probe",
            "frnn_embedding_forward", "frnn_embedding_backward", "frnn_embedding_backward_workspace", "frnn_layer_norm_forward",
-           "frnn_layer_norm_backward", "frnn_layer_norm_backward_workspace", "frnn_token_logprobs_forward", "frnn_token_logprobs_backward"]
+           "frnn_layer_norm_backward", "frnn_layer_norm_backward_workspace", "frnn_token_logprobs_forward", "frnn_token_logprobs_backward",
+           "frnn_gated_mlp_forward", "frnn_gated_mlp_forward_workspace", "frnn_gated_mlp_backward", "frnn_gated_mlp_backward_workspace",
+           "frnn_linear_logprobs_forward", "frnn_linear_logprobs_forward_workspace", "frnn_linear_logprobs_backward",
+           "frnn_linear_logprobs_backward_workspace", "frnn_rotary"]
 
 
 class FrnnError(RuntimeError):
@@ -105,6 +108,7 @@ def host():
             m.bind(*[address(f) for f in (L.frnn_launch, L.frnn_tensor_map_encode, L.frnn_last_error)])
             m.bind_lm({n: address(getattr(L, n)) for n in SYMBOLS if n.startswith(("frnn_embedding", "frnn_layer_norm", "frnn_token", "frnn_last"))},
                       _status_word, _status_raise)
+            m.bind_block({n: address(getattr(L, n)) for n in SYMBOLS if n.startswith(("frnn_gated_mlp", "frnn_linear_logprobs", "frnn_rotary"))})
             _host = m
     return _host
 

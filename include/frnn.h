@@ -238,6 +238,66 @@ int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64
                                  float temperature, int64_t ignore_index, const float* dlogprob, const float* dentropy, const float* stats,
                                  void* dlogits, void* stream);
 
+/*
+ * The gated feed-forward block: y = (act(x gate^T) * (x up^T)) down^T, x [n, width], gate and up [hidden, width], down
+ * [out_width, hidden], all of `dtype`; rows are runs of consecutive elements, `*_stride` elements apart.  The products run on
+ * the tensor cores with sums in 32 bits (fp32 operands as sums of three bf16 numbers); for bf16 and fp16 what lies between
+ * two products (the hidden vector, and backward its gradients) is rounded to that type, because the tensor cores read it so.
+ * y and all gradients are contiguous.  `hidden_a` and `hidden_b` are the two projections as the forward saves them for the
+ * backward (NULL: not), [n, hidden rounded up to a multiple of 8], on a 16-byte boundary.
+ */
+enum { FRNN_SILU = 0, FRNN_GELU = 1, FRNN_RELU = 2, FRNN_SIGMOID = 3 };
+typedef struct frnn_gated_mlp_call {
+    int32_t dtype, activation;
+    int64_t n, width, hidden, out_width;
+    const void *x, *gate, *up, *down;
+    int64_t x_stride, gate_stride, up_stride, down_stride;
+} frnn_gated_mlp_call;
+size_t frnn_gated_mlp_forward_workspace(const frnn_gated_mlp_call* call);
+int frnn_gated_mlp_forward(const frnn_gated_mlp_call* call, void* y, void* hidden_a, void* hidden_b, void* workspace, int* err_word, void* stream);
+
+/* Gradients of x, gate, up and down for the upstream gradient dy [n, out_width]; each may be NULL (not wanted). */
+size_t frnn_gated_mlp_backward_workspace(const frnn_gated_mlp_call* call, const void* dy, int64_t dy_stride);
+int frnn_gated_mlp_backward(const frnn_gated_mlp_call* call, const void* dy, int64_t dy_stride, const void* hidden_a, const void* hidden_b, void* dx, void* dgate, void* dup,
+                            void* ddown, void* workspace, int* err_word, void* stream);
+
+/*
+ * What frnn_token_logprobs_forward gives from logits = x weight^T, x [n, width], weight [vocab, width], without keeping the
+ * logits: log probabilities of the tokens and entropies, fp32 [n].  stats (may be NULL): fp32 [n][2] for the backward.
+ * The backward computes the logits again, a piece of the vocabulary at a time (pieces of up to 512 MB), and gives dx and
+ * dweight (contiguous; either may be NULL).  The logits' gradient is rounded to `dtype` for its products (fp16: after scaling by
+ * a power of two that keeps it in range).
+ */
+typedef struct frnn_linear_logprobs_call {
+    int32_t dtype, token_bytes;
+    int64_t n, vocab, width;
+    const void *x, *weight;
+    int64_t x_stride, weight_stride;
+    const void* tokens;
+    int64_t ignore_index;
+    float temperature;
+} frnn_linear_logprobs_call;
+size_t frnn_linear_logprobs_forward_workspace(const frnn_linear_logprobs_call* call);
+int frnn_linear_logprobs_forward(const frnn_linear_logprobs_call* call, float* logprob, float* entropy, float* stats, void* workspace, int* err_word, void* stream);
+size_t frnn_linear_logprobs_backward_workspace(const frnn_linear_logprobs_call* call);
+int frnn_linear_logprobs_backward(const frnn_linear_logprobs_call* call, const float* dlogprob, const float* dentropy, const float* stats, void* dx, void* dweight, void* workspace,
+                                  int* err_word, void* stream);
+
+/*
+ * Rotary positions: of each head of x[b, t, h, :] (element strides x_stride, heads runs of consecutive elements) the pairs
+ * (u, w) of its first 2 * pairs values become scale * (u cos - w sin), scale * (u sin + w cos), the others are copied.  Pair i
+ * is (x[i], x[pairs + i]), or (x[2 i], x[2 i + 1]) where interleaved; its angle is position * frequencies[i], negative where
+ * inverse.  positions: int32 or int64 at b * position_stride[0] + t * position_stride[1], or NULL: start + t.  frequencies: fp32
+ * or fp64 [pairs].  y may be x itself.
+ */
+typedef struct frnn_rotary_call {
+    int32_t dtype, interleaved, inverse, position_bytes, frequency_bytes;
+    float scale;
+    int64_t batch, length, heads, width, pairs, start;
+    int64_t x_stride[3], y_stride[3], position_stride[2];
+} frnn_rotary_call;
+int frnn_rotary(const frnn_rotary_call* call, const void* x, const void* positions, const void* frequencies, void* y, void* stream);
+
 /* ---- helpers compiled into the library (used by the benchmark harness) ---- */
 
 /* Overwrite `bytes` bytes at `buf` (device) with a byte pattern; writing a
