@@ -65,7 +65,7 @@ GatedMlp gated_mlp_call(const char* op, const Tensor& x, const Tensor& gate, con
     return m;
 }
 
-std::tuple<Tensor, Tensor, Tensor> gated_mlp_cuda(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation, bool save) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_cuda(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation, bool save) {
     c10::cuda::OptionalCUDAGuard guard;
     if (x.is_cuda()) guard.set_device(x.device());
     const GatedMlp m = gated_mlp_call("gated_mlp", x, gate, up, down, activation);
@@ -73,15 +73,17 @@ std::tuple<Tensor, Tensor, Tensor> gated_mlp_cuda(const Tensor& x, const Tensor&
     auto sizes = x.sizes().vec();
     sizes.back() = m.c.out_width;
     const int64_t n = save ? m.c.n : 0, ld = (m.c.hidden + 7) / 8 * 8;
-    Tensor y = make("the output", sizes, x.scalar_type(), x), a = make("the first projection", {n, ld}, x.scalar_type(), x), b = make("the second projection", {n, ld}, x.scalar_type(), x);
+    const bool wide = x.scalar_type() == at::kFloat;
+    Tensor y = make("the output", sizes, x.scalar_type(), x), by_gate = make("the derivatives by gate", {n, ld}, x.scalar_type(), x), by_up = make("the derivatives by up", {n, ld}, x.scalar_type(), x);
+    Tensor hidden = make("the hidden vectors", {wide ? 3 : 1, n, ld}, wide ? at::kBFloat16 : x.scalar_type(), x);
     if (m.c.n) {
         const Tensor work = workspace(g_gated_mlp_forward_workspace(&m.c), x);
-        ran(g_gated_mlp_forward(&m.c, y.data_ptr(), n ? a.data_ptr() : nullptr, n ? b.data_ptr() : nullptr, ptr(work), err, stream_of(x)), x);
+        ran(g_gated_mlp_forward(&m.c, y.data_ptr(), n ? by_gate.data_ptr() : nullptr, n ? by_up.data_ptr() : nullptr, n ? hidden.data_ptr() : nullptr, ptr(work), err, stream_of(x)), x);
     }
-    return {y, a, b};
+    return {y, by_gate, by_up, hidden};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_cuda(const Tensor& grad, const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const Tensor& a, const Tensor& b,
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_cuda(const Tensor& grad, const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const Tensor& by_gate, const Tensor& by_up, const Tensor& hidden,
                                                                    int64_t activation, bool want_x, bool want_gate, bool want_up, bool want_down) {
     const char* op = "gated_mlp_backward";
     c10::cuda::OptionalCUDAGuard guard;
@@ -91,17 +93,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_cuda(const Tensor&
                 ": the gradient has to have the shape and type of the output, got ", grad.sizes());
     check_one(op, "the gradient", grad, x);
     const int64_t ld = (m.c.hidden + 7) / 8 * 8;
-    for (const Tensor* t : {&a, &b}) {
-        TORCH_CHECK(t->dim() == 2 && t->size(0) == m.c.n && t->size(1) == ld && t->scalar_type() == x.scalar_type(), "flex_rnn_b200: ", op, ": the projections have to be those of the forward");
-        check_one(op, "a projection", *t, x);
+    const bool wide = x.scalar_type() == at::kFloat;
+    for (const Tensor* t : {&by_gate, &by_up, &hidden}) {
+        const bool h = t == &hidden;
+        TORCH_CHECK(t->dim() == (h ? 3 : 2) && t->size(-2) == m.c.n && t->size(-1) == ld && (!h || t->size(0) == (wide ? 3 : 1)) && t->scalar_type() == (h && wide ? at::kBFloat16 : x.scalar_type()),
+                    "flex_rnn_b200: ", op, ": what the forward kept has to be given as it was");
+        check_one(op, "what the forward kept", *t, x);
     }
     int* err = error_word(x.device().index());
     auto result = [&](bool want, const char* what, const Tensor& like) { return want ? make(what, like.sizes(), like.scalar_type(), like) : Tensor(); };
     Tensor dx = result(want_x, "x's gradient", x), dgate = result(want_gate, "gate's gradient", gate), dup = result(want_up, "up's gradient", up), ddown = result(want_down, "down's gradient", down);
     if (m.c.n) {
-        const Tensor g = as_rows(grad), sa = saved(a), sb = saved(b);
+        const Tensor g = as_rows(grad), sa = saved(by_gate), sb = saved(by_up), sh = saved(hidden);
         const Tensor work = workspace(g_gated_mlp_backward_workspace(&m.c, g.data_ptr(), g.stride(0)), x);
-        ran(g_gated_mlp_backward(&m.c, g.data_ptr(), g.stride(0), sa.data_ptr(), sb.data_ptr(), ptr(dx), ptr(dgate), ptr(dup), ptr(ddown), ptr(work), err, stream_of(x)), x);
+        ran(g_gated_mlp_backward(&m.c, g.data_ptr(), g.stride(0), sa.data_ptr(), sb.data_ptr(), sh.data_ptr(), ptr(dx), ptr(dgate), ptr(dup), ptr(ddown), ptr(work), err, stream_of(x)), x);
     } else {
         for (Tensor* t : {&dgate, &dup, &ddown})
             if (t->defined()) t->zero_();
@@ -262,15 +267,15 @@ struct GatedMlpBackward : Saving {
         for (int i = 0; i < 4; i++) want[i] = task_should_compute_output(i);
         if (!up[0].defined() || !(want[0] || want[1] || want[2] || want[3])) return variable_list(4);
         const variable_list k = unpack();
-        auto [dx, dgate, dup, ddown] = gated_mlp_backward().call(up[0], k[0], k[1], k[2], k[3], k[4], k[5], activation, want[0], want[1], want[2], want[3]);
+        auto [dx, dgate, dup, ddown] = gated_mlp_backward().call(up[0], k[0], k[1], k[2], k[3], k[4], k[5], k[6], activation, want[0], want[1], want[2], want[3]);
         return {want[0] ? dx : Tensor(), want[1] ? dgate : Tensor(), want[2] ? dup : Tensor(), want[3] ? ddown : Tensor()};
     }
 };
 
-std::tuple<Tensor, Tensor, Tensor> gated_mlp_autograd(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation, bool save) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_autograd(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation, bool save) {
     for (const Tensor* t : {&x, &gate, &up, &down}) no_tangent(*t);
     const bool grad = at::GradMode::is_enabled() && (needs(x) || needs(gate) || needs(up) || needs(down));
-    std::tuple<Tensor, Tensor, Tensor> r;
+    std::tuple<Tensor, Tensor, Tensor, Tensor> r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         r = gated_mlp().call(x, gate, up, down, activation, save || grad);
@@ -278,19 +283,19 @@ std::tuple<Tensor, Tensor, Tensor> gated_mlp_autograd(const Tensor& x, const Ten
     if (grad) {
         auto node = make_node<GatedMlpBackward>(x, gate, up, down);
         node->activation = activation;
-        for (const Tensor& t : {x, gate, up, down, std::get<1>(r), std::get<2>(r)}) node->save(t);
+        for (const Tensor& t : {x, gate, up, down, std::get<1>(r), std::get<2>(r), std::get<3>(r)}) node->save(t);
         torch::autograd::create_gradient_edge(std::get<0>(r), node);
     }
     return r;
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_autograd(const Tensor& grad, const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const Tensor& a, const Tensor& b,
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_autograd(const Tensor& grad, const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const Tensor& by_gate, const Tensor& by_up, const Tensor& hidden,
                                                                        int64_t activation, bool want_x, bool want_gate, bool want_up, bool want_down) {
     for (const Tensor* t : {&grad, &x, &gate, &up, &down}) no_tangent(*t);
     std::tuple<Tensor, Tensor, Tensor, Tensor> r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        r = gated_mlp_backward().call(grad, x, gate, up, down, a, b, activation, want_x, want_gate, want_up, want_down);
+        r = gated_mlp_backward().call(grad, x, gate, up, down, by_gate, by_up, hidden, activation, want_x, want_gate, want_up, want_down);
     }
     only_once({&std::get<0>(r), &std::get<1>(r), &std::get<2>(r), &std::get<3>(r)}, grad, x, gate, up, down);
     return r;
@@ -385,8 +390,8 @@ Tensor rotary_autograd(const Tensor& x, const optional<Tensor>& positions, int64
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(flex_rnn_b200, m) {
-    m.def("gated_mlp(Tensor x, Tensor gate, Tensor up, Tensor down, int activation, bool save) -> (Tensor, Tensor, Tensor)");
-    m.def("gated_mlp_backward(Tensor grad, Tensor x, Tensor gate, Tensor up, Tensor down, Tensor a, Tensor b, int activation, bool want_x, bool want_gate, bool want_up, bool want_down) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("gated_mlp(Tensor x, Tensor gate, Tensor up, Tensor down, int activation, bool save) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("gated_mlp_backward(Tensor grad, Tensor x, Tensor gate, Tensor up, Tensor down, Tensor by_gate, Tensor by_up, Tensor hidden, int activation, bool want_x, bool want_gate, bool want_up, bool want_down) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("linear_logprobs(Tensor x, Tensor weight, Tensor tokens, float temperature, int ignore_index, bool save) -> (Tensor, Tensor, Tensor)");
     m.def("linear_logprobs_backward(Tensor? dlogprob, Tensor? dentropy, Tensor x, Tensor weight, Tensor tokens, Tensor stats, float temperature, int ignore_index, bool want_x, bool want_weight) -> (Tensor, Tensor)");
     m.def("rotary(Tensor x, Tensor? positions, int start, Tensor frequencies, bool interleaved, float scale, bool inverse) -> Tensor");

@@ -2,10 +2,12 @@
 //
 //   a = x Wg^T, b = x Wu^T          one product, a tile holds columns of both; its epilogue makes h = act(a) b
 //   y = h Wd^T
-//   dh = dy Wd                      its epilogue makes db = dh act(a), da = dh b act'(a), and h again
+//   dh = dy Wd                      its epilogue makes da = dh (b act'(a)), db = dh act(a)
 //   dWd = dy^T h, dWg = da^T x, dWu = db^T x, dx = da Wg + db Wu (one product of twice the length)
 //
-// n D F (D = width = out_width): 6 operations a value forward, 12 backward.
+// n D F (D = width = out_width): 6 operations a value forward, 12 backward.  The forward keeps h and its two derivatives
+// b act'(a) and act(a), each rounded once: a and b kept instead, rounded, were rounded twice on the way to da, db and h (errors of the gradients in
+// bf16 against 64 bits 3.5e-3 instead of 2.9e-3), and the backward's epilogue computed the activation again.
 #include "frnn_product.cuh"
 
 using namespace frnn_lm;
@@ -37,7 +39,15 @@ Product product(const frnn_gated_mlp_call* c, int64_t m, int64_t n, int64_t k) {
     return q;
 }
 
-int forward(const frnn_gated_mlp_call* c, void* y, void* a, void* b, Scratch& s, int* err, cudaStream_t stream) {
+// The hidden vectors as the forward keeps them.
+Operand kept(const frnn_gated_mlp_call* c, const void* hidden) {
+    Scratch none = {nullptr};
+    Operand h = new_operand(none, c->dtype, c->n, c->hidden);
+    h.p = hidden;
+    return h;
+}
+
+int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, void* hidden, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "gated_mlp";
     Operand x, gate, up, down;
     int rc = as_operand(s, c->dtype, c->x, c->n, c->width, c->x_stride, x, stream);
@@ -45,7 +55,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* a, void* b, Scratch& s,
     if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->up, c->hidden, c->width, c->up_stride, up, stream);
     if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->down, c->out_width, c->hidden, c->down_stride, down, stream);
     if (rc != FRNN_OK) return rc;
-    const Operand h = new_operand(s, c->dtype, c->n, c->hidden);
+    const Operand h = hidden ? kept(c, hidden) : new_operand(s, c->dtype, c->n, c->hidden);
     {
         Product q = product(c, c->n, c->hidden, c->width);
         q.a = x;
@@ -53,9 +63,9 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* a, void* b, Scratch& s,
         q.b[1] = up;
         q.args.dual = 1;
         q.args.err = err;
-        q.args.save_a = a;
-        q.args.save_b = b;
-        q.args.save_ld = padded(c->hidden);
+        q.args.by_gate = by_gate;
+        q.args.by_up = by_up;
+        q.args.by_ld = padded(c->hidden);
         q.args.h = h.writable();
         rc = run_product<GLU_FORWARD, false, false>(what, q, s, stream);
         if (rc != FRNN_OK) return rc;
@@ -70,18 +80,18 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* a, void* b, Scratch& s,
     return run_product<STORE, false, false>(what, q, s, stream);
 }
 
-int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* a, const void* b, void* dx, void* dgate, void* dup, void* ddown, Scratch& s, int* err, cudaStream_t stream) {
+int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* by_gate, const void* by_up, const void* hidden, void* dx, void* dgate, void* dup, void* ddown, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "gated_mlp_backward";
-    const bool count = !s.base, want_x = count || dx, want_gate = count || dgate, want_up = count || dup, want_down = count || ddown;
+    const bool count = !s.base, want_x = count || dx, want_gate = count || dgate, want_up = count || dup, want_down = count || ddown, want_hidden = want_x || want_gate || want_up;
     Operand x, gate, up, down, g;
     int rc = as_operand(s, c->dtype, dy, c->n, c->out_width, dy_stride, g, stream);
     if (rc == FRNN_OK && (want_gate || want_up)) rc = as_operand(s, c->dtype, c->x, c->n, c->width, c->x_stride, x, stream);
     if (rc == FRNN_OK && want_x) rc = as_operand(s, c->dtype, c->gate, c->hidden, c->width, c->gate_stride, gate, stream);
     if (rc == FRNN_OK && want_x) rc = as_operand(s, c->dtype, c->up, c->hidden, c->width, c->up_stride, up, stream);
-    if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->down, c->out_width, c->hidden, c->down_stride, down, stream);
+    if (rc == FRNN_OK && want_hidden) rc = as_operand(s, c->dtype, c->down, c->out_width, c->hidden, c->down_stride, down, stream);
     if (rc != FRNN_OK) return rc;
     const int planes = planes_of(c->dtype);
-    const Operand h = new_operand(s, c->dtype, c->n, c->hidden), both = new_operand(s, c->dtype, c->n, c->hidden, 2);      // da, db
+    const Operand both = new_operand(s, c->dtype, c->n, c->hidden, 2);      // da, db
     Operand da = both, db = both;
     da.planes = db.planes = planes;
     db.p = (const char*)both.p + both.plane * planes * 2;
@@ -91,16 +101,15 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.out_dtype = c->dtype;
         q.out_ld = ld;
     };
-    {
+    if (want_hidden) {
         Product q = product(c, c->n, c->hidden, c->out_width);
         q.a = g;
         q.b[0] = down;
         q.bt = true;
         q.args.err = err;
-        q.args.save_a = const_cast<void*>(a);
-        q.args.save_b = const_cast<void*>(b);
-        q.args.save_ld = padded(c->hidden);
-        if (want_down) q.args.h = h.writable();
+        q.args.by_gate = const_cast<void*>(by_gate);
+        q.args.by_up = const_cast<void*>(by_up);
+        q.args.by_ld = padded(c->hidden);
         if (want_x || want_gate) q.args.da = da.writable();
         if (want_x || want_up) q.args.db = db.writable();
         rc = run_product<GLU_BACKWARD, false, true>(what, q, s, stream);
@@ -109,7 +118,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
     if (want_down) {
         Product q = product(c, c->out_width, c->hidden, c->n);
         q.a = g;
-        q.b[0] = h;
+        q.b[0] = kept(c, hidden);
         store(q, ddown, c->hidden);
         rc = run_product<STORE, true, true>(what, q, s, stream);
         if (rc != FRNN_OK) return rc;
@@ -142,37 +151,39 @@ extern "C" {
 size_t frnn_gated_mlp_forward_workspace(const frnn_gated_mlp_call* c) {
     if (check("gated_mlp", c) != FRNN_OK) return 0;
     Scratch s = {nullptr};
-    forward(c, nullptr, nullptr, nullptr, s, nullptr, nullptr);
+    forward(c, nullptr, nullptr, nullptr, nullptr, s, nullptr, nullptr);
     return s.used;
 }
 
-int frnn_gated_mlp_forward(const frnn_gated_mlp_call* c, void* y, void* a, void* b, void* workspace, int* err, void* stream) {
+int frnn_gated_mlp_forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, void* hidden, void* workspace, int* err, void* stream) {
     const int rc = check("gated_mlp", c);
     if (rc != FRNN_OK) return rc;
-    if (!y || !err || !workspace || !on_boundary(workspace, 16) || !on_boundary(y, dtype_bytes(c->dtype)) || !a != !b || !on_boundary(a, 16) || !on_boundary(b, 16))
+    if (!y || !err || !workspace || !on_boundary(workspace, 16) || !on_boundary(y, dtype_bytes(c->dtype)) || !by_gate != !by_up || !by_gate != !hidden || !on_boundary(by_gate, 16) || !on_boundary(by_up, 16) ||
+        !on_boundary(hidden, 16))
         return frnn_fail(FRNN_E_ARG, "gated_mlp: bad argument");
     Scratch s = {(char*)workspace};
-    return forward(c, y, a, b, s, err, (cudaStream_t)stream);
+    return forward(c, y, by_gate, by_up, hidden, s, err, (cudaStream_t)stream);
 }
 
 size_t frnn_gated_mlp_backward_workspace(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride) {
     if (check("gated_mlp_backward", c) != FRNN_OK) return 0;
     Scratch s = {nullptr};
-    backward(c, dy, dy_stride, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, s, nullptr, nullptr);
+    backward(c, dy, dy_stride, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, s, nullptr, nullptr);
     return s.used;
 }
 
-int frnn_gated_mlp_backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* a, const void* b, void* dx, void* dgate, void* dup, void* ddown, void* workspace, int* err,
-                            void* stream) {
+int frnn_gated_mlp_backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* by_gate, const void* by_up, const void* hidden, void* dx, void* dgate, void* dup,
+                            void* ddown, void* workspace, int* err, void* stream) {
     const int rc = check("gated_mlp_backward", c);
     if (rc != FRNN_OK) return rc;
     const size_t e = dtype_bytes(c->dtype);
-    if (!dy || !on_boundary(dy, e) || (c->n > 1 && (dy_stride < 0 || dy_stride >= (1ll << 36))) || !a || !b || !on_boundary(a, 16) || !on_boundary(b, 16) || !err || !workspace ||
+    if (!dy || !on_boundary(dy, e) || (c->n > 1 && (dy_stride < 0 || dy_stride >= (1ll << 36))) || !by_gate || !by_up || !hidden || !on_boundary(by_gate, 16) ||
+        !on_boundary(by_up, 16) || !on_boundary(hidden, 16) || !err || !workspace ||
         !on_boundary(workspace, 16) || !on_boundary(dx, e) || !on_boundary(dgate, e) || !on_boundary(dup, e) || !on_boundary(ddown, e))
         return frnn_fail(FRNN_E_ARG, "gated_mlp_backward: bad argument");
     if (!dx && !dgate && !dup && !ddown) return FRNN_OK;
     Scratch s = {(char*)workspace};
-    return backward(c, dy, dy_stride, a, b, dx, dgate, dup, ddown, s, err, (cudaStream_t)stream);
+    return backward(c, dy, dy_stride, by_gate, by_up, hidden, dx, dgate, dup, ddown, s, err, (cudaStream_t)stream);
 }
 
 }  // extern "C"

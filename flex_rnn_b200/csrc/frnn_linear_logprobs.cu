@@ -13,15 +13,17 @@ using namespace frnn_lm;
 
 namespace {
 
-enum { JOIN_ROWS = 8, JOIN_SLICES = 32 };
+enum { JOIN_ROWS = 8, JOIN_SLICES = 64 };
 
-// Rows of partial results [blocks][3][n] joined: 32 threads a row take every 32nd block, then their results in order.
+// Rows of partial results [blocks][3][n] joined: 64 threads a row take every 64th block, four at a time so that their loads are
+// under way together, then their results in order.
 __global__ void __launch_bounds__(JOIN_ROWS* JOIN_SLICES) join_kernel(const float* partial, const float* target, int64_t blocks, int64_t n, const void* tokens, int token_bytes, int64_t vocab,
                                                                       int64_t ignore_index, float* logprob, float* entropy, float* stats, int* err) {
     __shared__ float part[3][JOIN_SLICES][JOIN_ROWS];
     const int r = threadIdx.x % JOIN_ROWS, slice = threadIdx.x / JOIN_ROWS;
     const int64_t row = (int64_t)blockIdx.x * JOIN_ROWS + r;
-    float m = -3.4028235e38f, s = 0.f, t = 0.f;
+    const float lowest = -3.4028235e38f;
+    float m = lowest, s = 0.f, t = 0.f;
     auto add = [&](float m2, float s2, float t2) {
         const float top = fmaxf(m, m2), d1 = exp2_fast(m - top), d2 = exp2_fast(m2 - top);
         t = (s == 0.f ? 0.f : d1 * (t + s * (m - top))) + (s2 == 0.f ? 0.f : d2 * (t2 + s2 * (m2 - top)));
@@ -29,16 +31,32 @@ __global__ void __launch_bounds__(JOIN_ROWS* JOIN_SLICES) join_kernel(const floa
         m = top;
     };
     if (row < n)
-        for (int64_t b = slice; b < blocks; b += JOIN_SLICES) {
-            const float* p = partial + b * 3 * n + row;
-            add(p[0], p[n], p[2 * n]);
+        for (int64_t b = slice; b < blocks; b += 4 * JOIN_SLICES) {
+            float v[4][3];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool there = b + k * JOIN_SLICES < blocks;
+                const float* p = partial + (b + k * JOIN_SLICES) * 3 * n + row;
+                v[k][0] = there ? p[0] : lowest;
+                v[k][1] = there ? p[n] : 0.f;
+                v[k][2] = there ? p[2 * n] : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) add(v[k][0], v[k][1], v[k][2]);
         }
     part[0][slice][r] = m;
     part[1][slice][r] = s;
     part[2][slice][r] = t;
-    __syncthreads();
+    for (int half = JOIN_SLICES / 2; half; half /= 2) {
+        __syncthreads();
+        if (slice < half) {
+            add(part[0][slice + half][r], part[1][slice + half][r], part[2][slice + half][r]);
+            part[0][slice][r] = m;
+            part[1][slice][r] = s;
+            part[2][slice][r] = t;
+        }
+    }
     if (slice || row >= n) return;
-    for (int i = 1; i < JOIN_SLICES; i++) add(part[0][i][r], part[1][i][r], part[2][i][r]);
     const bool empty = s == 0.f;
     const float lse2 = empty ? -INFINITY : m + log2f(s), h = empty ? 0.f : 0.69314718055994531f * (log2f(s) - t / s);
     const int64_t token = token_at(tokens, token_bytes, row);

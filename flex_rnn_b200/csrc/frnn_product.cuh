@@ -64,8 +64,8 @@ struct alignas(64) ProductArgs {
     const float* alpha;         // a factor on the device, or NULL
     // GLU_*
     int io, activation;
-    void *save_a, *save_b;      // the two products, [M][save_ld] of the type of io; written forward (NULL: not), read backward
-    int64_t save_ld;
+    void *by_gate, *by_up;      // b act'(a) and act(a), [M][by_ld] of the type of io; written forward (NULL: not), read backward
+    int64_t by_ld;
     Planes h, da, db;
     // LOGPROB_*
     float c2;                   // log2(e) / temperature
@@ -217,29 +217,75 @@ template <class T> __device__ __forceinline__ void get_row(const T* p, int cols,
         }
     }
 }
-__device__ __forceinline__ void get_row_as(int dtype, const void* p, int64_t at, int cols, float* v) {
-    if (dtype == FRNN_F32) get_row((const float*)p + at, cols, v);
-    else if (dtype == FRNN_BF16) get_row((const __nv_bfloat16*)p + at, cols, v);
-    else get_row((const __half*)p + at, cols, v);
+// The way back: 32 values of each lane's row out of 32 rows, read by neighbouring lanes (aligned rows; undefined beyond rows and cols).
+template <class T> __device__ __forceinline__ void get_rows(unsigned char* staging, int lane, const T* src, int64_t ld, int rows, int cols, float* v) {
+    constexpr int W = WIDE<T>, CHUNKS = 32 / W, ROW = 32 * (int)sizeof(T), AT_ONCE = 32 / CHUNKS;
+    auto slot = [](int r, int c) { return r * ROW + ((c ^ (sizeof(T) == 2 ? (r >> 1) & 3 : r & 7)) * 16); };
+    const int c = lane % CHUNKS;
+    if ((c + 1) * W <= (cols + W - 1) / W * W) {          // (rows are padded to whole accesses)
+        Pack<T, W> x[CHUNKS];
+#pragma unroll
+        for (int k = 0; k < CHUNKS; k++) {
+            const int r = k * AT_ONCE + lane / CHUNKS;
+            if (r < rows) x[k].load(src + r * ld + c * W);
+        }
+#pragma unroll
+        for (int k = 0; k < CHUNKS; k++) {
+            const int r = k * AT_ONCE + lane / CHUNKS;
+            if (r < rows) x[k].store((T*)(staging + slot(r, c)));
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+        Pack<T, W> x;
+        x.load((const T*)(staging + slot(lane, k)));
+        x.to(v + k * W);
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ void get_rows_as(int dtype, unsigned char* staging, int lane, const void* src, int64_t at, int64_t ld, int rows, int cols, float* v) {
+    if (dtype == FRNN_F32) get_rows(staging, lane, (const float*)src + at, ld, rows, cols, v);
+    else if (dtype == FRNN_BF16) get_rows(staging, lane, (const __nv_bfloat16*)src + at, ld, rows, cols, v);
+    else get_rows(staging, lane, (const __half*)src + at, ld, rows, cols, v);
 }
 
 // ---- activations -----------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float logistic(float a) { return 1.f / (1.f + __expf(-a)); }
-__device__ __forceinline__ float activate(int kind, float a) {
-    switch (kind) {
-        case FRNN_SILU: return a * logistic(a);
-        case FRNN_GELU: return a * (0.5f * erfcf(-0.70710678118654752f * a));
-        case FRNN_RELU: return a > 0.f || a != a ? a : 0.f;
-        default: return logistic(a);
+// h = act(a) b of N values, and where asked for its derivatives by a and b, in their place.  (One choice for all of them:
+// chosen for each value, the code of all four no longer fit the instruction cache, and a tile took five times as long.)
+template <int KIND> __device__ __forceinline__ void activate(float a, float& act, float& slope) {
+    if constexpr (KIND == FRNN_SILU || KIND == FRNN_SIGMOID) {
+        const float s = __fdividef(1.f, 1.f + __expf(-a));
+        act = KIND == FRNN_SILU ? a * s : s;
+        slope = KIND == FRNN_SILU ? fmaf(act, 1.f - s, s) : s * (1.f - s);
+    } else if constexpr (KIND == FRNN_GELU) {
+        const float half = 0.5f * erfcf(-0.70710678118654752f * a);
+        act = a * half;
+        slope = fmaf(a, 0.39894228040143268f * __expf(-0.5f * a * a), half);
+    } else {
+        act = a > 0.f || a != a ? a : 0.f;
+        slope = a > 0.f ? 1.f : 0.f;
     }
 }
-__device__ __forceinline__ float slope(int kind, float a) {
+template <int KIND, int N> __device__ __forceinline__ void glu_of(float* a, float* b, float* h, bool derivatives) {
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        float act, slope;
+        activate<KIND>(a[j], act, slope);
+        h[j] = act * b[j];
+        if (derivatives) {
+            a[j] = b[j] * slope;
+            b[j] = act;
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* b, float* h, bool derivatives) {
     switch (kind) {
-        case FRNN_SILU: { const float s = logistic(a); return s * (1.f + a * (1.f - s)); }
-        case FRNN_GELU: return 0.5f * erfcf(-0.70710678118654752f * a) + a * (0.39894228040143268f * __expf(-0.5f * a * a));
-        case FRNN_RELU: return a > 0.f ? 1.f : 0.f;
-        default: { const float s = logistic(a); return s * (1.f - s); }
+        case FRNN_SILU: return glu_of<FRNN_SILU, N>(a, b, h, derivatives);
+        case FRNN_GELU: return glu_of<FRNN_GELU, N>(a, b, h, derivatives);
+        case FRNN_RELU: return glu_of<FRNN_RELU, N>(a, b, h, derivatives);
+        default: return glu_of<FRNN_SIGMOID, N>(a, b, h, derivatives);
     }
 }
 
@@ -249,7 +295,7 @@ __device__ __forceinline__ float slope(int kind, float a) {
 // bit, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096, 2e-5 at 8192 in six segments, where 32-bit
 // sums rounded to nearest lose some 3e-7).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
 // instead, from parts of FLUSH steps, in registers, half of a tile's columns a warp.
-enum { FLUSH = 4 };
+enum { FLUSH = 16 };
 
 // Column of accumulators that a warp's i-th value lies in: its half of the tile's columns, or of both products' columns.
 template <int EPI, int BN> __device__ __forceinline__ int column_of(int half, int i) {
@@ -295,50 +341,35 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, const fl
     } else if constexpr (EPI == GLU_FORWARD) {
 #pragma unroll ROUNDS
         for (int i = 0; i < BN / 4; i += 32) {
-            const int c = half * (BN / 4) + i;
-            float a[32], b[32];
+            float a[32], b[32], h[32];
             take(i, a);
             take(BN / 4 + i, b);
-            const int col = tn * (BN / 2) + c, cols = min(32, p.N - col);
+            const int col = tn * (BN / 2) + half * (BN / 4) + i, cols = min(32, p.N - col);
             if (rows <= 0 || cols <= 0) continue;
-            if (p.save_a) {
-                const int64_t at = row0 * p.save_ld + col;
-                put_rows_as(p.io, staging, lane, a, p.save_a, at, p.save_ld, rows, cols, true);
-                put_rows_as(p.io, staging, lane, b, p.save_b, at, p.save_ld, rows, cols, true);
+            glu<32>(p.activation, a, b, h, p.by_gate);
+            if (p.by_gate) {
+                const int64_t at = row0 * p.by_ld + col;
+                put_rows_as(p.io, staging, lane, a, p.by_gate, at, p.by_ld, rows, cols, true);
+                put_rows_as(p.io, staging, lane, b, p.by_up, at, p.by_ld, rows, cols, true);
             }
-#pragma unroll
-            for (int j = 0; j < 32; j++) a[j] = activate(p.activation, a[j]) * b[j];
-            put_planes(p.io, staging, lane, a, p.h, row0, col, rows, cols);
+            put_planes(p.io, staging, lane, h, p.h, row0, col, rows, cols);
         }
     } else if constexpr (EPI == GLU_BACKWARD) {
 #pragma unroll ROUNDS
         for (int i = 0; i < BN / 2; i += 32) {
-            const int c = half * (BN / 2) + i;
-            float d[32], a[32], b[32];
+            float d[32], f[32];
             take(i, d);
-            const int col = tn * BN + c, cols = min(32, p.N - col);
+            const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
             if (rows <= 0 || cols <= 0) continue;
-            const int64_t at = row * p.save_ld + col;
+#pragma unroll 1
+            for (int k = 0; k < 2; k++) {
+                const Planes& to = k ? p.db : p.da;
+                if (!to.p) continue;
+                get_rows_as(p.io, staging, lane, k ? p.by_up : p.by_gate, row0 * p.by_ld + col, p.by_ld, rows, cols, f);
 #pragma unroll
-            for (int j = 0; j < 32; j++) a[j] = b[j] = 0.f;
-            if (lane < rows) {
-                get_row_as(p.io, p.save_a, at, cols, a);
-                get_row_as(p.io, p.save_b, at, cols, b);
+                for (int j = 0; j < 32; j++) f[j] *= d[j];
+                put_planes(p.io, staging, lane, f, to, row0, col, rows, cols);
             }
-            if (p.da.p) {
-                float t[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) t[j] = d[j] * b[j] * slope(p.activation, a[j]);
-                put_planes(p.io, staging, lane, t, p.da, row0, col, rows, cols);
-            }
-#pragma unroll
-            for (int j = 0; j < 32; j++) {
-                const float s = activate(p.activation, a[j]);
-                a[j] = d[j] * s;
-                b[j] *= s;
-            }
-            if (p.db.p) put_planes(p.io, staging, lane, a, p.db, row0, col, rows, cols);
-            if (p.h.p) put_planes(p.io, staging, lane, b, p.h, row0, col, rows, cols);
         }
     } else if constexpr (EPI == LOGPROB_STATS) {
         int64_t token = -1;
@@ -488,7 +519,7 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
                             tma_load<CG>(at, &p.a, k * BK, m, pa, bar);
                         }
                         if constexpr (BT) {
-    #pragma unroll
+#pragma unroll
                             for (int part = 0; part < NB / 64; part++) tma_load<CG>(at + A_BYTES + part * 8192, &p.b[p.map_b[g]], n + part * 64, k * BK, pb, bar);
                         } else if (!p.dual) {
                             tma_load<CG>(at + A_BYTES, &p.b[p.map_b[g]], k * BK, n, pb, bar);
@@ -524,7 +555,7 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
                             frnn_tmem_fence_after_sync();
                             const u32 at = frnn_smem_addr(smem + s * STAGE_BYTES);
                             const u64 a = operand_desc(at, 8192), b = operand_desc(at + A_BYTES, 8192);
-    #pragma unroll
+#pragma unroll
                             for (int k = 0; k < BK / 16; k++)      // 16 values of k: 32 bytes of a row, or 16 rows
                                 mma_f16<CG>(d, a + k * (AT ? 2048 / 16 : 32 / 16), b + k * (BT ? 2048 / 16 : 32 / 16), p.idesc, i > from || k > 0);
                             mma_commit<CG>(&empty[s]);
@@ -551,7 +582,7 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
             frnn_tmem_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_block(&acc_empty[t & 1], 0)) : "memory");
+                if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_block(&acc_empty[t & 1], 0)) : "memory");
                 else frnn_mbar_arrive(&acc_empty[t & 1]);
             }
             t++;
@@ -634,22 +665,21 @@ template <int EPI> __global__ void __launch_bounds__(256) finish_kernel(const __
         for (int e = 0; e < 4; e++) {
             if (col + e >= p.N) break;
             float x = (&v.x)[e];
-            const float y = (&w.x)[e];
             if constexpr (EPI == STORE) {
                 x *= alpha;
                 if (p.add) x += p.add[row * p.add_ld + col + e];
                 store_as(to_dtype, to, row * to_ld + col + e, x);
             } else if constexpr (EPI == GLU_FORWARD) {
-                if (p.save_a) {
-                    store_as(p.io, p.save_a, row * p.save_ld + col + e, x);
-                    store_as(p.io, p.save_b, row * p.save_ld + col + e, y);
+                float y = (&w.x)[e], h;
+                glu<1>(p.activation, &x, &y, &h, p.by_gate);
+                if (p.by_gate) {
+                    store_as(p.io, p.by_gate, row * p.by_ld + col + e, x);
+                    store_as(p.io, p.by_up, row * p.by_ld + col + e, y);
                 }
-                store_planes(p.io, p.h, row, col + e, activate(p.activation, x) * y);
+                store_planes(p.io, p.h, row, col + e, h);
             } else {
-                const float a = load_as(p.io, p.save_a, row * p.save_ld + col + e), b = load_as(p.io, p.save_b, row * p.save_ld + col + e), s = activate(p.activation, a);
-                if (p.da.p) store_planes(p.io, p.da, row, col + e, x * b * slope(p.activation, a));
-                if (p.db.p) store_planes(p.io, p.db, row, col + e, x * s);
-                if (p.h.p) store_planes(p.io, p.h, row, col + e, b * s);
+                if (p.da.p) store_planes(p.io, p.da, row, col + e, x * load_as(p.io, p.by_gate, row * p.by_ld + col + e));
+                if (p.db.p) store_planes(p.io, p.db, row, col + e, x * load_as(p.io, p.by_up, row * p.by_ld + col + e));
             }
         }
     }
@@ -657,14 +687,40 @@ template <int EPI> __global__ void __launch_bounds__(256) finish_kernel(const __
 
 // ---- operands -------------------------------------------------------------------------------------------------------------------
 
-// Rows of any type and stride as a 16-bit operand: rows on 16-byte boundaries, fp32 as three planes.
-template <class T> __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, Planes to, int io) {
-    const int64_t quads = (cols + 3) / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / quads, col = i % quads * 4;
+// Rows of any type and stride as a 16-bit operand: rows on 16-byte boundaries, fp32 as three planes.  A thread takes 8 columns.
+template <class T, bool WIDE_LOADS> __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, Planes to) {
+    const int64_t eights = (cols + 7) / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * eights; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / eights, col = i % eights * 8;
+        const T* const from = x + row * stride + col;
+        float v[8];
+        if (WIDE_LOADS && col + 8 <= cols) {
+            constexpr int W = WIDE<T>;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (col + e < cols) store_planes(io, to, row, col + e, to_float(x[row * stride + col + e]));
+            for (int c = 0; c < 8; c += W) {
+                Pack<T, W> q;
+                q.load(from + c);
+                q.to(v + c);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = col + e < cols ? to_float(from[e]) : 0.f;
+        }
+        if constexpr (sizeof(T) == 2) {
+            Pack<T, 8> q;
+            q.from(v);
+            q.store((T*)to.p + row * to.ld + col);
+        } else {
+            float part[3][8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) split3(v[e], part[0][e], part[1][e], part[2][e]);
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                Pack<__nv_bfloat16, 8> q;
+                q.from(part[k]);
+                q.store((__nv_bfloat16*)to.p + k * to.plane + row * to.ld + col);
+            }
+        }
     }
 }
 
@@ -718,10 +774,11 @@ inline int as_operand(Scratch& s, int dtype, const void* x, int64_t rows, int64_
     }
     o = new_operand(s, dtype, rows, cols);
     if (!s.base) return FRNN_OK;
-    const int64_t blocks = std::min<int64_t>((rows * ((cols + 3) / 4) + 255) / 256, (int64_t)sm_count() * 16);
+    const int64_t blocks = std::min<int64_t>((rows * ((cols + 7) / 8) + 255) / 256, (int64_t)sm_count() * 16);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        pack_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>((const T*)x, rows, cols, stride, o.writable(), dtype);
+        if (on_boundary(x, 16) && (rows == 1 || stride * sizeof(T) % 16 == 0)) pack_kernel<T, true><<<(unsigned)blocks, 256, 0, stream>>>((const T*)x, rows, cols, stride, o.writable());
+        else pack_kernel<T, false><<<(unsigned)blocks, 256, 0, stream>>>((const T*)x, rows, cols, stride, o.writable());
         return launched("matrix product: operand");
     });
 }
