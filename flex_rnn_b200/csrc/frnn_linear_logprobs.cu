@@ -13,10 +13,10 @@ using namespace frnn_lm;
 
 namespace {
 
-enum { JOIN_ROWS = 8, JOIN_SLICES = 64 };
-
-// Rows of partial results [blocks][3][n] joined: 64 threads a row take every 64th block, four at a time so that their loads are
-// under way together, then their results in order.
+// Rows of partial results [blocks][3][n] joined: SLICES threads a row take every SLICES-th block, four at a time so that their
+// loads are under way together, then their results in order.  32 rows a block where there are many (whole lines of the
+// partial results), 8 and more threads to each where there are few.
+template <int JOIN_ROWS, int JOIN_SLICES>
 __global__ void __launch_bounds__(JOIN_ROWS* JOIN_SLICES) join_kernel(const float* partial, const float* target, int64_t blocks, int64_t n, const void* tokens, int token_bytes, int64_t vocab,
                                                                       int64_t ignore_index, float* logprob, float* entropy, float* stats, int* err) {
     __shared__ float part[3][JOIN_SLICES][JOIN_ROWS];
@@ -134,8 +134,11 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
     q.args.target = (float*)s.take((size_t)c->n * 4);
     rc = run_product<LOGPROB_STATS, false, false>(what, q, s, stream);
     if (rc != FRNN_OK || !s.base) return rc;
-    join_kernel<<<(unsigned)((c->n + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_ROWS * JOIN_SLICES, 0, stream>>>(q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab, c->ignore_index,
-                                                                                                      logprob, entropy, stats, err);
+    auto join = [&](auto kernel, int rows, int slices) {
+        kernel<<<(unsigned)((c->n + rows - 1) / rows), rows * slices, 0, stream>>>(q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab, c->ignore_index, logprob, entropy, stats, err);
+    };
+    if (c->n >= 2048) join(join_kernel<32, 16>, 32, 16);
+    else join(join_kernel<8, 128>, 8, 128);
     return launched(what);
 }
 

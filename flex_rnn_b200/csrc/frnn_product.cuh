@@ -202,18 +202,35 @@ __device__ __forceinline__ void put_planes(int io, unsigned char* staging, int l
         }
     }
 }
-// 32 values of a lane's row (aligned rows; zeros beyond `cols`)
-template <class T> __device__ __forceinline__ void get_row(const T* p, int cols, float* v) {
+// 16 values of a lane's row, straight from its registers (aligned rows).
+template <class T> __device__ __forceinline__ void put_row(const float* v, T* dst, int cols) {
     constexpr int W = WIDE<T>;
 #pragma unroll
-    for (int c = 0; c < 32 / W; c++) {
-        if ((c + 1) * W <= cols) {
-            Pack<T, W> x;
-            x.load(p + c * W);
-            x.to(v + c * W);
-        } else {
+    for (int c = 0; c < 16; c += W) {
+        Pack<T, W> x;
+        x.from(v + c);
+        if (c < cols) x.store(dst + c);          // (rows are padded to whole accesses)
+    }
+}
+__device__ __forceinline__ void put_row_as(int dtype, const float* v, void* dst, int64_t at, int cols) {
+    if (dtype == FRNN_F32) put_row(v, (float*)dst + at, cols);
+    else if (dtype == FRNN_BF16) put_row(v, (__nv_bfloat16*)dst + at, cols);
+    else put_row(v, (__half*)dst + at, cols);
+}
+__device__ __forceinline__ void put_row_planes(int io, float* v, const Planes& to, int64_t at, int cols) {
+    if (io != FRNN_F32) {
+        put_row_as(io, v, to.p, at, cols);
+    } else {
+#pragma unroll 1
+        for (int plane = 0; plane < 3; plane++) {          // each round leaves the rest of the one before
+            float part[16];
 #pragma unroll
-            for (int e = 0; e < W; e++) v[c * W + e] = c * W + e < cols ? to_float(p[c * W + e]) : 0.f;
+            for (int j = 0; j < 16; j++) {
+                float mid, lo;
+                split3(v[j], part[j], mid, lo);
+                v[j] = fabsf(part[j]) < INFINITY ? v[j] - part[j] : 0.f;
+            }
+            put_row(part, (__nv_bfloat16*)to.p + plane * to.plane + at, cols);
         }
     }
 }
@@ -294,73 +311,78 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 // The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last
 // bit, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096, 2e-5 at 8192 in six segments, where 32-bit
 // sums rounded to nearest lose some 3e-7).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
-// instead, from parts of FLUSH steps, in registers, half of a tile's columns a warp.
+// instead, from parts of FLUSH steps, in registers, half of a tile's columns a warp; the sums go back to where the last part was, and
+// the epilogue is the same for all.  (One that took them from registers had its loops unrolled, and its code did not fit the instruction cache.)
 enum { FLUSH = 16 };
 
-// Column of accumulators that a warp's i-th value lies in: its half of the tile's columns, or of both products' columns.
-template <int EPI, int BN> __device__ __forceinline__ int column_of(int half, int i) {
-    if (EPI == GLU_FORWARD) return i < BN / 4 ? half * (BN / 4) + i : BN / 2 + half * (BN / 4) + i - BN / 4;
-    return half * (BN / 2) + i;
+// 32 columns of accumulators, of the lane's row.  (Waited for apart: the next ones are under way while these are worked on.)
+__device__ __forceinline__ void ask(u32 taddr, float* v) { frnn_tmem_ld<32>(taddr, v); }
+template <int N> __device__ __forceinline__ void wait_for(float* v) {
+    frnn_tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < N; j++) asm volatile("" : "+f"(v[j]));      // (nothing that uses them moves up)
 }
 
-template <int EPI, int BN, bool PROMOTE>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, const float* sum, int64_t row0, int tn, int slice, int half, int lane, unsigned char* staging) {
-    constexpr int ROUNDS = PROMOTE ? BN / 64 : 1;      // (registers are not indexed: unrolled)
-    auto take = [&](int i, float* v) {
-        if constexpr (PROMOTE) {
+template <int EPI, int BN>
+__device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t row0, int tn, int slice, int half, int lane, unsigned char* staging) {
+    // body(i, v) for each 32 of this warp's half of the tile's columns, of which the i-th lies in column half * BN / 2 + i
+    auto each = [&](auto body) {
+        const u32 mine = acc + half * (BN / 2);
+        float v[32], next[32];
+        ask(mine, v);
+#pragma unroll 1
+        for (int i = 0; i < BN / 2; i += 32) {
+            wait_for<32>(v);
+            if (i + 32 < BN / 2) ask(mine + i + 32, next);
+            body(i, v);
+            if (i + 32 < BN / 2) {
+                wait_for<32>(next);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = sum[i + j];
-        } else {
-            frnn_tmem_ld<32>(acc + column_of<EPI, BN>(half, i), v);
-            frnn_tmem_wait_ld();
+                for (int j = 0; j < 32; j++) v[j] = next[j];
+            }
         }
     };
     const int rows = (int)min((int64_t)32, max((int64_t)0, p.M - row0));
     const int64_t row = row0 + lane;
     if constexpr (EPI == STORE) {
         const float alpha = p.alpha ? *p.alpha : 1.f;
-#pragma unroll ROUNDS
-        for (int i = 0; i < BN / 2; i += 32) {
-            const int c = half * (BN / 2) + i;
-            float v[32];
-            take(i, v);
-            const int col = p.dual ? tn * (BN / 2) + c % (BN / 2) : tn * BN + c;
-            const int cols = min(32, p.N - col);
-            if (rows <= 0 || cols <= 0) continue;
+        each([&](int i, float* v) {
+            const int c = half * (BN / 2) + i, col = p.dual ? tn * (BN / 2) + c % (BN / 2) : tn * BN + c, cols = min(32, p.N - col);
+            if (rows <= 0 || cols <= 0) return;
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] *= alpha;
-            if (p.add && lane < rows) {
+            if (p.add) {
                 float o[32];
-                get_row(p.add + row * p.add_ld + col, cols, o);
+                get_rows(staging, lane, p.add + row0 * p.add_ld + col, p.add_ld, rows, cols, o);
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += o[j];
             }
             const int64_t at = slice * p.out_slice + row0 * p.out_ld + col + (p.dual && c >= BN / 2 ? p.out_ld / 2 : 0);
             put_rows_as(p.out_dtype, staging, lane, v, p.out, at, p.out_ld, rows, cols, p.out_wide);
-        }
+        });
     } else if constexpr (EPI == GLU_FORWARD) {
-#pragma unroll ROUNDS
-        for (int i = 0; i < BN / 4; i += 32) {
-            float a[32], b[32], h[32];
-            take(i, a);
-            take(BN / 4 + i, b);
-            const int col = tn * (BN / 2) + half * (BN / 4) + i, cols = min(32, p.N - col);
-            if (rows <= 0 || cols <= 0) continue;
-            glu<32>(p.activation, a, b, h, p.by_gate);
+        const u32 mine = acc + half * (BN / 4);
+#pragma unroll 1
+        for (int i = 0; i < BN / 4; i += 16) {          // (16 values of each: full 32-byte sectors, and half the code)
+            float a[16], b[16], h[16];
+            frnn_tmem_ld<16>(mine + i, a);
+            frnn_tmem_ld<16>(mine + BN / 2 + i, b);
+            wait_for<16>(a);
+            wait_for<16>(b);
+            const int col = tn * (BN / 2) + half * (BN / 4) + i, cols = min(16, p.N - col);
+            if (lane >= rows || cols <= 0) continue;
+            glu<16>(p.activation, a, b, h, p.by_gate);
             if (p.by_gate) {
-                const int64_t at = row0 * p.by_ld + col;
-                put_rows_as(p.io, staging, lane, a, p.by_gate, at, p.by_ld, rows, cols, true);
-                put_rows_as(p.io, staging, lane, b, p.by_up, at, p.by_ld, rows, cols, true);
+                put_row_as(p.io, a, p.by_gate, row * p.by_ld + col, cols);
+                put_row_as(p.io, b, p.by_up, row * p.by_ld + col, cols);
             }
-            put_planes(p.io, staging, lane, h, p.h, row0, col, rows, cols);
+            put_row_planes(p.io, h, p.h, row * p.h.ld + col, cols);
         }
     } else if constexpr (EPI == GLU_BACKWARD) {
-#pragma unroll ROUNDS
-        for (int i = 0; i < BN / 2; i += 32) {
-            float d[32], f[32];
-            take(i, d);
+        each([&](int i, float* d) {
+            float f[32];
             const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
-            if (rows <= 0 || cols <= 0) continue;
+            if (rows <= 0 || cols <= 0) return;
 #pragma unroll 1
             for (int k = 0; k < 2; k++) {
                 const Planes& to = k ? p.db : p.da;
@@ -370,45 +392,37 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, const fl
                 for (int j = 0; j < 32; j++) f[j] *= d[j];
                 put_planes(p.io, staging, lane, f, to, row0, col, rows, cols);
             }
-        }
+        });
     } else if constexpr (EPI == LOGPROB_STATS) {
         int64_t token = -1;
         if (lane < rows) token = token_at(p.tokens, p.token_bytes, row);
         float m = -3.4028235e38f, s = 0.f, t = 0.f;
-#pragma unroll ROUNDS
-        for (int i = 0; i < BN / 2; i += 32) {
-            const int c = half * (BN / 2) + i;
-            float v[32];
-            take(i, v);
-            const int col = tn * BN + c, cols = min(32, p.N - col);
-            if (cols <= 0) continue;
-            float top = m;
+        each([&](int i, float* v) {
+            const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
+            if (cols <= 0) return;
+            const int64_t hit = token - p.first - col;
+            float top = m, x = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; j++) {
                 v[j] = j < cols ? v[j] * p.c2 : -INFINITY;
                 top = fmaxf(top, v[j]);
+                if (hit == j) x += v[j];          // (a choice of one becomes an index into registers, which then all live in memory)
             }
-            const int64_t hit = token - p.first - col;
-            if (hit >= 0 && hit < cols && lane < rows) {
-#pragma unroll 1
-                for (int j = 0; j < 32; j++) {
-                    float x = v[0];
-#pragma unroll
-                    for (int i = 1; i < 32; i++) x = i == j ? v[i] : x;
-                    if (j == (int)hit) p.target[row] = x;
-                }
-            }
+            if (hit >= 0 && hit < cols && lane < rows) p.target[row] = x;
             const float down = exp2_fast(m - top);
             t = s == 0.f ? 0.f : down * (t + s * (m - top));
             s *= down;
+            float s4[4] = {}, t4[4] = {};
 #pragma unroll
             for (int j = 0; j < 32; j++) {
                 const float u = v[j] - top, e = exp2_fast(u);
-                s += e;
-                t = fmaf(e, fmaxf(u, -1e30f), t);
+                s4[j % 4] += e;
+                t4[j % 4] = fmaf(e, fmaxf(u, -1e30f), t4[j % 4]);
             }
+            s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            t += (t4[0] + t4[1]) + (t4[2] + t4[3]);
             m = top;
-        }
+        });
         if (lane < rows) {
             float* to = p.partial + (int64_t)(tn * 2 + half) * 3 * p.M + row;
             to[0] = m;
@@ -428,13 +442,9 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, const fl
             empty = lse2 == -INFINITY;
         }
         const float k = p.inv_t * (p.scale ? *p.scale : 1.f);
-#pragma unroll ROUNDS
-        for (int i = 0; i < BN / 2; i += 32) {
-            const int c = half * (BN / 2) + i;
-            float v[32];
-            take(i, v);
-            const int col = tn * BN + c, cols = min(32, p.N - col);
-            if (rows <= 0 || cols <= 0) continue;
+        each([&](int i, float* v) {
+            const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
+            if (rows <= 0 || cols <= 0) return;
             const int64_t hit = token - p.first - col;
 #pragma unroll
             for (int j = 0; j < 32; j++) {
@@ -444,7 +454,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, const fl
                 v[j] = empty ? 0.f : d * k;
             }
             put_planes(p.io, staging, lane, v, p.grad, row0, col, rows, cols);
-        }
+        });
     }
 }
 
@@ -590,28 +600,40 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
         for (int u = first; ok && u < units; u += stride) {
             const Unit w = unit_of(p, u);
             const int64_t row0 = (int64_t)(w.tm * CG + (int)rank) * 128 + quarter * 32;
+            u32 acc = filled();
+            if (!ok) break;
             if constexpr (PROMOTE) {
-                float sum[BN / 2];
-                for (int from = w.from; from < w.to; from += FLUSH) {
-                    const u32 acc = filled();
+                if (w.from + FLUSH < w.to) {
+                    float sum[BN / 2];
+#pragma unroll
+                    for (int i = 0; i < BN / 2; i += 32) ask(acc + half * (BN / 2) + i, sum + i);
+                    wait_for<BN / 2>(sum);
+                    for (int from = w.from + FLUSH; from < w.to; from += FLUSH) {
+                        emptied();
+                        acc = filled();
+                        if (!ok) break;
+#pragma unroll
+                        for (int i = 0; i < BN / 2; i += 32) {
+                            float v[32];
+                            ask(acc + half * (BN / 2) + i, v);
+                            wait_for<32>(v);
+#pragma unroll
+                            for (int j = 0; j < 32; j++) sum[i + j] += v[j];
+                        }
+                    }
                     if (!ok) break;
 #pragma unroll
-                    for (int i = 0; i < BN / 2; i += 32) {
-                        float v[32];
-                        frnn_tmem_ld<32>(acc + column_of<EPI, BN>(half, i), v);
-                        frnn_tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; j++) sum[i + j] = from == w.from ? v[j] : sum[i + j] + v[j];
+                    for (int i = 0; i < BN / 2; i += 32) frnn_tmem_st<32>(acc + half * (BN / 2) + i, sum + i);
+                    frnn_tmem_wait_st();
+                    if constexpr (EPI == GLU_FORWARD) {      // (a warp's columns of the two products lie in both warps' halves)
+                        frnn_tmem_fence_before_sync();
+                        frnn_group_sync(1 + quarter, 64);
+                        frnn_tmem_fence_after_sync();
                     }
-                    emptied();
                 }
-                if (ok) epilogue<EPI, BN, true>(p, 0, sum, row0, w.tn, w.slice, half, lane, staging);
-            } else {
-                const u32 acc = filled();
-                if (!ok) break;
-                epilogue<EPI, BN, false>(p, acc, nullptr, row0, w.tn, w.slice, half, lane, staging);
-                emptied();
             }
+            epilogue<EPI, BN>(p, acc, row0, w.tn, w.slice, half, lane, staging);
+            emptied();
         }
     }
     frnn_tmem_fence_before_sync();
