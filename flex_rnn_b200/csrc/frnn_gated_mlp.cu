@@ -49,13 +49,13 @@ Operand kept(const frnn_gated_mlp_call* c, const void* hidden) {
 
 int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, void* hidden, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "gated_mlp";
-    Operand x, gate, up, down;
-    int rc = as_operand(s, c->dtype, c->x, c->n, c->width, c->x_stride, x, stream);
-    if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->gate, c->hidden, c->width, c->gate_stride, gate, stream);
-    if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->up, c->hidden, c->width, c->up_stride, up, stream);
-    if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->down, c->out_width, c->hidden, c->down_stride, down, stream);
-    if (rc != FRNN_OK) return rc;
+    Packs packs = {};
+    const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), gate = as_operand(s, packs, c->dtype, c->gate, c->hidden, c->width, c->gate_stride);
+    const Operand up = as_operand(s, packs, c->dtype, c->up, c->hidden, c->width, c->up_stride), down = as_operand(s, packs, c->dtype, c->down, c->out_width, c->hidden, c->down_stride);
     const Operand h = hidden ? kept(c, hidden) : new_operand(s, c->dtype, c->n, c->hidden);
+    if (!s.base) return FRNN_OK;
+    int rc = pack(packs, c->dtype, stream);
+    if (rc != FRNN_OK) return rc;
     {
         Product q = product(c, c->n, c->hidden, c->width);
         q.a = x;
@@ -67,7 +67,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, v
         q.args.by_up = by_up;
         q.args.by_ld = padded(c->hidden);
         q.args.h = h.writable();
-        rc = run_product<GLU_FORWARD, false, false>(what, q, s, stream);
+        rc = run_product<GLU_FORWARD, false, false>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }
     Product q = product(c, c->n, c->out_width, c->hidden);
@@ -77,24 +77,27 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, v
     q.out = y;
     q.out_dtype = c->dtype;
     q.out_ld = c->out_width;
-    return run_product<STORE, false, false>(what, q, s, stream);
+    return run_product<STORE, false, false>(what, q, stream);
 }
 
 int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* by_gate, const void* by_up, const void* hidden, void* dx, void* dgate, void* dup, void* ddown, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "gated_mlp_backward";
     const bool count = !s.base, want_x = count || dx, want_gate = count || dgate, want_up = count || dup, want_down = count || ddown, want_hidden = want_x || want_gate || want_up;
-    Operand x, gate, up, down, g;
-    int rc = as_operand(s, c->dtype, dy, c->n, c->out_width, dy_stride, g, stream);
-    if (rc == FRNN_OK && (want_gate || want_up)) rc = as_operand(s, c->dtype, c->x, c->n, c->width, c->x_stride, x, stream);
-    if (rc == FRNN_OK && want_x) rc = as_operand(s, c->dtype, c->gate, c->hidden, c->width, c->gate_stride, gate, stream);
-    if (rc == FRNN_OK && want_x) rc = as_operand(s, c->dtype, c->up, c->hidden, c->width, c->up_stride, up, stream);
-    if (rc == FRNN_OK && want_hidden) rc = as_operand(s, c->dtype, c->down, c->out_width, c->hidden, c->down_stride, down, stream);
-    if (rc != FRNN_OK) return rc;
+    Packs packs = {};
+    Operand x, gate, up, down;
+    const Operand g = as_operand(s, packs, c->dtype, dy, c->n, c->out_width, dy_stride);
+    if (want_gate || want_up) x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride);
+    if (want_x) gate = as_operand(s, packs, c->dtype, c->gate, c->hidden, c->width, c->gate_stride);
+    if (want_x) up = as_operand(s, packs, c->dtype, c->up, c->hidden, c->width, c->up_stride);
+    if (want_hidden) down = as_operand(s, packs, c->dtype, c->down, c->out_width, c->hidden, c->down_stride);
     const int planes = planes_of(c->dtype);
     const Operand both = new_operand(s, c->dtype, c->n, c->hidden, 2);      // da, db
     Operand da = both, db = both;
     da.planes = db.planes = planes;
     db.p = (const char*)both.p + both.plane * planes * 2;
+    if (count) return FRNN_OK;
+    int rc = pack(packs, c->dtype, stream);
+    if (rc != FRNN_OK) return rc;
     auto store = [&](Product& q, void* out, int64_t ld) {
         q.args.err = err;
         q.out = out;
@@ -105,14 +108,13 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         Product q = product(c, c->n, c->hidden, c->out_width);
         q.a = g;
         q.b[0] = down;
-        q.bt = true;
         q.args.err = err;
         q.args.by_gate = const_cast<void*>(by_gate);
         q.args.by_up = const_cast<void*>(by_up);
         q.args.by_ld = padded(c->hidden);
         if (want_x || want_gate) q.args.da = da.writable();
         if (want_x || want_up) q.args.db = db.writable();
-        rc = run_product<GLU_BACKWARD, false, true>(what, q, s, stream);
+        rc = run_product<GLU_BACKWARD, false, true>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }
     if (want_down) {
@@ -120,7 +122,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.a = g;
         q.b[0] = kept(c, hidden);
         store(q, ddown, c->hidden);
-        rc = run_product<STORE, true, true>(what, q, s, stream);
+        rc = run_product<STORE, true, true>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }
     for (int i = 0; i < 2; i++) {
@@ -129,7 +131,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.a = i ? db : da;
         q.b[0] = x;
         store(q, i ? dup : dgate, c->width);
-        rc = run_product<STORE, true, true>(what, q, s, stream);
+        rc = run_product<STORE, true, true>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }
     if (want_x) {
@@ -139,7 +141,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.b[1] = up;
         q.pairs = 2;
         store(q, dx, c->width);
-        rc = run_product<STORE, false, true>(what, q, s, stream);
+        rc = run_product<STORE, false, true>(what, q, stream);
     }
     return rc;
 }

@@ -124,16 +124,17 @@ Product logits(const frnn_linear_logprobs_call* c, const Operand& x, const Opera
 
 int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, float* stats, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "linear_logprobs";
-    Operand x, w;
-    int rc = as_operand(s, c->dtype, c->x, c->n, c->width, c->x_stride, x, stream);
-    if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->weight, c->vocab, c->width, c->weight_stride, w, stream);
-    if (rc != FRNN_OK) return rc;
+    Packs packs = {};
+    const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), w = as_operand(s, packs, c->dtype, c->weight, c->vocab, c->width, c->weight_stride);
     Product q = logits(c, x, w, 0, err);
-    const int64_t blocks = plan_product(q, false).tiles_n * 2;
+    const ProductPlan plan = plan_product<LOGPROB_STATS, false, false>(q);
+    const int64_t blocks = plan.tiles_n * (plan.form == PAIR ? 256 : 128) / plan.columns();
     q.args.partial = (float*)s.take((size_t)blocks * 3 * c->n * 4);
     q.args.target = (float*)s.take((size_t)c->n * 4);
-    rc = run_product<LOGPROB_STATS, false, false>(what, q, s, stream);
-    if (rc != FRNN_OK || !s.base) return rc;
+    if (!s.base) return FRNN_OK;
+    int rc = pack(packs, c->dtype, stream);
+    if (rc == FRNN_OK) rc = run_product<LOGPROB_STATS, false, false>(what, q, stream);
+    if (rc != FRNN_OK) return rc;
     auto join = [&](auto kernel, int rows, int slices) {
         kernel<<<(unsigned)((c->n + rows - 1) / rows), rows * slices, 0, stream>>>(q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab, c->ignore_index, logprob, entropy, stats, err);
     };
@@ -145,25 +146,23 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
 int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const float* dentropy, const float* stats, void* dx, void* dweight, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "linear_logprobs_backward";
     const bool count = !s.base, want_x = count || dx, want_w = count || dweight;
-    Operand x, w;
-    int rc = as_operand(s, c->dtype, c->x, c->n, c->width, c->x_stride, x, stream);
-    if (rc == FRNN_OK) rc = as_operand(s, c->dtype, c->weight, c->vocab, c->width, c->weight_stride, w, stream);
-    if (rc != FRNN_OK) return rc;
+    Packs packs = {};
+    const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), w = as_operand(s, packs, c->dtype, c->weight, c->vocab, c->width, c->weight_stride);
     // pieces of up to 2^28 elements of the logits' gradient (512 MB; half as many in three planes), whole tiles of 256 columns
     const int64_t most = std::max<int64_t>(256, ((c->dtype == FRNN_F32 ? 1ll << 27 : 1ll << 28) / c->n) / 256 * 256), pieces = (c->vocab + most - 1) / most;
     const int64_t piece = pieces == 1 ? c->vocab : std::min(most, ((c->vocab + pieces - 1) / pieces + 255) / 256 * 256);
     const Operand grad = new_operand(s, c->dtype, c->n, piece);
     float* const sum = pieces > 1 ? (float*)s.take((size_t)c->n * padded(c->width) * 4) : nullptr;
     float* const range = c->dtype == FRNN_F16 ? (float*)s.take(8) : nullptr;
-    if (range && !count) {
+    if (count) return FRNN_OK;
+    int rc = pack(packs, c->dtype, stream);
+    if (rc != FRNN_OK) return rc;
+    if (range) {
         range_kernel<<<1, 1024, 0, stream>>>(dlogprob, dentropy, c->n, (float)(1.0 / c->temperature), range);
         rc = launched(what);
         if (rc != FRNN_OK) return rc;
     }
-    const Scratch before = s;
-    size_t used = s.used;
     for (int64_t v = 0; v < c->vocab; v += piece) {
-        s = before;                                // (partial sums of one product are not needed by the next piece's)
         const int64_t cols = std::min(piece, c->vocab - v);
         const bool first = v == 0, last = v + cols == c->vocab;
         const Operand part = w.from_row(v, cols);
@@ -176,7 +175,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.args.stats = stats;
             q.args.scale = range;
             q.args.grad = g.writable();
-            rc = run_product<LOGPROB_GRAD, false, false>(what, q, s, stream);
+            rc = run_product<LOGPROB_GRAD, false, false>(what, q, stream);
             if (rc != FRNN_OK) return rc;
         }
         if (want_x) {
@@ -194,7 +193,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.out = last ? dx : sum;
             q.out_dtype = last ? c->dtype : (int)FRNN_F32;
             q.out_ld = last ? c->width : padded(c->width);
-            rc = run_product<STORE, false, true>(what, q, s, stream);
+            rc = run_product<STORE, false, true>(what, q, stream);
             if (rc != FRNN_OK) return rc;
         }
         if (want_w) {
@@ -207,15 +206,13 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.b[0] = x;
             q.args.err = err;
             q.args.alpha = range ? range + 1 : nullptr;
-            q.out = count ? nullptr : (char*)dweight + v * c->width * dtype_bytes(c->dtype);
+            q.out = (char*)dweight + v * c->width * dtype_bytes(c->dtype);
             q.out_dtype = c->dtype;
             q.out_ld = c->width;
-            rc = run_product<STORE, true, true>(what, q, s, stream);
+            rc = run_product<STORE, true, true>(what, q, stream);
             if (rc != FRNN_OK) return rc;
         }
-        used = std::max(used, s.used);
     }
-    s.used = used;
     return FRNN_OK;
 }
 

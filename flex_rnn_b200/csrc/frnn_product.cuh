@@ -13,13 +13,17 @@
 // edges TMA fills in zeros, so that sizes need not be multiples of anything; rows have to start on 16-byte boundaries.
 //
 // Roles: one thread issues copies (6 stages of 32 KB under way), one the products, 8 warps take finished accumulators out of
-// Tensor Memory (which holds two sets, so that the next tile's products run meanwhile).  Blocks stay for several tiles.  CG = 2:
-// a pair of blocks computes 256 rows, each holds half of B's rows, so that a byte of B in shared memory serves 256 rows; without
-// pairs (CG = 1, tiles of 128 x 128) small products spread over more multiprocessors, and k is split where that is not enough.
+// Tensor Memory (which holds two sets, so that the next tile's products run meanwhile).  Blocks stay for several tiles.  Three forms:
+//   PAIR   256 x 256 by a pair of blocks, each with half of B's rows, so that a byte of B in shared memory serves 256 rows
+//   ALONE  128 x 128 by a block: small products spread over more multiprocessors
+//   SPLIT  128 x 128 by a cluster of 2, 4 or 8 blocks, each with a part of k.  Each block then owns a part of the tile's columns: the others
+//          send it their sums of these (st.async into its shared memory), it adds them in the order of the blocks and has the epilogue
+//          to itself.  (4 stages, and 64 KB for what arrives.)
 #pragma once
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "frnn_lm.cuh"
 
@@ -31,10 +35,11 @@ int frnn_tensor_map_swizzled(void* out_map, const void* base, uint64_t cols, uin
 
 namespace frnn_lm {
 
-enum { BK = 64, STAGES = 6, STAGE_BYTES = 32768, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
+enum Form { PAIR, ALONE, SPLIT };
+enum { BK = 64, STAGE_BYTES = 32768, EXCHANGE_BYTES = 65536, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
 // Registers of the warps that copy and issue, and of the epilogue's: 128 x 56 + 256 x 224 = 384 x 168, what a block starts with.
 enum { CONTROL_REGISTERS = 56, EPILOGUE_REGISTERS = 224, START_REGISTERS = 168 };
-enum { PRODUCT_SHARED = STAGES * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };
+enum { PRODUCT_SHARED = 6 * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };      // (4 stages and what arrives: as much)
 enum { CODE_PRODUCT = 97 };       // error word: a wait inside a matrix product ran out
 
 // What becomes of a tile.
@@ -50,14 +55,14 @@ struct alignas(64) ProductArgs {
     CUtensorMap a, b[2];
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
     int ksteps, segments;       // steps of 64 along k in a segment
-    int tiles_m, tiles_n, slices, group;
+    int tiles_m, tiles_n, group;
     int dual;                   // a tile's columns are half of B0's rows and half of B1's
     unsigned idesc;
     int* err;
     unsigned char plane_a[MAX_SEGMENTS], map_b[MAX_SEGMENTS], plane_b[MAX_SEGMENTS];
     // STORE
     void* out;
-    int64_t out_ld, out_slice;  // out_slice: elements between the partial sums of two slices of k
+    int64_t out_ld;
     int out_dtype, out_wide;    // wide: rows start on 16-byte boundaries
     const float* add;           // fp32 [M][add_ld] to add, or NULL
     int64_t add_ld;
@@ -73,7 +78,7 @@ struct alignas(64) ProductArgs {
     const void* tokens;
     int token_bytes;
     int64_t ignore_index, first;      // first: token of column 0
-    float* partial;             // STATS: [block of columns][max, sum, sum of products][M]
+    float* partial;             // STATS: [columns / stats_columns][max, sum, sum of products][M]
     float* target;              // STATS: [M] of u at the row's token
     const float *stats, *dlogprob, *dentropy;      // GRAD: [M][2] log2 of the sum, entropy
     const float* scale;         // GRAD: a power of two that brings fp16 gradients into range, or NULL
@@ -90,6 +95,11 @@ __device__ __forceinline__ u32 cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ u32 cluster_blocks() {
+    u32 r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
 // the address of the same variable in block `rank` of the cluster
 __device__ __forceinline__ u32 in_block(const void* p, u32 rank) {
     u32 r;
@@ -101,6 +111,31 @@ template <int CG> __device__ __forceinline__ void tma_load(u32 dst, const CUtens
         asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((u64)map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
     else
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((u64)map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// 16 bytes to another block's shared memory, counted by its mbarrier when they are there
+__device__ __forceinline__ void send(u32 dst, float a, float b, float c, float d, u32 bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_at(u32 bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// frnn_mbar_wait for what other blocks of the cluster have written
+__device__ __forceinline__ bool wait_for_cluster(u64* bar, u32 parity, int* err) {
+    auto there = [&] {
+        u32 ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(frnn_smem_addr(bar)), "r"(parity) : "memory");
+        return ok != 0;
+    };
+    if (there()) return true;
+    const u64 from = frnn_now_ns();
+#pragma unroll 1
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (there()) return true;
+        if (frnn_now_ns() - from > FRNN_WAIT_LIMIT_NS) {
+            frnn_report(err, CODE_PRODUCT);
+            return false;
+        }
+    }
 }
 template <int CG> __device__ __forceinline__ void mma_f16(u32 d, u64 a, u64 b, u32 idesc, bool accumulate) {
     if constexpr (CG == 2)
@@ -323,19 +358,20 @@ template <int N> __device__ __forceinline__ void wait_for(float* v) {
     for (int j = 0; j < N; j++) asm volatile("" : "+f"(v[j]));      // (nothing that uses them moves up)
 }
 
-template <int EPI, int BN>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t row0, int tn, int slice, int half, int lane, unsigned char* staging) {
-    // body(i, v) for each 32 of this warp's half of the tile's columns, of which the i-th lies in column half * BN / 2 + i
+// `count` columns from the one numbered `first` on, whose accumulators lie at `acc` (of GLU_FORWARD's second product at `acc2`), of the 32
+// rows from row0 on.
+template <int EPI>
+__device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, u32 acc2, int64_t row0, int first, int count, int lane, unsigned char* staging) {
+    // body(col, cols, v) for each 32 columns
     auto each = [&](auto body) {
-        const u32 mine = acc + half * (BN / 2);
         float v[32], next[32];
-        ask(mine, v);
+        ask(acc, v);
 #pragma unroll 1
-        for (int i = 0; i < BN / 2; i += 32) {
+        for (int i = 0; i < count; i += 32) {
             wait_for<32>(v);
-            if (i + 32 < BN / 2) ask(mine + i + 32, next);
-            body(i, v);
-            if (i + 32 < BN / 2) {
+            if (i + 32 < count) ask(acc + i + 32, next);
+            body(first + i, min(32, min(count - i, p.N - first - i)), v);
+            if (i + 32 < count) {
                 wait_for<32>(next);
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = next[j];
@@ -346,8 +382,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
     const int64_t row = row0 + lane;
     if constexpr (EPI == STORE) {
         const float alpha = p.alpha ? *p.alpha : 1.f;
-        each([&](int i, float* v) {
-            const int c = half * (BN / 2) + i, col = p.dual ? tn * (BN / 2) + c % (BN / 2) : tn * BN + c, cols = min(32, p.N - col);
+        each([&](int col, int cols, float* v) {
             if (rows <= 0 || cols <= 0) return;
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] *= alpha;
@@ -357,19 +392,17 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += o[j];
             }
-            const int64_t at = slice * p.out_slice + row0 * p.out_ld + col + (p.dual && c >= BN / 2 ? p.out_ld / 2 : 0);
-            put_rows_as(p.out_dtype, staging, lane, v, p.out, at, p.out_ld, rows, cols, p.out_wide);
+            put_rows_as(p.out_dtype, staging, lane, v, p.out, row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide);
         });
     } else if constexpr (EPI == GLU_FORWARD) {
-        const u32 mine = acc + half * (BN / 4);
 #pragma unroll 1
-        for (int i = 0; i < BN / 4; i += 16) {          // (16 values of each: full 32-byte sectors, and half the code)
+        for (int i = 0; i < count; i += 16) {          // (16 values of each: full 32-byte sectors, and half the code)
             float a[16], b[16], h[16];
-            frnn_tmem_ld<16>(mine + i, a);
-            frnn_tmem_ld<16>(mine + BN / 2 + i, b);
+            frnn_tmem_ld<16>(acc + i, a);
+            frnn_tmem_ld<16>(acc2 + i, b);
             wait_for<16>(a);
             wait_for<16>(b);
-            const int col = tn * (BN / 2) + half * (BN / 4) + i, cols = min(16, p.N - col);
+            const int col = first + i, cols = min(16, min(count - i, p.N - col));
             if (lane >= rows || cols <= 0) continue;
             glu<16>(p.activation, a, b, h, p.by_gate);
             if (p.by_gate) {
@@ -379,9 +412,8 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
             put_row_planes(p.io, h, p.h, row * p.h.ld + col, cols);
         }
     } else if constexpr (EPI == GLU_BACKWARD) {
-        each([&](int i, float* d) {
+        each([&](int col, int cols, float* d) {
             float f[32];
-            const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
             if (rows <= 0 || cols <= 0) return;
 #pragma unroll 1
             for (int k = 0; k < 2; k++) {
@@ -397,8 +429,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
         int64_t token = -1;
         if (lane < rows) token = token_at(p.tokens, p.token_bytes, row);
         float m = -3.4028235e38f, s = 0.f, t = 0.f;
-        each([&](int i, float* v) {
-            const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
+        each([&](int col, int cols, float* v) {
             if (cols <= 0) return;
             const int64_t hit = token - p.first - col;
             float top = m, x = 0.f;
@@ -424,7 +455,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
             m = top;
         });
         if (lane < rows) {
-            float* to = p.partial + (int64_t)(tn * 2 + half) * 3 * p.M + row;
+            float* to = p.partial + (int64_t)(first / count) * 3 * p.M + row;
             to[0] = m;
             to[p.M] = s;
             to[2 * (int64_t)p.M] = t;
@@ -442,8 +473,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
             empty = lse2 == -INFINITY;
         }
         const float k = p.inv_t * (p.scale ? *p.scale : 1.f);
-        each([&](int i, float* v) {
-            const int col = tn * BN + half * (BN / 2) + i, cols = min(32, p.N - col);
+        each([&](int col, int cols, float* v) {
             if (rows <= 0 || cols <= 0) return;
             const int64_t hit = token - p.first - col;
 #pragma unroll
@@ -460,33 +490,31 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, int64_t 
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
-struct Unit { int tm, tn, slice, from, to; };      // a tile and a range of its steps along k
+struct Tile { int tm, tn; };
 
 // Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
-__device__ __forceinline__ Unit unit_of(const ProductArgs& p, int u) {
-    Unit r;
-    r.slice = u % p.slices;
-    const int tile = u / p.slices, a_group = p.group * p.tiles_n, g = tile / a_group, in = tile % a_group, high = min(p.group, p.tiles_m - g * p.group);
-    r.tm = g * p.group + in % high;
-    r.tn = in / high;
-    const int64_t steps = (int64_t)p.ksteps * p.segments;
-    r.from = (int)(steps * r.slice / p.slices);
-    r.to = (int)(steps * (r.slice + 1) / p.slices);
-    return r;
+__device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u) {
+    const int a_group = p.group * p.tiles_n, g = u / a_group, in = u % a_group, high = min(p.group, p.tiles_m - g * p.group);
+    return {g * p.group + in % high, in / high};
 }
 
 // AT, BT: the operand's rows run along m (n) instead of k.
-template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
+template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
+    constexpr int CG = FORM == PAIR ? 2 : 1, BN = FORM == PAIR ? 256 : 128, STAGES = FORM == SPLIT ? 4 : 6;
     constexpr int NB = BN / CG;                        // B's rows in this block
-    constexpr u32 A_BYTES = 128 * BK * 2, B_BYTES = NB * BK * 2, COLUMNS = 2 * BN;
+    constexpr u32 A_BYTES = 128 * BK * 2, B_BYTES = NB * BK * 2, COLUMNS = FORM == SPLIT ? 512 : 2 * BN;
     static_assert(A_BYTES + B_BYTES <= STAGE_BYTES && COLUMNS <= 512, "a stage or Tensor Memory is too small");
     extern __shared__ unsigned char raw[];
-    __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+    __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], arrived, taken;
     __shared__ u32 tmem;
     unsigned char* const smem = raw + (1024 - (frnn_smem_addr(raw) & 1023)) % 1024;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const u32 rank = CG == 2 ? cluster_rank() : 0;
-    const int units = p.tiles_m * p.tiles_n * p.slices, first = blockIdx.x / CG, stride = gridDim.x / CG;
+    const u32 rank = FORM == ALONE ? 0 : cluster_rank(), blocks = FORM == ALONE ? 1 : cluster_blocks();
+    const u32 half_m = FORM == PAIR ? rank : 0;        // which 128 of a tile's rows
+    const int tiles = p.tiles_m * p.tiles_n, first = blockIdx.x / blocks, stride = gridDim.x / blocks;
+    // this block's steps along k
+    const int64_t steps = (int64_t)p.ksteps * p.segments;
+    const int k_from = FORM == SPLIT ? (int)(steps * rank / blocks) : 0, k_to = FORM == SPLIT ? (int)(steps * (rank + 1) / blocks) : (int)steps;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -497,14 +525,22 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
             frnn_mbar_init(&acc_full[b], 1);
             frnn_mbar_init(&acc_empty[b], EPILOGUE_WARPS * CG);
         }
+        if (FORM == SPLIT) {
+            frnn_mbar_init(&arrived, 1);
+            frnn_mbar_init(&taken, EPILOGUE_WARPS * blocks);
+        }
         frnn_mbar_init_fence();
     }
+    if (warp == 1 && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"((u64)(lane ? &p.b[lane - 1] : &p.a)) : "memory");
     __syncwarp();
     if (warp == 2) tmem_alloc<CG>(&tmem, COLUMNS);
     frnn_tmem_fence_before_sync();
-    if constexpr (CG == 2) cluster_sync();
+    if constexpr (FORM != ALONE) cluster_sync();
     __syncthreads();
     frnn_tmem_fence_after_sync();
+    // Up to here nothing has been read that a kernel before this one may still be writing; the next one may come as far.
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
 
     if (warp < 4) {
         frnn_regs_release<CONTROL_REGISTERS>();
@@ -512,14 +548,14 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
             if (frnn_elect()) {
                 u32 it = 0;
                 bool ok = true;
-                for (int u = first; ok && u < units; u += stride) {
-                    const Unit w = unit_of(p, u);
-                    const int m = (w.tm * CG + (int)rank) * 128, n = p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)rank * NB;
-                    int g = w.from / p.ksteps, k = w.from % p.ksteps;
-                    for (int i = w.from; i < w.to; i++, it++) {
+                for (int u = first; ok && u < tiles; u += stride) {
+                    const Tile w = tile_of(p, u);
+                    const int m = (w.tm * CG + (int)half_m) * 128, n = p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)half_m * NB;
+                    int g = k_from / p.ksteps, k = k_from % p.ksteps;
+                    for (int i = k_from; i < k_to; i++, it++) {
                         const int s = it % STAGES;
                         if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
-                        if (rank == 0) frnn_mbar_expect_tx(&full[s], (A_BYTES + B_BYTES) * CG);
+                        if (half_m == 0) frnn_mbar_expect_tx(&full[s], (A_BYTES + B_BYTES) * CG);
                         const u32 bar = CG == 2 ? in_block(&full[s], 0) : frnn_smem_addr(&full[s]), at = frnn_smem_addr(smem + s * STAGE_BYTES);
                         const int pa = p.plane_a[g], pb = p.plane_b[g];
                         if constexpr (AT) {
@@ -535,7 +571,7 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
                             tma_load<CG>(at + A_BYTES, &p.b[p.map_b[g]], k * BK, n, pb, bar);
                             static_assert(BT || NB == 128, "a copy is 128 rows high");
                         } else if (CG == 2) {      // one block has B0's rows, the other B1's
-                            tma_load<CG>(at + A_BYTES, &p.b[rank], k * BK, n, pb, bar);
+                            tma_load<CG>(at + A_BYTES, &p.b[half_m], k * BK, n, pb, bar);
                         } else {                   // (copies of 64 rows)
                             tma_load<CG>(at + A_BYTES, &p.b[0], k * BK, n, pb, bar);
                             tma_load<CG>(at + A_BYTES + B_BYTES / 2, &p.b[1], k * BK, n, pb, bar);
@@ -549,13 +585,12 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
             }
             __syncwarp();
         } else if (warp == 1) {
-            if (rank == 0 && frnn_elect()) {
+            if (half_m == 0 && frnn_elect()) {
                 u32 it = 0, t = 0;
                 bool ok = true;
-                for (int u = first; ok && u < units; u += stride) {
-                    const Unit w = unit_of(p, u);
-                    for (int from = w.from; ok && from < w.to; t++) {
-                        const int to = PROMOTE ? min(from + FLUSH, w.to) : w.to;
+                for (int u = first; ok && u < tiles; u += stride) {
+                    for (int from = k_from; ok && from < k_to; t++) {
+                        const int to = PROMOTE ? min(from + FLUSH, k_to) : k_to;
                         const u32 buf = t & 1, d = tmem + buf * BN;
                         if (!(ok = frnn_mbar_wait(&acc_empty[buf], (t / 2 & 1) ^ 1, p.err, CODE_PRODUCT))) break;
                         frnn_tmem_fence_after_sync();
@@ -580,8 +615,9 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
     } else {
         frnn_regs_acquire<EPILOGUE_REGISTERS>();
         const int quarter = warp % 4, half = (warp - 4) / 4;
-        unsigned char* const staging = smem + STAGES * STAGE_BYTES + (warp - 4) * STAGING_BYTES;
-        u32 t = 0;
+        unsigned char* const staging = smem + 6 * STAGE_BYTES + (warp - 4) * STAGING_BYTES;
+        float4* const exchange = (float4*)(smem + STAGES * STAGE_BYTES);      // SPLIT: [block][own columns / 4][128 rows]
+        u32 t = 0, round = 0;
         bool ok = true;
         auto filled = [&] {            // waits for accumulators; their address
             ok = __all_sync(0xffffffffu, frnn_mbar_wait(&acc_full[t & 1], t / 2 & 1, p.err, CODE_PRODUCT));
@@ -592,23 +628,23 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
             frnn_tmem_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (CG == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_block(&acc_empty[t & 1], 0)) : "memory");
+                if constexpr (CG == 2) arrive_at(in_block(&acc_empty[t & 1], 0));
                 else frnn_mbar_arrive(&acc_empty[t & 1]);
             }
             t++;
         };
-        for (int u = first; ok && u < units; u += stride) {
-            const Unit w = unit_of(p, u);
-            const int64_t row0 = (int64_t)(w.tm * CG + (int)rank) * 128 + quarter * 32;
+        for (int u = first; ok && u < tiles; u += stride, round++) {
+            const Tile w = tile_of(p, u);
+            const int64_t row0 = (int64_t)(w.tm * CG + (int)half_m) * 128 + quarter * 32;
             u32 acc = filled();
             if (!ok) break;
-            if constexpr (PROMOTE) {
-                if (w.from + FLUSH < w.to) {
+            if constexpr (PROMOTE || FORM == SPLIT) {
+                if (FORM == SPLIT || k_from + FLUSH < k_to) {
                     float sum[BN / 2];
 #pragma unroll
                     for (int i = 0; i < BN / 2; i += 32) ask(acc + half * (BN / 2) + i, sum + i);
                     wait_for<BN / 2>(sum);
-                    for (int from = w.from + FLUSH; from < w.to; from += FLUSH) {
+                    for (int from = k_from + FLUSH; PROMOTE && from < k_to; from += FLUSH) {
                         emptied();
                         acc = filled();
                         if (!ok) break;
@@ -622,101 +658,101 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ vo
                         }
                     }
                     if (!ok) break;
+                    if constexpr (FORM == SPLIT) {
+                        emptied();
+                        // to the owners: of every block's columns those that this warp has, four at a time
+                        const int own = BN / (int)blocks, row = quarter * 32 + lane;      // (own: a power of two)
+                        ok = __all_sync(0xffffffffu, wait_for_cluster(&taken, (round & 1) ^ 1, p.err));
+                        if (!ok) break;
+                        if (warp == 4 && lane == 0) frnn_mbar_expect_tx(&arrived, EXCHANGE_BYTES);
 #pragma unroll
-                    for (int i = 0; i < BN / 2; i += 32) frnn_tmem_st<32>(acc + half * (BN / 2) + i, sum + i);
-                    frnn_tmem_wait_st();
-                    if constexpr (EPI == GLU_FORWARD) {      // (a warp's columns of the two products lie in both warps' halves)
-                        frnn_tmem_fence_before_sync();
-                        frnn_group_sync(1 + quarter, 64);
-                        frnn_tmem_fence_after_sync();
+                        for (int i = 0; i < BN / 2; i += 4) {
+                            const int c = half * (BN / 2) + i;
+                            int owner, at;
+                            if (EPI == GLU_FORWARD) {      // (an owner has the same columns of both products)
+                                owner = i >> (__ffs(own) - 2);
+                                at = (i & (own / 2 - 1)) + half * (own / 2);
+                            } else {
+                                owner = c >> (__ffs(own) - 1);
+                                at = c & (own - 1);
+                            }
+                            send(in_block(&exchange[((int)rank * own + at) / 4 * 128 + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3], in_block(&arrived, owner));
+                        }
+                        ok = __all_sync(0xffffffffu, wait_for_cluster(&arrived, round & 1, p.err));
+                        if (!ok) break;
+                        // the owner's columns: halves of 32 or 16, or all of them by the first warps
+                        const int width = EPI == GLU_FORWARD ? own / 2 : own, smallest = EPI == GLU_FORWARD ? 16 : 32;
+                        const int count = max(min(width, smallest), width / 2), from = half * count;
+                        const u32 place = tmem + 2 * BN + frnn_tmem_lane_base(quarter);
+                        if (from < width) {
+#pragma unroll 1
+                            for (int i = 0; i < (EPI == GLU_FORWARD ? 2 : 1) * count; i += 4) {
+                                const int at = i < count ? from + i : own / 2 + from + i - count;
+                                float v[4] = {};
+                                for (u32 b = 0; b < blocks; b++) {
+                                    const float4 x = exchange[((int)b * own + at) / 4 * 128 + row];
+                                    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+                                }
+                                frnn_tmem_st4(place + half * 64 + i, v);
+                            }
+                            frnn_tmem_wait_st();
+                        }
+                        __syncwarp();
+                        if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
+                        if (from < width) {
+                            const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
+                            epilogue<EPI>(p, place + half * 64, place + half * 64 + count, row0, tile_col + from, count, lane, staging);
+                        }
+                        continue;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < BN / 2; i += 32) frnn_tmem_st<32>(acc + half * (BN / 2) + i, sum + i);
+                        frnn_tmem_wait_st();
+                        if constexpr (EPI == GLU_FORWARD) {      // (a warp's columns of the two products lie in both warps' halves)
+                            frnn_tmem_fence_before_sync();
+                            frnn_group_sync(1 + quarter, 64);
+                            frnn_tmem_fence_after_sync();
+                        }
                     }
                 }
             }
-            epilogue<EPI, BN>(p, acc, row0, w.tn, w.slice, half, lane, staging);
+            constexpr int COUNT = EPI == GLU_FORWARD ? BN / 4 : BN / 2;
+            epilogue<EPI>(p, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, lane, staging);
             emptied();
         }
     }
     frnn_tmem_fence_before_sync();
     __syncthreads();
-    if constexpr (CG == 2) cluster_sync();
+    if constexpr (FORM != ALONE) cluster_sync();
     frnn_tmem_fence_after_sync();
     if (warp == 2) tmem_free<CG>(tmem, COLUMNS);
 }
 
-// ---- the rest of a product whose k was split: partial sums added in the order of the slices ----------------------------------------
-
-__device__ __forceinline__ void store_as(int dtype, void* p, int64_t at, float v) {
-    if (dtype == FRNN_F32) ((float*)p)[at] = v;
-    else if (dtype == FRNN_BF16) ((__nv_bfloat16*)p)[at] = from_float<__nv_bfloat16>(v);
-    else ((__half*)p)[at] = from_float<__half>(v);
-}
-__device__ __forceinline__ float load_as(int dtype, const void* p, int64_t at) {
-    return dtype == FRNN_F32 ? ((const float*)p)[at] : dtype == FRNN_BF16 ? to_float(((const __nv_bfloat16*)p)[at]) : to_float(((const __half*)p)[at]);
-}
-__device__ __forceinline__ void store_planes(int io, const Planes& to, int64_t row, int64_t col, float v) {
-    const int64_t at = row * to.ld + col;
-    if (io != FRNN_F32) {
-        store_as(io, to.p, at, v);
-    } else {
-        float hi, mid, lo;
-        split3(v, hi, mid, lo);
-        store_as(FRNN_BF16, to.p, at, hi);
-        store_as(FRNN_BF16, to.p, at + to.plane, mid);
-        store_as(FRNN_BF16, to.p, at + 2 * to.plane, lo);
-    }
-}
-
-// p.out: partial sums of p.slices slices as STORE left them; to / to_dtype / to_ld: where STORE's own result goes.
-template <int EPI> __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ ProductArgs p, void* to, int to_dtype, int64_t to_ld) {
-    const int quads = (p.N + 3) / 4;
-    const float alpha = EPI == STORE && p.alpha ? *p.alpha : 1.f;
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < (int64_t)p.M * quads; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / quads;
-        const int col = (int)(i % quads) * 4;
-        const float* from = (const float*)p.out + row * p.out_ld + col;
-        float4 v = make_float4(0, 0, 0, 0), w = v;
-        for (int s = 0; s < p.slices; s++) {
-            const float4 x = *(const float4*)(from + s * p.out_slice);
-            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-            if constexpr (EPI == GLU_FORWARD) {
-                const float4 y = *(const float4*)(from + s * p.out_slice + p.out_ld / 2);
-                w.x += y.x; w.y += y.y; w.z += y.z; w.w += y.w;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (col + e >= p.N) break;
-            float x = (&v.x)[e];
-            if constexpr (EPI == STORE) {
-                x *= alpha;
-                if (p.add) x += p.add[row * p.add_ld + col + e];
-                store_as(to_dtype, to, row * to_ld + col + e, x);
-            } else if constexpr (EPI == GLU_FORWARD) {
-                float y = (&w.x)[e], h;
-                glu<1>(p.activation, &x, &y, &h, p.by_gate);
-                if (p.by_gate) {
-                    store_as(p.io, p.by_gate, row * p.by_ld + col + e, x);
-                    store_as(p.io, p.by_up, row * p.by_ld + col + e, y);
-                }
-                store_planes(p.io, p.h, row, col + e, h);
-            } else {
-                if (p.da.p) store_planes(p.io, p.da, row, col + e, x * load_as(p.io, p.by_gate, row * p.by_ld + col + e));
-                if (p.db.p) store_planes(p.io, p.db, row, col + e, x * load_as(p.io, p.by_up, row * p.by_ld + col + e));
-            }
-        }
-    }
-}
-
 // ---- operands -------------------------------------------------------------------------------------------------------------------
 
-// Rows of any type and stride as a 16-bit operand: rows on 16-byte boundaries, fp32 as three planes.  A thread takes 8 columns.
-template <class T, bool WIDE_LOADS> __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, Planes to) {
-    const int64_t eights = (cols + 7) / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * eights; i += (int64_t)gridDim.x * 256) {
+// Rows of any type and stride as 16-bit operands: rows on 16-byte boundaries, fp32 as three planes.  A thread takes 8 columns;
+// blockIdx.y is the matrix.
+enum { MAX_PACKS = 5 };
+struct PackJob {
+    const void* x;
+    int64_t rows, cols, stride;
+    Planes to;
+    int wide;                   // rows of x start on 16-byte boundaries
+};
+struct Packs {
+    PackJob each[MAX_PACKS];
+    int count;
+};
+template <class T> __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs) {
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
+    const PackJob& m = packs.each[blockIdx.y];
+    const int64_t eights = (m.cols + 7) / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < m.rows * eights; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / eights, col = i % eights * 8;
-        const T* const from = x + row * stride + col;
+        const T* const from = (const T*)m.x + row * m.stride + col;
         float v[8];
-        if (WIDE_LOADS && col + 8 <= cols) {
+        if (m.wide && col + 8 <= m.cols) {
             constexpr int W = WIDE<T>;
 #pragma unroll
             for (int c = 0; c < 8; c += W) {
@@ -726,12 +762,12 @@ template <class T, bool WIDE_LOADS> __global__ void __launch_bounds__(256) pack_
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = col + e < cols ? to_float(from[e]) : 0.f;
+            for (int e = 0; e < 8; e++) v[e] = col + e < m.cols ? to_float(from[e]) : 0.f;
         }
         if constexpr (sizeof(T) == 2) {
             Pack<T, 8> q;
             q.from(v);
-            q.store((T*)to.p + row * to.ld + col);
+            q.store((T*)m.to.p + row * m.to.ld + col);
         } else {
             float part[3][8];
 #pragma unroll
@@ -740,7 +776,7 @@ template <class T, bool WIDE_LOADS> __global__ void __launch_bounds__(256) pack_
             for (int k = 0; k < 3; k++) {
                 Pack<__nv_bfloat16, 8> q;
                 q.from(part[k]);
-                q.store((__nv_bfloat16*)to.p + k * to.plane + row * to.ld + col);
+                q.store((__nv_bfloat16*)m.to.p + k * m.to.plane + row * m.to.ld + col);
             }
         }
     }
@@ -782,9 +818,10 @@ inline Operand new_operand(Scratch& s, int dtype, int64_t rows, int64_t cols, in
     o.p = s.take((size_t)o.plane * o.planes * 2);
     return o;
 }
-// The caller's matrix itself where the tensor cores can read it as it is, else a copy.
-inline int as_operand(Scratch& s, int dtype, const void* x, int64_t rows, int64_t cols, int64_t stride, Operand& o, cudaStream_t stream) {
+// The caller's matrix itself where the tensor cores can read it as it is, else a copy, which `packs` has to make.
+inline Operand as_operand(Scratch& s, Packs& packs, int dtype, const void* x, int64_t rows, int64_t cols, int64_t stride) {
     if (rows == 1) stride = padded(cols);
+    Operand o;
     if (dtype != FRNN_F32 && on_boundary(x, 16) && stride % 8 == 0 && stride >= cols) {
         o.p = x;
         o.rows = rows;
@@ -792,17 +829,18 @@ inline int as_operand(Scratch& s, int dtype, const void* x, int64_t rows, int64_
         o.ld = stride;
         o.plane = rows * stride;
         o.planes = 1;
-        return FRNN_OK;
+        return o;
     }
     o = new_operand(s, dtype, rows, cols);
-    if (!s.base) return FRNN_OK;
-    const int64_t blocks = std::min<int64_t>((rows * ((cols + 7) / 8) + 255) / 256, (int64_t)sm_count() * 16);
-    return with_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        if (on_boundary(x, 16) && (rows == 1 || stride * sizeof(T) % 16 == 0)) pack_kernel<T, true><<<(unsigned)blocks, 256, 0, stream>>>((const T*)x, rows, cols, stride, o.writable());
-        else pack_kernel<T, false><<<(unsigned)blocks, 256, 0, stream>>>((const T*)x, rows, cols, stride, o.writable());
-        return launched("matrix product: operand");
-    });
+    packs.each[packs.count++] = {x, rows, cols, stride, o.writable(), on_boundary(x, 16) && stride * dtype_bytes(dtype) % 16 == 0};
+    return o;
+}
+inline int pack(const Packs& packs, int dtype, cudaStream_t stream) {
+    if (!packs.count) return FRNN_OK;
+    int64_t most = 0;
+    for (int i = 0; i < packs.count; i++) most = std::max(most, packs.each[i].rows * ((packs.each[i].cols + 7) / 8));
+    const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, (int64_t)sm_count() * 16), packs.count);
+    return with_dtype(dtype, [&](auto t) { return launch("matrix product: operands", pack_kernel<decltype(t)>, grid, 256, 0, stream, true, 1, packs); });
 }
 
 // ---- products --------------------------------------------------------------------------------------------------------------------
@@ -811,7 +849,6 @@ struct Product {
     ProductArgs args = {};
     int dtype;                                    // of the operands: FRNN_F32 means planes
     Operand a, b[2];
-    bool at = false, bt = false;                  // stored [k][m], [k][n]
     int64_t m, n, k;
     int pairs = 1;                                // products that are added up: planes of a, b[0], b[1]
     void* out = nullptr;                          // STORE
@@ -820,37 +857,58 @@ struct Product {
 };
 
 struct ProductPlan {
-    bool pair;
-    int slices;
-    int64_t tiles_m, tiles_n, ld;
-    size_t bytes;                                 // partial sums
+    Form form;
+    int blocks;                                   // of a cluster
+    int64_t tiles_m, tiles_n;
+    int columns() const { return form == PAIR ? 128 : form == ALONE ? 64 : blocks == 8 ? 16 : 32; }      // that a warp of the epilogue has in a row
 };
 
-// Which kernel, and into how many slices k is split.  Cycles of a step of 64 along k in a block: 512 of 128 x 256 (pairs), and
-// for 128 x 128 the 256 of the products, but 340 with its copies; what a tile or slice costs besides, and a second kernel for
-// the partial sums, as measured.  A split takes whole-wave shapes: the fewest cycles of the busiest multiprocessor.
-inline ProductPlan plan_product(const Product& q, bool may_split) {
-    const int sms = sm_count();
+// Clusters of 1, 2, 4 or 8 blocks that run at once, one block to a multiprocessor.
+template <auto KERNEL> inline int clusters_at_once(int blocks) {
+    static std::atomic<int> known[64][9];
+    if (blocks == 1) return sm_count();
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return sm_count() / blocks; }
+    int n = known[dev][blocks].load(std::memory_order_relaxed);
+    if (!n) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(blocks * sm_count());
+        config.blockDim = dim3(PRODUCT_THREADS);
+        config.dynamicSmemBytes = PRODUCT_SHARED;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = blocks;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        if (!allow_shared<KERNEL>(PRODUCT_SHARED) || cudaOccupancyMaxActiveClusters(&n, KERNEL, &config) != cudaSuccess || n <= 0) n = sm_count() / blocks;
+        cudaGetLastError();
+        known[dev][blocks].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// Which form.  Cycles, as measured: a step of 64 along k in a block 520 of PAIR, 340 of the others (of the products 256, their
+// copies are what takes longer); a tile besides, in PAIR 2000, else 1500 and where it is SPLIT 1500 more for the exchange; 9000 a kernel.
+// The fewest cycles of the busiest multiprocessor win.
+template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    ProductPlan best = {true, 1, up(q.m, 256), up(q.n * width, 256), 0, 0};
-    if (q.args.dual) best.tiles_n = up(q.n, 128);
-    double cost = (double)up(best.tiles_m * best.tiles_n, sms / 2) * (steps * 512 + 1000) + 4000;
-    const int64_t tm = up(q.m, 128), tn = q.args.dual ? up(q.n, 64) : up(q.n, 128), ld = padded(q.n) * width;
-    for (int s = 1; s <= (may_split ? 16 : 1) && s <= steps; s++) {
-        const size_t bytes = s > 1 ? (size_t)s * q.m * ld * 4 : 0;
-        if (bytes > ((size_t)64 << 20)) break;
-        const double c = (double)up(tm * tn * s, sms) * ((double)up(steps, s) * 340 + 1000) + 4000 + (s > 1 ? 5000 + bytes / 2000.0 : 0);
+    ProductPlan best = {PAIR, 2, up(q.m, 256), up(q.n * width, 256)};
+    int64_t cost = up(best.tiles_m * best.tiles_n, clusters_at_once<product_kernel<SPLIT, AT, BT, EPI, true>>(2)) * (steps * 520 + 2000);
+    const int64_t tm = up(q.m, 128), tn = up(q.n * width, 128);
+    for (int blocks = 1; blocks <= 8 && blocks <= steps; blocks *= 2) {
+        const int64_t c = up(tm * tn, clusters_at_once<product_kernel<SPLIT, AT, BT, EPI, true>>(blocks)) * (up(steps, blocks) * 340 + (blocks > 1 ? 3000 : 1500));
         if (c < cost) {
             cost = c;
-            best = {false, s, tm, tn, ld, bytes};
+            best = {blocks > 1 ? SPLIT : ALONE, blocks, tm, tn};
         }
     }
     return best;
 }
 
-template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_product(const char* what, const ProductArgs& p, cudaStream_t stream) {
-    constexpr auto kernel = product_kernel<CG, BN, AT, BT, EPI, PROMOTE>;
+template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_product(const char* what, const ProductArgs& p, int blocks, cudaStream_t stream) {
+    constexpr auto kernel = product_kernel<FORM, AT, BT, EPI, PROMOTE>;
     // (the warps would wait for registers that the block does not have)
     static const bool enough = [] {
         cudaFuncAttributes a = {};
@@ -860,27 +918,22 @@ template <int CG, int BN, bool AT, bool BT, int EPI, bool PROMOTE> inline int la
     }();
     if (!enough) return frnn_fail(FRNN_E_LAUNCH, "%s: the kernel was not built for %d registers a thread, or there is no GPU to run it", what, (int)START_REGISTERS);
     if (!allow_shared<kernel>(PRODUCT_SHARED)) { cudaGetLastError(); return frnn_fail(FRNN_E_LAUNCH, "%s: no room in shared memory", what); }
-    const int64_t units = (int64_t)p.tiles_m * p.tiles_n * p.slices;
-    return launch(what, kernel, dim3((unsigned)(std::min<int64_t>(units, sm_count() / CG) * CG)), PRODUCT_THREADS, PRODUCT_SHARED, stream, false, CG, p);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, clusters = std::min<int64_t>(tiles, clusters_at_once<product_kernel<SPLIT, AT, BT, EPI, true>>(blocks));
+    return launch(what, kernel, dim3((unsigned)(clusters * blocks)), PRODUCT_THREADS, PRODUCT_SHARED, stream, true, blocks, p);
 }
 
-// One product.  Without memory behind `s` only its scratch is counted.
-template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Product& q, Scratch& s, cudaStream_t stream) {
-    constexpr bool MAY_SPLIT = EPI != LOGPROB_STATS && EPI != LOGPROB_GRAD;
+template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Product& q, cudaStream_t stream) {
     ProductArgs& p = q.args;
-    const ProductPlan plan = plan_product(q, MAY_SPLIT);
-    void* const partial = plan.slices > 1 ? s.take(plan.bytes) : nullptr;
-    if (!s.base) return FRNN_OK;
-    if (plan.tiles_m * plan.tiles_n * plan.slices >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "%s: too many tiles", what);
+    const ProductPlan plan = plan_product<EPI, AT, BT>(q);
+    if (plan.tiles_m * plan.tiles_n >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "%s: too many tiles", what);
     p.M = (int)q.m;
     p.N = (int)q.n;
     p.ksteps = (int)((q.k + BK - 1) / BK);
     p.tiles_m = (int)plan.tiles_m;
     p.tiles_n = (int)plan.tiles_n;
-    p.slices = plan.slices;
-    p.group = plan.pair ? 16 : 32;
-    const unsigned type = q.dtype == FRNN_F16 ? 0 : 1, bn = plan.pair ? 256 : 128, bm = plan.pair ? 256 : 128;
-    p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((unsigned)AT << 15) | ((unsigned)BT << 16) | ((bn >> 3) << 17) | ((bm >> 4) << 24);
+    p.group = plan.form == PAIR ? 16 : 32;
+    const unsigned type = q.dtype == FRNN_F16 ? 0 : 1, side = plan.form == PAIR ? 256 : 128;
+    p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((unsigned)AT << 15) | ((unsigned)BT << 16) | ((side >> 3) << 17) | ((side >> 4) << 24);
     static const unsigned char first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};      // planes of a and b, small terms first
     const int terms = q.dtype == FRNN_F32 ? 6 : 1;
     p.segments = 0;
@@ -890,37 +943,30 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
             p.plane_b[p.segments] = terms == 6 ? second[t] : 0;
             p.map_b[p.segments] = (unsigned char)(q.pairs > 1 ? pair : 0);
         }
+    if ((int64_t)p.ksteps * p.segments >= (1ll << 31) - 64) return frnn_fail(FRNN_E_ARG, "%s: too long", what);
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);
     };
     int rc = encode(p.a, q.a, AT, 128);
-    for (int i = 0; i < 2 && rc == FRNN_OK; i++) rc = encode(p.b[i], q.b[i].p ? q.b[i] : q.b[0], BT, p.dual && !plan.pair ? 64 : 128);
-    if (rc != FRNN_OK) return rc;
-    if (plan.slices > 1) {
-        if constexpr (MAY_SPLIT) {
-            ProductArgs part = p;
-            part.out = partial;
-            part.out_ld = plan.ld;
-            part.out_slice = q.m * plan.ld;
-            part.out_dtype = FRNN_F32;
-            part.out_wide = 1;
-            part.add = part.alpha = nullptr;
-            rc = q.dtype == FRNN_F32 ? launch_product<1, 128, AT, BT, STORE, true>(what, part, stream) : launch_product<1, 128, AT, BT, STORE, false>(what, part, stream);
-            if (rc != FRNN_OK) return rc;
-            part.add = p.add;
-            part.alpha = p.alpha;
-            const int64_t blocks = std::min<int64_t>((q.m * ((q.n + 3) / 4) + 255) / 256, (int64_t)sm_count() * 8);
-            finish_kernel<EPI><<<(unsigned)blocks, 256, 0, stream>>>(part, q.out, q.out_dtype, q.out_ld);
-            return launched(what);
-        }
+    for (int i = 0; i < 2 && rc == FRNN_OK; i++) {
+        if (i && !q.b[1].p) p.b[1] = p.b[0];
+        else rc = encode(p.b[i], q.b[i], BT, p.dual && plan.form != PAIR ? 64 : 128);
     }
+    if (rc != FRNN_OK) return rc;
     p.out = q.out;
     p.out_dtype = q.out_dtype;
     p.out_ld = q.out_ld;
     p.out_wide = on_boundary(q.out, 16) && q.out_ld * (int64_t)dtype_bytes(q.out_dtype) % 16 == 0;
-    if (q.dtype == FRNN_F32) return plan.pair ? launch_product<2, 256, AT, BT, EPI, true>(what, p, stream) : launch_product<1, 128, AT, BT, EPI, true>(what, p, stream);
     constexpr bool EXACT = EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
-    return plan.pair ? launch_product<2, 256, AT, BT, EPI, EXACT>(what, p, stream) : launch_product<1, 128, AT, BT, EPI, EXACT>(what, p, stream);
+    auto run = [&](auto form) {
+        constexpr Form FORM = decltype(form)::value;
+        return q.dtype == FRNN_F32 ? launch_product<FORM, AT, BT, EPI, true>(what, p, plan.blocks, stream) : launch_product<FORM, AT, BT, EPI, EXACT>(what, p, plan.blocks, stream);
+    };
+    switch (plan.form) {
+        case PAIR: return run(std::integral_constant<Form, PAIR>());
+        case ALONE: return run(std::integral_constant<Form, ALONE>());
+        default: return run(std::integral_constant<Form, SPLIT>());
+    }
 }
 
 }  // namespace frnn_lm
