@@ -72,7 +72,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_cuda(const Tensor& x, const
     int* err = error_word(x.device().index());
     auto sizes = x.sizes().vec();
     sizes.back() = m.c.out_width;
-    const int64_t n = save ? m.c.n : 0, ld = (m.c.hidden + 7) / 8 * 8;
+    const int64_t n = save ? m.c.n : 0, ld = (m.c.hidden + 63) / 64 * 64;
     const bool wide = x.scalar_type() == at::kFloat;
     Tensor y = make("the output", sizes, x.scalar_type(), x), by_gate = make("the derivatives by gate", {n, ld}, x.scalar_type(), x), by_up = make("the derivatives by up", {n, ld}, x.scalar_type(), x);
     Tensor hidden = make("the hidden vectors", {wide ? 3 : 1, n, ld}, wide ? at::kBFloat16 : x.scalar_type(), x);
@@ -92,7 +92,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_cuda(const Tensor&
     TORCH_CHECK(grad.scalar_type() == x.scalar_type() && grad.dim() == x.dim() && grad.size(-1) == m.c.out_width && grad.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1), "flex_rnn_b200: ", op,
                 ": the gradient has to have the shape and type of the output, got ", grad.sizes());
     check_one(op, "the gradient", grad, x);
-    const int64_t ld = (m.c.hidden + 7) / 8 * 8;
+    const int64_t ld = (m.c.hidden + 63) / 64 * 64;
     const bool wide = x.scalar_type() == at::kFloat;
     for (const Tensor* t : {&by_gate, &by_up, &hidden}) {
         const bool h = t == &hidden;

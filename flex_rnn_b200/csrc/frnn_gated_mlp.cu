@@ -73,6 +73,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, v
     Product q = product(c, c->n, c->out_width, c->hidden);
     q.a = h;
     q.b[0] = down;
+    q.args.b_ready = 1;
     q.args.err = err;
     q.out = y;
     q.out_dtype = c->dtype;
@@ -99,6 +100,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
     int rc = pack(packs, c->dtype, stream);
     if (rc != FRNN_OK) return rc;
     auto store = [&](Product& q, void* out, int64_t ld) {
+        q.args.b_ready = 1;                // (the hidden gradients, which the first product writes, are always A)
         q.args.err = err;
         q.out = out;
         q.out_dtype = c->dtype;
@@ -122,6 +124,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.a = g;
         q.b[0] = kept(c, hidden);
         store(q, ddown, c->hidden);
+        q.args.b_ready = want_hidden;      // (else it is the first: what is before it is not known)
         rc = run_product<STORE, true, true>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }

@@ -20,6 +20,7 @@ template <int JOIN_ROWS, int JOIN_SLICES>
 __global__ void __launch_bounds__(JOIN_ROWS* JOIN_SLICES) join_kernel(const float* partial, const float* target, int64_t blocks, int64_t n, const void* tokens, int token_bytes, int64_t vocab,
                                                                       int64_t ignore_index, float* logprob, float* entropy, float* stats, int* err) {
     __shared__ float part[3][JOIN_SLICES][JOIN_ROWS];
+    cudaGridDependencySynchronize();
     const int r = threadIdx.x % JOIN_ROWS, slice = threadIdx.x / JOIN_ROWS;
     const int64_t row = (int64_t)blockIdx.x * JOIN_ROWS + r;
     const float lowest = -3.4028235e38f;
@@ -136,11 +137,10 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
     if (rc == FRNN_OK) rc = run_product<LOGPROB_STATS, false, false>(what, q, stream);
     if (rc != FRNN_OK) return rc;
     auto join = [&](auto kernel, int rows, int slices) {
-        kernel<<<(unsigned)((c->n + rows - 1) / rows), rows * slices, 0, stream>>>(q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab, c->ignore_index, logprob, entropy, stats, err);
+        return launch(what, kernel, dim3((unsigned)((c->n + rows - 1) / rows)), rows * slices, 0, stream, true, 1, q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab,
+                      c->ignore_index, logprob, entropy, stats, err);
     };
-    if (c->n >= 2048) join(join_kernel<32, 16>, 32, 16);
-    else join(join_kernel<8, 128>, 8, 128);
-    return launched(what);
+    return c->n >= 2048 ? join(join_kernel<32, 16>, 32, 16) : join(join_kernel<8, 128>, 8, 128);
 }
 
 int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const float* dentropy, const float* stats, void* dx, void* dweight, Scratch& s, int* err, cudaStream_t stream) {
@@ -186,6 +186,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.k = cols;
             q.a = g;
             q.b[0] = part;
+            q.args.b_ready = 1;
             q.args.err = err;
             q.args.alpha = range ? range + 1 : nullptr;
             q.args.add = first ? nullptr : sum;
@@ -204,6 +205,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.k = c->n;
             q.a = g;
             q.b[0] = x;
+            q.args.b_ready = 1;
             q.args.err = err;
             q.args.alpha = range ? range + 1 : nullptr;
             q.out = (char*)dweight + v * c->width * dtype_bytes(c->dtype);

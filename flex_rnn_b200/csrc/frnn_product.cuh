@@ -19,6 +19,9 @@
 //   SPLIT  128 x 128 by a cluster of 2, 4 or 8 blocks, each with a part of k.  Each block then owns a part of the tile's columns: the others
 //          send it their sums of these (st.async into its shared memory), it adds them in the order of the blocks and has the epilogue
 //          to itself.  (4 stages, and 64 KB for what arrives.)
+// THIN (ALONE or SPLIT, up to 32 rows, as in generation): only 32 of A's rows are copied, so that 10 stages of B are under way, 160 KB a
+// multiprocessor: such products are as fast as their weights come.  The tensor cores read 128 rows all the same: what they find
+// behind the 32 ends in rows of the result that nobody looks at.
 #pragma once
 #include <cuda.h>
 
@@ -36,10 +39,10 @@ int frnn_tensor_map_swizzled(void* out_map, const void* base, uint64_t cols, uin
 namespace frnn_lm {
 
 enum Form { PAIR, ALONE, SPLIT };
-enum { BK = 64, STAGE_BYTES = 32768, EXCHANGE_BYTES = 65536, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
+enum { BK = 64, STAGE_BYTES = 32768, THIN_ROWS = 32, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
 // Registers of the warps that copy and issue, and of the epilogue's: 128 x 56 + 256 x 224 = 384 x 168, what a block starts with.
 enum { CONTROL_REGISTERS = 56, EPILOGUE_REGISTERS = 224, START_REGISTERS = 168 };
-enum { PRODUCT_SHARED = 6 * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };      // (4 stages and what arrives: as much)
+enum { PRODUCT_SHARED = 6 * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };      // (6 stages; 4 and 64 KB for what arrives; 10 thin ones, 16 KB and less staging: as much each)
 enum { CODE_PRODUCT = 97 };       // error word: a wait inside a matrix product ran out
 
 // What becomes of a tile.
@@ -56,6 +59,7 @@ struct alignas(64) ProductArgs {
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
     int ksteps, segments;       // steps of 64 along k in a segment
     int tiles_m, tiles_n, group;
+    int b_ready;                // the kernel before this one writes nothing of B: its copies begin before that one ends
     int dual;                   // a tile's columns are half of B0's rows and half of B1's
     unsigned idesc;
     int* err;
@@ -499,11 +503,14 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u) {
 }
 
 // AT, BT: the operand's rows run along m (n) instead of k.
-template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
-    constexpr int CG = FORM == PAIR ? 2 : 1, BN = FORM == PAIR ? 256 : 128, STAGES = FORM == SPLIT ? 4 : 6;
+template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
+    constexpr int CG = FORM == PAIR ? 2 : 1, BN = FORM == PAIR ? 256 : 128, STAGES = THIN ? 10 : FORM == SPLIT ? 4 : 6;
     constexpr int NB = BN / CG;                        // B's rows in this block
-    constexpr u32 A_BYTES = 128 * BK * 2, B_BYTES = NB * BK * 2, COLUMNS = FORM == SPLIT ? 512 : 2 * BN;
-    static_assert(A_BYTES + B_BYTES <= STAGE_BYTES && COLUMNS <= 512, "a stage or Tensor Memory is too small");
+    constexpr int ROWS = THIN ? (int)THIN_ROWS : 128;  // of A, that are copied and that have a result
+    constexpr u32 A_BYTES = ROWS * BK * 2, B_BYTES = NB * BK * 2, STAGE = A_BYTES + B_BYTES, COLUMNS = FORM == SPLIT ? 512 : 2 * BN;
+    constexpr u32 EXCHANGE = FORM == SPLIT ? ROWS * BN * 4 : 0;
+    static_assert(STAGES * STAGE + EXCHANGE + ROWS / 32 * 2 * STAGING_BYTES + 1024 <= PRODUCT_SHARED && COLUMNS <= 512, "shared memory or Tensor Memory is too small");
+    static_assert(!THIN || (!AT && FORM != PAIR), "only rows along k can be left out");
     extern __shared__ unsigned char raw[];
     __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], arrived, taken;
     __shared__ u32 tmem;
@@ -538,9 +545,12 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
     if constexpr (FORM != ALONE) cluster_sync();
     __syncthreads();
     frnn_tmem_fence_after_sync();
-    // Up to here nothing has been read that a kernel before this one may still be writing; the next one may come as far.
-    cudaGridDependencySynchronize();
-    cudaTriggerProgrammaticLaunchCompletion();
+    // Up to here nothing has been read that a kernel before this one may still be writing; the next one may come as far.  (That one finds
+    // everything written that was before this kernel's own predecessor ended.)
+    if (warp != 0) {
+        cudaGridDependencySynchronize();
+        cudaTriggerProgrammaticLaunchCompletion();
+    }
 
     if (warp < 4) {
         frnn_regs_release<CONTROL_REGISTERS>();
@@ -548,34 +558,49 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
             if (frnn_elect()) {
                 u32 it = 0;
                 bool ok = true;
+                auto bar_of = [&](int s) { return CG == 2 ? in_block(&full[s], 0) : frnn_smem_addr(&full[s]); };
+                auto load_b = [&](int s, int n, int g, int k) {
+                    const u32 bar = bar_of(s), at = frnn_smem_addr(smem + s * STAGE) + A_BYTES;
+                    const int plane = p.plane_b[g];
+                    if (half_m == 0) frnn_mbar_expect_tx(&full[s], STAGE * CG);      // (a's bytes too)
+                    if constexpr (BT) {
+#pragma unroll
+                        for (int part = 0; part < NB / 64; part++) tma_load<CG>(at + part * 8192, &p.b[p.map_b[g]], n + part * 64, k * BK, plane, bar);
+                    } else if (!p.dual) {
+                        tma_load<CG>(at, &p.b[p.map_b[g]], k * BK, n, plane, bar);
+                        static_assert(BT || NB == 128, "a copy is 128 rows high");
+                    } else if (CG == 2) {      // one block has B0's rows, the other B1's
+                        tma_load<CG>(at, &p.b[half_m], k * BK, n, plane, bar);
+                    } else {                   // (copies of 64 rows)
+                        tma_load<CG>(at, &p.b[0], k * BK, n, plane, bar);
+                        tma_load<CG>(at + B_BYTES / 2, &p.b[1], k * BK, n, plane, bar);
+                    }
+                };
+                auto load_a = [&](int s, int m, int g, int k) {
+                    const u32 bar = bar_of(s), at = frnn_smem_addr(smem + s * STAGE);
+                    const int plane = p.plane_a[g];
+                    if constexpr (AT) {
+                        tma_load<CG>(at, &p.a, m, k * BK, plane, bar);
+                        tma_load<CG>(at + A_BYTES / 2, &p.a, m + 64, k * BK, plane, bar);
+                    } else {
+                        tma_load<CG>(at, &p.a, k * BK, m, plane, bar);
+                    }
+                };
+                auto column = [&](const Tile& w) { return p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)half_m * NB; };
+                const int early = p.b_ready && first < tiles ? min(STAGES, k_to - k_from) : 0;
+                for (int i = 0; i < early; i++) load_b(i, column(tile_of(p, first)), (k_from + i) / p.ksteps, (k_from + i) % p.ksteps);
+                cudaGridDependencySynchronize();
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u);
-                    const int m = (w.tm * CG + (int)half_m) * 128, n = p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)half_m * NB;
+                    const int m = (w.tm * CG + (int)half_m) * 128, n = column(w);
                     int g = k_from / p.ksteps, k = k_from % p.ksteps;
                     for (int i = k_from; i < k_to; i++, it++) {
                         const int s = it % STAGES;
-                        if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
-                        if (half_m == 0) frnn_mbar_expect_tx(&full[s], (A_BYTES + B_BYTES) * CG);
-                        const u32 bar = CG == 2 ? in_block(&full[s], 0) : frnn_smem_addr(&full[s]), at = frnn_smem_addr(smem + s * STAGE_BYTES);
-                        const int pa = p.plane_a[g], pb = p.plane_b[g];
-                        if constexpr (AT) {
-                            tma_load<CG>(at, &p.a, m, k * BK, pa, bar);
-                            tma_load<CG>(at + A_BYTES / 2, &p.a, m + 64, k * BK, pa, bar);
-                        } else {
-                            tma_load<CG>(at, &p.a, k * BK, m, pa, bar);
+                        if (it >= (u32)early) {
+                            if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
+                            load_b(s, n, g, k);
                         }
-                        if constexpr (BT) {
-#pragma unroll
-                            for (int part = 0; part < NB / 64; part++) tma_load<CG>(at + A_BYTES + part * 8192, &p.b[p.map_b[g]], n + part * 64, k * BK, pb, bar);
-                        } else if (!p.dual) {
-                            tma_load<CG>(at + A_BYTES, &p.b[p.map_b[g]], k * BK, n, pb, bar);
-                            static_assert(BT || NB == 128, "a copy is 128 rows high");
-                        } else if (CG == 2) {      // one block has B0's rows, the other B1's
-                            tma_load<CG>(at + A_BYTES, &p.b[half_m], k * BK, n, pb, bar);
-                        } else {                   // (copies of 64 rows)
-                            tma_load<CG>(at + A_BYTES, &p.b[0], k * BK, n, pb, bar);
-                            tma_load<CG>(at + A_BYTES + B_BYTES / 2, &p.b[1], k * BK, n, pb, bar);
-                        }
+                        load_a(s, m, g, k);
                         if (++k == p.ksteps) { k = 0; g++; }
                     }
                 }
@@ -598,7 +623,7 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
                             const int s = it % STAGES;
                             if (!(ok = frnn_mbar_wait(&full[s], it / STAGES & 1, p.err, CODE_PRODUCT))) break;
                             frnn_tmem_fence_after_sync();
-                            const u32 at = frnn_smem_addr(smem + s * STAGE_BYTES);
+                            const u32 at = frnn_smem_addr(smem + s * STAGE);
                             const u64 a = operand_desc(at, 8192), b = operand_desc(at + A_BYTES, 8192);
 #pragma unroll
                             for (int k = 0; k < BK / 16; k++)      // 16 values of k: 32 bytes of a row, or 16 rows
@@ -615,8 +640,9 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
     } else {
         frnn_regs_acquire<EPILOGUE_REGISTERS>();
         const int quarter = warp % 4, half = (warp - 4) / 4;
-        unsigned char* const staging = smem + 6 * STAGE_BYTES + (warp - 4) * STAGING_BYTES;
-        float4* const exchange = (float4*)(smem + STAGES * STAGE_BYTES);      // SPLIT: [block][own columns / 4][128 rows]
+        const bool idle = quarter * 32 >= ROWS;                               // none of this warp's rows has a result
+        unsigned char* const staging = smem + STAGES * STAGE + EXCHANGE + (half * (ROWS / 32) + (idle ? 0 : quarter)) * STAGING_BYTES;
+        float4* const exchange = (float4*)(smem + STAGES * STAGE);            // SPLIT: [block][own columns / 4][rows]
         u32 t = 0, round = 0;
         bool ok = true;
         auto filled = [&] {            // waits for accumulators; their address
@@ -664,9 +690,9 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
                         const int own = BN / (int)blocks, row = quarter * 32 + lane;      // (own: a power of two)
                         ok = __all_sync(0xffffffffu, wait_for_cluster(&taken, (round & 1) ^ 1, p.err));
                         if (!ok) break;
-                        if (warp == 4 && lane == 0) frnn_mbar_expect_tx(&arrived, EXCHANGE_BYTES);
+                        if (warp == 4 && lane == 0) frnn_mbar_expect_tx(&arrived, EXCHANGE);
 #pragma unroll
-                        for (int i = 0; i < BN / 2; i += 4) {
+                        for (int i = 0; i < BN / 2 && !idle; i += 4) {
                             const int c = half * (BN / 2) + i;
                             int owner, at;
                             if (EPI == GLU_FORWARD) {      // (an owner has the same columns of both products)
@@ -676,7 +702,7 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
                                 owner = c >> (__ffs(own) - 1);
                                 at = c & (own - 1);
                             }
-                            send(in_block(&exchange[((int)rank * own + at) / 4 * 128 + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3], in_block(&arrived, owner));
+                            send(in_block(&exchange[((int)rank * own + at) / 4 * ROWS + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3], in_block(&arrived, owner));
                         }
                         ok = __all_sync(0xffffffffu, wait_for_cluster(&arrived, round & 1, p.err));
                         if (!ok) break;
@@ -684,13 +710,14 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
                         const int width = EPI == GLU_FORWARD ? own / 2 : own, smallest = EPI == GLU_FORWARD ? 16 : 32;
                         const int count = max(min(width, smallest), width / 2), from = half * count;
                         const u32 place = tmem + 2 * BN + frnn_tmem_lane_base(quarter);
-                        if (from < width) {
+                        const bool works = from < width && !idle && row0 < p.M;
+                        if (works) {
 #pragma unroll 1
                             for (int i = 0; i < (EPI == GLU_FORWARD ? 2 : 1) * count; i += 4) {
                                 const int at = i < count ? from + i : own / 2 + from + i - count;
                                 float v[4] = {};
                                 for (u32 b = 0; b < blocks; b++) {
-                                    const float4 x = exchange[((int)b * own + at) / 4 * 128 + row];
+                                    const float4 x = exchange[((int)b * own + at) / 4 * ROWS + row];
                                     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
                                 }
                                 frnn_tmem_st4(place + half * 64 + i, v);
@@ -699,7 +726,7 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
                         }
                         __syncwarp();
                         if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
-                        if (from < width) {
+                        if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
                             epilogue<EPI>(p, place + half * 64, place + half * 64 + count, row0, tile_col + from, count, lane, staging);
                         }
@@ -717,7 +744,7 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __
                 }
             }
             constexpr int COUNT = EPI == GLU_FORWARD ? BN / 4 : BN / 2;
-            epilogue<EPI>(p, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, lane, staging);
+            if (!idle && row0 < p.M) epilogue<EPI>(p, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, lane, staging);
             emptied();
         }
     }
@@ -793,7 +820,8 @@ struct Scratch {
     }
 };
 
-inline int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+// Rows of 16-bit operands begin on whole lines: a box' rows of 128 bytes that straddle two cost two requests each.
+inline int64_t padded(int64_t n) { return (n + 63) / 64 * 64; }
 inline int planes_of(int dtype) { return dtype == FRNN_F32 ? 3 : 1; }
 
 struct Operand {                  // a [rows][cols] matrix in 16 bits
@@ -895,10 +923,10 @@ template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Produ
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     ProductPlan best = {PAIR, 2, up(q.m, 256), up(q.n * width, 256)};
-    int64_t cost = up(best.tiles_m * best.tiles_n, clusters_at_once<product_kernel<SPLIT, AT, BT, EPI, true>>(2)) * (steps * 520 + 2000);
+    int64_t cost = up(best.tiles_m * best.tiles_n, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(2)) * (steps * 520 + 2000);
     const int64_t tm = up(q.m, 128), tn = up(q.n * width, 128);
     for (int blocks = 1; blocks <= 8 && blocks <= steps; blocks *= 2) {
-        const int64_t c = up(tm * tn, clusters_at_once<product_kernel<SPLIT, AT, BT, EPI, true>>(blocks)) * (up(steps, blocks) * 340 + (blocks > 1 ? 3000 : 1500));
+        const int64_t c = up(tm * tn, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks)) * (up(steps, blocks) * 340 + (blocks > 1 ? 3000 : 1500));
         if (c < cost) {
             cost = c;
             best = {blocks > 1 ? SPLIT : ALONE, blocks, tm, tn};
@@ -907,8 +935,8 @@ template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Produ
     return best;
 }
 
-template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_product(const char* what, const ProductArgs& p, int blocks, cudaStream_t stream) {
-    constexpr auto kernel = product_kernel<FORM, AT, BT, EPI, PROMOTE>;
+template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_product(const char* what, const ProductArgs& p, int blocks, cudaStream_t stream) {
+    constexpr auto kernel = product_kernel<FORM, THIN, AT, BT, EPI, PROMOTE>;
     // (the warps would wait for registers that the block does not have)
     static const bool enough = [] {
         cudaFuncAttributes a = {};
@@ -918,7 +946,7 @@ template <Form FORM, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_
     }();
     if (!enough) return frnn_fail(FRNN_E_LAUNCH, "%s: the kernel was not built for %d registers a thread, or there is no GPU to run it", what, (int)START_REGISTERS);
     if (!allow_shared<kernel>(PRODUCT_SHARED)) { cudaGetLastError(); return frnn_fail(FRNN_E_LAUNCH, "%s: no room in shared memory", what); }
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, clusters = std::min<int64_t>(tiles, clusters_at_once<product_kernel<SPLIT, AT, BT, EPI, true>>(blocks));
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, clusters = std::min<int64_t>(tiles, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks));
     return launch(what, kernel, dim3((unsigned)(clusters * blocks)), PRODUCT_THREADS, PRODUCT_SHARED, stream, true, blocks, p);
 }
 
@@ -947,7 +975,8 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);
     };
-    int rc = encode(p.a, q.a, AT, 128);
+    const bool thin = !AT && plan.form != PAIR && q.m <= THIN_ROWS;
+    int rc = encode(p.a, q.a, AT, thin ? THIN_ROWS : 128);
     for (int i = 0; i < 2 && rc == FRNN_OK; i++) {
         if (i && !q.b[1].p) p.b[1] = p.b[0];
         else rc = encode(p.b[i], q.b[i], BT, p.dual && plan.form != PAIR ? 64 : 128);
@@ -958,15 +987,18 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     p.out_ld = q.out_ld;
     p.out_wide = on_boundary(q.out, 16) && q.out_ld * (int64_t)dtype_bytes(q.out_dtype) % 16 == 0;
     constexpr bool EXACT = EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
-    auto run = [&](auto form) {
+    auto run = [&](auto form, auto rows) {
         constexpr Form FORM = decltype(form)::value;
-        return q.dtype == FRNN_F32 ? launch_product<FORM, AT, BT, EPI, true>(what, p, plan.blocks, stream) : launch_product<FORM, AT, BT, EPI, EXACT>(what, p, plan.blocks, stream);
+        constexpr bool THIN = decltype(rows)::value;
+        return q.dtype == FRNN_F32 ? launch_product<FORM, THIN, AT, BT, EPI, true>(what, p, plan.blocks, stream) : launch_product<FORM, THIN, AT, BT, EPI, EXACT>(what, p, plan.blocks, stream);
     };
-    switch (plan.form) {
-        case PAIR: return run(std::integral_constant<Form, PAIR>());
-        case ALONE: return run(std::integral_constant<Form, ALONE>());
-        default: return run(std::integral_constant<Form, SPLIT>());
+    const std::false_type all;
+    if (plan.form == PAIR) return run(std::integral_constant<Form, PAIR>(), all);
+    if constexpr (!AT) {
+        const std::true_type few;
+        if (thin) return plan.form == ALONE ? run(std::integral_constant<Form, ALONE>(), few) : run(std::integral_constant<Form, SPLIT>(), few);
     }
+    return plan.form == ALONE ? run(std::integral_constant<Form, ALONE>(), all) : run(std::integral_constant<Form, SPLIT>(), all);
 }
 
 }  // namespace frnn_lm

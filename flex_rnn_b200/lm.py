@@ -257,7 +257,7 @@ def _register_fakes():
 
     @fake("flex_rnn_b200::gated_mlp")
     def _(x, gate, up, down, activation, save):
-        kept = (x.numel() // x.shape[-1] if save else 0, (gate.shape[0] + 7) // 8 * 8)
+        kept = (x.numel() // x.shape[-1] if save else 0, (gate.shape[0] + 63) // 64 * 64)
         hidden = x.new_empty((3, *kept), dtype=th.bfloat16) if x.dtype == th.float32 else x.new_empty((1, *kept))
         return x.new_empty((*x.shape[:-1], down.shape[0])), x.new_empty(kept), x.new_empty(kept), hidden
 

@@ -244,7 +244,7 @@ int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64
  * the tensor cores with sums in 32 bits (fp32 operands as sums of three bf16 numbers); for bf16 and fp16 what lies between
  * two products (the hidden vector, and backward its gradients) is rounded to that type, because the tensor cores read it so.
  * y and all gradients are contiguous.  What the forward keeps for the backward (all three or none: NULL), on 16-byte boundaries,
- * with H = hidden rounded up to a multiple of 8: `by_gate` and `by_up` [n, H] of `dtype`, the hidden vectors' derivatives by the two
+ * with H = hidden rounded up to a multiple of 64: `by_gate` and `by_up` [n, H] of `dtype`, the hidden vectors' derivatives by the two
  * projections; `kept` [n, H] of `dtype`, for fp32 [3, n, H] bf16, the hidden vectors.
  */
 enum { FRNN_SILU = 0, FRNN_GELU = 1, FRNN_RELU = 2, FRNN_SIGMOID = 3 };
