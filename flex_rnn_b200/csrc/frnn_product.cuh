@@ -17,7 +17,7 @@
 //   PAIR   256 x 256 by a pair of blocks, each with half of B's rows, so that a byte of B in shared memory serves 256 rows
 //   ALONE  128 x 128 by a block: small products spread over more multiprocessors
 //   SPLIT  128 x 128 by a cluster of 2, 4 or 8 blocks, each with a part of k.  Each block then owns a part of the tile's columns: the others
-//          send it their sums of these (st.async into its shared memory), it adds them in the order of the blocks and has the epilogue
+//          send it their sums of these (into its shared memory), it adds them in the order of the blocks and has the epilogue
 //          to itself.  (4 stages, and 64 KB for what arrives.)
 // THIN (ALONE or SPLIT, up to 32 rows, as in generation): only 32 of A's rows are copied, so that 10 stages of B are under way, 160 KB a
 // multiprocessor: such products are as fast as their weights come.  The tensor cores read 128 rows all the same: what they find
@@ -116,10 +116,12 @@ template <int CG> __device__ __forceinline__ void tma_load(u32 dst, const CUtens
     else
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((u64)map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
-// 16 bytes to another block's shared memory, counted by its mbarrier when they are there
-__device__ __forceinline__ void send(u32 dst, float a, float b, float c, float d, u32 bar) {
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d), "r"(bar) : "memory");
+// 16 bytes to another block's shared memory.  (st.async, which counts each of them on an mbarrier, took 5 us for a block's 64 KB.)
+__device__ __forceinline__ void send(u32 dst, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
+// an arrival that says that what this warp has sent is there
+__device__ __forceinline__ void arrive_after_sending(u32 bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void arrive_at(u32 bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // frnn_mbar_wait for what other blocks of the cluster have written
 __device__ __forceinline__ bool wait_for_cluster(u64* bar, u32 parity, int* err) {
@@ -181,8 +183,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // ---- rows of 32 values --------------------------------------------------------------------------------------------------------
 
 // Each lane has 32 consecutive values of its row; they go to dst (rows ld elements apart) by way of shared memory, so that
-// neighbouring lanes write neighbouring bytes.  Of the warp's 32 rows `rows` exist, of the 32 columns `cols`.
-template <class T> __device__ __forceinline__ void put_rows(unsigned char* staging, int lane, const float* v, T* dst, int64_t ld, int rows, int cols, bool wide) {
+// neighbouring lanes write neighbouring bytes.  Of the warp's 32 rows `rows` exist, of the 32 columns `cols`.  `wide`: rows of dst begin on 16-byte
+// boundaries; `padded`: what lies behind a row's end up to such a boundary is nobody's.
+template <class T> __device__ __forceinline__ void put_rows(unsigned char* staging, int lane, const float* v, T* dst, int64_t ld, int rows, int cols, bool wide, bool padded) {
     constexpr int W = WIDE<T>, CHUNKS = 32 / W, ROW = 32 * (int)sizeof(T);       // 4 chunks of 8, or 8 of 4
     auto slot = [](int r, int c) { return r * ROW + ((c ^ (sizeof(T) == 2 ? (r >> 1) & 3 : r & 7)) * 16); };
 #pragma unroll
@@ -192,7 +195,7 @@ template <class T> __device__ __forceinline__ void put_rows(unsigned char* stagi
         x.store((T*)(staging + slot(lane, c)));
     }
     __syncwarp();
-    if (wide && cols == 32) {
+    if (wide && (padded || cols % W == 0)) {
         constexpr int AT_ONCE = 32 / CHUNKS;      // rows
         const int c = lane % CHUNKS;
 #pragma unroll
@@ -200,17 +203,17 @@ template <class T> __device__ __forceinline__ void put_rows(unsigned char* stagi
             const int r = r0 + lane / CHUNKS;
             Pack<T, W> x;
             x.load((const T*)(staging + slot(r, c)));
-            if (r < rows) x.store(dst + r * ld + c * W);
+            if (r < rows && c * W < cols) x.store(dst + r * ld + c * W);
         }
     } else if (lane < cols) {
         for (int r = 0; r < rows; r++) dst[r * ld + lane] = *(const T*)(staging + slot(r, lane / W) + lane % W * sizeof(T));
     }
     __syncwarp();
 }
-__device__ __forceinline__ void put_rows_as(int dtype, unsigned char* staging, int lane, const float* v, void* dst, int64_t at, int64_t ld, int rows, int cols, bool wide) {
-    if (dtype == FRNN_F32) put_rows(staging, lane, v, (float*)dst + at, ld, rows, cols, wide);
-    else if (dtype == FRNN_BF16) put_rows(staging, lane, v, (__nv_bfloat16*)dst + at, ld, rows, cols, wide);
-    else put_rows(staging, lane, v, (__half*)dst + at, ld, rows, cols, wide);
+__device__ __forceinline__ void put_rows_as(int dtype, unsigned char* staging, int lane, const float* v, void* dst, int64_t at, int64_t ld, int rows, int cols, bool wide, bool padded) {
+    if (dtype == FRNN_F32) put_rows(staging, lane, v, (float*)dst + at, ld, rows, cols, wide, padded);
+    else if (dtype == FRNN_BF16) put_rows(staging, lane, v, (__nv_bfloat16*)dst + at, ld, rows, cols, wide, padded);
+    else put_rows(staging, lane, v, (__half*)dst + at, ld, rows, cols, wide, padded);
 }
 // x = hi + mid + lo in bf16, exactly (values above the largest bf16 are cut off first; what is not finite stays in hi alone).
 __device__ __forceinline__ void split3(float x, float& hi, float& mid, float& lo) {
@@ -221,13 +224,9 @@ __device__ __forceinline__ void split3(float x, float& hi, float& mid, float& lo
     mid = whole ? __bfloat162float(__float2bfloat16_rn(rest)) : 0.f;
     lo = whole ? rest - mid : 0.f;
 }
-__device__ __forceinline__ void put_planes(int io, unsigned char* staging, int lane, float* v, const Planes& to, int64_t row, int col, int rows, int cols) {
+template <bool FP32> __device__ __forceinline__ void put_planes(int io, unsigned char* staging, int lane, float* v, const Planes& to, int64_t row, int col, int rows, int cols) {
     const int64_t at = row * to.ld + col;
-    if (io == FRNN_F16) {
-        put_rows(staging, lane, v, (__half*)to.p + at, to.ld, rows, cols, true);
-    } else if (io == FRNN_BF16) {
-        put_rows(staging, lane, v, (__nv_bfloat16*)to.p + at, to.ld, rows, cols, true);
-    } else {
+    if constexpr (FP32) {
 #pragma unroll 1
         for (int plane = 0; plane < 3; plane++) {          // each round leaves the rest of the one before
             float part[32];
@@ -237,74 +236,47 @@ __device__ __forceinline__ void put_planes(int io, unsigned char* staging, int l
                 split3(v[j], part[j], mid, lo);
                 v[j] = fabsf(part[j]) < INFINITY ? v[j] - part[j] : 0.f;
             }
-            put_rows(staging, lane, part, (__nv_bfloat16*)to.p + plane * to.plane + at, to.ld, rows, cols, true);
+            put_rows(staging, lane, part, (__nv_bfloat16*)to.p + plane * to.plane + at, to.ld, rows, cols, true, true);
         }
-    }
-}
-// 16 values of a lane's row, straight from its registers (aligned rows).
-template <class T> __device__ __forceinline__ void put_row(const float* v, T* dst, int cols) {
-    constexpr int W = WIDE<T>;
-#pragma unroll
-    for (int c = 0; c < 16; c += W) {
-        Pack<T, W> x;
-        x.from(v + c);
-        if (c < cols) x.store(dst + c);          // (rows are padded to whole accesses)
-    }
-}
-__device__ __forceinline__ void put_row_as(int dtype, const float* v, void* dst, int64_t at, int cols) {
-    if (dtype == FRNN_F32) put_row(v, (float*)dst + at, cols);
-    else if (dtype == FRNN_BF16) put_row(v, (__nv_bfloat16*)dst + at, cols);
-    else put_row(v, (__half*)dst + at, cols);
-}
-__device__ __forceinline__ void put_row_planes(int io, float* v, const Planes& to, int64_t at, int cols) {
-    if (io != FRNN_F32) {
-        put_row_as(io, v, to.p, at, cols);
+    } else if (io == FRNN_F16) {
+        put_rows(staging, lane, v, (__half*)to.p + at, to.ld, rows, cols, true, true);
     } else {
-#pragma unroll 1
-        for (int plane = 0; plane < 3; plane++) {          // each round leaves the rest of the one before
-            float part[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                float mid, lo;
-                split3(v[j], part[j], mid, lo);
-                v[j] = fabsf(part[j]) < INFINITY ? v[j] - part[j] : 0.f;
-            }
-            put_row(part, (__nv_bfloat16*)to.p + plane * to.plane + at, cols);
-        }
+        put_rows(staging, lane, v, (__nv_bfloat16*)to.p + at, to.ld, rows, cols, true, true);
     }
+}
+template <bool FP32> __device__ __forceinline__ void put_rows_io(int io, unsigned char* staging, int lane, const float* v, void* dst, int64_t at, int64_t ld, int rows, int cols) {
+    if constexpr (FP32) put_rows(staging, lane, v, (float*)dst + at, ld, rows, cols, true, true);
+    else if (io == FRNN_BF16) put_rows(staging, lane, v, (__nv_bfloat16*)dst + at, ld, rows, cols, true, true);
+    else put_rows(staging, lane, v, (__half*)dst + at, ld, rows, cols, true, true);
 }
 // The way back: 32 values of each lane's row out of 32 rows, read by neighbouring lanes (aligned rows; undefined beyond rows and cols).
-template <class T> __device__ __forceinline__ void get_rows(unsigned char* staging, int lane, const T* src, int64_t ld, int rows, int cols, float* v) {
-    constexpr int W = WIDE<T>, CHUNKS = 32 / W, ROW = 32 * (int)sizeof(T), AT_ONCE = 32 / CHUNKS;
-    auto slot = [](int r, int c) { return r * ROW + ((c ^ (sizeof(T) == 2 ? (r >> 1) & 3 : r & 7)) * 16); };
-    const int c = lane % CHUNKS;
-    if ((c + 1) * W <= (cols + W - 1) / W * W) {          // (rows are padded to whole accesses)
-        Pack<T, W> x[CHUNKS];
+// Asked for first, turned over by way of shared memory later.
+template <class T> struct Rows {
+    static constexpr int W = WIDE<T>, CHUNKS = 32 / W, AT_ONCE = 32 / CHUNKS;
+    Pack<T, W> x[CHUNKS];
+    __device__ __forceinline__ void ask(int lane, const T* src, int64_t ld, int rows, int cols) {
+        const int c = lane % CHUNKS;
 #pragma unroll
         for (int k = 0; k < CHUNKS; k++) {
             const int r = k * AT_ONCE + lane / CHUNKS;
-            if (r < rows) x[k].load(src + r * ld + c * W);
+            if (r < rows && c * W < cols) x[k].load(src + r * ld + c * W);      // (rows are padded to whole accesses)
         }
+    }
+    __device__ __forceinline__ void get(unsigned char* staging, int lane, float* v) const {
+        constexpr int ROW = 32 * (int)sizeof(T);
+        auto slot = [](int r, int c) { return r * ROW + ((c ^ (sizeof(T) == 2 ? (r >> 1) & 3 : r & 7)) * 16); };
+#pragma unroll
+        for (int k = 0; k < CHUNKS; k++) x[k].store((T*)(staging + slot(k * AT_ONCE + lane / CHUNKS, lane % CHUNKS)));
+        __syncwarp();
 #pragma unroll
         for (int k = 0; k < CHUNKS; k++) {
-            const int r = k * AT_ONCE + lane / CHUNKS;
-            if (r < rows) x[k].store((T*)(staging + slot(r, c)));
+            Pack<T, W> y;
+            y.load((const T*)(staging + slot(lane, k)));
+            y.to(v + k * W);
         }
+        __syncwarp();
     }
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < CHUNKS; k++) {
-        Pack<T, W> x;
-        x.load((const T*)(staging + slot(lane, k)));
-        x.to(v + k * W);
-    }
-    __syncwarp();
-}
-__device__ __forceinline__ void get_rows_as(int dtype, unsigned char* staging, int lane, const void* src, int64_t at, int64_t ld, int rows, int cols, float* v) {
-    if (dtype == FRNN_F32) get_rows(staging, lane, (const float*)src + at, ld, rows, cols, v);
-    else if (dtype == FRNN_BF16) get_rows(staging, lane, (const __nv_bfloat16*)src + at, ld, rows, cols, v);
-    else get_rows(staging, lane, (const __half*)src + at, ld, rows, cols, v);
-}
+};
 
 // ---- activations -----------------------------------------------------------------------------------------------------------
 
@@ -362,10 +334,65 @@ template <int N> __device__ __forceinline__ void wait_for(float* v) {
     for (int j = 0; j < N; j++) asm volatile("" : "+f"(v[j]));      // (nothing that uses them moves up)
 }
 
+// da = dh (b act'(a)), db = dh act(a), 32 columns at a time; the next ones' factors are on their way meanwhile.
+template <class T>
+__device__ __forceinline__ void glu_backward(const ProductArgs& p, u32 acc, int64_t row0, int first, int count, int rows, int lane, unsigned char* staging) {
+    Rows<T> gate, up;
+    auto fetch = [&](Rows<T>& to, const void* from, int i) {
+        const int col = first + i;
+        if (i < count) to.ask(lane, (const T*)from + row0 * p.by_ld + col, p.by_ld, rows, min(32, min(count - i, p.N - col)));
+    };
+    if (p.da.p) fetch(gate, p.by_gate, 0);
+    if (p.db.p) fetch(up, p.by_up, 0);
+#pragma unroll 1
+    for (int i = 0; i < count; i += 32) {
+        float d[32], f[32];
+        ask(acc + i, d);
+        wait_for<32>(d);
+        const int col = first + i, cols = min(32, min(count - i, p.N - col));
+        if (rows <= 0 || cols <= 0) break;
+        if (p.da.p) {
+            gate.get(staging, lane, f);
+            fetch(gate, p.by_gate, i + 32);
+#pragma unroll
+            for (int j = 0; j < 32; j++) f[j] *= d[j];
+            put_planes<sizeof(T) == 4>(p.io, staging, lane, f, p.da, row0, col, rows, cols);
+        }
+        if (p.db.p) {
+            up.get(staging, lane, f);
+            fetch(up, p.by_up, i + 32);
+#pragma unroll
+            for (int j = 0; j < 32; j++) f[j] *= d[j];
+            put_planes<sizeof(T) == 4>(p.io, staging, lane, f, p.db, row0, col, rows, cols);
+        }
+    }
+}
+
+// What the epilogues of log probabilities know of a lane's row, asked for before the accumulators are there.
+struct RowData {
+    int64_t token;
+    float lse2, entropy, g, h;
+};
+template <int EPI> __device__ __forceinline__ RowData row_data(const ProductArgs& p, int64_t row) {
+    RowData d = {-1, 0.f, 0.f, 0.f, 0.f};
+    if constexpr (EPI == LOGPROB_STATS || EPI == LOGPROB_GRAD) {
+        if (row < p.M) {
+            d.token = token_at(p.tokens, p.token_bytes, row);
+            if constexpr (EPI == LOGPROB_GRAD) {
+                d.lse2 = p.stats[2 * row];
+                d.entropy = p.stats[2 * row + 1];
+                if (p.dlogprob) d.g = p.dlogprob[row];
+                if (p.dentropy) d.h = p.dentropy[row];
+            }
+        }
+    }
+    return d;
+}
+
 // `count` columns from the one numbered `first` on, whose accumulators lie at `acc` (of GLU_FORWARD's second product at `acc2`), of the 32
 // rows from row0 on.
-template <int EPI>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, u32 acc2, int64_t row0, int first, int count, int lane, unsigned char* staging) {
+template <int EPI, bool FP32>
+__device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& data, u32 acc, u32 acc2, int64_t row0, int first, int count, int lane, unsigned char* staging) {
     // body(col, cols, v) for each 32 columns
     auto each = [&](auto body) {
         float v[32], next[32];
@@ -392,46 +419,38 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, u32 acc2
             for (int j = 0; j < 32; j++) v[j] *= alpha;
             if (p.add) {
                 float o[32];
-                get_rows(staging, lane, p.add + row0 * p.add_ld + col, p.add_ld, rows, cols, o);
+                Rows<float> sum;
+                sum.ask(lane, p.add + row0 * p.add_ld + col, p.add_ld, rows, cols);
+                sum.get(staging, lane, o);
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += o[j];
             }
-            put_rows_as(p.out_dtype, staging, lane, v, p.out, row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide);
+            put_rows_as(p.out_dtype, staging, lane, v, p.out, row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide, false);
         });
     } else if constexpr (EPI == GLU_FORWARD) {
 #pragma unroll 1
-        for (int i = 0; i < count; i += 16) {          // (16 values of each: full 32-byte sectors, and half the code)
-            float a[16], b[16], h[16];
-            frnn_tmem_ld<16>(acc + i, a);
-            frnn_tmem_ld<16>(acc2 + i, b);
-            wait_for<16>(a);
-            wait_for<16>(b);
-            const int col = first + i, cols = min(16, min(count - i, p.N - col));
-            if (lane >= rows || cols <= 0) continue;
-            glu<16>(p.activation, a, b, h, p.by_gate);
+        for (int i = 0; i < count; i += 32) {
+            float a[32], b[32], h[32];
+            ask(acc + i, a);
+            ask(acc2 + i, b);
+            wait_for<32>(a);
+            wait_for<32>(b);
+            const int col = first + i, cols = min(32, min(count - i, p.N - col));
+            if (rows <= 0 || cols <= 0) continue;
+            glu<32>(p.activation, a, b, h, p.by_gate);
             if (p.by_gate) {
-                put_row_as(p.io, a, p.by_gate, row * p.by_ld + col, cols);
-                put_row_as(p.io, b, p.by_up, row * p.by_ld + col, cols);
+                const int64_t at = row0 * p.by_ld + col;
+                put_rows_io<FP32>(p.io, staging, lane, a, p.by_gate, at, p.by_ld, rows, cols);
+                put_rows_io<FP32>(p.io, staging, lane, b, p.by_up, at, p.by_ld, rows, cols);
             }
-            put_row_planes(p.io, h, p.h, row * p.h.ld + col, cols);
+            put_planes<FP32>(p.io, staging, lane, h, p.h, row0, col, rows, cols);
         }
     } else if constexpr (EPI == GLU_BACKWARD) {
-        each([&](int col, int cols, float* d) {
-            float f[32];
-            if (rows <= 0 || cols <= 0) return;
-#pragma unroll 1
-            for (int k = 0; k < 2; k++) {
-                const Planes& to = k ? p.db : p.da;
-                if (!to.p) continue;
-                get_rows_as(p.io, staging, lane, k ? p.by_up : p.by_gate, row0 * p.by_ld + col, p.by_ld, rows, cols, f);
-#pragma unroll
-                for (int j = 0; j < 32; j++) f[j] *= d[j];
-                put_planes(p.io, staging, lane, f, to, row0, col, rows, cols);
-            }
-        });
+        if constexpr (FP32) glu_backward<float>(p, acc, row0, first, count, rows, lane, staging);
+        else if (p.io == FRNN_BF16) glu_backward<__nv_bfloat16>(p, acc, row0, first, count, rows, lane, staging);
+        else glu_backward<__half>(p, acc, row0, first, count, rows, lane, staging);
     } else if constexpr (EPI == LOGPROB_STATS) {
-        int64_t token = -1;
-        if (lane < rows) token = token_at(p.tokens, p.token_bytes, row);
+        const int64_t token = data.token;
         float m = -3.4028235e38f, s = 0.f, t = 0.f;
         each([&](int col, int cols, float* v) {
             if (cols <= 0) return;
@@ -465,17 +484,9 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, u32 acc2
             to[2 * (int64_t)p.M] = t;
         }
     } else {
-        int64_t token = -1;
-        float lse2 = 0.f, entropy = 0.f, g = 0.f, h = 0.f;
-        bool empty = false;
-        if (lane < rows) {
-            token = token_at(p.tokens, p.token_bytes, row);
-            lse2 = p.stats[2 * row];
-            entropy = p.stats[2 * row + 1];
-            g = p.dlogprob && token != p.ignore_index ? p.dlogprob[row] : 0.f;
-            h = p.dentropy ? p.dentropy[row] : 0.f;
-            empty = lse2 == -INFINITY;
-        }
+        const int64_t token = data.token;
+        const float lse2 = data.lse2, entropy = data.entropy, g = token != p.ignore_index ? data.g : 0.f, h = data.h;
+        const bool empty = lse2 == -INFINITY;
         const float k = p.inv_t * (p.scale ? *p.scale : 1.f);
         each([&](int col, int cols, float* v) {
             if (rows <= 0 || cols <= 0) return;
@@ -487,7 +498,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, u32 acc, u32 acc2
                 if (hit == j) d += g;
                 v[j] = empty ? 0.f : d * k;
             }
-            put_planes(p.io, staging, lane, v, p.grad, row0, col, rows, cols);
+            put_planes<FP32>(p.io, staging, lane, v, p.grad, row0, col, rows, cols);
         });
     }
 }
@@ -533,7 +544,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
             frnn_mbar_init(&acc_empty[b], EPILOGUE_WARPS * CG);
         }
         if (FORM == SPLIT) {
-            frnn_mbar_init(&arrived, 1);
+            frnn_mbar_init(&arrived, EPILOGUE_WARPS * blocks);
             frnn_mbar_init(&taken, EPILOGUE_WARPS * blocks);
         }
         frnn_mbar_init_fence();
@@ -662,6 +673,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
         for (int u = first; ok && u < tiles; u += stride, round++) {
             const Tile w = tile_of(p, u);
             const int64_t row0 = (int64_t)(w.tm * CG + (int)half_m) * 128 + quarter * 32;
+            const RowData data = row_data<EPI>(p, row0 + lane);
             u32 acc = filled();
             if (!ok) break;
             if constexpr (PROMOTE || FORM == SPLIT) {
@@ -690,7 +702,6 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         const int own = BN / (int)blocks, row = quarter * 32 + lane;      // (own: a power of two)
                         ok = __all_sync(0xffffffffu, wait_for_cluster(&taken, (round & 1) ^ 1, p.err));
                         if (!ok) break;
-                        if (warp == 4 && lane == 0) frnn_mbar_expect_tx(&arrived, EXCHANGE);
 #pragma unroll
                         for (int i = 0; i < BN / 2 && !idle; i += 4) {
                             const int c = half * (BN / 2) + i;
@@ -702,33 +713,36 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                                 owner = c >> (__ffs(own) - 1);
                                 at = c & (own - 1);
                             }
-                            send(in_block(&exchange[((int)rank * own + at) / 4 * ROWS + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3], in_block(&arrived, owner));
+                            send(in_block(&exchange[((int)rank * own + at) / 4 * ROWS + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
                         }
+                        __syncwarp();
+                        if (lane < (int)blocks) arrive_after_sending(in_block(&arrived, lane));
                         ok = __all_sync(0xffffffffu, wait_for_cluster(&arrived, round & 1, p.err));
                         if (!ok) break;
-                        // the owner's columns: halves of 32 or 16, or all of them by the first warps
-                        const int width = EPI == GLU_FORWARD ? own / 2 : own, smallest = EPI == GLU_FORWARD ? 16 : 32;
-                        const int count = max(min(width, smallest), width / 2), from = half * count;
-                        const u32 place = tmem + 2 * BN + frnn_tmem_lane_base(quarter);
+                        // the owner's columns: half of them each, but whole accesses of 8 (both products' of GLU_FORWARD)
+                        const int width = EPI == GLU_FORWARD ? own / 2 : own, count = max(8, width / 2), from = half * count;
+                        const u32 place = tmem + 2 * BN + frnn_tmem_lane_base(quarter) + half * 64;
                         const bool works = from < width && !idle && row0 < p.M;
                         if (works) {
-#pragma unroll 1
-                            for (int i = 0; i < (EPI == GLU_FORWARD ? 2 : 1) * count; i += 4) {
-                                const int at = i < count ? from + i : own / 2 + from + i - count;
-                                float v[4] = {};
-                                for (u32 b = 0; b < blocks; b++) {
+                            const int values = (EPI == GLU_FORWARD ? 2 : 1) * count;
+                            float v[32] = {};
+                            for (u32 b = 0; b < blocks; b++) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4) {
+                                    if (i >= values) continue;
+                                    const int at = i < count ? from + i : own / 2 + from + i - count;
                                     const float4 x = exchange[((int)b * own + at) / 4 * ROWS + row];
-                                    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+                                    v[i] += x.x; v[i + 1] += x.y; v[i + 2] += x.z; v[i + 3] += x.w;
                                 }
-                                frnn_tmem_st4(place + half * 64 + i, v);
                             }
+                            frnn_tmem_st<32>(place, v);
                             frnn_tmem_wait_st();
                         }
                         __syncwarp();
                         if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
                         if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
-                            epilogue<EPI>(p, place + half * 64, place + half * 64 + count, row0, tile_col + from, count, lane, staging);
+                            epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, lane, staging);
                         }
                         continue;
                     } else {
@@ -744,7 +758,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 }
             }
             constexpr int COUNT = EPI == GLU_FORWARD ? BN / 4 : BN / 2;
-            if (!idle && row0 < p.M) epilogue<EPI>(p, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, lane, staging);
+            if (!idle && row0 < p.M) epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, lane, staging);
             emptied();
         }
     }
@@ -888,7 +902,7 @@ struct ProductPlan {
     Form form;
     int blocks;                                   // of a cluster
     int64_t tiles_m, tiles_n;
-    int columns() const { return form == PAIR ? 128 : form == ALONE ? 64 : blocks == 8 ? 16 : 32; }      // that a warp of the epilogue has in a row
+    int columns() const { return form == PAIR ? 128 : form == ALONE ? 64 : 64 / blocks; }      // that a warp of the epilogue has in a row
 };
 
 // Clusters of 1, 2, 4 or 8 blocks that run at once, one block to a multiprocessor.
@@ -916,20 +930,37 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
     return n;
 }
 
-// Which form.  Cycles, as measured: a step of 64 along k in a block 520 of PAIR, 340 of the others (of the products 256, their
-// copies are what takes longer); a tile besides, in PAIR 2000, else 1500 and where it is SPLIT 1500 more for the exchange; 9000 a kernel.
-// The fewest cycles of the busiest multiprocessor win.
+// Which form: the one that is done first, by what was measured (ns, on a B200).  A step of 64 along k takes 285 in PAIR (for 128 x 256 in
+// each block; the tensor cores' own time is 270), 205 in ALONE and 268 in SPLIT (for 128 x 128; 135, but 8 KB of operands for each 16
+// values of k are as much as shared memory gives, and the copies come on top).  A tile leaves in `leave` (STORE, GLU_FORWARD,
+// GLU_BACKWARD, LOGPROB_STATS, LOGPROB_GRAD), while the next one is computed; in SPLIT that has the exchange in it.
+// THIN products read 16 KB of weights a step: 372 when all multiprocessors do (6.5 TB/s), 225 at least (the tensor cores read 128 rows
+// of A whatever is in them).
+// Measured, us: 256 x 512 of K = 2048 PAIR 14.9, ALONE 9.7, SPLIT 9.9, 8.8 and 8.8 (2, 4 and 8 blocks); K = 16384 ALONE 55, SPLIT in 4 23.
+// A block of 16 rows, 4096 wide, 12288 hidden (both products): ALONE and 4 63, 2 and 4 58, 4 and 4 66; 2048 wide, 8192 hidden: ALONE and 4 29, 2 and 4 32.
+// Log probabilities of 16 rows, 65536 tokens, 4096 wide: ALONE 105, SPLIT in 2 115.
+inline bool is_thin(const Product& q, bool at, Form form) { return !at && form != PAIR && q.m <= THIN_ROWS; }
 template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
+    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2300, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 268};
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    auto cost = [&](Form form, int blocks, int64_t tiles) {
+        const int64_t at_once = clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks), rounds = up(tiles, at_once), out = leave[form][EPI];
+        auto k_time = [&](int64_t tiles) {
+            return (form == SPLIT ? up(steps, blocks) : steps) * (is_thin(q, AT, form) ? std::max<int64_t>(225, 372 * tiles * blocks / sm_count()) : step[form]);
+        };
+        const int64_t last = k_time(tiles - (rounds - 1) * at_once), start = (form == ALONE ? 1000 : 2000) + (form == SPLIT ? 1000 * rounds : 0);      // (its blocks wait for one another)
+        return rounds == 1 ? start + last + out : start + k_time(at_once) + (rounds - 2) * std::max(k_time(at_once), out) + std::max(last, out) + out;
+    };
     ProductPlan best = {PAIR, 2, up(q.m, 256), up(q.n * width, 256)};
-    int64_t cost = up(best.tiles_m * best.tiles_n, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(2)) * (steps * 520 + 2000);
+    int64_t least = cost(PAIR, 2, best.tiles_m * best.tiles_n);
     const int64_t tm = up(q.m, 128), tn = up(q.n * width, 128);
     for (int blocks = 1; blocks <= 8 && blocks <= steps; blocks *= 2) {
-        const int64_t c = up(tm * tn, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks)) * (up(steps, blocks) * 340 + (blocks > 1 ? 3000 : 1500));
-        if (c < cost) {
-            cost = c;
-            best = {blocks > 1 ? SPLIT : ALONE, blocks, tm, tn};
+        const Form form = blocks > 1 ? SPLIT : ALONE;
+        const int64_t c = cost(form, blocks, tm * tn);
+        if (c < least) {
+            least = c;
+            best = {form, blocks, tm, tn};
         }
     }
     return best;
@@ -975,7 +1006,7 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);
     };
-    const bool thin = !AT && plan.form != PAIR && q.m <= THIN_ROWS;
+    const bool thin = is_thin(q, AT, plan.form);
     int rc = encode(p.a, q.a, AT, thin ? THIN_ROWS : 128);
     for (int i = 0; i < 2 && rc == FRNN_OK; i++) {
         if (i && !q.b[1].p) p.b[1] = p.b[0];
