@@ -128,12 +128,15 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         rc = run_product<STORE, true, true>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }
-    for (int i = 0; i < 2; i++) {
-        if (!(i ? want_up : want_gate)) continue;
+    if (want_gate || want_up) {             // both in one: half of a small product would leave multiprocessors idle
         Product q = product(c, c->hidden, c->width, c->n);
-        q.a = i ? db : da;
+        q.a = want_gate ? both : db;
         q.b[0] = x;
-        store(q, i ? dup : dgate, c->width);
+        if (want_gate && want_up) {
+            q.args.stacked = planes;
+            q.args.out2 = dup;
+        }
+        store(q, want_gate ? dgate : dup, c->width);
         rc = run_product<STORE, true, true>(what, q, stream);
         if (rc != FRNN_OK) return rc;
     }

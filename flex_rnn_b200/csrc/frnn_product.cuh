@@ -59,6 +59,8 @@ struct alignas(64) ProductArgs {
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
     int ksteps, segments;       // steps of 64 along k in a segment
     int tiles_m, tiles_n, group;
+    int stacked;                // two products with the same B: the second's A is this many planes further on, its result at out2 (0: one)
+    void* out2;
     int b_ready;                // the kernel before this one writes nothing of B: its copies begin before that one ends
     int dual;                   // a tile's columns are half of B0's rows and half of B1's
     unsigned idesc;
@@ -392,7 +394,7 @@ template <int EPI> __device__ __forceinline__ RowData row_data(const ProductArgs
 // `count` columns from the one numbered `first` on, whose accumulators lie at `acc` (of GLU_FORWARD's second product at `acc2`), of the 32
 // rows from row0 on.
 template <int EPI, bool FP32>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& data, u32 acc, u32 acc2, int64_t row0, int first, int count, int lane, unsigned char* staging) {
+__device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& data, u32 acc, u32 acc2, int64_t row0, int first, int count, bool second, int lane, unsigned char* staging) {
     // body(col, cols, v) for each 32 columns
     auto each = [&](auto body) {
         float v[32], next[32];
@@ -425,7 +427,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += o[j];
             }
-            put_rows_as(p.out_dtype, staging, lane, v, p.out, row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide, false);
+            put_rows_as(p.out_dtype, staging, lane, v, second ? p.out2 : p.out, row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide, false);
         });
     } else if constexpr (EPI == GLU_FORWARD) {
 #pragma unroll 1
@@ -505,12 +507,14 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
-struct Tile { int tm, tn; };
+struct Tile { int tm, tn; bool second; };
 
 // Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
 __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u) {
     const int a_group = p.group * p.tiles_n, g = u / a_group, in = u % a_group, high = min(p.group, p.tiles_m - g * p.group);
-    return {g * p.group + in % high, in / high};
+    const int tm = g * p.group + in % high, half = p.tiles_m / 2;
+    const bool second = p.stacked && tm >= half;
+    return {second ? tm - half : tm, in / high, second};
 }
 
 // AT, BT: the operand's rows run along m (n) instead of k.
@@ -587,9 +591,8 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         tma_load<CG>(at + B_BYTES / 2, &p.b[1], k * BK, n, plane, bar);
                     }
                 };
-                auto load_a = [&](int s, int m, int g, int k) {
+                auto load_a = [&](int s, int m, int plane, int k) {
                     const u32 bar = bar_of(s), at = frnn_smem_addr(smem + s * STAGE);
-                    const int plane = p.plane_a[g];
                     if constexpr (AT) {
                         tma_load<CG>(at, &p.a, m, k * BK, plane, bar);
                         tma_load<CG>(at + A_BYTES / 2, &p.a, m + 64, k * BK, plane, bar);
@@ -603,7 +606,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 cudaGridDependencySynchronize();
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u);
-                    const int m = (w.tm * CG + (int)half_m) * 128, n = column(w);
+                    const int m = (w.tm * CG + (int)half_m) * 128, n = column(w), further = w.second ? p.stacked : 0;
                     int g = k_from / p.ksteps, k = k_from % p.ksteps;
                     for (int i = k_from; i < k_to; i++, it++) {
                         const int s = it % STAGES;
@@ -611,7 +614,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                             if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
                             load_b(s, n, g, k);
                         }
-                        load_a(s, m, g, k);
+                        load_a(s, m, p.plane_a[g] + further, k);
                         if (++k == p.ksteps) { k = 0; g++; }
                     }
                 }
@@ -742,7 +745,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
                         if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
-                            epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, lane, staging);
+                            epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, w.second, lane, staging);
                         }
                         continue;
                     } else {
@@ -758,7 +761,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 }
             }
             constexpr int COUNT = EPI == GLU_FORWARD ? BN / 4 : BN / 2;
-            if (!idle && row0 < p.M) epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, lane, staging);
+            if (!idle && row0 < p.M) epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, w.second, lane, staging);
             emptied();
         }
     }
@@ -934,8 +937,8 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
 // each block; the tensor cores' own time is 270), 205 in ALONE and 268 in SPLIT (for 128 x 128; 135, but 8 KB of operands for each 16
 // values of k are as much as shared memory gives, and the copies come on top).  A tile leaves in `leave` (STORE, GLU_FORWARD,
 // GLU_BACKWARD, LOGPROB_STATS, LOGPROB_GRAD), while the next one is computed; in SPLIT that has the exchange in it.
-// THIN products read 16 KB of weights a step: 372 when all multiprocessors do (6.5 TB/s), 225 at least (the tensor cores read 128 rows
-// of A whatever is in them).
+// Products of up to 128 rows read 16 KB of weights a step that nobody else reads: 372 when all multiprocessors do (6.5 TB/s).  THIN takes 225
+// at least (the tensor cores read 128 rows of A whatever is in them).
 // Measured, us: 256 x 512 of K = 2048 PAIR 14.9, ALONE 9.7, SPLIT 9.9, 8.8 and 8.8 (2, 4 and 8 blocks); K = 16384 ALONE 55, SPLIT in 4 23.
 // A block of 16 rows, 4096 wide, 12288 hidden (both products): ALONE and 4 63, 2 and 4 58, 4 and 4 66; 2048 wide, 8192 hidden: ALONE and 4 29, 2 and 4 32.
 // Log probabilities of 16 rows, 65536 tokens, 4096 wide: ALONE 105, SPLIT in 2 115.
@@ -943,18 +946,20 @@ inline bool is_thin(const Product& q, bool at, Form form) { return !at && form !
 template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
     static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2300, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 268};
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
+    const bool few = !AT && q.m <= 128;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     auto cost = [&](Form form, int blocks, int64_t tiles) {
         const int64_t at_once = clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks), rounds = up(tiles, at_once), out = leave[form][EPI];
         auto k_time = [&](int64_t tiles) {
-            return (form == SPLIT ? up(steps, blocks) : steps) * (is_thin(q, AT, form) ? std::max<int64_t>(225, 372 * tiles * blocks / sm_count()) : step[form]);
+            return (form == SPLIT ? up(steps, blocks) : steps) * std::max<int64_t>(is_thin(q, AT, form) ? 225 : step[form], few ? 372 * tiles * blocks / sm_count() : 0);
         };
         const int64_t last = k_time(tiles - (rounds - 1) * at_once), start = (form == ALONE ? 1000 : 2000) + (form == SPLIT ? 1000 * rounds : 0);      // (its blocks wait for one another)
         return rounds == 1 ? start + last + out : start + k_time(at_once) + (rounds - 2) * std::max(k_time(at_once), out) + std::max(last, out) + out;
     };
-    ProductPlan best = {PAIR, 2, up(q.m, 256), up(q.n * width, 256)};
+    const int64_t stack = q.args.stacked ? 2 : 1;
+    ProductPlan best = {PAIR, 2, up(q.m, 256) * stack, up(q.n * width, 256)};
     int64_t least = cost(PAIR, 2, best.tiles_m * best.tiles_n);
-    const int64_t tm = up(q.m, 128), tn = up(q.n * width, 128);
+    const int64_t tm = up(q.m, 128) * stack, tn = up(q.n * width, 128);
     for (int blocks = 1; blocks <= 8 && blocks <= steps; blocks *= 2) {
         const Form form = blocks > 1 ? SPLIT : ALONE;
         const int64_t c = cost(form, blocks, tm * tn);
@@ -1016,7 +1021,7 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     p.out = q.out;
     p.out_dtype = q.out_dtype;
     p.out_ld = q.out_ld;
-    p.out_wide = on_boundary(q.out, 16) && q.out_ld * (int64_t)dtype_bytes(q.out_dtype) % 16 == 0;
+    p.out_wide = on_boundary(q.out, 16) && on_boundary(p.out2, 16) && q.out_ld * (int64_t)dtype_bytes(q.out_dtype) % 16 == 0;
     constexpr bool EXACT = EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
     auto run = [&](auto form, auto rows) {
         constexpr Form FORM = decltype(form)::value;

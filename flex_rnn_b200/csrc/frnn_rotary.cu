@@ -2,10 +2,11 @@
 //
 //   u' = scale (u cos - w sin),  w' = scale (u sin + w cos);   the gradient is the turn back, scaled the same
 //
-// Bound by memory: x once, y once.  A lane takes E pairs of a place (of a batch and a position): their sines and cosines
-// are computed once, in registers, and turn the pairs of all heads that the lane's warp passes.  Angles: position * frequency
-// in 64 bits, taken modulo a turn there (a position of 10^6 at frequency 1 is 1.6 10^5 turns: in 32 bits 2 % of a turn would be
-// lost), then sine and cosine of the rest in 32 bits.
+// Bound by memory: x once, y once.  A warp has a place (of a batch and a position) and some or all of its heads.  Its lanes compute
+// the place's sines and cosines once, each a few, into a table in shared memory; a lane then keeps those of its E pairs in
+// registers for all heads that it passes, U of them at a time, whose loads are under way together and before the table is made.
+// Angles: position * frequency in 64 bits, taken modulo a turn there (a position of 10^6 at frequency 1 is 1.6 10^5 turns: in 32 bits
+// 2 % of a turn would be lost), then sine and cosine of the rest in 32 bits.
 #include <algorithm>
 
 #include "frnn_lm.cuh"
@@ -50,51 +51,85 @@ __device__ __forceinline__ void turn(double position, double frequency, float sc
 }
 
 template <class T, int E, bool INTERLEAVED> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+    constexpr int U = E >= 4 ? 4 : 8;
+    __shared__ float2 tables[8][32 * E];
     const int lane = threadIdx.x % 32, in_head = lane % a.lanes, heads_at_once = 32 / a.lanes;
     const int64_t warp = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
     if (warp >= a.warps) return;
+    float2* const table = tables[threadIdx.x / 32];
     const int64_t place = warp / a.per_place, b = place / a.length, t = place % a.length;
     const int64_t first = warp % a.per_place * a.heads_each, last = min(a.heads, first + a.heads_each);
     const T* const x = (const T*)a.x + b * a.x_stride[0] + t * a.x_stride[1];
     T* const y = (T*)a.y + b * a.y_stride[0] + t * a.y_stride[1];
     const double position = a.positions ? (double)token_at(a.positions, a.position_bytes, b * a.p_stride[0] + t * a.p_stride[1]) : (double)(a.start + t);
     const int items = (int)(a.pairs / E);
-    for (int i = in_head; i < items; i += a.lanes) {
+    for (int i0 = 0; i0 < items; i0 += a.lanes) {
+        const int i = i0 + in_head;
+        const bool mine = i < items;
+        const int64_t u = INTERLEAVED ? 2 * E * i : E * i, w = INTERLEAVED ? 2 * E * i + E : a.pairs + E * i;
+        T p[U][E], q[U][E];
+        auto fetch = [&](int64_t h) {
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int64_t at = h + k * heads_at_once;
+                if (mine && at < last) {
+                    load_few<T, E>(x + at * a.x_stride[2] + u, p[k]);
+                    load_few<T, E>(x + at * a.x_stride[2] + w, q[k]);
+                }
+            }
+        };
+        int64_t h = first + lane / a.lanes;
+        fetch(h);
+        __syncwarp();                     // (the table of the pairs before these has been read)
+        for (int k = lane; k < min(a.lanes, items - i0) * E; k += 32) {
+            const int pair = i0 * E + k;
+            turn(position, a.frequency_bytes == 8 ? ((const double*)a.frequencies)[pair] : (double)((const float*)a.frequencies)[pair], a.scale, a.direction, table[k].x, table[k].y);
+        }
+        __syncwarp();
         float c[E], s[E];
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            turn(position, a.frequency_bytes == 8 ? ((const double*)a.frequencies)[i * E + e] : (double)((const float*)a.frequencies)[i * E + e], a.scale, a.direction, c[e], s[e]);
-        const int64_t u = INTERLEAVED ? 2 * E * i : E * i, w = INTERLEAVED ? 2 * E * i + E : a.pairs + E * i;
-#pragma unroll 2
-        for (int64_t h = first + lane / a.lanes; h < last; h += heads_at_once) {
-            T p[E], q[E];
-            load_few<T, E>(x + h * a.x_stride[2] + u, p);
-            load_few<T, E>(x + h * a.x_stride[2] + w, q);
-            auto rotate = [&](T& p0, T& q0, float c0, float s0) {
-                const float f = to_float(p0), g = to_float(q0);
-                p0 = from_float<T>(f * c0 - g * s0);
-                q0 = from_float<T>(f * s0 + g * c0);
-            };
-            if constexpr (INTERLEAVED && E > 1) {      // E pairs lie in a row, half of them in p
+        for (int e = 0; e < E; e++) {
+            const float2 z = mine ? table[in_head * E + e] : make_float2(0.f, 0.f);
+            c[e] = z.x;
+            s[e] = z.y;
+        }
+        while (h < last) {
 #pragma unroll
-                for (int e = 0; e < E / 2; e++) {
-                    rotate(p[2 * e], p[2 * e + 1], c[e], s[e]);
-                    rotate(q[2 * e], q[2 * e + 1], c[E / 2 + e], s[E / 2 + e]);
+            for (int k = 0; k < U; k++) {
+                const int64_t at = h + k * heads_at_once;
+                if (!mine || at >= last) continue;
+                auto rotate = [&](T& p0, T& q0, float c0, float s0) {
+                    const float f = to_float(p0), g = to_float(q0);
+                    p0 = from_float<T>(f * c0 - g * s0);
+                    q0 = from_float<T>(f * s0 + g * c0);
+                };
+                if constexpr (INTERLEAVED && E > 1) {      // E pairs lie in a row, half of them in p
+#pragma unroll
+                    for (int e = 0; e < E / 2; e++) {
+                        rotate(p[k][2 * e], p[k][2 * e + 1], c[e], s[e]);
+                        rotate(q[k][2 * e], q[k][2 * e + 1], c[E / 2 + e], s[E / 2 + e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e++) rotate(p[k][e], q[k][e], c[e], s[e]);
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) rotate(p[e], q[e], c[e], s[e]);
+                store_few<T, E>(y + at * a.y_stride[2] + u, p[k]);
+                store_few<T, E>(y + at * a.y_stride[2] + w, q[k]);
             }
-            store_few<T, E>(y + h * a.y_stride[2] + u, p);
-            store_few<T, E>(y + h * a.y_stride[2] + w, q);
+            h += U * heads_at_once;
+            if (h < last) fetch(h);
         }
     }
     const int rest = (int)((a.width - 2 * a.pairs) / E);
     for (int i = in_head; i < rest; i += a.lanes)
-        for (int64_t h = first + lane / a.lanes; h < last; h += heads_at_once) {
-            T p[E];
-            load_few<T, E>(x + h * a.x_stride[2] + 2 * a.pairs + E * i, p);
-            store_few<T, E>(y + h * a.y_stride[2] + 2 * a.pairs + E * i, p);
+        for (int64_t h = first + lane / a.lanes; h < last; h += U * heads_at_once) {
+            T p[U][E];
+#pragma unroll
+            for (int k = 0; k < U; k++)
+                if (h + k * heads_at_once < last) load_few<T, E>(x + (h + k * heads_at_once) * a.x_stride[2] + 2 * a.pairs + E * i, p[k]);
+#pragma unroll
+            for (int k = 0; k < U; k++)
+                if (h + k * heads_at_once < last) store_few<T, E>(y + (h + k * heads_at_once) * a.y_stride[2] + 2 * a.pairs + E * i, p[k]);
         }
 }
 
