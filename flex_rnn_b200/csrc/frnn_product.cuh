@@ -457,14 +457,24 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
         each([&](int col, int cols, float* v) {
             if (cols <= 0) return;
             const int64_t hit = token - p.first - col;
-            float top = m, x = 0.f;
+            float tops[4] = {m, m, m, m};
+            if (cols == 32) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-                v[j] = j < cols ? v[j] * p.c2 : -INFINITY;
-                top = fmaxf(top, v[j]);
-                if (hit == j) x += v[j];          // (a choice of one becomes an index into registers, which then all live in memory)
+                for (int j = 0; j < 32; j++) v[j] *= p.c2;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = j < cols ? v[j] * p.c2 : -INFINITY;
             }
-            if (hit >= 0 && hit < cols && lane < rows) p.target[row] = x;
+#pragma unroll
+            for (int j = 0; j < 32; j++) tops[j % 4] = fmaxf(tops[j % 4], v[j]);
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            if (__any_sync(0xffffffffu, hit >= 0 && hit < cols)) {          // (one chunk of thousands)
+                float x = 0.f;          // (a choice of one becomes an index into registers, which then all live in memory)
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (hit == j) x += v[j];
+                if (hit >= 0 && hit < cols && lane < rows) p.target[row] = x;
+            }
             const float down = exp2_fast(m - top);
             t = s == 0.f ? 0.f : down * (t + s * (m - top));
             s *= down;
@@ -489,16 +499,23 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
         const int64_t token = data.token;
         const float lse2 = data.lse2, entropy = data.entropy, g = token != p.ignore_index ? data.g : 0.f, h = data.h;
         const bool empty = lse2 == -INFINITY;
-        const float k = p.inv_t * (p.scale ? *p.scale : 1.f);
+        const float k = p.inv_t * (p.scale ? *p.scale : 1.f), gk = -g * k, hk = -h * k;
         each([&](int col, int cols, float* v) {
             if (rows <= 0 || cols <= 0) return;
             const int64_t hit = token - p.first - col;
 #pragma unroll
             for (int j = 0; j < 32; j++) {
                 const float u = fmaf(v[j], p.c2, -lse2), e = exp2_fast(u);
-                float d = -e * fmaf(h, fmaf(fmaxf(u, -1e30f), 0.69314718055994531f, entropy), g);
-                if (hit == j) d += g;
-                v[j] = empty ? 0.f : d * k;
+                v[j] = e * fmaf(hk, fmaf(fmaxf(u, -1e30f), 0.69314718055994531f, entropy), gk);
+            }
+            if (__any_sync(0xffffffffu, hit >= 0 && hit < cols)) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (hit == j) v[j] -= gk;
+            }
+            if (__any_sync(0xffffffffu, empty)) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = empty ? 0.f : v[j];
             }
             put_planes<FP32>(p.io, staging, lane, v, p.grad, row0, col, rows, cols);
         });

@@ -1,7 +1,9 @@
 """A small recurrent language model that runs the operators of this package together: embedding, layer norms, Gated Delta
-Rule scans (``jit``), a layer norm of each head, log probabilities.
+Rule scans (``jit``), a layer norm of each head, log probabilities; as options rotary positions on queries and keys, a gated
+feed-forward block behind each scan, and a loss without logits.
 
     python -m flex_rnn_b200.language_model                  # trains on synthetic text, scores it, continues it
+    python -m flex_rnn_b200.language_model --hidden 704 --turned 32 --without-logits
 
 Training: ``model.loss(tokens)`` and its gradients.  Scoring: ``model.score(tokens, top=5)``.  Generation: ``model.generate``
 reads a prompt once and then one token a call, with the layers' states handed on.  ``plain=True`` computes the same from
@@ -10,7 +12,7 @@ the operators' definitions in plain PyTorch, on any device and in any precision.
 from __future__ import annotations
 
 import argparse
-from typing import List, Optional, Tuple
+from typing import List, Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -25,9 +27,10 @@ scan = jit(gated_delta_rule)
 
 class Layer(nn.Module):
     """x + W_out norm_of_heads(scan(projections of norm(x) at this place and the one before)).  Its state: the scan's, and
-    norm(x) of the last place."""
+    norm(x) of the last place.  ``turned`` values of each head's query and key carry rotary positions; with ``hidden``, a gated
+    feed-forward block of that many values follows: x + block(norm(x))."""
 
-    def __init__(self, width: int, heads: int, head_width: int):
+    def __init__(self, width: int, heads: int, head_width: int, hidden: int = 0, turned: int = 0):
         super().__init__()
         self.heads, self.head_width = heads, head_width
         n = heads * head_width
@@ -35,28 +38,45 @@ class Layer(nn.Module):
         self.project = nn.Linear(2 * width, 3 * n + 2 * heads, bias=False)
         self.head_weight, self.head_bias = nn.Parameter(torch.ones(heads, head_width)), nn.Parameter(torch.zeros(heads, head_width))
         self.out = nn.Linear(n, width, bias=False)
+        self.hidden, self.turned = hidden, turned
+        if turned:
+            # (not a buffer: a model that changes its type keeps its frequencies in 64 bits)
+            self.frequencies = lm.rotary_frequencies(turned, base=500.0)
+        if hidden:
+            self.block_weight, self.block_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
+            self.gate, self.up, self.down = nn.Linear(width, hidden, bias=False), nn.Linear(width, hidden, bias=False), nn.Linear(hidden, width, bias=False)
 
-    def forward(self, x, state, ops):
+    def forward(self, x, state, ops, position: int = 0):
         B, T, _ = x.shape
         H, M = self.heads, self.head_width
         state, last = state
         h = ops.layer_norm(x, self.norm_weight, self.norm_bias)
         before = torch.cat([last[:, None], h[:, :-1]], 1)
         q, k, v, g, beta = self.project(torch.cat([h, before], -1)).split([H * M, H * M, H * M, H, H], dim=-1)
-        row = lambda t: F.normalize(t.view(B, T, H, 1, M), dim=-1)
+        # (padding has zero vectors; 1e-12, the usual bound, is zero in fp16)
+        row = lambda t: F.normalize(t.view(B, T, H, 1, M), dim=-1, eps=max(1e-12, torch.finfo(t.dtype).tiny))
         scalar = lambda t: torch.sigmoid(t).view(B, T, H, 1, 1)
+        q, k = row(q), row(k)
+        if self.turned:
+            self.frequencies = self.frequencies.to(x.device)
+            q, k = ops.rotary(q, position, self.frequencies), ops.rotary(k, position, self.frequencies)
         # states are kept in 32 bits from call to call; the outputs have their type
-        y, state = ops.scan(row(q), row(k), v.reshape(B, T, H, M, 1), scalar(g + 3), scalar(beta), state)
+        y, state = ops.scan(q, k, v.reshape(B, T, H, M, 1), scalar(g + 3), scalar(beta), state)
         y = ops.layer_norm(y.to(x.dtype), self.head_weight, self.head_bias)
-        return x + self.out(y.reshape(B, T, H * M)), (state, h[:, -1])
+        x = x + self.out(y.reshape(B, T, H * M))
+        if self.hidden:
+            x = x + ops.gated_mlp(ops.layer_norm(x, self.block_weight, self.block_bias), self.gate.weight, self.up.weight, self.down.weight)
+        return x, (state, h[:, -1])
 
 
 class _Fast:
     embedding, layer_norm, token_logprobs, scan = staticmethod(lm.embedding), staticmethod(lm.layer_norm), staticmethod(lm.token_logprobs), staticmethod(scan)
+    rotary, gated_mlp, linear_logprobs = staticmethod(lm.rotary), staticmethod(lm.gated_mlp), staticmethod(lm.linear_logprobs)
 
 
 class _Plain:
     embedding, layer_norm, token_logprobs = staticmethod(lm.naive_embedding), staticmethod(lm.naive_layer_norm), staticmethod(lm.naive_token_logprobs)
+    rotary, gated_mlp, linear_logprobs = staticmethod(lm.naive_rotary), staticmethod(lm.naive_gated_mlp), staticmethod(lm.naive_linear_logprobs)
 
     @staticmethod
     def scan(*args):
@@ -64,12 +84,16 @@ class _Plain:
 
 
 class RecurrentLM(nn.Module):
-    def __init__(self, vocabulary: int, width: int = 256, layers: int = 2, heads: int = 4, head_width: int = 64, plain: bool = False):
+    """``hidden`` and ``turned``: see ``Layer``.  Without ``keep_logits``, ``loss`` and scores without alternatives are computed
+    from the vectors before the last projection."""
+
+    def __init__(self, vocabulary: int, width: int = 256, layers: int = 2, heads: int = 4, head_width: int = 64, plain: bool = False, hidden: int = 0, turned: int = 0, keep_logits: bool = True):
         super().__init__()
+        self.keep_logits = keep_logits
         self.ops = _Plain if plain else _Fast
         self.scale = width ** 0.5
         self.weight = nn.Parameter(torch.randn(vocabulary, width) * width ** -0.5)
-        self.layers = nn.ModuleList(Layer(width, heads, head_width) for _ in range(layers))
+        self.layers = nn.ModuleList(Layer(width, heads, head_width, hidden, turned) for _ in range(layers))
         self.norm_weight, self.norm_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
         self.head = nn.Linear(width, vocabulary, bias=False)
 
@@ -78,17 +102,25 @@ class RecurrentLM(nn.Module):
         dtype = torch.promote_types(p.dtype, torch.float32)
         return [(torch.zeros(batch, l.heads, l.head_width, l.head_width, dtype=dtype, device=p.device), p.new_zeros(batch, p.shape[1])) for l in self.layers]
 
-    def forward(self, tokens, states: Optional[list] = None) -> Tuple[torch.Tensor, list]:
-        """tokens [B,T] (``-100``: padding, a zero input), the layers' states -> logits [B,T,vocabulary], new states"""
+    def features(self, tokens, states: Optional[list] = None, position: int = 0) -> Tuple[torch.Tensor, list]:
+        """tokens [B,T] (``-100``: padding, a zero input), the layers' states, the first token's position -> what the last
+        projection takes [B,T,width], new states"""
         states = self.states(tokens.shape[0]) if states is None else states
         x, new = self.ops.embedding(tokens, self.weight, scale=self.scale), []
         for layer, state in zip(self.layers, states):
-            x, state = layer(x, state, self.ops)
+            x, state = layer(x, state, self.ops, position)
             new.append(state)
-        return self.head(self.ops.layer_norm(x, self.norm_weight, self.norm_bias)), new
+        return self.ops.layer_norm(x, self.norm_weight, self.norm_bias), new
 
-    def score(self, tokens, top: int = 0, temperature: float = 1.0) -> lm.TokenLogprobs:
+    def forward(self, tokens, states: Optional[list] = None, position: int = 0) -> Tuple[torch.Tensor, list]:
+        """As ``features``, but with logits [B,T,vocabulary]."""
+        x, new = self.features(tokens, states, position)
+        return self.head(x), new
+
+    def score(self, tokens, top: int = 0, temperature: float = 1.0) -> Union[lm.TokenLogprobs, lm.LinearLogprobs]:
         """Log probability of each token but the first of tokens [B,T] after those before it; padding counts as 0."""
+        if not self.keep_logits and not top:
+            return self.ops.linear_logprobs(self.features(tokens[:, :-1])[0], self.head.weight, tokens[:, 1:], temperature=temperature)
         logits, _ = self(tokens[:, :-1])
         return self.ops.token_logprobs(logits, tokens[:, 1:], top=top, temperature=temperature)
 
@@ -103,12 +135,12 @@ class RecurrentLM(nn.Module):
         """The most probable continuation, token by token, of prompt [B,T]: tokens [B,steps] and their log probabilities."""
         logits, states = self(prompt)
         last, tokens, logprobs = logits[:, -1], [], []
-        for _ in range(steps):
+        for step in range(steps):
             # (the alternatives come with the log probability of any token; 0 stands in for it)
             best = self.ops.token_logprobs(last, torch.zeros_like(prompt[:, 0]), top=1, temperature=temperature)
             tokens.append(best.top_token)
             logprobs.append(best.top_logprob)
-            logits, states = self(best.top_token, states)
+            logits, states = self(best.top_token, states, prompt.shape[1] + step)
             last = logits[:, 0]
         return torch.cat(tokens, 1), torch.cat(logprobs, 1)
 
@@ -128,9 +160,12 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--length", type=int, default=128)
     ap.add_argument("--vocabulary", type=int, default=512)
+    ap.add_argument("--hidden", type=int, default=0, help="values of a gated feed-forward block behind each scan (0: none)")
+    ap.add_argument("--turned", type=int, default=0, help="values of each head's query and key that carry rotary positions")
+    ap.add_argument("--without-logits", action="store_true", help="the loss from the vectors before the last projection")
     a = ap.parse_args(argv)
     torch.manual_seed(0)
-    model = RecurrentLM(a.vocabulary).cuda()
+    model = RecurrentLM(a.vocabulary, hidden=a.hidden, turned=a.turned, keep_logits=not a.without_logits).cuda()
     optimiser = torch.optim.AdamW(model.parameters(), lr=3e-3)
     for step in range(a.steps):
         loss = model.loss(synthetic_text(a.batch, a.length, a.vocabulary, seed=step).cuda(), entropy_weight=0.001)

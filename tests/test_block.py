@@ -9,6 +9,9 @@ is rounded to the operands' type (half a unit in the last place, UNIT); how thes
 is computed next to the exact results, term by term, with absolute values."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -666,6 +669,30 @@ def test_guard_bands(monkeypatch):
             logprobs_check(*logprobs_case(n, V, D, dtype))
         for B, T, H, N, pairs in [(1, 1, 1, 2, 1), (2, 3, 4, 64, 32), (1, 7, 3, 97, 31)]:
             rotary_check(rand(B, T, H, N).to(dtype), 3, lm.rotary_frequencies(2 * pairs, device="cuda"), True)
+
+
+@pytest.mark.gpu
+def test_first_use_is_a_captured_one():
+    """A process whose first use of each operator, forward and backward, is captured into a graph."""
+    program = """
+import torch, flex_rnn_b200 as fr
+g = torch.Generator(device="cuda").manual_seed(0)
+r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16().requires_grad_()
+x, gate, up, down, w, t = r(300, 96), r(200, 96), r(200, 96), r(96, 200), r(1000, 96), torch.arange(300, device="cuda")
+f = fr.rotary_frequencies(96, device="cuda")
+def step():
+    y = fr.gated_mlp(fr.rotary(x.view(1, 300, 1, 96), 5, f).view(300, 96), gate, up, down)
+    lp = fr.linear_logprobs(y, w, t).logprob
+    return [lp, *torch.autograd.grad(lp.sum(), [x, gate, up, down, w])]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+print(all(torch.equal(a, b) for a, b in zip(got, step())))
+"""
+    r = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=600)
+    assert r.stdout.split() == ["True"], r.stdout + r.stderr[-2000:]
 
 
 # ---- what is refused ----------------------------------------------------------------------------------------------------------------
