@@ -74,11 +74,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_cuda(const Tensor& x, const
     sizes.back() = m.c.out_width;
     const int64_t n = save ? m.c.n : 0, ld = (m.c.hidden + 63) / 64 * 64;
     const bool wide = x.scalar_type() == at::kFloat;
-    Tensor y = make("the output", sizes, x.scalar_type(), x), by_gate = make("the derivatives by gate", {n, ld}, x.scalar_type(), x), by_up = make("the derivatives by up", {n, ld}, x.scalar_type(), x);
+    Tensor y = make("the output", sizes, x.scalar_type(), x), by_gate = make("the derivatives by gate", {n, ld}, at::kFloat, x), by_up = make("the derivatives by up", {n, ld}, at::kFloat, x);
     Tensor hidden = make("the hidden vectors", {wide ? 3 : 1, n, ld}, wide ? at::kBFloat16 : x.scalar_type(), x);
     if (m.c.n) {
         const Tensor work = workspace(g_gated_mlp_forward_workspace(&m.c), x);
-        ran(g_gated_mlp_forward(&m.c, y.data_ptr(), n ? by_gate.data_ptr() : nullptr, n ? by_up.data_ptr() : nullptr, n ? hidden.data_ptr() : nullptr, ptr(work), err, stream_of(x)), x);
+        ran(g_gated_mlp_forward(&m.c, y.data_ptr(), n ? by_gate.data_ptr<float>() : nullptr, n ? by_up.data_ptr<float>() : nullptr, n ? hidden.data_ptr() : nullptr, ptr(work), err, stream_of(x)), x);
     }
     return {y, by_gate, by_up, hidden};
 }
@@ -96,7 +96,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_cuda(const Tensor&
     const bool wide = x.scalar_type() == at::kFloat;
     for (const Tensor* t : {&by_gate, &by_up, &hidden}) {
         const bool h = t == &hidden;
-        TORCH_CHECK(t->dim() == (h ? 3 : 2) && t->size(-2) == m.c.n && t->size(-1) == ld && (!h || t->size(0) == (wide ? 3 : 1)) && t->scalar_type() == (h && wide ? at::kBFloat16 : x.scalar_type()),
+        TORCH_CHECK(t->dim() == (h ? 3 : 2) && t->size(-2) == m.c.n && t->size(-1) == ld && (!h || t->size(0) == (wide ? 3 : 1)) && t->scalar_type() == (!h ? at::kFloat : wide ? at::kBFloat16 : x.scalar_type()),
                     "flex_rnn_b200: ", op, ": what the forward kept has to be given as it was");
         check_one(op, "what the forward kept", *t, x);
     }
@@ -106,7 +106,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_mlp_backward_cuda(const Tensor&
     if (m.c.n) {
         const Tensor g = as_rows(grad), sa = saved(by_gate), sb = saved(by_up), sh = saved(hidden);
         const Tensor work = workspace(g_gated_mlp_backward_workspace(&m.c, g.data_ptr(), g.stride(0)), x);
-        ran(g_gated_mlp_backward(&m.c, g.data_ptr(), g.stride(0), sa.data_ptr(), sb.data_ptr(), sh.data_ptr(), ptr(dx), ptr(dgate), ptr(dup), ptr(ddown), ptr(work), err, stream_of(x)), x);
+        ran(g_gated_mlp_backward(&m.c, g.data_ptr(), g.stride(0), sa.data_ptr<float>(), sb.data_ptr<float>(), sh.data_ptr(), ptr(dx), ptr(dgate), ptr(dup), ptr(ddown), ptr(work), err, stream_of(x)), x);
     } else {
         for (Tensor* t : {&dgate, &dup, &ddown})
             if (t->defined()) t->zero_();

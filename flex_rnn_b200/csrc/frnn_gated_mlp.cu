@@ -5,9 +5,9 @@
 //   dh = dy Wd                      its epilogue makes da = dh (b act'(a)), db = dh act(a)
 //   dWd = dy^T h, dWg = da^T x, dWu = db^T x, dx = da Wg + db Wu (one product of twice the length)
 //
-// n D F (D = width = out_width): 6 operations a value forward, 12 backward.  The forward keeps h and its two derivatives
-// b act'(a) and act(a), each rounded once: a and b kept instead, rounded, were rounded twice on the way to da, db and h (errors of the gradients in
-// bf16 against 64 bits 3.5e-3 instead of 2.9e-3), and the backward's epilogue computed the activation again.
+// n D F (D = width = out_width): 6 operations a value forward, 12 backward.  The forward keeps h, as it is multiplied, and its two
+// derivatives b act'(a) and act(a) in 32 bits.  (Errors of the gradients in bf16 against 64 bits: 2.4e-3 so, 2.9e-3 with derivatives in 16 bits,
+// 3.5e-3 with a and b kept instead, which the backward's epilogue took through the activation again; 1.7e-3 is the rounding of the result alone.)
 #include "frnn_product.cuh"
 
 using namespace frnn_lm;
@@ -47,7 +47,7 @@ Operand kept(const frnn_gated_mlp_call* c, const void* hidden) {
     return h;
 }
 
-int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, void* hidden, Scratch& s, int* err, cudaStream_t stream) {
+int forward(const frnn_gated_mlp_call* c, void* y, float* by_gate, float* by_up, void* hidden, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "gated_mlp";
     Packs packs = {};
     const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), gate = as_operand(s, packs, c->dtype, c->gate, c->hidden, c->width, c->gate_stride);
@@ -81,7 +81,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, v
     return run_product<STORE, false, false>(what, q, stream);
 }
 
-int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* by_gate, const void* by_up, const void* hidden, void* dx, void* dgate, void* dup, void* ddown, Scratch& s, int* err, cudaStream_t stream) {
+int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const float* by_gate, const float* by_up, const void* hidden, void* dx, void* dgate, void* dup, void* ddown, Scratch& s, int* err, cudaStream_t stream) {
     const char* what = "gated_mlp_backward";
     const bool count = !s.base, want_x = count || dx, want_gate = count || dgate, want_up = count || dup, want_down = count || ddown, want_hidden = want_x || want_gate || want_up;
     Packs packs = {};
@@ -111,8 +111,8 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.a = g;
         q.b[0] = down;
         q.args.err = err;
-        q.args.by_gate = const_cast<void*>(by_gate);
-        q.args.by_up = const_cast<void*>(by_up);
+        q.args.by_gate = const_cast<float*>(by_gate);
+        q.args.by_up = const_cast<float*>(by_up);
         q.args.by_ld = padded(c->hidden);
         if (want_x || want_gate) q.args.da = da.writable();
         if (want_x || want_up) q.args.db = db.writable();
@@ -163,7 +163,7 @@ size_t frnn_gated_mlp_forward_workspace(const frnn_gated_mlp_call* c) {
     return s.used;
 }
 
-int frnn_gated_mlp_forward(const frnn_gated_mlp_call* c, void* y, void* by_gate, void* by_up, void* hidden, void* workspace, int* err, void* stream) {
+int frnn_gated_mlp_forward(const frnn_gated_mlp_call* c, void* y, float* by_gate, float* by_up, void* hidden, void* workspace, int* err, void* stream) {
     const int rc = check("gated_mlp", c);
     if (rc != FRNN_OK) return rc;
     if (!y || !err || !workspace || !on_boundary(workspace, 16) || !on_boundary(y, dtype_bytes(c->dtype)) || !by_gate != !by_up || !by_gate != !hidden || !on_boundary(by_gate, 16) || !on_boundary(by_up, 16) ||
@@ -180,7 +180,7 @@ size_t frnn_gated_mlp_backward_workspace(const frnn_gated_mlp_call* c, const voi
     return s.used;
 }
 
-int frnn_gated_mlp_backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const void* by_gate, const void* by_up, const void* hidden, void* dx, void* dgate, void* dup,
+int frnn_gated_mlp_backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const float* by_gate, const float* by_up, const void* hidden, void* dx, void* dgate, void* dup,
                             void* ddown, void* workspace, int* err, void* stream) {
     const int rc = check("gated_mlp_backward", c);
     if (rc != FRNN_OK) return rc;

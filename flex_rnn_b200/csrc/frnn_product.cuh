@@ -75,7 +75,7 @@ struct alignas(64) ProductArgs {
     const float* alpha;         // a factor on the device, or NULL
     // GLU_*
     int io, activation;
-    void *by_gate, *by_up;      // b act'(a) and act(a), [M][by_ld] of the type of io; written forward (NULL: not), read backward
+    float *by_gate, *by_up;     // b act'(a) and act(a), [M][by_ld]; written forward (NULL: not), read backward
     int64_t by_ld;
     Planes h, da, db;
     // LOGPROB_*
@@ -246,11 +246,7 @@ template <bool FP32> __device__ __forceinline__ void put_planes(int io, unsigned
         put_rows(staging, lane, v, (__nv_bfloat16*)to.p + at, to.ld, rows, cols, true, true);
     }
 }
-template <bool FP32> __device__ __forceinline__ void put_rows_io(int io, unsigned char* staging, int lane, const float* v, void* dst, int64_t at, int64_t ld, int rows, int cols) {
-    if constexpr (FP32) put_rows(staging, lane, v, (float*)dst + at, ld, rows, cols, true, true);
-    else if (io == FRNN_BF16) put_rows(staging, lane, v, (__nv_bfloat16*)dst + at, ld, rows, cols, true, true);
-    else put_rows(staging, lane, v, (__half*)dst + at, ld, rows, cols, true, true);
-}
+
 // The way back: 32 values of each lane's row out of 32 rows, read by neighbouring lanes (aligned rows; undefined beyond rows and cols).
 // Asked for first, turned over by way of shared memory later.
 template <class T> struct Rows {
@@ -323,10 +319,10 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 
 // The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last
 // bit, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096, 2e-5 at 8192 in six segments, where 32-bit
-// sums rounded to nearest lose some 3e-7).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
+// sums rounded to nearest lose some 7e-7; from parts of 16 steps 3e-6, of 8 1.5e-6, of 4 7e-7, which costs up to 5 % of the time).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
 // instead, from parts of FLUSH steps, in registers, half of a tile's columns a warp; the sums go back to where the last part was, and
 // the epilogue is the same for all.  (One that took them from registers had its loops unrolled, and its code did not fit the instruction cache.)
-enum { FLUSH = 16 };
+enum { FLUSH = 4 };
 
 // 32 columns of accumulators, of the lane's row.  (Waited for apart: the next ones are under way while these are worked on.)
 __device__ __forceinline__ void ask(u32 taddr, float* v) { frnn_tmem_ld<32>(taddr, v); }
@@ -337,12 +333,12 @@ template <int N> __device__ __forceinline__ void wait_for(float* v) {
 }
 
 // da = dh (b act'(a)), db = dh act(a), 32 columns at a time; the next ones' factors are on their way meanwhile.
-template <class T>
+template <bool FP32>
 __device__ __forceinline__ void glu_backward(const ProductArgs& p, u32 acc, int64_t row0, int first, int count, int rows, int lane, unsigned char* staging) {
-    Rows<T> gate, up;
-    auto fetch = [&](Rows<T>& to, const void* from, int i) {
+    Rows<float> gate, up;
+    auto fetch = [&](Rows<float>& to, const float* from, int i) {
         const int col = first + i;
-        if (i < count) to.ask(lane, (const T*)from + row0 * p.by_ld + col, p.by_ld, rows, min(32, min(count - i, p.N - col)));
+        if (i < count) to.ask(lane, from + row0 * p.by_ld + col, p.by_ld, rows, min(32, min(count - i, p.N - col)));
     };
     if (p.da.p) fetch(gate, p.by_gate, 0);
     if (p.db.p) fetch(up, p.by_up, 0);
@@ -358,14 +354,14 @@ __device__ __forceinline__ void glu_backward(const ProductArgs& p, u32 acc, int6
             fetch(gate, p.by_gate, i + 32);
 #pragma unroll
             for (int j = 0; j < 32; j++) f[j] *= d[j];
-            put_planes<sizeof(T) == 4>(p.io, staging, lane, f, p.da, row0, col, rows, cols);
+            put_planes<FP32>(p.io, staging, lane, f, p.da, row0, col, rows, cols);
         }
         if (p.db.p) {
             up.get(staging, lane, f);
             fetch(up, p.by_up, i + 32);
 #pragma unroll
             for (int j = 0; j < 32; j++) f[j] *= d[j];
-            put_planes<sizeof(T) == 4>(p.io, staging, lane, f, p.db, row0, col, rows, cols);
+            put_planes<FP32>(p.io, staging, lane, f, p.db, row0, col, rows, cols);
         }
     }
 }
@@ -442,15 +438,13 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
             glu<32>(p.activation, a, b, h, p.by_gate);
             if (p.by_gate) {
                 const int64_t at = row0 * p.by_ld + col;
-                put_rows_io<FP32>(p.io, staging, lane, a, p.by_gate, at, p.by_ld, rows, cols);
-                put_rows_io<FP32>(p.io, staging, lane, b, p.by_up, at, p.by_ld, rows, cols);
+                put_rows(staging, lane, a, p.by_gate + at, p.by_ld, rows, cols, true, true);
+                put_rows(staging, lane, b, p.by_up + at, p.by_ld, rows, cols, true, true);
             }
             put_planes<FP32>(p.io, staging, lane, h, p.h, row0, col, rows, cols);
         }
     } else if constexpr (EPI == GLU_BACKWARD) {
-        if constexpr (FP32) glu_backward<float>(p, acc, row0, first, count, rows, lane, staging);
-        else if (p.io == FRNN_BF16) glu_backward<__nv_bfloat16>(p, acc, row0, first, count, rows, lane, staging);
-        else glu_backward<__half>(p, acc, row0, first, count, rows, lane, staging);
+        glu_backward<FP32>(p, acc, row0, first, count, rows, lane, staging);
     } else if constexpr (EPI == LOGPROB_STATS) {
         const int64_t token = data.token;
         float m = -3.4028235e38f, s = 0.f, t = 0.f;

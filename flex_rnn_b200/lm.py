@@ -108,8 +108,9 @@ def gated_mlp(x: th.Tensor, gate: th.Tensor, up: th.Tensor, down: th.Tensor, act
     ``ACTIVATIONS``.
 
     The products run on the tensor cores, with sums in 32 bits (fp32 numbers as sums of three bf16 ones, so that nothing of them
-    is lost).  In bf16 and fp16 the hidden vectors, their derivatives that are kept for the backward and the gradients of the two
-    projections are rounded to that type, as the tensor cores read them."""
+    is lost).  In bf16 and fp16 the hidden vectors and the gradients of the two projections are rounded to
+    that type, as the tensor cores read them.  For the backward a call keeps the hidden vectors and, in 32 bits, their
+    derivatives by the two projections."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"flex_rnn_b200: gated_mlp: activation has to be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     _operators()
@@ -259,7 +260,8 @@ def _register_fakes():
     def _(x, gate, up, down, activation, save):
         kept = (x.numel() // x.shape[-1] if save else 0, (gate.shape[0] + 63) // 64 * 64)
         hidden = x.new_empty((3, *kept), dtype=th.bfloat16) if x.dtype == th.float32 else x.new_empty((1, *kept))
-        return x.new_empty((*x.shape[:-1], down.shape[0])), x.new_empty(kept), x.new_empty(kept), hidden
+        by = x.new_empty((2, *kept), dtype=th.float32)
+        return x.new_empty((*x.shape[:-1], down.shape[0])), by[0].clone(), by[1].clone(), hidden
 
     @fake("flex_rnn_b200::gated_mlp_backward")
     def _(grad, x, gate, up, down, by_gate, by_up, hidden, activation, want_x, want_gate, want_up, want_down):

@@ -244,7 +244,7 @@ int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64
  * the tensor cores with sums in 32 bits (fp32 operands as sums of three bf16 numbers); for bf16 and fp16 what lies between
  * two products (the hidden vector, and backward its gradients) is rounded to that type, because the tensor cores read it so.
  * y and all gradients are contiguous.  What the forward keeps for the backward (all three or none: NULL), on 16-byte boundaries,
- * with H = hidden rounded up to a multiple of 64: `by_gate` and `by_up` [n, H] of `dtype`, the hidden vectors' derivatives by the two
+ * with H = hidden rounded up to a multiple of 64: `by_gate` and `by_up` fp32 [n, H], the hidden vectors' derivatives by the two
  * projections; `kept` [n, H] of `dtype`, for fp32 [3, n, H] bf16, the hidden vectors.
  */
 enum { FRNN_SILU = 0, FRNN_GELU = 1, FRNN_RELU = 2, FRNN_SIGMOID = 3 };
@@ -255,11 +255,11 @@ typedef struct frnn_gated_mlp_call {
     int64_t x_stride, gate_stride, up_stride, down_stride;
 } frnn_gated_mlp_call;
 size_t frnn_gated_mlp_forward_workspace(const frnn_gated_mlp_call* call);
-int frnn_gated_mlp_forward(const frnn_gated_mlp_call* call, void* y, void* by_gate, void* by_up, void* kept, void* workspace, int* err_word, void* stream);
+int frnn_gated_mlp_forward(const frnn_gated_mlp_call* call, void* y, float* by_gate, float* by_up, void* kept, void* workspace, int* err_word, void* stream);
 
 /* Gradients of x, gate, up and down for the upstream gradient dy [n, out_width]; each may be NULL (not wanted). */
 size_t frnn_gated_mlp_backward_workspace(const frnn_gated_mlp_call* call, const void* dy, int64_t dy_stride);
-int frnn_gated_mlp_backward(const frnn_gated_mlp_call* call, const void* dy, int64_t dy_stride, const void* by_gate, const void* by_up, const void* kept, void* dx,
+int frnn_gated_mlp_backward(const frnn_gated_mlp_call* call, const void* dy, int64_t dy_stride, const float* by_gate, const float* by_up, const void* kept, void* dx,
                             void* dgate, void* dup, void* ddown, void* workspace, int* err_word, void* stream);
 
 /*

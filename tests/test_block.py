@@ -92,8 +92,8 @@ def mlp_exact(x, gate, up, down, dy, activation):
     edh = lost(O, dtype) * (dy.abs() @ down.abs())
     es = second * ea + FAST * (a.abs() + 1) + (torch.where(a.abs() <= ea, 1.0, 0.0) if activation == "relu" else 0.0)
     db, da = dh * s, dh * b * slope
-    edb = edh * s.abs() + (dh.abs() + edh) * (first * ea + FAST * (s.abs() + 1) + u * s.abs() + tiny) + u * db.abs() + tiny
-    eda = edh * (b * slope).abs() + (dh.abs() + edh) * (eb * slope.abs() + (b.abs() + eb) * es + u * (b * slope).abs() + tiny) + u * da.abs() + tiny
+    edb = edh * s.abs() + (dh.abs() + edh) * (first * ea + FAST * (s.abs() + 1)) + u * db.abs() + tiny
+    eda = edh * (b * slope).abs() + (dh.abs() + edh) * (eb * slope.abs() + (b.abs() + eb) * es) + u * da.abs() + tiny
     edx = eda @ gate.abs() + edb @ up.abs() + lost(2 * F, dtype) * (da.abs() @ gate.abs() + db.abs() @ up.abs())
     ew = [e.T @ x.abs() + lost(n, dtype) * (v.abs().T @ x.abs()) for e, v in ((eda, da), (edb, db))]
     edown = dy.abs().T @ of_h(ea, eb) + lost(n, dtype) * (dy.abs().T @ h.abs())
@@ -107,7 +107,7 @@ def mlp_check(tensors, dy, activation="silu"):
     flat = [tensors[0].reshape(-1, tensors[0].shape[-1]), *tensors[1:]]
     want, tol = mlp_exact(*flat, dy.reshape(-1, dy.shape[-1]), activation)
     assert y.is_contiguous() and y.dtype == tensors[0].dtype and y.shape == dy.shape
-    for g, like, w, t, roundings in zip(got, [y, *tensors], want, tol, (2, 3, 3, 3, 2)):
+    for g, like, w, t, roundings in zip(got, [y, *tensors], want, tol, (2, 2, 2, 2, 2)):
         assert g.shape == like.shape and g.dtype == like.dtype
         within(g.reshape(w.shape), w, t)
         near_in_norm(g.reshape(w.shape), w, roundings)
