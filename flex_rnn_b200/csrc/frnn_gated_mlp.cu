@@ -53,8 +53,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, float* by_gate, float* by_up,
     const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), gate = as_operand(s, packs, c->dtype, c->gate, c->hidden, c->width, c->gate_stride);
     const Operand up = as_operand(s, packs, c->dtype, c->up, c->hidden, c->width, c->up_stride), down = as_operand(s, packs, c->dtype, c->down, c->out_width, c->hidden, c->down_stride);
     const Operand h = hidden ? kept(c, hidden) : new_operand(s, c->dtype, c->n, c->hidden);
-    if (!s.base) return FRNN_OK;
-    int rc = pack(packs, c->dtype, stream);
+    int rc = s.base ? pack(packs, c->dtype, stream) : (int)FRNN_OK;
     if (rc != FRNN_OK) return rc;
     {
         Product q = product(c, c->n, c->hidden, c->width);
@@ -67,7 +66,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, float* by_gate, float* by_up,
         q.args.by_up = by_up;
         q.args.by_ld = padded(c->hidden);
         q.args.h = h.writable();
-        rc = run_product<GLU_FORWARD, false, false>(what, q, stream);
+        rc = run_product<GLU_FORWARD, false, false>(what, q, s, stream);
         if (rc != FRNN_OK) return rc;
     }
     Product q = product(c, c->n, c->out_width, c->hidden);
@@ -78,7 +77,7 @@ int forward(const frnn_gated_mlp_call* c, void* y, float* by_gate, float* by_up,
     q.out = y;
     q.out_dtype = c->dtype;
     q.out_ld = c->out_width;
-    return run_product<STORE, false, false>(what, q, stream);
+    return run_product<STORE, false, false>(what, q, s, stream);
 }
 
 int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const float* by_gate, const float* by_up, const void* hidden, void* dx, void* dgate, void* dup, void* ddown, Scratch& s, int* err, cudaStream_t stream) {
@@ -96,8 +95,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
     Operand da = both, db = both;
     da.planes = db.planes = planes;
     db.p = (const char*)both.p + both.plane * planes * 2;
-    if (count) return FRNN_OK;
-    int rc = pack(packs, c->dtype, stream);
+    int rc = count ? (int)FRNN_OK : pack(packs, c->dtype, stream);
     if (rc != FRNN_OK) return rc;
     auto store = [&](Product& q, void* out, int64_t ld) {
         q.args.b_ready = 1;                // (the hidden gradients, which the first product writes, are always A)
@@ -116,7 +114,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.args.by_ld = padded(c->hidden);
         if (want_x || want_gate) q.args.da = da.writable();
         if (want_x || want_up) q.args.db = db.writable();
-        rc = run_product<GLU_BACKWARD, false, true>(what, q, stream);
+        rc = run_product<GLU_BACKWARD, false, true>(what, q, s, stream);
         if (rc != FRNN_OK) return rc;
     }
     if (want_down) {
@@ -125,19 +123,19 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.b[0] = kept(c, hidden);
         store(q, ddown, c->hidden);
         q.args.b_ready = want_hidden;      // (else it is the first: what is before it is not known)
-        rc = run_product<STORE, true, true>(what, q, stream);
+        rc = run_product<STORE, true, true>(what, q, s, stream);
         if (rc != FRNN_OK) return rc;
     }
-    if (want_gate || want_up) {             // both in one: half of a small product would leave multiprocessors idle
+    // both in one, because half of a small product would leave multiprocessors idle (counted is what one of them alone asks for: more)
+    if (want_gate || want_up) {
+        const bool two = want_gate && want_up && !count;
         Product q = product(c, c->hidden, c->width, c->n);
         q.a = want_gate ? both : db;
         q.b[0] = x;
-        if (want_gate && want_up) {
-            q.args.stacked = planes;
-            q.args.out2 = dup;
-        }
+        q.args.stacked = two ? planes : 0;
+        q.args.out2 = two ? dup : nullptr;
         store(q, want_gate ? dgate : dup, c->width);
-        rc = run_product<STORE, true, true>(what, q, stream);
+        rc = run_product<STORE, true, true>(what, q, s, stream);
         if (rc != FRNN_OK) return rc;
     }
     if (want_x) {
@@ -147,7 +145,7 @@ int backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, co
         q.b[1] = up;
         q.pairs = 2;
         store(q, dx, c->width);
-        rc = run_product<STORE, false, true>(what, q, stream);
+        rc = run_product<STORE, false, true>(what, q, s, stream);
     }
     return rc;
 }
@@ -160,7 +158,7 @@ size_t frnn_gated_mlp_forward_workspace(const frnn_gated_mlp_call* c) {
     if (check("gated_mlp", c) != FRNN_OK) return 0;
     Scratch s = {nullptr};
     forward(c, nullptr, nullptr, nullptr, nullptr, s, nullptr, nullptr);
-    return s.used;
+    return s.most;
 }
 
 int frnn_gated_mlp_forward(const frnn_gated_mlp_call* c, void* y, float* by_gate, float* by_up, void* hidden, void* workspace, int* err, void* stream) {
@@ -177,7 +175,7 @@ size_t frnn_gated_mlp_backward_workspace(const frnn_gated_mlp_call* c, const voi
     if (check("gated_mlp_backward", c) != FRNN_OK) return 0;
     Scratch s = {nullptr};
     backward(c, dy, dy_stride, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, s, nullptr, nullptr);
-    return s.used;
+    return s.most;
 }
 
 int frnn_gated_mlp_backward(const frnn_gated_mlp_call* c, const void* dy, int64_t dy_stride, const float* by_gate, const float* by_up, const void* hidden, void* dx, void* dgate, void* dup,

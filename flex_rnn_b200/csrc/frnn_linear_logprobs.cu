@@ -134,7 +134,7 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
     q.args.target = (float*)s.take((size_t)c->n * 4);
     if (!s.base) return FRNN_OK;
     int rc = pack(packs, c->dtype, stream);
-    if (rc == FRNN_OK) rc = run_product<LOGPROB_STATS, false, false>(what, q, stream);
+    if (rc == FRNN_OK) rc = run_product<LOGPROB_STATS, false, false>(what, q, s, stream);
     if (rc != FRNN_OK) return rc;
     auto join = [&](auto kernel, int rows, int slices) {
         return launch(what, kernel, dim3((unsigned)((c->n + rows - 1) / rows)), rows * slices, 0, stream, true, 1, q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab,
@@ -154,15 +154,16 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
     const Operand grad = new_operand(s, c->dtype, c->n, piece);
     float* const sum = pieces > 1 ? (float*)s.take((size_t)c->n * padded(c->width) * 4) : nullptr;
     float* const range = c->dtype == FRNN_F16 ? (float*)s.take(8) : nullptr;
-    if (count) return FRNN_OK;
-    int rc = pack(packs, c->dtype, stream);
+    int rc = count ? (int)FRNN_OK : pack(packs, c->dtype, stream);
     if (rc != FRNN_OK) return rc;
-    if (range) {
+    if (range && !count) {
         range_kernel<<<1, 1024, 0, stream>>>(dlogprob, dentropy, c->n, (float)(1.0 / c->temperature), range);
         rc = launched(what);
         if (rc != FRNN_OK) return rc;
     }
+    const size_t kept = s.used;
     for (int64_t v = 0; v < c->vocab; v += piece) {
+        s.used = kept;                             // (what slices of the piece before left has been added up)
         const int64_t cols = std::min(piece, c->vocab - v);
         const bool first = v == 0, last = v + cols == c->vocab;
         const Operand part = w.from_row(v, cols);
@@ -175,7 +176,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.args.stats = stats;
             q.args.scale = range;
             q.args.grad = g.writable();
-            rc = run_product<LOGPROB_GRAD, false, false>(what, q, stream);
+            rc = run_product<LOGPROB_GRAD, false, false>(what, q, s, stream);
             if (rc != FRNN_OK) return rc;
         }
         if (want_x) {
@@ -194,7 +195,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.out = last ? dx : sum;
             q.out_dtype = last ? c->dtype : (int)FRNN_F32;
             q.out_ld = last ? c->width : padded(c->width);
-            rc = run_product<STORE, false, true>(what, q, stream);
+            rc = run_product<STORE, false, true>(what, q, s, stream);
             if (rc != FRNN_OK) return rc;
         }
         if (want_w) {
@@ -208,10 +209,10 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.args.b_ready = 1;
             q.args.err = err;
             q.args.alpha = range ? range + 1 : nullptr;
-            q.out = (char*)dweight + v * c->width * dtype_bytes(c->dtype);
+            q.out = count ? nullptr : (char*)dweight + v * c->width * dtype_bytes(c->dtype);
             q.out_dtype = c->dtype;
             q.out_ld = c->width;
-            rc = run_product<STORE, true, true>(what, q, stream);
+            rc = run_product<STORE, true, true>(what, q, s, stream);
             if (rc != FRNN_OK) return rc;
         }
     }
@@ -226,7 +227,7 @@ size_t frnn_linear_logprobs_forward_workspace(const frnn_linear_logprobs_call* c
     if (check("linear_logprobs", c) != FRNN_OK) return 0;
     Scratch s = {nullptr};
     forward(c, nullptr, nullptr, nullptr, s, nullptr, nullptr);
-    return s.used;
+    return s.most;
 }
 
 int frnn_linear_logprobs_forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, float* stats, void* workspace, int* err, void* stream) {
@@ -242,7 +243,7 @@ size_t frnn_linear_logprobs_backward_workspace(const frnn_linear_logprobs_call* 
     if (check("linear_logprobs_backward", c) != FRNN_OK) return 0;
     Scratch s = {nullptr};
     backward(c, nullptr, nullptr, nullptr, nullptr, nullptr, s, nullptr, nullptr);
-    return s.used;
+    return s.most;
 }
 
 int frnn_linear_logprobs_backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const float* dentropy, const float* stats, void* dx, void* dweight, void* workspace, int* err, void* stream) {

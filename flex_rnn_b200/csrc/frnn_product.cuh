@@ -58,7 +58,7 @@ struct alignas(64) ProductArgs {
     CUtensorMap a, b[2];
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
     int ksteps, segments;       // steps of 64 along k in a segment
-    int tiles_m, tiles_n, group;
+    int tiles_m, tiles_n, group, slices;      // slices of k, each with a result of its own (STORE)
     int stacked;                // two products with the same B: the second's A is this many planes further on, its result at out2 (0: one)
     void* out2;
     int b_ready;                // the kernel before this one writes nothing of B: its copies begin before that one ends
@@ -68,7 +68,7 @@ struct alignas(64) ProductArgs {
     unsigned char plane_a[MAX_SEGMENTS], map_b[MAX_SEGMENTS], plane_b[MAX_SEGMENTS];
     // STORE
     void* out;
-    int64_t out_ld;
+    int64_t out_ld, out_slice;  // out_slice: elements between two slices' results
     int out_dtype, out_wide;    // wide: rows start on 16-byte boundaries
     const float* add;           // fp32 [M][add_ld] to add, or NULL
     int64_t add_ld;
@@ -387,10 +387,12 @@ template <int EPI> __device__ __forceinline__ RowData row_data(const ProductArgs
     return d;
 }
 
+struct Tile { int tm, tn, slice, from, to; bool second; };      // from, to: steps along k of a block
+
 // `count` columns from the one numbered `first` on, whose accumulators lie at `acc` (of GLU_FORWARD's second product at `acc2`), of the 32
 // rows from row0 on.
 template <int EPI, bool FP32>
-__device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& data, u32 acc, u32 acc2, int64_t row0, int first, int count, bool second, int lane, unsigned char* staging) {
+__device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& data, u32 acc, u32 acc2, int64_t row0, int first, int count, const Tile& w, int lane, unsigned char* staging) {
     // body(col, cols, v) for each 32 columns
     auto each = [&](auto body) {
         float v[32], next[32];
@@ -423,7 +425,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += o[j];
             }
-            put_rows_as(p.out_dtype, staging, lane, v, second ? p.out2 : p.out, row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide, false);
+            put_rows_as(p.out_dtype, staging, lane, v, w.second ? p.out2 : p.out, w.slice * p.out_slice + row0 * p.out_ld + col, p.out_ld, rows, cols, p.out_wide, false);
         });
     } else if constexpr (EPI == GLU_FORWARD) {
 #pragma unroll 1
@@ -518,14 +520,15 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
-struct Tile { int tm, tn; bool second; };
 
 // Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
-__device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u) {
-    const int a_group = p.group * p.tiles_n, g = u / a_group, in = u % a_group, high = min(p.group, p.tiles_m - g * p.group);
+__device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 rank, u32 blocks) {
+    const int tiles = p.tiles_m * p.tiles_n, slice = p.slices > 1 ? u / tiles : 0, in_slice = u - slice * tiles;
+    const int a_group = p.group * p.tiles_n, g = in_slice / a_group, in = in_slice % a_group, high = min(p.group, p.tiles_m - g * p.group);
     const int tm = g * p.group + in % high, half = p.tiles_m / 2;
     const bool second = p.stacked && tm >= half;
-    return {second ? tm - half : tm, in / high, second};
+    const int64_t steps = (int64_t)p.ksteps * p.segments, parts = (int64_t)p.slices * blocks, part = (int64_t)slice * blocks + rank;
+    return {second ? tm - half : tm, in / high, slice, (int)(steps * part / parts), (int)(steps * (part + 1) / parts), second};
 }
 
 // AT, BT: the operand's rows run along m (n) instead of k.
@@ -544,10 +547,8 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const u32 rank = FORM == ALONE ? 0 : cluster_rank(), blocks = FORM == ALONE ? 1 : cluster_blocks();
     const u32 half_m = FORM == PAIR ? rank : 0;        // which 128 of a tile's rows
-    const int tiles = p.tiles_m * p.tiles_n, first = blockIdx.x / blocks, stride = gridDim.x / blocks;
-    // this block's steps along k
-    const int64_t steps = (int64_t)p.ksteps * p.segments;
-    const int k_from = FORM == SPLIT ? (int)(steps * rank / blocks) : 0, k_to = FORM == SPLIT ? (int)(steps * (rank + 1) / blocks) : (int)steps;
+    const int tiles = p.tiles_m * p.tiles_n * p.slices, first = blockIdx.x / blocks, stride = gridDim.x / blocks;
+    const u32 part = FORM == SPLIT ? rank : 0, parts = FORM == SPLIT ? blocks : 1;       // of a tile's steps along k
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -612,14 +613,18 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                     }
                 };
                 auto column = [&](const Tile& w) { return p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)half_m * NB; };
-                const int early = p.b_ready && first < tiles ? min(STAGES, k_to - k_from) : 0;
-                for (int i = 0; i < early; i++) load_b(i, column(tile_of(p, first)), (k_from + i) / p.ksteps, (k_from + i) % p.ksteps);
+                int early = 0;
+                if (p.b_ready && first < tiles) {
+                    const Tile w = tile_of(p, first, part, parts);
+                    early = min(STAGES, w.to - w.from);
+                    for (int i = 0; i < early; i++) load_b(i, column(w), (w.from + i) / p.ksteps, (w.from + i) % p.ksteps);
+                }
                 cudaGridDependencySynchronize();
                 for (int u = first; ok && u < tiles; u += stride) {
-                    const Tile w = tile_of(p, u);
+                    const Tile w = tile_of(p, u, part, parts);
                     const int m = (w.tm * CG + (int)half_m) * 128, n = column(w), further = w.second ? p.stacked : 0;
-                    int g = k_from / p.ksteps, k = k_from % p.ksteps;
-                    for (int i = k_from; i < k_to; i++, it++) {
+                    int g = w.from / p.ksteps, k = w.from % p.ksteps;
+                    for (int i = w.from; i < w.to; i++, it++) {
                         const int s = it % STAGES;
                         if (it >= (u32)early) {
                             if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
@@ -639,8 +644,9 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 u32 it = 0, t = 0;
                 bool ok = true;
                 for (int u = first; ok && u < tiles; u += stride) {
-                    for (int from = k_from; ok && from < k_to; t++) {
-                        const int to = PROMOTE ? min(from + FLUSH, k_to) : k_to;
+                    const Tile w = tile_of(p, u, part, parts);
+                    for (int from = w.from; ok && from < w.to; t++) {
+                        const int to = PROMOTE ? min(from + FLUSH, w.to) : w.to;
                         const u32 buf = t & 1, d = tmem + buf * BN;
                         if (!(ok = frnn_mbar_wait(&acc_empty[buf], (t / 2 & 1) ^ 1, p.err, CODE_PRODUCT))) break;
                         frnn_tmem_fence_after_sync();
@@ -685,18 +691,18 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
             t++;
         };
         for (int u = first; ok && u < tiles; u += stride, round++) {
-            const Tile w = tile_of(p, u);
+            const Tile w = tile_of(p, u, part, parts);
             const int64_t row0 = (int64_t)(w.tm * CG + (int)half_m) * 128 + quarter * 32;
             const RowData data = row_data<EPI>(p, row0 + lane);
             u32 acc = filled();
             if (!ok) break;
             if constexpr (PROMOTE || FORM == SPLIT) {
-                if (FORM == SPLIT || k_from + FLUSH < k_to) {
+                if (FORM == SPLIT || w.from + FLUSH < w.to) {
                     float sum[BN / 2];
 #pragma unroll
                     for (int i = 0; i < BN / 2; i += 32) ask(acc + half * (BN / 2) + i, sum + i);
                     wait_for<BN / 2>(sum);
-                    for (int from = k_from + FLUSH; PROMOTE && from < k_to; from += FLUSH) {
+                    for (int from = w.from + FLUSH; PROMOTE && from < w.to; from += FLUSH) {
                         emptied();
                         acc = filled();
                         if (!ok) break;
@@ -756,7 +762,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
                         if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
-                            epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, w.second, lane, staging);
+                            epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
                         }
                         continue;
                     } else {
@@ -772,7 +778,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 }
             }
             constexpr int COUNT = EPI == GLU_FORWARD ? BN / 4 : BN / 2;
-            if (!idle && row0 < p.M) epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, w.second, lane, staging);
+            if (!idle && row0 < p.M) epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, w, lane, staging);
             emptied();
         }
     }
@@ -781,6 +787,34 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
     if constexpr (FORM != ALONE) cluster_sync();
     frnn_tmem_fence_after_sync();
     if (warp == 2) tmem_free<CG>(tmem, COLUMNS);
+}
+
+// The results of `slices` slices of k, fp32 [slices][M][ld] at p.out, added in their order.
+static __global__ void __launch_bounds__(256) join_slices(const __grid_constant__ ProductArgs p, void* to, int to_dtype, int64_t to_ld) {
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int64_t quads = (p.N + 3) / 4;
+    const float alpha = p.alpha ? *p.alpha : 1.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.M * quads; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / quads, col = i % quads * 4;
+        const float* const from = (const float*)p.out + row * p.out_ld + col;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = 0; s < p.slices; s++) {
+            const float4 x = *(const float4*)(from + s * p.out_slice);
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (col + e >= p.N) break;
+            float x = (&v.x)[e] * alpha;
+            if (p.add) x += p.add[row * p.add_ld + col + e];
+            const int64_t at = row * to_ld + col + e;
+            if (to_dtype == FRNN_F32) ((float*)to)[at] = x;
+            else if (to_dtype == FRNN_BF16) ((__nv_bfloat16*)to)[at] = from_float<__nv_bfloat16>(x);
+            else ((__half*)to)[at] = from_float<__half>(x);
+        }
+    }
 }
 
 // ---- operands -------------------------------------------------------------------------------------------------------------------
@@ -837,13 +871,15 @@ template <class T> __global__ void __launch_bounds__(256) pack_kernel(const __gr
     }
 }
 
-// Scratch handed out piece by piece; without memory behind it, the sum of what is asked for.
+// Scratch handed out piece by piece; `used` may be set back when what came after is no longer needed.  Without memory behind it,
+// `most` is what is asked for.
 struct Scratch {
     char* base;
-    size_t used = 0;
+    size_t used = 0, most = 0;
     void* take(size_t bytes) {
         void* const p = base ? base + used : nullptr;
         used += (bytes + 255) / 256 * 256;
+        most = std::max(most, used);
         return p;
     }
 };
@@ -914,8 +950,9 @@ struct Product {
 
 struct ProductPlan {
     Form form;
-    int blocks;                                   // of a cluster
+    int blocks, slices;                           // of a cluster; of k beyond that
     int64_t tiles_m, tiles_n;
+    size_t scratch;                               // the slices' results
     int columns() const { return form == PAIR ? 128 : form == ALONE ? 64 : 64 / blocks; }      // that a warp of the epilogue has in a row
 };
 
@@ -959,24 +996,29 @@ template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Produ
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     const bool few = !AT && q.m <= 128;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    auto cost = [&](Form form, int blocks, int64_t tiles) {
+    auto cost = [&](Form form, int blocks, int64_t tiles, int slices) {
         const int64_t at_once = clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks), rounds = up(tiles, at_once), out = leave[form][EPI];
         auto k_time = [&](int64_t tiles) {
-            return (form == SPLIT ? up(steps, blocks) : steps) * std::max<int64_t>(is_thin(q, AT, form) ? 225 : step[form], few ? 372 * tiles * blocks / sm_count() : 0);
+            return up(steps, form == SPLIT ? blocks * slices : slices) * std::max<int64_t>(is_thin(q, AT, form) ? 225 : step[form], few ? 372 * tiles * blocks / sm_count() : 0);
         };
         const int64_t last = k_time(tiles - (rounds - 1) * at_once), start = (form == ALONE ? 1000 : 2000) + (form == SPLIT ? 1000 * rounds : 0);      // (its blocks wait for one another)
         return rounds == 1 ? start + last + out : start + k_time(at_once) + (rounds - 2) * std::max(k_time(at_once), out) + std::max(last, out) + out;
     };
     const int64_t stack = q.args.stacked ? 2 : 1;
-    ProductPlan best = {PAIR, 2, up(q.m, 256) * stack, up(q.n * width, 256)};
-    int64_t least = cost(PAIR, 2, best.tiles_m * best.tiles_n);
+    ProductPlan best = {PAIR, 2, 1, up(q.m, 256) * stack, up(q.n * width, 256), 0};
+    int64_t least = cost(PAIR, 2, best.tiles_m * best.tiles_n, 1);
     const int64_t tm = up(q.m, 128) * stack, tn = up(q.n * width, 128);
     for (int blocks = 1; blocks <= 8 && blocks <= steps; blocks *= 2) {
         const Form form = blocks > 1 ? SPLIT : ALONE;
-        const int64_t c = cost(form, blocks, tm * tn);
-        if (c < least) {
-            least = c;
-            best = {form, blocks, tm, tn};
+        // a long sum for few tiles: slices of at least 32 steps a block, whose results (up to 32 MB) a second kernel adds up
+        for (int slices = 1; slices <= (EPI == STORE && !q.args.stacked ? 32 : 1); slices *= 2) {
+            const size_t scratch = slices > 1 ? (size_t)slices * q.m * padded(q.n) * 4 : 0;
+            if (slices > 1 && (steps < 32ll * blocks * slices || scratch > (32u << 20))) break;
+            const int64_t c = cost(form, blocks, tm * tn * slices, slices) + (slices > 1 ? 4000 + (int64_t)(scratch >> 12) : 0);
+            if (c < least) {
+                least = c;
+                best = {form, blocks, slices, tm, tn, scratch};
+            }
         }
     }
     return best;
@@ -993,20 +1035,24 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> inline 
     }();
     if (!enough) return frnn_fail(FRNN_E_LAUNCH, "%s: the kernel was not built for %d registers a thread, or there is no GPU to run it", what, (int)START_REGISTERS);
     if (!allow_shared<kernel>(PRODUCT_SHARED)) { cudaGetLastError(); return frnn_fail(FRNN_E_LAUNCH, "%s: no room in shared memory", what); }
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, clusters = std::min<int64_t>(tiles, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks));
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.slices, clusters = std::min<int64_t>(tiles, clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks));
     return launch(what, kernel, dim3((unsigned)(clusters * blocks)), PRODUCT_THREADS, PRODUCT_SHARED, stream, true, blocks, p);
 }
 
-template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Product& q, cudaStream_t stream) {
+// One product.  Without memory behind `s` only its scratch is counted.
+template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Product& q, Scratch& s, cudaStream_t stream) {
     ProductArgs& p = q.args;
     const ProductPlan plan = plan_product<EPI, AT, BT>(q);
-    if (plan.tiles_m * plan.tiles_n >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "%s: too many tiles", what);
+    void* const sliced = plan.slices > 1 ? s.take(plan.scratch) : nullptr;
+    if (!s.base) return FRNN_OK;
+    if (plan.tiles_m * plan.tiles_n * plan.slices >= (1ll << 31)) return frnn_fail(FRNN_E_ARG, "%s: too many tiles", what);
     p.M = (int)q.m;
     p.N = (int)q.n;
     p.ksteps = (int)((q.k + BK - 1) / BK);
     p.tiles_m = (int)plan.tiles_m;
     p.tiles_n = (int)plan.tiles_n;
     p.group = plan.form == PAIR ? 16 : 32;
+    p.slices = plan.slices;
     const unsigned type = q.dtype == FRNN_F16 ? 0 : 1, side = plan.form == PAIR ? 256 : 128;
     p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((unsigned)AT << 15) | ((unsigned)BT << 16) | ((side >> 3) << 17) | ((side >> 4) << 24);
     static const unsigned char first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};      // planes of a and b, small terms first
@@ -1032,7 +1078,15 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     p.out = q.out;
     p.out_dtype = q.out_dtype;
     p.out_ld = q.out_ld;
-    p.out_wide = on_boundary(q.out, 16) && on_boundary(p.out2, 16) && q.out_ld * (int64_t)dtype_bytes(q.out_dtype) % 16 == 0;
+    const float *const add = p.add, *const alpha = p.alpha;
+    if (sliced) {
+        p.out = sliced;
+        p.out_dtype = FRNN_F32;
+        p.out_ld = padded(q.n);
+        p.out_slice = q.m * p.out_ld;
+        p.add = p.alpha = nullptr;
+    }
+    p.out_wide = on_boundary(p.out, 16) && on_boundary(p.out2, 16) && p.out_ld * (int64_t)dtype_bytes(p.out_dtype) % 16 == 0;
     constexpr bool EXACT = EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
     auto run = [&](auto form, auto rows) {
         constexpr Form FORM = decltype(form)::value;
@@ -1040,12 +1094,15 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
         return q.dtype == FRNN_F32 ? launch_product<FORM, THIN, AT, BT, EPI, true>(what, p, plan.blocks, stream) : launch_product<FORM, THIN, AT, BT, EPI, EXACT>(what, p, plan.blocks, stream);
     };
     const std::false_type all;
-    if (plan.form == PAIR) return run(std::integral_constant<Form, PAIR>(), all);
-    if constexpr (!AT) {
-        const std::true_type few;
-        if (thin) return plan.form == ALONE ? run(std::integral_constant<Form, ALONE>(), few) : run(std::integral_constant<Form, SPLIT>(), few);
-    }
-    return plan.form == ALONE ? run(std::integral_constant<Form, ALONE>(), all) : run(std::integral_constant<Form, SPLIT>(), all);
+    const std::true_type few;
+    if (plan.form == PAIR) rc = run(std::integral_constant<Form, PAIR>(), all);
+    else if (!thin) rc = plan.form == ALONE ? run(std::integral_constant<Form, ALONE>(), all) : run(std::integral_constant<Form, SPLIT>(), all);
+    else if constexpr (!AT) rc = plan.form == ALONE ? run(std::integral_constant<Form, ALONE>(), few) : run(std::integral_constant<Form, SPLIT>(), few);
+    if (rc != FRNN_OK || !sliced) return rc;
+    p.add = add;
+    p.alpha = alpha;
+    const int64_t blocks = std::min<int64_t>((q.m * ((q.n + 3) / 4) + 255) / 256, (int64_t)sm_count() * 8);
+    return launch(what, join_slices, dim3((unsigned)blocks), 256, 0, stream, true, 1, p, q.out, q.out_dtype, q.out_ld);
 }
 
 }  // namespace frnn_lm
