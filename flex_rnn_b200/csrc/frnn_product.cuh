@@ -18,7 +18,8 @@
 //   ALONE  128 x 128 by a block: small products spread over more multiprocessors
 //   SPLIT  128 x 128 by a cluster of 2, 4 or 8 blocks, each with a part of k.  Each block then owns a part of the tile's columns: the others
 //          send it their sums of these (into its shared memory), it adds them in the order of the blocks and has the epilogue
-//          to itself.  (4 stages, and 64 KB for what arrives.)
+//          to itself.  (5 stages, and 64 KB for what arrives, where the
+//          epilogue turns its rows over afterwards.)
 // THIN (ALONE or SPLIT, up to 32 rows, as in generation): only 32 of A's rows are copied, so that 10 stages of B are under way, 160 KB a
 // multiprocessor: such products are as fast as their weights come.  The tensor cores read 128 rows all the same: what they find
 // behind the 32 ends in rows of the result that nobody looks at.
@@ -42,7 +43,7 @@ enum Form { PAIR, ALONE, SPLIT };
 enum { BK = 64, STAGE_BYTES = 32768, THIN_ROWS = 32, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
 // Registers of the warps that copy and issue, and of the epilogue's: 128 x 56 + 256 x 224 = 384 x 168, what a block starts with.
 enum { CONTROL_REGISTERS = 56, EPILOGUE_REGISTERS = 224, START_REGISTERS = 168 };
-enum { PRODUCT_SHARED = 6 * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };      // (6 stages; 4 and 64 KB for what arrives; 10 thin ones, 16 KB and less staging: as much each)
+enum { PRODUCT_SHARED = 6 * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };      // (6 stages; 5 and 64 KB for what arrives; 10 thin ones, 16 KB and less staging)
 enum { CODE_PRODUCT = 97 };       // error word: a wait inside a matrix product ran out
 
 // What becomes of a tile.
@@ -533,12 +534,13 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 rank, u
 
 // AT, BT: the operand's rows run along m (n) instead of k.
 template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
-    constexpr int CG = FORM == PAIR ? 2 : 1, BN = FORM == PAIR ? 256 : 128, STAGES = THIN ? 10 : FORM == SPLIT ? 4 : 6;
+    constexpr int CG = FORM == PAIR ? 2 : 1, BN = FORM == PAIR ? 256 : 128, STAGES = THIN ? 10 : FORM == SPLIT ? 5 : 6;
     constexpr int NB = BN / CG;                        // B's rows in this block
     constexpr int ROWS = THIN ? (int)THIN_ROWS : 128;  // of A, that are copied and that have a result
     constexpr u32 A_BYTES = ROWS * BK * 2, B_BYTES = NB * BK * 2, STAGE = A_BYTES + B_BYTES, COLUMNS = FORM == SPLIT ? 512 : 2 * BN;
     constexpr u32 EXCHANGE = FORM == SPLIT ? ROWS * BN * 4 : 0;
-    static_assert(STAGES * STAGE + EXCHANGE + ROWS / 32 * 2 * STAGING_BYTES + 1024 <= PRODUCT_SHARED && COLUMNS <= 512, "shared memory or Tensor Memory is too small");
+    constexpr bool SHARE = FORM == SPLIT && !THIN;     // staging lies where the sums arrived
+    static_assert(STAGES * STAGE + EXCHANGE + (SHARE ? 0 : ROWS / 32 * 2 * STAGING_BYTES) + 1024 <= PRODUCT_SHARED && COLUMNS <= 512, "shared memory or Tensor Memory is too small");
     static_assert(!THIN || (!AT && FORM != PAIR), "only rows along k can be left out");
     extern __shared__ unsigned char raw[];
     __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], arrived, taken;
@@ -672,7 +674,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
         frnn_regs_acquire<EPILOGUE_REGISTERS>();
         const int quarter = warp % 4, half = (warp - 4) / 4;
         const bool idle = quarter * 32 >= ROWS;                               // none of this warp's rows has a result
-        unsigned char* const staging = smem + STAGES * STAGE + EXCHANGE + (half * (ROWS / 32) + (idle ? 0 : quarter)) * STAGING_BYTES;
+        unsigned char* const staging = smem + STAGES * STAGE + (SHARE ? 0 : EXCHANGE) + (half * (ROWS / 32) + (idle ? 0 : quarter)) * STAGING_BYTES;
         float4* const exchange = (float4*)(smem + STAGES * STAGE);            // SPLIT: [block][own columns / 4][rows]
         u32 t = 0, round = 0;
         bool ok = true;
@@ -758,12 +760,17 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                             frnn_tmem_st<32>(place, v);
                             frnn_tmem_wait_st();
                         }
-                        __syncwarp();
-                        if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
+                        auto done_with = [&] {
+                            __syncwarp();
+                            if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
+                        };
+                        if constexpr (SHARE) frnn_group_sync(5, EPILOGUE_WARPS * 32);
+                        else done_with();
                         if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
                             epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
                         }
+                        if constexpr (SHARE) done_with();
                         continue;
                     } else {
 #pragma unroll
@@ -982,7 +989,7 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
 }
 
 // Which form: the one that is done first, by what was measured (ns, on a B200).  A step of 64 along k takes 285 in PAIR (for 128 x 256 in
-// each block; the tensor cores' own time is 270), 205 in ALONE and 268 in SPLIT (for 128 x 128; 135, but 8 KB of operands for each 16
+// each block; the tensor cores' own time is 270), 205 in ALONE and 225 in SPLIT (for 128 x 128; 135, but 8 KB of operands for each 16
 // values of k are as much as shared memory gives, and the copies come on top).  A tile leaves in `leave` (STORE, GLU_FORWARD,
 // GLU_BACKWARD, LOGPROB_STATS, LOGPROB_GRAD), while the next one is computed; in SPLIT that has the exchange in it.
 // Products of up to 128 rows read 16 KB of weights a step that nobody else reads: 372 when all multiprocessors do (6.5 TB/s).  THIN takes 225
@@ -992,7 +999,7 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
 // Log probabilities of 16 rows, 65536 tokens, 4096 wide: ALONE 105, SPLIT in 2 115.
 inline bool is_thin(const Product& q, bool at, Form form) { return !at && form != PAIR && q.m <= THIN_ROWS; }
 template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
-    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2300, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 268};
+    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2300, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 225};
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     const bool few = !AT && q.m <= 128;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
