@@ -523,13 +523,29 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
 
 
 // Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
-__device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 rank, u32 blocks) {
-    const int tiles = p.tiles_m * p.tiles_n, slice = p.slices > 1 ? u / tiles : 0, in_slice = u - slice * tiles;
-    const int a_group = p.group * p.tiles_n, g = in_slice / a_group, in = in_slice % a_group, high = min(p.group, p.tiles_m - g * p.group);
-    const int tm = g * p.group + in % high, half = p.tiles_m / 2;
-    const bool second = p.stacked && tm >= half;
-    const int64_t steps = (int64_t)p.ksteps * p.segments, parts = (int64_t)p.slices * blocks, part = (int64_t)slice * blocks + rank;
-    return {second ? tm - half : tm, in / high, slice, (int)(steps * part / parts), (int)(steps * (part + 1) / parts), second};
+// Part `part` of `parts` of a tile's (a slice's) steps along k.
+__device__ __forceinline__ void steps_of(const ProductArgs& p, Tile& w, u32 part, u32 parts) {
+    const int steps = p.ksteps * p.segments;
+    if (p.slices * parts == 1) {                   // (64-bit divisions take as long as a small tile's products)
+        w.from = 0;
+        w.to = steps;
+    } else {
+        const int64_t all = (int64_t)p.slices * parts, at = (int64_t)w.slice * parts + part;
+        w.from = (int)(steps * at / all);
+        w.to = (int)(steps * (at + 1) / all);
+    }
+}
+__device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 part, u32 parts) {
+    Tile w;
+    const int tiles = p.tiles_m * p.tiles_n;
+    w.slice = p.slices > 1 ? u / tiles : 0;
+    const int in_slice = u - w.slice * tiles, a_group = p.group * p.tiles_n, g = in_slice / a_group, in = in_slice - g * a_group, high = min(p.group, p.tiles_m - g * p.group);
+    w.tn = in / high;
+    w.tm = g * p.group + in - w.tn * high;
+    w.second = p.stacked && w.tm >= p.tiles_m / 2;
+    if (w.second) w.tm -= p.tiles_m / 2;
+    steps_of(p, w, part, parts);
+    return w;
 }
 
 // AT, BT: the operand's rows run along m (n) instead of k.
@@ -692,10 +708,21 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
             }
             t++;
         };
+        auto row_of = [&](const Tile& w) { return (int64_t)(w.tm * CG + (int)half_m) * 128 + quarter * 32; };
+        Tile next = {};
+        RowData next_data = {};
+        if (first < tiles) {
+            next = tile_of(p, first, part, parts);
+            next_data = row_data<EPI>(p, row_of(next) + lane);
+        }
         for (int u = first; ok && u < tiles; u += stride, round++) {
-            const Tile w = tile_of(p, u, part, parts);
-            const int64_t row0 = (int64_t)(w.tm * CG + (int)half_m) * 128 + quarter * 32;
-            const RowData data = row_data<EPI>(p, row0 + lane);
+            const Tile w = next;
+            const RowData data = next_data;
+            const int64_t row0 = row_of(w);
+            if (u + stride < tiles) {          // (its data is on its way while this one leaves)
+                next = tile_of(p, u + stride, part, parts);
+                next_data = row_data<EPI>(p, row_of(next) + lane);
+            }
             u32 acc = filled();
             if (!ok) break;
             if constexpr (PROMOTE || FORM == SPLIT) {
