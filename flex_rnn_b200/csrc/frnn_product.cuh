@@ -58,6 +58,7 @@ struct Planes {
 struct alignas(64) ProductArgs {
     CUtensorMap a, b[2];
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
+    int flush;                  // PROMOTE: steps along k of a part
     int ksteps, segments;       // steps of 64 along k in a segment
     int tiles_m, tiles_n, group, slices;      // slices of k, each with a result of its own (STORE)
     int stacked;                // two products with the same B: the second's A is this many planes further on, its result at out2 (0: one)
@@ -321,9 +322,9 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 // The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last
 // bit, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096, 2e-5 at 8192 in six segments, where 32-bit
 // sums rounded to nearest lose some 7e-7; from parts of 16 steps 3e-6, of 8 1.5e-6, of 4 7e-7, which costs up to 5 % of the time).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
-// instead, from parts of FLUSH steps, in registers, half of a tile's columns a warp; the sums go back to where the last part was, and
+// instead, from parts of `flush` steps, in registers, half of a tile's columns a warp; the sums go back to where the last part was, and
 // the epilogue is the same for all.  (One that took them from registers had its loops unrolled, and its code did not fit the instruction cache.)
-enum { FLUSH = 4 };
+// Parts of 4 where the operands are fp32; of 16 for the fp32 results of 16-bit operands (4e-7).
 
 // 32 columns of accumulators, of the lane's row.  (Waited for apart: the next ones are under way while these are worked on.)
 __device__ __forceinline__ void ask(u32 taddr, float* v) { frnn_tmem_ld<32>(taddr, v); }
@@ -664,7 +665,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u, part, parts);
                     for (int from = w.from; ok && from < w.to; t++) {
-                        const int to = PROMOTE ? min(from + FLUSH, w.to) : w.to;
+                        const int to = PROMOTE ? min(from + p.flush, w.to) : w.to;
                         const u32 buf = t & 1, d = tmem + buf * BN;
                         if (!(ok = frnn_mbar_wait(&acc_empty[buf], (t / 2 & 1) ^ 1, p.err, CODE_PRODUCT))) break;
                         frnn_tmem_fence_after_sync();
@@ -726,12 +727,12 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
             u32 acc = filled();
             if (!ok) break;
             if constexpr (PROMOTE || FORM == SPLIT) {
-                if (FORM == SPLIT || w.from + FLUSH < w.to) {
+                if (FORM == SPLIT || w.from + p.flush < w.to) {
                     float sum[BN / 2];
 #pragma unroll
                     for (int i = 0; i < BN / 2; i += 32) ask(acc + half * (BN / 2) + i, sum + i);
                     wait_for<BN / 2>(sum);
-                    for (int from = w.from + FLUSH; PROMOTE && from < w.to; from += FLUSH) {
+                    for (int from = w.from + p.flush; PROMOTE && from < w.to; from += p.flush) {
                         emptied();
                         acc = filled();
                         if (!ok) break;
@@ -1026,7 +1027,7 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
 // Log probabilities of 16 rows, 65536 tokens, 4096 wide: ALONE 105, SPLIT in 2 115.
 inline bool is_thin(const Product& q, bool at, Form form) { return !at && form != PAIR && q.m <= THIN_ROWS; }
 template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
-    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2300, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 225};
+    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 1700, 2600}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 225};
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     const bool few = !AT && q.m <= 128;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
@@ -1087,6 +1088,7 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     p.tiles_n = (int)plan.tiles_n;
     p.group = plan.form == PAIR ? 16 : 32;
     p.slices = plan.slices;
+    p.flush = q.dtype == FRNN_F32 ? 4 : 16;
     const unsigned type = q.dtype == FRNN_F16 ? 0 : 1, side = plan.form == PAIR ? 256 : 128;
     p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((unsigned)AT << 15) | ((unsigned)BT << 16) | ((side >> 3) << 17) | ((side >> 4) << 24);
     static const unsigned char first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};      // planes of a and b, small terms first
