@@ -127,11 +127,14 @@ __device__ __forceinline__ void send(u32 dst, float a, float b, float c, float d
 // an arrival that says that what this warp has sent is there
 __device__ __forceinline__ void arrive_after_sending(u32 bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void arrive_at(u32 bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// frnn_mbar_wait for what other blocks of the cluster have written
-__device__ __forceinline__ bool wait_for_cluster(u64* bar, u32 parity, int* err) {
+// A bounded wait (as frnn_mbar_wait) on a barrier given by its address; CLUSTER: for what other blocks of the cluster have written.
+template <bool CLUSTER = false> __device__ __forceinline__ bool wait_at(u32 bar, u32 parity, int* err) {
     auto there = [&] {
         u32 ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(frnn_smem_addr(bar)), "r"(parity) : "memory");
+        if constexpr (CLUSTER)
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         return ok != 0;
     };
     if (there()) return true;
@@ -147,18 +150,19 @@ __device__ __forceinline__ bool wait_for_cluster(u64* bar, u32 parity, int* err)
         }
     }
 }
-template <int CG> __device__ __forceinline__ void mma_f16(u32 d, u64 a, u64 b, u32 idesc, bool accumulate) {
+__device__ __forceinline__ void expect_bytes(u32 bar, u32 bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+template <int CG> __device__ __forceinline__ void mma_f16(u32 d, u64 a, u64 b, u32 idesc, u32 accumulate) {
     if constexpr (CG == 2)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((u32)accumulate) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((u32)accumulate) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // An arrival on `bar` (of both blocks of a pair) when the products issued so far are done.
-template <int CG> __device__ __forceinline__ void mma_commit(u64* bar) {
+template <int CG> __device__ __forceinline__ void mma_commit(u32 bar) {
     if constexpr (CG == 2)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(frnn_smem_addr(bar)), "h"((unsigned short)3) : "memory");
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
     else
-        frnn_mma_commit(bar);
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 template <int CG> __device__ __forceinline__ void tmem_alloc(u32* at, u32 columns) {
     if constexpr (CG == 2) {
@@ -558,14 +562,14 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
     constexpr u32 EXCHANGE = FORM == SPLIT ? ROWS * BN * 4 : 0;
     constexpr bool SHARE = FORM == SPLIT && !THIN;     // staging lies where the sums arrived
     static_assert(STAGES * STAGE + EXCHANGE + (SHARE ? 0 : ROWS / 32 * 2 * STAGING_BYTES) + 1024 <= PRODUCT_SHARED && COLUMNS <= 512, "shared memory or Tensor Memory is too small");
-    static_assert(!THIN || (!AT && FORM != PAIR), "only rows along k can be left out");
+    static_assert(!THIN || (!AT && CG == 1), "only rows along k can be left out");
     extern __shared__ unsigned char raw[];
     __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], arrived, taken;
     __shared__ u32 tmem;
     unsigned char* const smem = raw + (1024 - (frnn_smem_addr(raw) & 1023)) % 1024;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const u32 rank = FORM == ALONE ? 0 : cluster_rank(), blocks = FORM == ALONE ? 1 : cluster_blocks();
-    const u32 half_m = FORM == PAIR ? rank : 0;        // which 128 of a tile's rows
+    const u32 half_m = CG == 2 ? rank : 0;        // which 128 of a tile's rows
     const int tiles = p.tiles_m * p.tiles_n * p.slices, first = blockIdx.x / blocks, stride = gridDim.x / blocks;
     const u32 part = FORM == SPLIT ? rank : 0, parts = FORM == SPLIT ? blocks : 1;       // of a tile's steps along k
 
@@ -601,86 +605,103 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
     if (warp < 4) {
         frnn_regs_release<CONTROL_REGISTERS>();
         if (warp == 0) {
+            // (One thread each copies and issues: of few instructions a step, because a step of 128 x 128 is done in 256 cycles.)
             if (frnn_elect()) {
-                u32 it = 0;
+                const u32 base = frnn_smem_addr(smem), empty0 = frnn_smem_addr(&empty[0]), full0 = frnn_smem_addr(&full[0]), full_lead = CG == 2 ? in_block(&full[0], 0) : full0;
+                u32 s = 0, phase = 1, issued = 0;
                 bool ok = true;
-                auto bar_of = [&](int s) { return CG == 2 ? in_block(&full[s], 0) : frnn_smem_addr(&full[s]); };
-                auto load_b = [&](int s, int n, int g, int k) {
-                    const u32 bar = bar_of(s), at = frnn_smem_addr(smem + s * STAGE) + A_BYTES;
-                    const int plane = p.plane_b[g];
-                    if (half_m == 0) frnn_mbar_expect_tx(&full[s], STAGE * CG);      // (a's bytes too)
+                auto load_b = [&](u32 s, const CUtensorMap* map, int n, int plane, int k) {
+                    const u32 bar = full_lead + s * 8, at = base + s * STAGE + A_BYTES;
+                    if (CG == 1 || half_m == 0) expect_bytes(full0 + s * 8, STAGE * CG);      // (a's bytes too)
                     if constexpr (BT) {
 #pragma unroll
-                        for (int part = 0; part < NB / 64; part++) tma_load<CG>(at + part * 8192, &p.b[p.map_b[g]], n + part * 64, k * BK, plane, bar);
-                    } else if (!p.dual) {
-                        tma_load<CG>(at, &p.b[p.map_b[g]], k * BK, n, plane, bar);
-                        static_assert(BT || NB == 128, "a copy is 128 rows high");
-                    } else if (CG == 2) {      // one block has B0's rows, the other B1's
-                        tma_load<CG>(at, &p.b[half_m], k * BK, n, plane, bar);
-                    } else {                   // (copies of 64 rows)
-                        tma_load<CG>(at, &p.b[0], k * BK, n, plane, bar);
-                        tma_load<CG>(at + B_BYTES / 2, &p.b[1], k * BK, n, plane, bar);
+                        for (int part = 0; part < NB / 64; part++) tma_load<CG>(at + part * 8192, map, n + part * 64, k, plane, bar);
+                    } else {
+                        tma_load<CG>(at, map, k, n, plane, bar);
+                        if (CG == 1 && p.dual) tma_load<CG>(at + B_BYTES / 2, &p.b[1], k, n, plane, bar);      // (copies of 64 rows)
                     }
                 };
-                auto load_a = [&](int s, int m, int plane, int k) {
-                    const u32 bar = bar_of(s), at = frnn_smem_addr(smem + s * STAGE);
+                auto load_a = [&](u32 s, int m, int plane, int k) {
+                    const u32 bar = full_lead + s * 8, at = base + s * STAGE;
                     if constexpr (AT) {
-                        tma_load<CG>(at, &p.a, m, k * BK, plane, bar);
-                        tma_load<CG>(at + A_BYTES / 2, &p.a, m + 64, k * BK, plane, bar);
+                        tma_load<CG>(at, &p.a, m, k, plane, bar);
+                        tma_load<CG>(at + A_BYTES / 2, &p.a, m + 64, k, plane, bar);
                     } else {
-                        tma_load<CG>(at, &p.a, k * BK, m, plane, bar);
+                        tma_load<CG>(at, &p.a, k, m, plane, bar);
                     }
                 };
                 auto column = [&](const Tile& w) { return p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)half_m * NB; };
-                int early = 0;
+                // (of two B a pair's blocks have one each)
+                auto map_of = [&](int g) { return &p.b[p.dual ? (CG == 2 ? (int)half_m : 0) : p.map_b[g]]; };
+                u32 early = 0;
                 if (p.b_ready && first < tiles) {
                     const Tile w = tile_of(p, first, part, parts);
                     early = min(STAGES, w.to - w.from);
-                    for (int i = 0; i < early; i++) load_b(i, column(w), (w.from + i) / p.ksteps, (w.from + i) % p.ksteps);
+                    for (u32 i = 0; i < early; i++) {
+                        const int g = (w.from + (int)i) / p.ksteps;
+                        load_b(i, map_of(g), column(w), p.plane_b[g], (w.from + (int)i - g * p.ksteps) * BK);
+                    }
                 }
                 cudaGridDependencySynchronize();
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u, part, parts);
                     const int m = (w.tm * CG + (int)half_m) * 128, n = column(w), further = w.second ? p.stacked : 0;
-                    int g = w.from / p.ksteps, k = w.from % p.ksteps;
-                    for (int i = w.from; i < w.to; i++, it++) {
-                        const int s = it % STAGES;
-                        if (it >= (u32)early) {
-                            if (!(ok = frnn_mbar_wait(&empty[s], (it / STAGES & 1) ^ 1, p.err, CODE_PRODUCT))) break;
-                            load_b(s, n, g, k);
+                    int g = w.from / p.ksteps, k = (w.from - g * p.ksteps) * BK, left = w.to - w.from;
+                    for (; ok && left > 0; g++, k = 0) {
+                        const CUtensorMap* const map = map_of(g);
+                        const int pa = p.plane_a[g] + further, pb = p.plane_b[g], end = min(p.ksteps * BK, k + left * BK);
+                        left -= (end - k) / BK;
+#pragma unroll 1
+                        for (; k < end; k += BK) {
+                            if (issued >= early) {
+                                if (!(ok = wait_at(empty0 + s * 8, phase, p.err))) break;
+                                load_b(s, map, n, pb, k);
+                            }
+                            load_a(s, m, pa, k);
+                            issued++;
+                            if (++s == STAGES) {
+                                s = 0;
+                                phase ^= 1;
+                            }
                         }
-                        load_a(s, m, p.plane_a[g] + further, k);
-                        if (++k == p.ksteps) { k = 0; g++; }
                     }
                 }
                 // every copy has been used, and every arrival has come, before the block leaves
-                for (u32 i = it > STAGES ? it - STAGES : 0; i < it; i++)
-                    if (!frnn_mbar_wait(&empty[i % STAGES], i / STAGES & 1, p.err, CODE_PRODUCT)) break;
+                for (u32 i = issued > STAGES ? issued - STAGES : 0; i < issued; i++)
+                    if (!wait_at(empty0 + i % STAGES * 8, i / STAGES & 1, p.err)) break;
             }
             __syncwarp();
         } else if (warp == 1) {
             if (half_m == 0 && frnn_elect()) {
-                u32 it = 0, t = 0;
+                const u32 full0 = frnn_smem_addr(&full[0]), empty0 = frnn_smem_addr(&empty[0]);
+                const u64 a0 = operand_desc(frnn_smem_addr(smem), 8192), b0 = operand_desc(frnn_smem_addr(smem) + A_BYTES, 8192);
+                u32 s = 0, phase = 0, t = 0;
                 bool ok = true;
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u, part, parts);
                     for (int from = w.from; ok && from < w.to; t++) {
                         const int to = PROMOTE ? min(from + p.flush, w.to) : w.to;
                         const u32 buf = t & 1, d = tmem + buf * BN;
-                        if (!(ok = frnn_mbar_wait(&acc_empty[buf], (t / 2 & 1) ^ 1, p.err, CODE_PRODUCT))) break;
+                        if (!(ok = wait_at(frnn_smem_addr(&acc_empty[buf]), (t / 2 & 1) ^ 1, p.err))) break;
                         frnn_tmem_fence_after_sync();
-                        for (int i = from; i < to; i++, it++) {
-                            const int s = it % STAGES;
-                            if (!(ok = frnn_mbar_wait(&full[s], it / STAGES & 1, p.err, CODE_PRODUCT))) break;
+                        u32 more = 0;                      // (the first product of a part overwrites what was there)
+#pragma unroll 1
+                        for (int i = from; i < to; i++) {
+                            if (!(ok = wait_at(full0 + s * 8, phase, p.err))) break;
                             frnn_tmem_fence_after_sync();
-                            const u32 at = frnn_smem_addr(smem + s * STAGE);
-                            const u64 a = operand_desc(at, 8192), b = operand_desc(at + A_BYTES, 8192);
+                            const u64 a = a0 + s * (STAGE / 16), b = b0 + s * (STAGE / 16);
 #pragma unroll
-                            for (int k = 0; k < BK / 16; k++)      // 16 values of k: 32 bytes of a row, or 16 rows
-                                mma_f16<CG>(d, a + k * (AT ? 2048 / 16 : 32 / 16), b + k * (BT ? 2048 / 16 : 32 / 16), p.idesc, i > from || k > 0);
-                            mma_commit<CG>(&empty[s]);
+                            for (int k = 0; k < BK / 16; k++) {      // 16 values of k: 32 bytes of a row, or 16 rows
+                                mma_f16<CG>(d, a + k * (AT ? 2048 / 16 : 32 / 16), b + k * (BT ? 2048 / 16 : 32 / 16), p.idesc, more);
+                                more = 1;
+                            }
+                            mma_commit<CG>(empty0 + s * 8);
+                            if (++s == STAGES) {
+                                s = 0;
+                                phase ^= 1;
+                            }
                         }
-                        mma_commit<CG>(&acc_full[buf]);
+                        mma_commit<CG>(frnn_smem_addr(&acc_full[buf]));
                         from = to;
                     }
                 }
@@ -696,7 +717,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
         u32 t = 0, round = 0;
         bool ok = true;
         auto filled = [&] {            // waits for accumulators; their address
-            ok = __all_sync(0xffffffffu, frnn_mbar_wait(&acc_full[t & 1], t / 2 & 1, p.err, CODE_PRODUCT));
+            ok = __all_sync(0xffffffffu, wait_at(frnn_smem_addr(&acc_full[t & 1]), t / 2 & 1, p.err));
             frnn_tmem_fence_after_sync();
             return tmem + (t & 1) * BN + frnn_tmem_lane_base(quarter);
         };
@@ -750,7 +771,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         emptied();
                         // to the owners: of every block's columns those that this warp has, four at a time
                         const int own = BN / (int)blocks, row = quarter * 32 + lane;      // (own: a power of two)
-                        ok = __all_sync(0xffffffffu, wait_for_cluster(&taken, (round & 1) ^ 1, p.err));
+                        ok = __all_sync(0xffffffffu, wait_at<true>(frnn_smem_addr(&taken), (round & 1) ^ 1, p.err));
                         if (!ok) break;
 #pragma unroll
                         for (int i = 0; i < BN / 2 && !idle; i += 4) {
@@ -767,7 +788,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         }
                         __syncwarp();
                         if (lane < (int)blocks) arrive_after_sending(in_block(&arrived, lane));
-                        ok = __all_sync(0xffffffffu, wait_for_cluster(&arrived, round & 1, p.err));
+                        ok = __all_sync(0xffffffffu, wait_at<true>(frnn_smem_addr(&arrived), round & 1, p.err));
                         if (!ok) break;
                         // the owner's columns: half of them each, but whole accesses of 8 (both products' of GLU_FORWARD)
                         const int width = EPI == GLU_FORWARD ? own / 2 : own, count = max(8, width / 2), from = half * count;
@@ -988,7 +1009,7 @@ struct ProductPlan {
     int blocks, slices;                           // of a cluster; of k beyond that
     int64_t tiles_m, tiles_n;
     size_t scratch;                               // the slices' results
-    int columns() const { return form == PAIR ? 128 : form == ALONE ? 64 : 64 / blocks; }      // that a warp of the epilogue has in a row
+    int columns() const { return form == PAIR ? 128 : form == SPLIT ? 64 / blocks : 64; }      // that a warp of the epilogue has in a row
 };
 
 // Clusters of 1, 2, 4 or 8 blocks that run at once, one block to a multiprocessor.
@@ -1017,17 +1038,18 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
 }
 
 // Which form: the one that is done first, by what was measured (ns, on a B200).  A step of 64 along k takes 285 in PAIR (for 128 x 256 in
-// each block; the tensor cores' own time is 270), 205 in ALONE and 225 in SPLIT (for 128 x 128; 135, but 8 KB of operands for each 16
-// values of k are as much as shared memory gives, and the copies come on top).  A tile leaves in `leave` (STORE, GLU_FORWARD,
-// GLU_BACKWARD, LOGPROB_STATS, LOGPROB_GRAD), while the next one is computed; in SPLIT that has the exchange in it.
+// each block; the tensor cores' own time is 270), 215 in ALONE and 225 in SPLIT (for 128 x 128; 135, but the 32 KB that are copied for it are 78
+// bytes a cycle, about what a multiprocessor takes in; 256 x 128 by a pair, 24 KB each, took 180 and was ahead by 5 % at a few sizes: left out).
+// A tile leaves in `leave` (STORE, GLU_FORWARD, GLU_BACKWARD, LOGPROB_STATS, LOGPROB_GRAD), while the next one is computed; in SPLIT that
+// has the exchange in it.
 // Products of up to 128 rows read 16 KB of weights a step that nobody else reads: 372 when all multiprocessors do (6.5 TB/s).  THIN takes 225
 // at least (the tensor cores read 128 rows of A whatever is in them).
 // Measured, us: 256 x 512 of K = 2048 PAIR 14.9, ALONE 9.7, SPLIT 9.9, 8.8 and 8.8 (2, 4 and 8 blocks); K = 16384 ALONE 55, SPLIT in 4 23.
 // A block of 16 rows, 4096 wide, 12288 hidden (both products): ALONE and 4 63, 2 and 4 58, 4 and 4 66; 2048 wide, 8192 hidden: ALONE and 4 29, 2 and 4 32.
 // Log probabilities of 16 rows, 65536 tokens, 4096 wide: ALONE 105, SPLIT in 2 115.
-inline bool is_thin(const Product& q, bool at, Form form) { return !at && form != PAIR && q.m <= THIN_ROWS; }
+inline bool is_thin(const Product& q, bool at, Form form) { return !at && (form == ALONE || form == SPLIT) && q.m <= THIN_ROWS; }
 template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
-    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 1700, 2600}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 205, 225};
+    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2500, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 215, 225};
     const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
     const bool few = !AT && q.m <= 128;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
