@@ -646,11 +646,13 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u, part, parts);
                     const int m = (w.tm * CG + (int)half_m) * 128, n = column(w), further = w.second ? p.stacked : 0;
-                    int g = w.from / p.ksteps, k = (w.from - g * p.ksteps) * BK, left = w.to - w.from;
-                    for (; ok && left > 0; g++, k = 0) {
+                    int g = w.from / p.ksteps, at = w.from - g * p.ksteps, left = w.to - w.from;      // (in steps: all segments together may pass 2^31 values)
+                    for (; ok && left > 0; g++, at = 0) {
                         const CUtensorMap* const map = map_of(g);
-                        const int pa = p.plane_a[g] + further, pb = p.plane_b[g], end = min(p.ksteps * BK, k + left * BK);
-                        left -= (end - k) / BK;
+                        const int pa = p.plane_a[g] + further, pb = p.plane_b[g], some = min(p.ksteps - at, left);
+                        left -= some;
+                        int k = at * BK;
+                        const int end = k + some * BK;
 #pragma unroll 1
                         for (; k < end; k += BK) {
                             if (issued >= early) {
