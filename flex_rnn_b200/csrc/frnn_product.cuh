@@ -526,8 +526,6 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
-
-// Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
 // Part `part` of `parts` of a tile's (a slice's) steps along k.
 __device__ __forceinline__ void steps_of(const ProductArgs& p, Tile& w, u32 part, u32 parts) {
     const int steps = p.ksteps * p.segments;
@@ -540,6 +538,7 @@ __device__ __forceinline__ void steps_of(const ProductArgs& p, Tile& w, u32 part
         w.to = (int)(steps * (at + 1) / all);
     }
 }
+// Tiles in groups of `group` rows of tiles, column after column: A's rows of a group stay in L2 while B passes by once.
 __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 part, u32 parts) {
     Tile w;
     const int tiles = p.tiles_m * p.tiles_n;
@@ -564,7 +563,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
     static_assert(STAGES * STAGE + EXCHANGE + (SHARE ? 0 : ROWS / 32 * 2 * STAGING_BYTES) + 1024 <= PRODUCT_SHARED && COLUMNS <= 512, "shared memory or Tensor Memory is too small");
     static_assert(!THIN || (!AT && CG == 1), "only rows along k can be left out");
     extern __shared__ unsigned char raw[];
-    __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], arrived, taken;
+    __shared__ u64 full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], arrived, taken, summed, halves[4];
     __shared__ u32 tmem;
     unsigned char* const smem = raw + (1024 - (frnn_smem_addr(raw) & 1023)) % 1024;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -585,7 +584,9 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
         if (FORM == SPLIT) {
             frnn_mbar_init(&arrived, EPILOGUE_WARPS * blocks);
             frnn_mbar_init(&taken, EPILOGUE_WARPS * blocks);
+            frnn_mbar_init(&summed, EPILOGUE_WARPS);
         }
+        for (int q = 0; q < 4; q++) frnn_mbar_init(&halves[q], 2);
         frnn_mbar_init_fence();
     }
     if (warp == 1 && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"((u64)(lane ? &p.b[lane - 1] : &p.a)) : "memory");
@@ -739,6 +740,12 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
             next = tile_of(p, first, part, parts);
             next_data = row_data<EPI>(p, row_of(next) + lane);
         }
+        // waits for other warps of this block, once a round (with a limit, as all waits: a warp that gave up does not come)
+        auto met = [&](u64* bar) {
+            __syncwarp();
+            if (lane == 0) frnn_mbar_arrive(bar);
+            ok = __all_sync(0xffffffffu, wait_at(frnn_smem_addr(bar), round & 1, p.err));
+        };
         for (int u = first; ok && u < tiles; u += stride, round++) {
             const Tile w = next;
             const RowData data = next_data;
@@ -815,8 +822,12 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                             __syncwarp();
                             if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
                         };
-                        if constexpr (SHARE) frnn_group_sync(5, EPILOGUE_WARPS * 32);
-                        else done_with();
+                        if constexpr (SHARE) {
+                            met(&summed);
+                            if (!ok) break;
+                        } else {
+                            done_with();
+                        }
                         if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
                             epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
@@ -829,8 +840,9 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         frnn_tmem_wait_st();
                         if constexpr (EPI == GLU_FORWARD) {      // (a warp's columns of the two products lie in both warps' halves)
                             frnn_tmem_fence_before_sync();
-                            frnn_group_sync(1 + quarter, 64);
+                            met(&halves[quarter]);
                             frnn_tmem_fence_after_sync();
+                            if (!ok) break;
                         }
                     }
                 }
