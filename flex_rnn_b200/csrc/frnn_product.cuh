@@ -1,11 +1,11 @@
 // Matrix products on the tensor cores (tcgen05) with what follows them done on the tile that leaves Tensor Memory: the products
 // of frnn_gated_mlp.cu and frnn_linear_logprobs.cu.
 //
-//   C[m, n] = sum over segments g and k of A[plane_a(g)][m, k] B_g[plane_b(g)][n, k]
+//   C[m, n] = sum over pairs g and k of A_g[m, k] B_g[n, k]          (a second pair: da Wg + db Wu)
 //
 // Operands are 16-bit (bf16 or fp16), accumulators 32-bit.  fp32 operands are three bf16 planes hi + mid + lo (each the rest of
-// the one before, rounded to nearest: 24 bits, exactly), a product of them six segments, the terms above 2^-24: lo hi, hi lo,
-// mid mid, mid hi, hi mid, hi hi, the small ones first.  A sum of two products (da Wg + db Wu) is segments too.
+// the one before, rounded to nearest: 24 bits, exactly), and a product of them six, the terms above 2^-24: lo hi, hi lo, mid mid,
+// mid hi, hi mid, hi hi.  A step copies the three planes of both once for all six.
 //
 // Layout.  A block computes 128 rows.  Operands come by TMA, 64 values of k a stage, swizzled over 128 bytes.  An operand whose
 // rows run along k lies in shared memory as rows of 128 bytes (8 rows and 1024 bytes an atom); one that runs along m or n as
@@ -40,7 +40,7 @@ int frnn_tensor_map_swizzled(void* out_map, const void* base, uint64_t cols, uin
 namespace frnn_lm {
 
 enum Form { PAIR, ALONE, SPLIT };
-enum { BK = 64, STAGE_BYTES = 32768, THIN_ROWS = 32, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096, MAX_SEGMENTS = 12 };
+enum { BK = 64, STAGE_BYTES = 32768, THIN_ROWS = 32, EPILOGUE_WARPS = 8, PRODUCT_THREADS = 384, STAGING_BYTES = 4096 };
 // Registers of the warps that copy and issue, and of the epilogue's: 128 x 56 + 256 x 224 = 384 x 168, what a block starts with.
 enum { CONTROL_REGISTERS = 56, EPILOGUE_REGISTERS = 224, START_REGISTERS = 168 };
 enum { PRODUCT_SHARED = 6 * STAGE_BYTES + EPILOGUE_WARPS * STAGING_BYTES + 1024 };      // (6 stages; 5 and 64 KB for what arrives; 10 thin ones, 16 KB and less staging)
@@ -59,7 +59,8 @@ struct alignas(64) ProductArgs {
     CUtensorMap a, b[2];
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
     int flush;                  // PROMOTE: steps along k of a part
-    int ksteps, segments;       // steps of 64 along k in a segment
+    int pairs;                  // products that are added up
+    int ksteps, segments;       // steps of 64 along k in a segment; segments: pairs, where fp32 takes one product a step six times as many
     int tiles_m, tiles_n, group, slices;      // slices of k, each with a result of its own (STORE)
     int stacked;                // two products with the same B: the second's A is this many planes further on, its result at out2 (0: one)
     void* out2;
@@ -67,7 +68,6 @@ struct alignas(64) ProductArgs {
     int dual;                   // a tile's columns are half of B0's rows and half of B1's
     unsigned idesc;
     int* err;
-    unsigned char plane_a[MAX_SEGMENTS], map_b[MAX_SEGMENTS], plane_b[MAX_SEGMENTS];
     // STORE
     void* out;
     int64_t out_ld, out_slice;  // out_slice: elements between two slices' results
@@ -323,12 +323,13 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 
 // ---- epilogues ---------------------------------------------------------------------------------------------------------------
 
-// The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last
-// bit, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096, 2e-5 at 8192 in six segments, where 32-bit
-// sums rounded to nearest lose some 7e-7; from parts of 16 steps 3e-6, of 8 1.5e-6, of 4 7e-7, which costs up to 5 % of the time).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps
-// instead, from parts of `flush` steps, in registers, half of a tile's columns a warp; the sums go back to where the last part was, and
-// the epilogue is the same for all.  (One that took them from registers had its loops unrolled, and its code did not fit the instruction cache.)
-// Parts of 4 where the operands are fp32; of 16 for the fp32 results of 16-bit operands (4e-7).
+// The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last bit, all in
+// one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096 in 16 bits, 2e-5 at 8192 in fp32, where 32-bit sums rounded to
+// nearest lose some 9e-7).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps instead, in registers, half of a
+// tile's columns a warp, from parts of `flush` steps; the sums go back to where the last part was, and the epilogue is the same for
+// all.  (One that took them from registers had its loops unrolled, and its code did not fit the instruction cache.)  fp32 where a step is
+// six products: parts of one, whose small products come first, while the accumulator is small: 3e-7 (of two steps 1.6e-6 and 4 % faster); fp32 in SPLIT:
+// parts of 4, 6e-7; fp32 results of 16-bit operands: of 16, 4e-7.
 
 // 32 columns of accumulators, of the lane's row.  (Waited for apart: the next ones are under way while these are worked on.)
 __device__ __forceinline__ void ask(u32 taddr, float* v) { frnn_tmem_ld<32>(taddr, v); }
@@ -553,7 +554,12 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 part, u
 }
 
 // AT, BT: the operand's rows run along m (n) instead of k.
-template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
+template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool FP32> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
+    constexpr bool PROMOTE = FP32 || EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
+    // fp32: a step copies three planes of each operand and multiplies them six times; in SPLIT, whose stages hold no two such steps, it is one
+    // product of two planes, and the six follow one another over all of k
+    constexpr bool FUSED = FP32 && (FORM != SPLIT || THIN);
+    constexpr int PLANES = FUSED ? 3 : 1;
     constexpr int CG = FORM == PAIR ? 2 : 1, BN = FORM == PAIR ? 256 : 128, STAGES = THIN ? 10 : FORM == SPLIT ? 5 : 6;
     constexpr int NB = BN / CG;                        // B's rows in this block
     constexpr int ROWS = THIN ? (int)THIN_ROWS : 128;  // of A, that are copied and that have a result
@@ -633,14 +639,25 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 };
                 auto column = [&](const Tile& w) { return p.dual ? w.tn * (BN / 2) : w.tn * BN + (int)half_m * NB; };
                 // (of two B a pair's blocks have one each)
-                auto map_of = [&](int g) { return &p.b[p.dual ? (CG == 2 ? (int)half_m : 0) : p.map_b[g]]; };
+                auto map_of = [&](int g) { return &p.b[p.dual ? (CG == 2 ? (int)half_m : 0) : FP32 && !FUSED ? g % p.pairs : g]; };
+                // planes of a and b in segment g (fp32 in SPLIT: small terms first)
+                auto plane_a = [&](int g) {
+                    if (!FP32 || FUSED) return g * PLANES;
+                    const int t = g / p.pairs;
+                    return (t == 0 ? 2 : t == 2 || t == 3 ? 1 : 0) + g % p.pairs * 3;
+                };
+                auto plane_b = [&](int g) {
+                    if (!FP32 || FUSED) return 0;
+                    const int t = g / p.pairs;
+                    return t == 1 ? 2 : t == 2 || t == 4 ? 1 : 0;
+                };
                 u32 early = 0;
                 if (p.b_ready && first < tiles) {
                     const Tile w = tile_of(p, first, part, parts);
-                    early = min(STAGES, w.to - w.from);
+                    early = min(STAGES, min(STAGES, w.to - w.from) * PLANES);
                     for (u32 i = 0; i < early; i++) {
-                        const int g = (w.from + (int)i) / p.ksteps;
-                        load_b(i, map_of(g), column(w), p.plane_b[g], (w.from + (int)i - g * p.ksteps) * BK);
+                        const int step = w.from + (int)i / PLANES, g = step / p.ksteps;
+                        load_b(i, map_of(g), column(w), plane_b(g) + (int)i % PLANES, (step - g * p.ksteps) * BK);
                     }
                 }
                 cudaGridDependencySynchronize();
@@ -650,21 +667,24 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                     int g = w.from / p.ksteps, at = w.from - g * p.ksteps, left = w.to - w.from;      // (in steps: all segments together may pass 2^31 values)
                     for (; ok && left > 0; g++, at = 0) {
                         const CUtensorMap* const map = map_of(g);
-                        const int pa = p.plane_a[g] + further, pb = p.plane_b[g], some = min(p.ksteps - at, left);
+                        const int pa = plane_a(g) + further, pb = plane_b(g), some = min(p.ksteps - at, left);
                         left -= some;
                         int k = at * BK;
                         const int end = k + some * BK;
 #pragma unroll 1
-                        for (; k < end; k += BK) {
-                            if (issued >= early) {
-                                if (!(ok = wait_at(empty0 + s * 8, phase, p.err))) break;
-                                load_b(s, map, n, pb, k);
-                            }
-                            load_a(s, m, pa, k);
-                            issued++;
-                            if (++s == STAGES) {
-                                s = 0;
-                                phase ^= 1;
+                        for (; ok && k < end; k += BK) {
+#pragma unroll
+                            for (int plane = 0; plane < PLANES; plane++) {
+                                if (issued >= early) {
+                                    if (!(ok = wait_at(empty0 + s * 8, phase, p.err))) break;
+                                    load_b(s, map, n, pb + plane, k);
+                                }
+                                load_a(s, m, pa + plane, k);
+                                issued++;
+                                if (++s == STAGES) {
+                                    s = 0;
+                                    phase ^= 1;
+                                }
                             }
                         }
                     }
@@ -690,19 +710,32 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         u32 more = 0;                      // (the first product of a part overwrites what was there)
 #pragma unroll 1
                         for (int i = from; i < to; i++) {
-                            if (!(ok = wait_at(full0 + s * 8, phase, p.err))) break;
-                            frnn_tmem_fence_after_sync();
-                            const u64 a = a0 + s * (STAGE / 16), b = b0 + s * (STAGE / 16);
+                            u32 at[PLANES];                // the stages of a step's planes
 #pragma unroll
-                            for (int k = 0; k < BK / 16; k++) {      // 16 values of k: 32 bytes of a row, or 16 rows
-                                mma_f16<CG>(d, a + k * (AT ? 2048 / 16 : 32 / 16), b + k * (BT ? 2048 / 16 : 32 / 16), p.idesc, more);
-                                more = 1;
+                            for (int plane = 0; plane < PLANES; plane++) {
+                                at[plane] = s;
+                                if (ok) ok = wait_at(full0 + s * 8, phase, p.err);
+                                if (++s == STAGES) {
+                                    s = 0;
+                                    phase ^= 1;
+                                }
                             }
-                            mma_commit<CG>(empty0 + s * 8);
-                            if (++s == STAGES) {
-                                s = 0;
-                                phase ^= 1;
+                            if (!ok) break;
+                            frnn_tmem_fence_after_sync();
+                            // of three planes the products above 2^-24 of the largest, the small ones first, while the accumulators are small
+                            constexpr int PRODUCTS = FUSED ? 6 : 1;
+#pragma unroll
+                            for (int q = 0; q < PRODUCTS; q++) {
+                                const int of_a = !FUSED ? 0 : q == 0 ? 2 : q == 2 || q == 3 ? 1 : 0, of_b = !FUSED ? 0 : q == 1 ? 2 : q == 2 || q == 4 ? 1 : 0;
+                                const u64 a = a0 + at[of_a] * (STAGE / 16), b = b0 + at[of_b] * (STAGE / 16);
+#pragma unroll
+                                for (int k = 0; k < BK / 16; k++) {      // 16 values of k: 32 bytes of a row, or 16 rows
+                                    mma_f16<CG>(d, a + k * (AT ? 2048 / 16 : 32 / 16), b + k * (BT ? 2048 / 16 : 32 / 16), p.idesc, more);
+                                    more = 1;
+                                }
                             }
+#pragma unroll
+                            for (int plane = 0; plane < PLANES; plane++) mma_commit<CG>(empty0 + at[plane] * 8);
                         }
                         mma_commit<CG>(frnn_smem_addr(&acc_full[buf]));
                         from = to;
@@ -830,7 +863,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                         }
                         if (works) {
                             const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
-                            epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
+                            epilogue<EPI, FP32>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
                         }
                         if constexpr (SHARE) done_with();
                         continue;
@@ -848,7 +881,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> __globa
                 }
             }
             constexpr int COUNT = EPI == GLU_FORWARD ? BN / 4 : BN / 2;
-            if (!idle && row0 < p.M) epilogue<EPI, PROMOTE && EPI != LOGPROB_STATS>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, w, lane, staging);
+            if (!idle && row0 < p.M) epilogue<EPI, FP32>(p, data, acc + half * COUNT, acc + half * COUNT + BN / 2, row0, w.tn * 2 * COUNT + half * COUNT, COUNT, w, lane, staging);
             emptied();
         }
     }
@@ -1012,7 +1045,7 @@ struct Product {
     int dtype;                                    // of the operands: FRNN_F32 means planes
     Operand a, b[2];
     int64_t m, n, k;
-    int pairs = 1;                                // products that are added up: planes of a, b[0], b[1]
+    int pairs = 1;                                // products that are added up: of a's planes (groups of them) with b[0], b[1]
     void* out = nullptr;                          // STORE
     int out_dtype = 0;
     int64_t out_ld = 0;
@@ -1051,7 +1084,7 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
     return n;
 }
 
-// Which form: the one that is done first, by what was measured (ns, on a B200).  A step of 64 along k takes 285 in PAIR (for 128 x 256 in
+// Which form: the one that is done first, by what was measured (ns, on a B200; 16-bit operands, then fp32, whose steps but for SPLIT are six products).  A step of 64 along k takes 285 in PAIR (for 128 x 256 in
 // each block; the tensor cores' own time is 270), 215 in ALONE and 225 in SPLIT (for 128 x 128; 135, but the 32 KB that are copied for it are 78
 // bytes a cycle, about what a multiprocessor takes in; 256 x 128 by a pair, 24 KB each, took 180 and was ahead by 5 % at a few sizes: left out).
 // A tile leaves in `leave` (STORE, GLU_FORWARD, GLU_BACKWARD, LOGPROB_STATS, LOGPROB_GRAD), while the next one is computed; in SPLIT that
@@ -1063,14 +1096,16 @@ template <auto KERNEL> inline int clusters_at_once(int blocks) {
 // Log probabilities of 16 rows, 65536 tokens, 4096 wide: ALONE 105, SPLIT in 2 115.
 inline bool is_thin(const Product& q, bool at, Form form) { return !at && (form == ALONE || form == SPLIT) && q.m <= THIN_ROWS; }
 template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Product& q) {
-    static const int leave[3][5] = {{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2500, 3000}, {4000, 6000, 7000, 4500, 5000}}, step[3] = {285, 215, 225};
-    const int64_t steps = (q.k + BK - 1) / BK * q.pairs * (q.dtype == FRNN_F32 ? 6 : 1), width = q.args.dual ? 2 : 1;
-    const bool few = !AT && q.m <= 128;
+    static const int leave[2][3][5] = {{{3100, 5800, 10900, 4500, 5900}, {1600, 3400, 6000, 2500, 3000}, {4000, 6000, 7000, 4500, 5000}},
+                                       {{5000, 20000, 26000, 4500, 12000}, {2500, 12500, 16000, 2500, 6000}, {5000, 9000, 12000, 4500, 7000}}}, step[2][3] = {{285, 215, 225}, {1650, 1150, 225}};
+    const int64_t steps = (q.k + BK - 1) / BK * q.pairs, width = q.args.dual ? 2 : 1;
+    const bool few = !AT && q.m <= 128, fp32 = q.dtype == FRNN_F32;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     auto cost = [&](Form form, int blocks, int64_t tiles, int slices) {
-        const int64_t at_once = clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks), rounds = up(tiles, at_once), out = leave[form][EPI];
+        const int64_t at_once = clusters_at_once<product_kernel<SPLIT, false, AT, BT, EPI, true>>(blocks), rounds = up(tiles, at_once), out = leave[fp32][form][EPI];
         auto k_time = [&](int64_t tiles) {
-            return up(steps, form == SPLIT ? blocks * slices : slices) * std::max<int64_t>(is_thin(q, AT, form) ? 225 : step[form], few ? 372 * tiles * blocks / sm_count() : 0);
+            const bool apart = fp32 && form == SPLIT && !is_thin(q, AT, form);      // (six steps of one product)
+            return up(steps * (apart ? 6 : 1), form == SPLIT ? blocks * slices : slices) * std::max<int64_t>(is_thin(q, AT, form) ? (fp32 ? 900 : 225) : step[fp32][form], few ? (!fp32 ? 1 : apart ? 2 : 3) * 372 * tiles * blocks / sm_count() : 0);
         };
         const int64_t last = k_time(tiles - (rounds - 1) * at_once), start = (form == ALONE ? 1000 : 2000) + (form == SPLIT ? 1000 * rounds : 0);      // (its blocks wait for one another)
         return rounds == 1 ? start + last + out : start + k_time(at_once) + (rounds - 2) * std::max(k_time(at_once), out) + std::max(last, out) + out;
@@ -1084,8 +1119,8 @@ template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Produ
         // a long sum for few tiles: slices of at least 32 steps a block, whose results (up to 32 MB) a second kernel adds up
         for (int slices = 1; slices <= (EPI == STORE && !q.args.stacked ? 32 : 1); slices *= 2) {
             const size_t scratch = slices > 1 ? (size_t)slices * q.m * padded(q.n) * 4 : 0;
-            if (slices > 1 && (steps < 32ll * blocks * slices || scratch > (32u << 20))) break;
-            const int64_t c = cost(form, blocks, tm * tn * slices, slices) + (slices > 1 ? 4000 + (int64_t)(scratch >> 12) : 0);
+            if (slices > 1 && (steps < (fp32 ? 8ll : 32ll) * blocks * slices || scratch > (32u << 20))) break;
+            const int64_t c = cost(form, blocks, tm * tn * slices, slices) + (slices > 1 ? 8000 + (int64_t)(scratch >> 12) : 0);
             if (c < least) {
                 least = c;
                 best = {form, blocks, slices, tm, tn, scratch};
@@ -1095,8 +1130,8 @@ template <int EPI, bool AT, bool BT> inline ProductPlan plan_product(const Produ
     return best;
 }
 
-template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool PROMOTE> inline int launch_product(const char* what, const ProductArgs& p, int blocks, cudaStream_t stream) {
-    constexpr auto kernel = product_kernel<FORM, THIN, AT, BT, EPI, PROMOTE>;
+template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool FP32> inline int launch_product(const char* what, const ProductArgs& p, int blocks, cudaStream_t stream) {
+    constexpr auto kernel = product_kernel<FORM, THIN, AT, BT, EPI, FP32>;
     // (the warps would wait for registers that the block does not have)
     static const bool enough = [] {
         cudaFuncAttributes a = {};
@@ -1124,23 +1159,16 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     p.tiles_n = (int)plan.tiles_n;
     p.group = plan.form == PAIR ? 16 : 32;
     p.slices = plan.slices;
-    p.flush = q.dtype == FRNN_F32 ? 4 : 16;
     const unsigned type = q.dtype == FRNN_F16 ? 0 : 1, side = plan.form == PAIR ? 256 : 128;
     p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((unsigned)AT << 15) | ((unsigned)BT << 16) | ((side >> 3) << 17) | ((side >> 4) << 24);
-    static const unsigned char first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};      // planes of a and b, small terms first
-    const int terms = q.dtype == FRNN_F32 ? 6 : 1;
-    p.segments = 0;
-    for (int t = 0; t < terms; t++)
-        for (int pair = 0; pair < q.pairs; pair++, p.segments++) {
-            p.plane_a[p.segments] = (unsigned char)((terms == 6 ? first[t] : 0) + pair * planes_of(q.dtype));
-            p.plane_b[p.segments] = terms == 6 ? second[t] : 0;
-            p.map_b[p.segments] = (unsigned char)(q.pairs > 1 ? pair : 0);
-        }
+    const bool thin = is_thin(q, AT, plan.form), fp32 = q.dtype == FRNN_F32, fused = fp32 && (plan.form != SPLIT || thin);
+    p.pairs = q.pairs;
+    p.segments = q.pairs * (fp32 && !fused ? 6 : 1);
+    p.flush = fused ? 1 : fp32 ? 4 : 16;
     if ((int64_t)p.ksteps * p.segments >= (1ll << 31) - 64) return frnn_fail(FRNN_E_ARG, "%s: too long", what);
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);
     };
-    const bool thin = is_thin(q, AT, plan.form);
     int rc = encode(p.a, q.a, AT, thin ? THIN_ROWS : 128);
     for (int i = 0; i < 2 && rc == FRNN_OK; i++) {
         if (i && !q.b[1].p) p.b[1] = p.b[0];
@@ -1159,11 +1187,10 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
         p.add = p.alpha = nullptr;
     }
     p.out_wide = on_boundary(p.out, 16) && on_boundary(p.out2, 16) && p.out_ld * (int64_t)dtype_bytes(p.out_dtype) % 16 == 0;
-    constexpr bool EXACT = EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
     auto run = [&](auto form, auto rows) {
         constexpr Form FORM = decltype(form)::value;
         constexpr bool THIN = decltype(rows)::value;
-        return q.dtype == FRNN_F32 ? launch_product<FORM, THIN, AT, BT, EPI, true>(what, p, plan.blocks, stream) : launch_product<FORM, THIN, AT, BT, EPI, EXACT>(what, p, plan.blocks, stream);
+        return q.dtype == FRNN_F32 ? launch_product<FORM, THIN, AT, BT, EPI, true>(what, p, plan.blocks, stream) : launch_product<FORM, THIN, AT, BT, EPI, false>(what, p, plan.blocks, stream);
     };
     const std::false_type all;
     const std::true_type few;
