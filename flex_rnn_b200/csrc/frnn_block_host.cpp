@@ -202,7 +202,7 @@ bool heads_of(const Tensor& x, int64_t& heads, int64_t& stride) {
     return true;
 }
 
-Tensor rotary_cuda(const Tensor& x, const optional<Tensor>& positions, int64_t start, const Tensor& frequencies, bool interleaved, double scale, bool inverse) {
+Tensor rotary_cuda(const Tensor& x, const optional<Tensor>& positions, c10::SymInt start, const Tensor& frequencies, bool interleaved, double scale, bool inverse) {
     const char* op = "rotary";
     frnn_rotary_call c = {};
     c.dtype = dtype_of(op, "x", x);
@@ -241,7 +241,7 @@ Tensor rotary_cuda(const Tensor& x, const optional<Tensor>& positions, int64_t s
     c.length = x.size(1);
     c.width = x.size(-1);
     c.pairs = f.size(0);
-    c.start = start;
+    c.start = start.expect_int();
     for (int d = 0; d < 2; d++) c.x_stride[d] = x.size(d) > 1 ? from.stride(d) : 0;
     c.y_stride[2] = c.heads > 1 ? c.width : 0;
     c.y_stride[1] = c.length > 1 ? c.heads * c.width : 0;
@@ -350,10 +350,11 @@ std::tuple<Tensor, Tensor> linear_logprobs_backward_autograd(const optional<Tens
     return r;
 }
 
-// A rotation is linear and its gradient the rotation back: the same operator, differentiable in its turn.
+// A rotation is linear and its gradient the rotation back: the same operator, differentiable in its turn.  (A compiled program
+// may have `start` as a symbol: generation goes on from another position each call.)
 struct RotaryBackward : Saving {
     using Saving::Saving;
-    int64_t start;
+    c10::SymInt start;
     bool interleaved, inverse, positions;
     double scale;
     std::string name() const override { return "RotaryBackward"; }
@@ -364,7 +365,7 @@ struct RotaryBackward : Saving {
     }
 };
 
-Tensor rotary_autograd(const Tensor& x, const optional<Tensor>& positions, int64_t start, const Tensor& frequencies, bool interleaved, double scale, bool inverse) {
+Tensor rotary_autograd(const Tensor& x, const optional<Tensor>& positions, c10::SymInt start, const Tensor& frequencies, bool interleaved, double scale, bool inverse) {
     no_tangent(x);
     no_tangent(frequencies);
     TORCH_CHECK(!at::GradMode::is_enabled() || !needs(frequencies), "flex_rnn_b200: rotary: the frequencies carry no gradient");
@@ -394,7 +395,7 @@ TORCH_LIBRARY_FRAGMENT(flex_rnn_b200, m) {
     m.def("gated_mlp_backward(Tensor grad, Tensor x, Tensor gate, Tensor up, Tensor down, Tensor by_gate, Tensor by_up, Tensor hidden, int activation, bool want_x, bool want_gate, bool want_up, bool want_down) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("linear_logprobs(Tensor x, Tensor weight, Tensor tokens, float temperature, int ignore_index, bool save) -> (Tensor, Tensor, Tensor)");
     m.def("linear_logprobs_backward(Tensor? dlogprob, Tensor? dentropy, Tensor x, Tensor weight, Tensor tokens, Tensor stats, float temperature, int ignore_index, bool want_x, bool want_weight) -> (Tensor, Tensor)");
-    m.def("rotary(Tensor x, Tensor? positions, int start, Tensor frequencies, bool interleaved, float scale, bool inverse) -> Tensor");
+    m.def("rotary(Tensor x, Tensor? positions, SymInt start, Tensor frequencies, bool interleaved, float scale, bool inverse) -> Tensor");
 }
 
 #define FRNN_ALL(how) \

@@ -16,10 +16,9 @@
 // Tensor Memory (which holds two sets, so that the next tile's products run meanwhile).  Blocks stay for several tiles.  Three forms:
 //   PAIR   256 x 256 by a pair of blocks, each with half of B's rows, so that a byte of B in shared memory serves 256 rows
 //   ALONE  128 x 128 by a block: small products spread over more multiprocessors
-//   SPLIT  128 x 128 by a cluster of 2, 4 or 8 blocks, each with a part of k.  Each block then owns a part of the tile's columns: the others
-//          send it their sums of these (into its shared memory), it adds them in the order of the blocks and has the epilogue
-//          to itself.  (5 stages, and 64 KB for what arrives, where the
-//          epilogue turns its rows over afterwards.)
+//   SPLIT  128 x 128 by a cluster of 2, 4 or 8 blocks, each with a part of k.  Each block then owns a part of the tile's columns:
+//          the others send it their sums of these (into its shared memory), it adds them in the order of the blocks and has the
+//          epilogue to itself.  (5 stages, and 64 KB for what arrives, where the epilogue turns its rows over afterwards.)
 // THIN (ALONE or SPLIT, up to 32 rows, as in generation): only 32 of A's rows are copied, so that 10 stages of B are under way, 160 KB a
 // multiprocessor: such products are as fast as their weights come.  The tensor cores read 128 rows all the same: what they find
 // behind the 32 ends in rows of the result that nobody looks at.

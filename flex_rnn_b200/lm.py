@@ -93,7 +93,7 @@ def linear_logprobs(x: th.Tensor, weight: th.Tensor, tokens: th.Tensor, temperat
     """``token_logprobs(x @ weight.T, tokens, ...)`` without the logits: log probabilities of ``tokens`` [...] and entropies
     from the vectors ``x`` [..., width] and the last projection's ``weight`` [vocabulary, width], of one type.
 
-    The products run on the tensor cores, with sums in 32 bits; the logits leave them a tile at a time and are not kept, and
+    The products run on the tensor cores, with sums in 32 bits (of fp32 as in ``gated_mlp``); the logits leave them a tile at a time and are not kept, and
     the backward computes them again, a piece of the vocabulary at a time (its workspace holds 2^28 of their gradients, in
     fp32 2^27, or 256 columns where there are more rows).  In bf16 and fp16 their gradient is rounded to that type before it
     is multiplied with ``weight`` and ``x``.  Results are fp32 and both differentiable.  Tokens equal to ``ignore_index`` have
@@ -109,7 +109,7 @@ def gated_mlp(x: th.Tensor, gate: th.Tensor, up: th.Tensor, down: th.Tensor, act
     ``ACTIVATIONS``.
 
     The products run on the tensor cores, with sums in 32 bits (fp32 numbers as sums of three bf16 ones, so that nothing of them
-    is lost).  In bf16 and fp16 the hidden vectors and the gradients of the two projections are rounded to
+    is lost; an infinity among them gives NaN).  In bf16 and fp16 the hidden vectors and the gradients of the two projections are rounded to
     that type, as the tensor cores read them.  For the backward a call keeps the hidden vectors and, in 32 bits, their
     derivatives by the two projections."""
     if activation not in ACTIVATIONS:

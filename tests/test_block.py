@@ -4,7 +4,8 @@ Tolerances of the matrix products.  Operands are exact: 16-bit numbers, or fp32 
 2^-24 are left out.  Accumulators have 32 bits and truncate: each instruction adds 16 products and may lose a unit of the last
 place, 2^-23 of a partial sum, which is at most the sum S of the terms' absolute values; ``lost(k, dtype)`` counts twice
 that for each instruction of a chain (its own alignment of 16 products loses as much at most): k / 16 of them in 16 bits, 16 where parts are added
-up in registers, and a rounding for each part of 256 values (fp32: in six products).  What lies between two products
+up in registers, and a rounding for each part of 256 values (fp32: in six products; or 24 for each 64 values, of which
+those of the small products, 2^-8 of the sum at most, count for nothing, and a rounding for each).  What lies between two products
 is rounded to the operands' type (half a unit in the last place, UNIT); how these errors go on through the formulas
 is computed next to the exact results, term by term, with absolute values."""
 import ctypes
@@ -847,3 +848,26 @@ def test_compiled_for_any_batch(name):
     for b in (6, 7, 9):
         f, leaves, up = of_batch(name, b, "cuda")
         assert all(torch.equal(a, g) for a, g in zip(both(lambda *a: compiled(f, a), leaves, up), both(f, leaves, up)))
+
+
+def turned_from(device):
+    """A compiled rotation of single tokens, as generation calls it, from many positions: two programs, not one for each."""
+    lm._operators()
+    torch._dynamo.reset()
+    f = torch.linspace(1, 0.1, 4, dtype=torch.float64, device=device)
+    x = torch.ones(2, 1, 3, 10, device=device, requires_grad=True)
+    compiled = torch.compile(lambda x, p: fr.rotary(x, p, f), fullgraph=True, backend="aot_eager")
+    for p in [0, 5, 2 ** 40, *range(7, 30)]:
+        y = compiled(x, p)
+        yield x, y, fr.rotary(x, p, f)
+
+
+def test_symbolic_position():
+    for x, y, want in turned_from("meta"):
+        assert y.shape == want.shape and torch.autograd.grad(y.sum(), x)[0].shape == x.shape
+
+
+@pytest.mark.gpu
+def test_compiled_for_any_position():
+    for x, y, want in turned_from("cuda"):
+        assert torch.equal(y, want) and torch.equal(*(torch.autograd.grad(v.sum(), x)[0] for v in (y, want)))
