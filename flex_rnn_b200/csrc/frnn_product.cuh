@@ -285,15 +285,28 @@ template <class T> struct Rows {
 
 // h = act(a) b of N values, and where asked for its derivatives by a and b, in their place.  (One choice for all of them:
 // chosen for each value, the code of all four no longer fit the instruction cache, and a tile took five times as long.)
+// gelu: a Phi(a), Phi(-t) = exp(-t^2 / 2) R(t) with R(t) = erfcx(t / sqrt 2) / 2, which is smooth: s = 1 / (1 + 0.26 t) times a polynomial
+// in s, fitted over 0 <= t <= 14.5 (beyond, Phi(-t) is 0) for the least relative error by reweighted least squares: 2.8e-8, in 32 bits 4e-7 and
+// t^2 2^-23.  (8192 x 1024 to 4096 in bf16, us without and with derivatives: silu 84 and 118, gelu 102 and 129, gelu with erfcf 123 and 166.)
 template <int KIND> __device__ __forceinline__ void activate(float a, float& act, float& slope) {
     if constexpr (KIND == FRNN_SILU || KIND == FRNN_SIGMOID) {
         const float s = __fdividef(1.f, 1.f + __expf(-a));
         act = KIND == FRNN_SILU ? a * s : s;
         slope = KIND == FRNN_SILU ? fmaf(act, 1.f - s, s) : s * (1.f - s);
     } else if constexpr (KIND == FRNN_GELU) {
-        const float half = 0.5f * erfcf(-0.70710678118654752f * a);
-        act = a * half;
-        slope = fmaf(a, 0.39894228040143268f * __expf(-0.5f * a * a), half);
+        const float t = fminf(fabsf(a), 14.5f), s = __fdividef(1.f, fmaf(0.26f, t, 1.f)), e = exp2_fast(-0.72134752044448170f * (t * t));
+        float r = 3.023032099e-02f;
+        r = fmaf(r, s, -1.514945477e-01f);
+        r = fmaf(r, s, 2.487334311e-01f);
+        r = fmaf(r, s, -1.477895379e-01f);
+        r = fmaf(r, s, 1.587588638e-01f);
+        r = fmaf(r, s, 5.196479708e-02f);
+        r = fmaf(r, s, 1.027886793e-01f);
+        r = fmaf(r, s, 1.030509695e-01f);
+        r = fmaf(r, s, 1.037570164e-01f);
+        const float low = e * (r * s), share = a > 0.f ? 1.f - low : low;
+        act = a * share;
+        slope = fmaf(a, 0.39894228040143268f * e, share);
     } else {
         act = a > 0.f || a != a ? a : 0.f;
         slope = a > 0.f ? 1.f : 0.f;

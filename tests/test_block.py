@@ -871,3 +871,23 @@ def test_symbolic_position():
 def test_compiled_for_any_position():
     for x, y, want in turned_from("cuda"):
         assert torch.equal(y, want) and torch.equal(*(torch.autograd.grad(v.sum(), x)[0] for v in (y, want)))
+
+
+@pytest.mark.gpu
+def test_gelu_everywhere():
+    """gelu and its derivative alone, from x = (a, 1), gate (1, 0), up (0, 1), down 1.  Relative errors in units of 2^-24, with t = |a|: the exponent
+    t^2 / 2 is rounded three times (1.5 t^2), an exponential 4, a reciprocal 5 (times 1.3, as it goes into the polynomial), the polynomial 4, four
+    roundings behind it, products on the way 4: 24 + 1.5 t^2 of each term."""
+    a = torch.cat([torch.linspace(-12, 12, 20001), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 30.0, -30.0, 1e30, -1e30])]).cuda()
+    x = torch.stack([a, torch.ones_like(a)], -1).requires_grad_()
+    gate, up, down = torch.tensor([[1.0, 0.0]]).cuda(), torch.tensor([[0.0, 1.0]]).cuda(), torch.ones(1, 1).cuda()
+    y = fr.gated_mlp(x, gate, up, down, "gelu")
+    slope = torch.autograd.grad(y.sum(), x)[0][:, 0].double()
+    t = a.double()
+    share, density = 0.5 * torch.special.erfc(-t / 2 ** 0.5), torch.exp(-t * t / 2) / (2 * math.pi) ** 0.5
+    tol = (24 + 1.5 * t * t) * 2.0 ** -24
+    for got, terms in ((y[:, 0].double(), (t * share,)), (slope, (share, torch.where(density == 0, 0.0, t * density)))):
+        off = (got - sum(terms)).abs() - tol.clamp(max=1.0) * sum(v.abs() for v in terms) - 2.0 ** -120
+        assert float(off.max()) <= 0, (float(a[off.argmax()]), float(off.max()))
+    inf = fr.gated_mlp(torch.tensor([[math.nan, 1.0]]).cuda(), gate, up, down, "gelu")
+    assert inf.isnan().all()
