@@ -151,7 +151,11 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
     // pieces of up to 2^28 elements of the logits' gradient (512 MB; half as many in three planes), whole tiles of 256 columns
     const int64_t most = std::max<int64_t>(256, ((c->dtype == FRNN_F32 ? 1ll << 27 : 1ll << 28) / c->n) / 256 * 256), pieces = (c->vocab + most - 1) / most;
     const int64_t piece = pieces == 1 ? c->vocab : std::min(most, ((c->vocab + pieces - 1) / pieces + 255) / 256 * 256);
-    const Operand grad = new_operand(s, c->dtype, c->n, piece);
+    // Up to 128 rows the gradient is two 16-bit planes, what rounding leaves is the second: few rows' gradients at their own tokens are nearly
+    // all of a result, and their rounding did not average out (9 rows, half of them ignored, bf16: 2.7e-3 against 64 bits, where the result's own
+    // rounding is 1.6e-3).  Products of so few rows wait for the weights' copies.
+    const int planes = c->dtype != FRNN_F32 && c->n <= 128 ? 2 : 1;
+    const Operand grad = new_operand(s, c->dtype, c->n, piece, planes);
     float* const sum = pieces > 1 ? (float*)s.take((size_t)c->n * padded(c->width) * 4) : nullptr;
     float* const range = c->dtype == FRNN_F16 ? (float*)s.take(8) : nullptr;
     int rc = count ? (int)FRNN_OK : pack(packs, c->dtype, stream);
@@ -176,6 +180,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.args.stats = stats;
             q.args.scale = range;
             q.args.grad = g.writable();
+            q.args.rest = planes == 2;
             rc = run_product<LOGPROB_GRAD, false, false>(what, q, s, stream);
             if (rc != FRNN_OK) return rc;
         }
@@ -186,7 +191,8 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.n = c->width;
             q.k = cols;
             q.a = g;
-            q.b[0] = part;
+            q.b[0] = q.b[1] = part;
+            q.pairs = planes;
             q.args.b_ready = 1;
             q.args.err = err;
             q.args.alpha = range ? range + 1 : nullptr;
@@ -205,7 +211,8 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
             q.n = c->width;
             q.k = c->n;
             q.a = g;
-            q.b[0] = x;
+            q.b[0] = q.b[1] = x;
+            q.pairs = planes;
             q.args.b_ready = 1;
             q.args.err = err;
             q.args.alpha = range ? range + 1 : nullptr;

@@ -90,6 +90,7 @@ struct alignas(64) ProductArgs {
     const float *stats, *dlogprob, *dentropy;      // GRAD: [M][2] log2 of the sum, entropy
     const float* scale;         // GRAD: a power of two that brings fp16 gradients into range, or NULL
     Planes grad;
+    int rest;                   // 16 bits: what rounding takes off the gradient is a second plane
 };
 
 // ---- instructions -----------------------------------------------------------------------------------------------------------
@@ -533,6 +534,14 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
                 for (int j = 0; j < 32; j++) v[j] = empty ? 0.f : v[j];
             }
             put_planes<FP32>(p.io, staging, lane, v, p.grad, row0, col, rows, cols);
+            if (!FP32 && p.rest) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const float near = p.io == FRNN_F16 ? __half2float(__float2half_rn(v[j])) : __bfloat162float(__float2bfloat16_rn(v[j]));
+                    v[j] = fabsf(near) < INFINITY ? v[j] - near : 0.f;
+                }
+                put_planes<FP32>(p.io, staging, lane, v, p.grad, row0 + p.M, col, rows, cols);      // (its rows follow the first plane's)
+            }
         });
     }
 }

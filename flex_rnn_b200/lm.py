@@ -96,7 +96,7 @@ def linear_logprobs(x: th.Tensor, weight: th.Tensor, tokens: th.Tensor, temperat
     The products run on the tensor cores, with sums in 32 bits (of fp32 as in ``gated_mlp``); the logits leave them a tile at a time and are not kept, and
     the backward computes them again, a piece of the vocabulary at a time (its workspace holds 2^28 of their gradients, in
     fp32 2^27, or 256 columns where there are more rows).  In bf16 and fp16 their gradient is rounded to that type before it
-    is multiplied with ``weight`` and ``x``.  Results are fp32 and both differentiable.  Tokens equal to ``ignore_index`` have
+    is multiplied with ``weight`` and ``x`` (up to 128 rows to twice its bits).  Results are fp32 and both differentiable.  Tokens equal to ``ignore_index`` have
     log probability 0 and no gradient through it; tokens outside the vocabulary have NaN, and the next call on that GPU raises
     ``FrnnError``."""
     _operators()

@@ -850,6 +850,26 @@ def test_compiled_for_any_batch(name):
         assert all(torch.equal(a, g) for a, g in zip(both(lambda *a: compiled(f, a), leaves, up), both(f, leaves, up)))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("n,V,D", [(1, 300, 64), (9, 3000, 383), (40, 1000, 72), (128, 515, 200)])
+def test_gradients_of_few_rows(n, V, D, dtype):
+    """Up to 128 rows the logits' gradient G is multiplied in two parts, 2^-16 of it (fp16: 2^-22, but not below its least number): beside the
+    result's rounding there are 2^-14 of |G| |W| and |G|^T |x|, in which logits' and sums' errors (2^-17 each) have room."""
+    x, w = rand(n, D).to(dtype), rand(V, D, scale=D ** -0.5).to(dtype)
+    t, g, h = torch.arange(n).cuda() * 7 % V, rand(n, seed=1), rand(n, seed=2, scale=0.01)
+    t[n // 2] = -100
+    leaves = [v.requires_grad_() for v in (x, w)]
+    exact = [v.detach().double().requires_grad_() for v in leaves]
+    r = fr.linear_logprobs(*leaves, t, temperature=0.7)
+    got = torch.autograd.grad([r.logprob, r.entropy], leaves, [g, h])
+    logits = (exact[0] @ exact[1].t()).detach().requires_grad_()
+    s = lm.naive_token_logprobs(logits, t, 0, 0.7)
+    G, = torch.autograd.grad([s[0], s[1]], logits, [g.double(), h.double()])
+    for a, b, size in ((got[0], G @ exact[1], G.abs() @ exact[1].abs()), (got[1], G.t() @ exact[0], G.abs().t() @ exact[0].abs())):
+        within(a, b.detach(), 2.0 ** -14 * size.detach())
+
+
 def turned_from(device):
     """A compiled rotation of single tokens, as generation calls it, from many positions: two programs, not one for each."""
     lm._operators()
