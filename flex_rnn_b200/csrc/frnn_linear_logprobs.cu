@@ -76,19 +76,23 @@ __global__ void __launch_bounds__(JOIN_ROWS* JOIN_SLICES) join_kernel(const floa
 }
 
 // A power of two that brings the logits' gradient, at most (|g| + (ln V + 1) |h|) / T, up to 2^13, and its inverse: fp16 has
-// normal numbers from 2^-14 to 2^16, and most of the gradient lies many powers below its largest values.
-__global__ void __launch_bounds__(1024) range_kernel(const float* g, const float* h, int64_t n, float inv_t, float* out) {
+// normal numbers from 2^-14 to 2^16, and most of the gradient lies many powers below its largest values.  Counted is what reaches
+// the logits: g only where the token is not ignored (whatever stands there, it is no gradient), and no row whose gradients are not
+// finite (its own results are lost at any scale, the other rows' are not).
+__global__ void __launch_bounds__(1024) range_kernel(const float* g, const float* h, const void* tokens, int token_bytes, int64_t ignore_index, int64_t n, float inv_t, float* out) {
     __shared__ float part[32];
     float most = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) most = fmaxf(most, (g ? fabsf(g[i]) : 0.f) + 23.f * (h ? fabsf(h[i]) : 0.f));
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const float a = g && token_at(tokens, token_bytes, i) != ignore_index ? fabsf(g[i]) : 0.f, b = (a + 23.f * (h ? fabsf(h[i]) : 0.f)) * inv_t;
+        if (b < INFINITY) most = fmaxf(most, b);
+    }
     for (int d = 16; d; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = most;
     __syncthreads();
     if (threadIdx.x) return;
     for (int i = 1; i < 32; i++) most = fmaxf(most, part[i]);
-    most *= inv_t;
     int e = 0;
-    if (most > 0.f && most < INFINITY) e = max(-100, min(100, 13 - ilogbf(most)));
+    if (most > 0.f) e = max(-100, min(100, 13 - ilogbf(most)));
     out[0] = ldexpf(1.f, e);
     out[1] = ldexpf(1.f, -e);
 }
@@ -161,7 +165,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
     int rc = count ? (int)FRNN_OK : pack(packs, c->dtype, stream);
     if (rc != FRNN_OK) return rc;
     if (range && !count) {
-        range_kernel<<<1, 1024, 0, stream>>>(dlogprob, dentropy, c->n, (float)(1.0 / c->temperature), range);
+        range_kernel<<<1, 1024, 0, stream>>>(dlogprob, dentropy, c->tokens, c->token_bytes, c->ignore_index, c->n, (float)(1.0 / c->temperature), range);
         rc = launched(what);
         if (rc != FRNN_OK) return rc;
     }
