@@ -124,7 +124,7 @@ template <int CG> __device__ __forceinline__ void tma_load(u32 dst, const CUtens
 __device__ __forceinline__ void send(u32 dst, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
-// an arrival that says that what this warp has sent is there
+// an arrival that says that what this warp has done in shared memory, its own block's or another's, is done
 __device__ __forceinline__ void arrive_after_sending(u32 bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void arrive_at(u32 bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A bounded wait (as frnn_mbar_wait) on a barrier given by its address; CLUSTER: for what other blocks of the cluster have written.
@@ -872,9 +872,12 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool FP32> __global__
                             frnn_tmem_st<32>(place, v);
                             frnn_tmem_wait_st();
                         }
+                        // The others may write here again, what has been read and (SHARE) staged here lies before that: a release to the cluster, which their
+                        // wait acquires.  It waits for this warp's stores of the tile, so it comes only where another round does.
                         auto done_with = [&] {
+                            if (u + stride >= tiles) return;
                             __syncwarp();
-                            if (lane < (int)blocks) arrive_at(in_block(&taken, lane));
+                            if (lane < (int)blocks) arrive_after_sending(in_block(&taken, lane));
                         };
                         if constexpr (SHARE) {
                             met(&summed);

@@ -6,7 +6,7 @@ import torch
 
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm
-from test_block import DTYPES, UNIT, logprobs_case, lost, rand
+from test_block import DTYPES, logprobs_case, mlp_case, mlp_check
 
 
 # ---- log probabilities without logits: upstream gradients ------------------------------------------------------------------------
@@ -51,3 +51,18 @@ def test_upstream_gradients_that_are_not_finite(n, dtype):
             other[k][~rows] = bad
             dx, _ = logprobs_grads(x, w, t, other)
             assert torch.equal(dx[rows], want[rows]) and not torch.isfinite(dx[~rows]).any()
+
+
+# ---- products by clusters -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n,D,F,O", [(torch.bfloat16, 16, 4096, 12288, 64), (torch.float16, 30, 4096, 11000, 72), (torch.float32, 16, 4096, 12288, 64), (torch.float32, 1000, 2000, 2500, 300), (torch.float32, 300, 1024, 4096, 64)])
+def test_clusters_with_several_tiles(dtype, n, D, F, O):
+    """More tiles than clusters that run at once: a block's exchange buffer is used again, by its neighbours, after it has read it.  Right, and the
+    same bits every time."""
+    tensors, dy = mlp_case(n, D, F, O, dtype)
+    want = mlp_check(tensors, dy)
+    leaves = [v.requires_grad_() for v in tensors]
+    for _ in range(20):
+        y = fr.gated_mlp(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip([y, *torch.autograd.grad(y, leaves, dy)], want))
