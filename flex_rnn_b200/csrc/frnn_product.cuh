@@ -57,7 +57,7 @@ struct Planes {
 struct alignas(64) ProductArgs {
     CUtensorMap a, b[2];
     int M, N;                   // rows and columns of the result (N: of each of the two products where dual)
-    int flush;                  // PROMOTE: steps along k of a part
+    int flush;                  // steps along k of a part
     int pairs;                  // products that are added up
     int ksteps, segments;       // steps of 64 along k in a segment; segments: pairs, where fp32 takes one product a step six times as many
     int tiles_m, tiles_n, group, slices;      // slices of k, each with a result of its own (STORE)
@@ -338,11 +338,13 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 
 // The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last bit, all in
 // one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096 in 16 bits, 2e-5 at 8192 in fp32, where 32-bit sums rounded to
-// nearest lose some 9e-7).  Results that are held to 32 bits (PROMOTE) are summed by the epilogue's warps instead, in registers, half of a
-// tile's columns a warp, from parts of `flush` steps; the sums go back to where the last part was, and the epilogue is the same for
-// all.  (One that took them from registers had its loops unrolled, and its code did not fit the instruction cache.)  fp32 where a step is
-// six products: parts of one, whose small products come first, while the accumulator is small: 3e-7 (of two steps 1.6e-6 and 4 % faster); fp32 in SPLIT:
-// parts of 4, 6e-7; fp32 results of 16-bit operands: of 16, 4e-7.
+// nearest lose some 9e-7).  So sums along k come in parts of `flush` steps, which the epilogue's warps add up in registers, half of a
+// tile's columns a warp; the sums go back to where the last part was, and the epilogue is the same for all.  (One that took them
+// from registers had its loops unrolled, and its code did not fit the instruction cache.)  Results in 16 bits: parts of 64 steps, so that no length of k
+// loses more than those 7e-6 beside a rounding of 2e-4 (a vocabulary of 150000 in one part: 2.6e-4).  Log probabilities of 16-bit operands: of 16, 4e-7, and
+// the same in their backward, because a probability is an exponential of the difference between its logits and the forward's log of
+// the sum.  fp32 where a step is six products: parts of one, whose small products come first, while the accumulator is small: 3e-7 (of two steps
+// 1.6e-6 and 4 % faster); fp32 in SPLIT: parts of 4, 6e-7.
 
 // 32 columns of accumulators, of the lane's row.  (Waited for apart: the next ones are under way while these are worked on.)
 __device__ __forceinline__ void ask(u32 taddr, float* v) { frnn_tmem_ld<32>(taddr, v); }
@@ -576,7 +578,6 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int u, u32 part, u
 
 // AT, BT: the operand's rows run along m (n) instead of k.
 template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool FP32> __global__ void __launch_bounds__(PRODUCT_THREADS, 1) product_kernel(const __grid_constant__ ProductArgs p) {
-    constexpr bool PROMOTE = FP32 || EPI == LOGPROB_STATS;      // (its results are fp32 whatever the operands are)
     // fp32: a step copies three planes of each operand and multiplies them six times; in SPLIT, whose stages hold no two such steps, it is one
     // product of two planes, and the six follow one another over all of k
     constexpr bool FUSED = FP32 && (FORM != SPLIT || THIN);
@@ -724,7 +725,7 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool FP32> __global__
                 for (int u = first; ok && u < tiles; u += stride) {
                     const Tile w = tile_of(p, u, part, parts);
                     for (int from = w.from; ok && from < w.to; t++) {
-                        const int to = PROMOTE ? min(from + p.flush, w.to) : w.to;
+                        const int to = min(from + p.flush, w.to);
                         const u32 buf = t & 1, d = tmem + buf * BN;
                         if (!(ok = wait_at(frnn_smem_addr(&acc_empty[buf]), (t / 2 & 1) ^ 1, p.err))) break;
                         frnn_tmem_fence_after_sync();
@@ -810,97 +811,95 @@ template <Form FORM, bool THIN, bool AT, bool BT, int EPI, bool FP32> __global__
             }
             u32 acc = filled();
             if (!ok) break;
-            if constexpr (PROMOTE || FORM == SPLIT) {
-                if (FORM == SPLIT || w.from + p.flush < w.to) {
-                    float sum[BN / 2];
+            if (FORM == SPLIT || w.from + p.flush < w.to) {
+                float sum[BN / 2];
 #pragma unroll
-                    for (int i = 0; i < BN / 2; i += 32) ask(acc + half * (BN / 2) + i, sum + i);
-                    wait_for<BN / 2>(sum);
-                    for (int from = w.from + p.flush; PROMOTE && from < w.to; from += p.flush) {
-                        emptied();
-                        acc = filled();
-                        if (!ok) break;
-#pragma unroll
-                        for (int i = 0; i < BN / 2; i += 32) {
-                            float v[32];
-                            ask(acc + half * (BN / 2) + i, v);
-                            wait_for<32>(v);
-#pragma unroll
-                            for (int j = 0; j < 32; j++) sum[i + j] += v[j];
-                        }
-                    }
+                for (int i = 0; i < BN / 2; i += 32) ask(acc + half * (BN / 2) + i, sum + i);
+                wait_for<BN / 2>(sum);
+                for (int from = w.from + p.flush; from < w.to; from += p.flush) {
+                    emptied();
+                    acc = filled();
                     if (!ok) break;
-                    if constexpr (FORM == SPLIT) {
-                        emptied();
-                        // to the owners: of every block's columns those that this warp has, four at a time
-                        const int own = BN / (int)blocks, row = quarter * 32 + lane;      // (own: a power of two)
-                        ok = __all_sync(0xffffffffu, wait_at<true>(frnn_smem_addr(&taken), (round & 1) ^ 1, p.err));
-                        if (!ok) break;
 #pragma unroll
-                        for (int i = 0; i < BN / 2 && !idle; i += 4) {
-                            const int c = half * (BN / 2) + i;
-                            int owner, at;
-                            if (EPI == GLU_FORWARD) {      // (an owner has the same columns of both products)
-                                owner = i >> (__ffs(own) - 2);
-                                at = (i & (own / 2 - 1)) + half * (own / 2);
-                            } else {
-                                owner = c >> (__ffs(own) - 1);
-                                at = c & (own - 1);
-                            }
-                            send(in_block(&exchange[((int)rank * own + at) / 4 * ROWS + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
-                        }
-                        __syncwarp();
-                        if (lane < (int)blocks) arrive_after_sending(in_block(&arrived, lane));
-                        ok = __all_sync(0xffffffffu, wait_at<true>(frnn_smem_addr(&arrived), round & 1, p.err));
-                        if (!ok) break;
-                        // the owner's columns: half of them each, but whole accesses of 8 (both products' of GLU_FORWARD)
-                        const int width = EPI == GLU_FORWARD ? own / 2 : own, count = max(8, width / 2), from = half * count;
-                        const u32 place = tmem + 2 * BN + frnn_tmem_lane_base(quarter) + half * 64;
-                        const bool works = from < width && !idle && row0 < p.M;
-                        if (works) {
-                            const int values = (EPI == GLU_FORWARD ? 2 : 1) * count;
-                            float v[32] = {};
-                            for (u32 b = 0; b < blocks; b++) {
+                    for (int i = 0; i < BN / 2; i += 32) {
+                        float v[32];
+                        ask(acc + half * (BN / 2) + i, v);
+                        wait_for<32>(v);
 #pragma unroll
-                                for (int i = 0; i < 32; i += 4) {
-                                    if (i >= values) continue;
-                                    const int at = i < count ? from + i : own / 2 + from + i - count;
-                                    const float4 x = exchange[((int)b * own + at) / 4 * ROWS + row];
-                                    v[i] += x.x; v[i + 1] += x.y; v[i + 2] += x.z; v[i + 3] += x.w;
-                                }
-                            }
-                            frnn_tmem_st<32>(place, v);
-                            frnn_tmem_wait_st();
-                        }
-                        // The others may write here again, what has been read and (SHARE) staged here lies before that: a release to the cluster, which their
-                        // wait acquires.  It waits for this warp's stores of the tile, so it comes only where another round does.
-                        auto done_with = [&] {
-                            if (u + stride >= tiles) return;
-                            __syncwarp();
-                            if (lane < (int)blocks) arrive_after_sending(in_block(&taken, lane));
-                        };
-                        if constexpr (SHARE) {
-                            met(&summed);
-                            if (!ok) break;
+                        for (int j = 0; j < 32; j++) sum[i + j] += v[j];
+                    }
+                }
+                if (!ok) break;
+                if constexpr (FORM == SPLIT) {
+                    emptied();
+                    // to the owners: of every block's columns those that this warp has, four at a time
+                    const int own = BN / (int)blocks, row = quarter * 32 + lane;      // (own: a power of two)
+                    ok = __all_sync(0xffffffffu, wait_at<true>(frnn_smem_addr(&taken), (round & 1) ^ 1, p.err));
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < BN / 2 && !idle; i += 4) {
+                        const int c = half * (BN / 2) + i;
+                        int owner, at;
+                        if (EPI == GLU_FORWARD) {      // (an owner has the same columns of both products)
+                            owner = i >> (__ffs(own) - 2);
+                            at = (i & (own / 2 - 1)) + half * (own / 2);
                         } else {
-                            done_with();
+                            owner = c >> (__ffs(own) - 1);
+                            at = c & (own - 1);
                         }
-                        if (works) {
-                            const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
-                            epilogue<EPI, FP32>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
-                        }
-                        if constexpr (SHARE) done_with();
-                        continue;
-                    } else {
+                        send(in_block(&exchange[((int)rank * own + at) / 4 * ROWS + row], owner), sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+                    }
+                    __syncwarp();
+                    if (lane < (int)blocks) arrive_after_sending(in_block(&arrived, lane));
+                    ok = __all_sync(0xffffffffu, wait_at<true>(frnn_smem_addr(&arrived), round & 1, p.err));
+                    if (!ok) break;
+                    // the owner's columns: half of them each, but whole accesses of 8 (both products' of GLU_FORWARD)
+                    const int width = EPI == GLU_FORWARD ? own / 2 : own, count = max(8, width / 2), from = half * count;
+                    const u32 place = tmem + 2 * BN + frnn_tmem_lane_base(quarter) + half * 64;
+                    const bool works = from < width && !idle && row0 < p.M;
+                    if (works) {
+                        const int values = (EPI == GLU_FORWARD ? 2 : 1) * count;
+                        float v[32] = {};
+                        for (u32 b = 0; b < blocks; b++) {
 #pragma unroll
-                        for (int i = 0; i < BN / 2; i += 32) frnn_tmem_st<32>(acc + half * (BN / 2) + i, sum + i);
-                        frnn_tmem_wait_st();
-                        if constexpr (EPI == GLU_FORWARD) {      // (a warp's columns of the two products lie in both warps' halves)
-                            frnn_tmem_fence_before_sync();
-                            met(&halves[quarter]);
-                            frnn_tmem_fence_after_sync();
-                            if (!ok) break;
+                            for (int i = 0; i < 32; i += 4) {
+                                if (i >= values) continue;
+                                const int at = i < count ? from + i : own / 2 + from + i - count;
+                                const float4 x = exchange[((int)b * own + at) / 4 * ROWS + row];
+                                v[i] += x.x; v[i + 1] += x.y; v[i + 2] += x.z; v[i + 3] += x.w;
+                            }
                         }
+                        frnn_tmem_st<32>(place, v);
+                        frnn_tmem_wait_st();
+                    }
+                    // The others may write here again, what has been read and (SHARE) staged here lies before that: a release to the cluster, which their
+                    // wait acquires.  It waits for this warp's stores of the tile, so it comes only where another round does.
+                    auto done_with = [&] {
+                        if (u + stride >= tiles) return;
+                        __syncwarp();
+                        if (lane < (int)blocks) arrive_after_sending(in_block(&taken, lane));
+                    };
+                    if constexpr (SHARE) {
+                        met(&summed);
+                        if (!ok) break;
+                    } else {
+                        done_with();
+                    }
+                    if (works) {
+                        const int tile_col = w.tn * (EPI == GLU_FORWARD ? BN / 2 : BN) + (int)rank * width;
+                        epilogue<EPI, FP32>(p, data, place, place + count, row0, tile_col + from, count, w, lane, staging);
+                    }
+                    if constexpr (SHARE) done_with();
+                    continue;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < BN / 2; i += 32) frnn_tmem_st<32>(acc + half * (BN / 2) + i, sum + i);
+                    frnn_tmem_wait_st();
+                    if constexpr (EPI == GLU_FORWARD) {      // (a warp's columns of the two products lie in both warps' halves)
+                        frnn_tmem_fence_before_sync();
+                        met(&halves[quarter]);
+                        frnn_tmem_fence_after_sync();
+                        if (!ok) break;
                     }
                 }
             }
@@ -1188,7 +1187,7 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     const bool thin = is_thin(q, AT, plan.form), fp32 = q.dtype == FRNN_F32, fused = fp32 && (plan.form != SPLIT || thin);
     p.pairs = q.pairs;
     p.segments = q.pairs * (fp32 && !fused ? 6 : 1);
-    p.flush = fused ? 1 : fp32 ? 4 : 16;
+    p.flush = fused ? 1 : fp32 ? 4 : EPI == LOGPROB_STATS || EPI == LOGPROB_GRAD ? 16 : 64;
     if ((int64_t)p.ksteps * p.segments >= (1ll << 31) - 64) return frnn_fail(FRNN_E_ARG, "%s: too long", what);
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);

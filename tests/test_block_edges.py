@@ -66,3 +66,51 @@ def test_clusters_with_several_tiles(dtype, n, D, F, O):
     for _ in range(20):
         y = fr.gated_mlp(*leaves)
         assert all(torch.equal(a, b) for a, b in zip([y, *torch.autograd.grad(y, leaves, dy)], want))
+
+
+# ---- sums along k ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [9000, 100000])
+def test_long_sums_in_16_bits_lean_to_neither_side(k, dtype):
+    """Accumulators truncate: a unit of the last place at most of the sum so far for each 16 values, in the mean half a unit of half the
+    sum.  That is 256 times 2^-25 in a part of 64 steps of 64 values, 2^-17 of the result, whatever k; without parts k / 16 times 2^-25, at 100000 1.9e-4.
+    All terms here are positive, so that the loss is on one side and shows in the mean over the results.  These are not independent in their roundings:
+    a row's results lie within k^-1/2 of one another, in bf16 less than a step (of 15 different x0 there is 3.4e-4 in the mean of the exact results'
+    roundings alone).  So they are compared with the exact results rounded to the same type: of those a part s (steps a result) that lies within the shift
+    from a border goes one step, which in the mean is the shift again, times at most 0.4 steps over the spread's k^-1/2 where a border cuts the middle of
+    them (bf16, k = 100000: 1.0): 2^-16 is twice what the parts lose.  (The hidden vectors are exact: relu(1) times whole numbers up to 225.  There
+    are results enough that k is not cut into slices.)"""
+    n, D, O = 2100, 8, 2048
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, gate, up = (torch.zeros(m, D, device="cuda") for m in (n, k, k))
+    x[:, 0], up[:, 0] = torch.randint(1, 16, (n,), generator=g, device="cuda"), torch.randint(1, 16, (k,), generator=g, device="cuda")
+    x[:, 1], gate[:, 1] = 1.0, 1.0
+    down = (torch.rand(O, k, generator=g, device="cuda") + 0.5) * 2.0 ** -10
+    x, gate, up, down = (v.to(dtype) for v in (x, gate, up, down))
+    y = fr.gated_mlp(x, gate, up, down, activation="relu").double()
+    want = lm.naive_gated_mlp(*(v.double() for v in (x, gate, up, down)), "relu")
+    assert abs(float(((y - want.to(dtype).double()) / want).mean())) <= 2.0 ** -16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [30, 300])
+def test_gradients_of_confident_rows(n, dtype):
+    """Tokens whose probability is near 1, from long sums: the gradient is in proportion to 1 - p, p = exp of the difference between a logit and the
+    log of the sum, and loses 1 / (1 - p) times what the two disagree by.  Logits are sums of positive terms, about 40; in parts of 1024 values each is
+    short by 2^-19 at most (64 times 2^-25, see above), so the two by 40 2^-19, and 1 - p = 1.2e-3 or more is off by 6.4 % at most."""
+    D, V = 16384, 1000
+    g = torch.Generator().manual_seed(4)
+    x, w = torch.rand(n, D, generator=g) + 0.5, torch.rand(V, D, generator=g) + 0.5
+    w *= 26.5 / D
+    w[7] *= 40 / 26.5
+    x, w = x.cuda().to(dtype), w.cuda().to(dtype)
+    t = torch.full((n,), 7, device="cuda")
+    leaves, exact = [v.requires_grad_() for v in (x, w)], [v.detach().double().requires_grad_() for v in (x, w)]
+    got = torch.autograd.grad(fr.linear_logprobs(*leaves, t).logprob.sum(), leaves)
+    r = lm.naive_linear_logprobs(*exact, t)
+    assert 2e-4 < float(-r.logprob.detach().mean()) < 5e-3
+    for a, b in zip(got, torch.autograd.grad(r.logprob.sum(), exact)):
+        assert float((a.double() - b).norm()) <= 0.07 * float(b.norm())
