@@ -2,7 +2,7 @@
 //
 // With u = log2(e) / T x W^T, of each row in blocks of columns: m = max u, s = sum 2^(u - m), t = sum 2^(u - m) (u - m), from
 // the tile that leaves Tensor Memory; a second kernel joins the blocks:
-//   log p[token] = ln 2 (u[token] - m - log2 s),   H = ln 2 (log2 s - t / s)
+//   log p[token] = ln 2 ((u[token] - m) - log2 s),   H = ln 2 (log2 s - t / s)
 // Backward, a piece of the vocabulary at a time: the logits again, their gradient
 //   G = (g (1[v = token] - p) - h p (ln p + H)) / T
 // as a 16-bit operand, dx += G W, dW of the piece = G^T x.  2 n V D operations forward, 6 n V D backward (2 of them for the
@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(JOIN_ROWS* JOIN_SLICES) join_kernel(const floa
     float lp = 0.f;
     if (token != ignore_index) {
         const bool inside = token >= 0 && token < vocab;
-        lp = inside ? (empty ? -INFINITY : 0.69314718055994531f * (target[row] - lse2)) : NAN;
+        // (u - m first: of the likeliest token it is 0, and what is left as exact as s, whatever m; from lse2, at m of some tens, 2^-19 is lost)
+        lp = inside ? (empty ? -INFINITY : 0.69314718055994531f * ((target[row] - m) - log2f(s))) : NAN;
         if (!inside) frnn_report(err, CODE_TOKEN);
     }
     logprob[row] = lp;

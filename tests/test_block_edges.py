@@ -114,3 +114,21 @@ def test_gradients_of_confident_rows(n, dtype):
     assert 2e-4 < float(-r.logprob.detach().mean()) < 5e-3
     for a, b in zip(got, torch.autograd.grad(r.logprob.sum(), exact)):
         assert float((a.double() - b).norm()) <= 0.07 * float(b.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [5, 300, 3000])
+def test_log_probabilities_near_zero(n, dtype):
+    """The log probability of the likeliest token, -log(1 + rest), has the rounding of 1 + rest and an exponential's error of the rest, whatever the
+    logits' size: logits are whole numbers here (width 1), exact in every type."""
+    V = 700
+    w = torch.zeros(V, 1, device="cuda")
+    w[3], w[11] = 1.0, 0.875
+    for size in (16.0, 64.0, 96.0, 200.0):
+        x = torch.full((n, 1), size, device="cuda")
+        r = fr.linear_logprobs(x.to(dtype), w.to(dtype), torch.full((n,), 3, device="cuda"))
+        want = lm.naive_linear_logprobs(x.double(), w.double(), torch.full((n,), 3, device="cuda"))
+        # rest = exp(-size / 8) + 698 exp(-size): 2^-24 of size for each of both logits' roundings after their factor, and of their difference's; 2^-21 of an exponential
+        rest = math.exp(-size / 8)
+        assert float((r.logprob.double() - want.logprob).abs().max()) <= 2.0 ** -22 + (size * 2.0 ** -22 + 2.0 ** -21) * rest
