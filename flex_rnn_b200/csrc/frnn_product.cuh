@@ -341,8 +341,9 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 // nearest lose some 9e-7).  So sums along k come in parts of `flush` steps, which the epilogue's warps add up in registers, half of a
 // tile's columns a warp; the sums go back to where the last part was, and the epilogue is the same for all.  (One that took them
 // from registers had its loops unrolled, and its code did not fit the instruction cache.)  Results in 16 bits: parts of 64 steps, so that no length of k
-// loses more than those 7e-6 beside a rounding of 2e-4 (a vocabulary of 150000 in one part: 2.6e-4).  Log probabilities of 16-bit operands: of 16, 4e-7, and
-// the same in their backward, because a probability is an exponential of the difference between its logits and the forward's log of
+// loses more than those 7e-6 (of positive terms 2.4e-5) beside a rounding of 2e-4 (a vocabulary of 150000 in one part: 2.6e-4).  Log probabilities of 16-bit operands: of 16, 4e-7
+// (up to 128 rows, which wait for weights and not for the epilogue, of 4: 16 rows of 4096 against
+// 65536 tokens 6.3e-7 -> 9e-8 for 104 -> 107 us), and the same in their backward, because a probability is an exponential of the difference between its logits and the forward's log of
 // the sum.  fp32 where a step is six products: parts of one, whose small products come first, while the accumulator is small: 3e-7 (of two steps
 // 1.6e-6 and 4 % faster); fp32 in SPLIT: parts of 4, 6e-7.
 
@@ -1187,7 +1188,7 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     const bool thin = is_thin(q, AT, plan.form), fp32 = q.dtype == FRNN_F32, fused = fp32 && (plan.form != SPLIT || thin);
     p.pairs = q.pairs;
     p.segments = q.pairs * (fp32 && !fused ? 6 : 1);
-    p.flush = fused ? 1 : fp32 ? 4 : EPI == LOGPROB_STATS || EPI == LOGPROB_GRAD ? 16 : 64;
+    p.flush = fused ? 1 : fp32 ? 4 : EPI != LOGPROB_STATS && EPI != LOGPROB_GRAD ? 64 : q.m <= 128 ? 4 : 16;
     if ((int64_t)p.ksteps * p.segments >= (1ll << 31) - 64) return frnn_fail(FRNN_E_ARG, "%s: too long", what);
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);

@@ -75,7 +75,7 @@ def test_clusters_with_several_tiles(dtype, n, D, F, O):
 @pytest.mark.parametrize("k", [9000, 100000])
 def test_long_sums_in_16_bits_lean_to_neither_side(k, dtype):
     """Accumulators truncate: a unit of the last place at most of the sum so far for each 16 values, in the mean half a unit of half the
-    sum.  That is 256 times 2^-25 in a part of 64 steps of 64 values, 2^-17 of the result, whatever k; without parts k / 16 times 2^-25, at 100000 1.9e-4.
+    sum (and the products' own alignment, which of 8 by 11 bits loses hardly any).  That is 256 times 2^-25 in a part of 64 steps of 64 values, 2^-17 of the result, whatever k; without parts k / 16 times 2^-25, at 100000 1.9e-4.
     All terms here are positive, so that the loss is on one side and shows in the mean over the results.  These are not independent in their roundings:
     a row's results lie within k^-1/2 of one another, in bf16 less than a step (of 15 different x0 there is 3.4e-4 in the mean of the exact results'
     roundings alone).  So they are compared with the exact results rounded to the same type: of those a part s (steps a result) that lies within the shift
@@ -132,3 +132,19 @@ def test_log_probabilities_near_zero(n, dtype):
         # rest = exp(-size / 8) + 698 exp(-size): 2^-24 of size for each of both logits' roundings after their factor, and of their difference's; 2^-21 of an exponential
         rest = math.exp(-size / 8)
         assert float((r.logprob.double() - want.logprob).abs().max()) <= 2.0 ** -22 + (size * 2.0 ** -22 + 2.0 ** -21) * rest
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,parts", [(1, 2.0 ** -19), (16, 2.0 ** -19), (128, 2.0 ** -19), (300, 2.0 ** -17)])
+def test_logits_of_16_bit_operands(n, parts, dtype):
+    """Long sums of positive terms.  An instruction loses two units of the last place at most (test_block), 2^-22 of the part's sum so far, which is half
+    of the whole in the mean: 16 times 2^-23 in parts of 4 steps (up to 128 rows), 64 times in parts of 16.  Of two logits, z and 0, the log
+    probability of the second is -log(1 + exp(z)), -z for z of 20."""
+    D = 16384
+    g = torch.Generator().manual_seed(5)
+    x, w = (torch.rand(n, D, generator=g) + 0.5).cuda().to(dtype), torch.zeros(2, D)
+    w[0] = (torch.rand(D, generator=g) + 0.5) * 20 / D
+    w, t = w.cuda().to(dtype), torch.ones(n, dtype=torch.int64, device="cuda")
+    want = lm.naive_linear_logprobs(x.double(), w.double(), t).logprob
+    assert abs(float(((fr.linear_logprobs(x, w, t).logprob.double() - want) / want).mean())) <= parts
