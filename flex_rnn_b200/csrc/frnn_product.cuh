@@ -518,7 +518,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& p, const RowData& da
         const int64_t token = data.token;
         const float lse2 = data.lse2, entropy = data.entropy, g = token != p.ignore_index ? data.g : 0.f, h = data.h;
         const bool empty = lse2 == -INFINITY;
-        const float k = p.inv_t * (p.scale ? *p.scale : 1.f), gk = -g * k, hk = -h * k;
+        const float scale = p.scale ? *p.scale : 1.f, gk = -g * p.inv_t * scale, hk = -h * p.inv_t * scale;      // (g first: 1 / T alone times the factor may pass 2^128)
         each([&](int col, int cols, float* v) {
             if (rows <= 0 || cols <= 0) return;
             const int64_t hit = token - p.first - col;

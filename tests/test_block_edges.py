@@ -6,7 +6,7 @@ import torch
 
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm
-from test_block import DTYPES, logprobs_case, mlp_case, mlp_check
+from test_block import DTYPES, TINY, UNIT, logprobs_case, mlp_case, mlp_check
 
 
 # ---- log probabilities without logits: upstream gradients ------------------------------------------------------------------------
@@ -148,3 +148,23 @@ def test_logits_of_16_bit_operands(n, parts, dtype):
     w, t = w.cuda().to(dtype), torch.ones(n, dtype=torch.int64, device="cuda")
     want = lm.naive_linear_logprobs(x.double(), w.double(), t).logprob
     assert abs(float(((fr.linear_logprobs(x, w, t).logprob.double() - want) / want).mean())) <= parts
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [60, 300])
+def test_gradients_at_the_least_temperature(n, dtype):
+    """1 / T and fp16's factor for small gradients are each in range where their product is not.  Logits are 0: of x the weight's zeros see the only
+    column that is not 0.  Errors in norm: UNIT for the rounding of the logits' gradient and of the result, and half of fp16's least number (2^-24) for each
+    result that is not 0: the weight's gradients, sums of 3e-36 / T / 700 and the like, lie at that number."""
+    x, w, t, up = logprobs_case(n, 700, 64, dtype, seed=11)
+    x.zero_()
+    x[:, 0] = 1
+    w *= 32
+    w[:, 0] = 0
+    up = [3e-36 * u.clamp(-3, 3) for u in up]
+    exact = [v.detach().double().requires_grad_() for v in (x, w)]
+    T = float(torch.tensor(1e-30))
+    want = torch.autograd.grad(lm.naive_linear_logprobs(*exact, t, T), exact, [u.double() for u in up])
+    for a, b in zip(logprobs_grads(x, w, t, up, temperature=1e-30), want):
+        assert float((a.double() - b).norm()) <= (2 * UNIT[dtype] + 2.0 ** -18) * float(b.norm()) + (TINY[dtype] / 2) * float((b != 0).sum()) ** 0.5
