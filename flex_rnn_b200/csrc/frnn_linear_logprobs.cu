@@ -132,20 +132,31 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
     const char* what = "linear_logprobs";
     Packs packs = {};
     const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), w = as_operand(s, packs, c->dtype, c->weight, c->vocab, c->width, c->weight_stride);
-    Product q = logits(c, x, w, 0, err);
-    const ProductPlan plan = plan_product<LOGPROB_STATS, false, false>(q);
-    const int64_t blocks = plan.tiles_n * (plan.form == PAIR ? 256 : 128) / plan.columns();
-    q.args.partial = (float*)s.take((size_t)blocks * 3 * c->n * 4);
-    q.args.target = (float*)s.take((size_t)c->n * 4);
-    if (!s.base) return FRNN_OK;
-    int rc = pack(packs, c->dtype, stream);
-    if (rc == FRNN_OK) rc = run_product<LOGPROB_STATS, false, false>(what, q, s, stream);
-    if (rc != FRNN_OK) return rc;
-    auto join = [&](auto kernel, int rows, int slices) {
-        return launch(what, kernel, dim3((unsigned)((c->n + rows - 1) / rows)), rows * slices, 0, stream, true, 1, q.args.partial, q.args.target, blocks, c->n, c->tokens, c->token_bytes, c->vocab,
-                      c->ignore_index, logprob, entropy, stats, err);
-    };
-    return c->n >= 2048 ? join(join_kernel<32, 16>, 32, 16) : join(join_kernel<8, 128>, 8, 128);
+    // pieces of rows whose partial results, 12 bytes for each row and 64 columns, take 256 MB (of large tiles, for each 128 columns, 128 MB)
+    const int64_t most = std::max<int64_t>(256, (1ll << 28) / (24 * ((c->vocab + 127) / 128)) / 256 * 256), pieces = (c->n + most - 1) / most;
+    const int64_t piece = pieces == 1 ? c->n : ((c->n + pieces - 1) / pieces + 255) / 256 * 256;
+    int rc = s.base ? pack(packs, c->dtype, stream) : (int)FRNN_OK;
+    const size_t kept = s.used;
+    for (int64_t r = 0; r < c->n && rc == FRNN_OK; r += piece) {
+        s.used = kept;
+        frnn_linear_logprobs_call some = *c;
+        some.n = std::min(piece, c->n - r);
+        some.tokens = (const char*)c->tokens + r * c->token_bytes;
+        Product q = logits(&some, x.from_row(r, some.n), w, 0, err);
+        const ProductPlan plan = plan_product<LOGPROB_STATS, false, false>(q);
+        const int64_t blocks = plan.tiles_n * (plan.form == PAIR ? 256 : 128) / plan.columns();
+        q.args.partial = (float*)s.take((size_t)blocks * 3 * some.n * 4);
+        q.args.target = (float*)s.take((size_t)some.n * 4);
+        if (!s.base) continue;
+        rc = run_product<LOGPROB_STATS, false, false>(what, q, s, stream);
+        if (rc != FRNN_OK) return rc;
+        auto join = [&](auto kernel, int rows, int slices) {
+            return launch(what, kernel, dim3((unsigned)((some.n + rows - 1) / rows)), rows * slices, 0, stream, true, 1, q.args.partial, q.args.target, blocks, some.n, some.tokens, c->token_bytes, c->vocab,
+                          c->ignore_index, logprob + r, entropy + r, stats ? stats + 2 * r : nullptr, err);
+        };
+        rc = some.n >= 2048 ? join(join_kernel<32, 16>, 32, 16) : join(join_kernel<8, 128>, 8, 128);
+    }
+    return rc;
 }
 
 int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const float* dentropy, const float* stats, void* dx, void* dweight, Scratch& s, int* err, cudaStream_t stream) {

@@ -1,12 +1,13 @@
 """Calls of gated_mlp, linear_logprobs and rotary (flex_rnn_b200.lm) at their edges; tolerances are those of test_block."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import flex_rnn_b200 as fr
-from flex_rnn_b200 import lm
-from test_block import DTYPES, TINY, UNIT, logprobs_case, mlp_case, mlp_check
+from flex_rnn_b200 import lm, runtime
+from test_block import DTYPES, TINY, UNIT, logprobs_case, logprobs_exact, mlp_case, mlp_check, rand, within
 
 
 # ---- log probabilities without logits: upstream gradients ------------------------------------------------------------------------
@@ -168,3 +169,38 @@ def test_gradients_at_the_least_temperature(n, dtype):
     want = torch.autograd.grad(lm.naive_linear_logprobs(*exact, t, T), exact, [u.double() for u in up])
     for a, b in zip(logprobs_grads(x, w, t, up, temperature=1e-30), want):
         assert float((a.double() - b).norm()) <= (2 * UNIT[dtype] + 2.0 ** -18) * float(b.norm()) + (TINY[dtype] / 2) * float((b != 0).sum()) ** 0.5
+
+
+# ---- log probabilities without logits: memory -----------------------------------------------------------------------------------------
+
+class Logprobs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("token_bytes", ctypes.c_int32), *[(k, ctypes.c_int64) for k in ("n", "vocab", "width")], ("x", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64), ("tokens", ctypes.c_void_p), ("ignore_index", ctypes.c_int64), ("temperature", ctypes.c_float)]
+
+
+def test_workspace_of_the_forward_is_bounded():
+    """What lies between the two kernels of a forward takes 256 MB at most (and 4 bytes a row), however many rows there are."""
+    workspace = runtime.lib().frnn_linear_logprobs_forward_workspace
+    workspace.restype = ctypes.c_size_t
+    for n in (1, 300, 20000, 262144, 2 ** 24):
+        for V in (1, 50257, 131072, 2 ** 20):
+            size = workspace(ctypes.byref(Logprobs(1, 8, n, V, 64, 4096, 4096, 64, 64, 4096, -100, 1.0)))
+            assert 0 < size <= 2 ** 28 + 2 ** 20 * 4 * 3 + 4 * n + 1024, (n, V, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_in_pieces(dtype):
+    """More rows than a forward takes at once: those of both pieces have their own tokens, and the results that they have alone."""
+    n, V, D = 15001, 100003, 24
+    x, w, t, _ = logprobs_case(n, V, D, dtype)
+    t[::7] = -100
+    leaf = x.requires_grad_()
+    r = fr.linear_logprobs(leaf, w, t)
+    g = rand(n, seed=12)
+    (dx,) = torch.autograd.grad(r.logprob, leaf, g)
+    for lo in range(0, n, 1500):
+        s = slice(lo, lo + 1500)
+        want, tol = logprobs_exact(x.detach()[s], w, t[s], [g[s], torch.zeros_like(g[s])], 1.0, -100)
+        for got, e, far in zip((r.logprob[s], r.entropy[s], dx[s]), want, tol):
+            within(got, e, far)
