@@ -26,8 +26,8 @@ scan = jit(gated_delta_rule)
 
 
 class Layer(nn.Module):
-    """x + W_out norm_of_heads(scan(projections of norm(x) at this place and the one before)).  Its state: the scan's, and
-    norm(x) of the last place.  ``turned`` values of each head's query and key carry rotary positions; with ``hidden``, a gated
+    """x + W_out norm_of_heads(scan(projections of norm(x) at this place and the one before)).  Its state: the scan's,
+    norm(x) of the last place, and the next place's position.  ``turned`` values of each head's query and key carry rotary positions; with ``hidden``, a gated
     feed-forward block of that many values follows: x + block(norm(x))."""
 
     def __init__(self, width: int, heads: int, head_width: int, hidden: int = 0, turned: int = 0):
@@ -46,10 +46,12 @@ class Layer(nn.Module):
             self.block_weight, self.block_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
             self.gate, self.up, self.down = nn.Linear(width, hidden, bias=False), nn.Linear(width, hidden, bias=False), nn.Linear(hidden, width, bias=False)
 
-    def forward(self, x, state, ops, position: int = 0):
+    def forward(self, x, state, ops, position: Optional[int] = None):
         B, T, _ = x.shape
         H, M = self.heads, self.head_width
-        state, last = state
+        state, last, *at = state          # (without a position: at the beginning)
+        if position is None:
+            position = at[0] if at else 0
         h = ops.layer_norm(x, self.norm_weight, self.norm_bias)
         before = torch.cat([last[:, None], h[:, :-1]], 1)
         q, k, v, g, beta = self.project(torch.cat([h, before], -1)).split([H * M, H * M, H * M, H, H], dim=-1)
@@ -66,7 +68,7 @@ class Layer(nn.Module):
         x = x + self.out(y.reshape(B, T, H * M))
         if self.hidden:
             x = x + ops.gated_mlp(ops.layer_norm(x, self.block_weight, self.block_bias), self.gate.weight, self.up.weight, self.down.weight)
-        return x, (state, h[:, -1])
+        return x, (state, h[:, -1], position + T)
 
 
 class _Fast:
@@ -97,14 +99,14 @@ class RecurrentLM(nn.Module):
         self.norm_weight, self.norm_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
         self.head = nn.Linear(width, vocabulary, bias=False)
 
-    def states(self, batch: int) -> List[Tuple[torch.Tensor, torch.Tensor]]:
+    def states(self, batch: int) -> List[Tuple[torch.Tensor, torch.Tensor, int]]:
         p = self.weight
         dtype = torch.promote_types(p.dtype, torch.float32)
-        return [(torch.zeros(batch, l.heads, l.head_width, l.head_width, dtype=dtype, device=p.device), p.new_zeros(batch, p.shape[1])) for l in self.layers]
+        return [(torch.zeros(batch, l.heads, l.head_width, l.head_width, dtype=dtype, device=p.device), p.new_zeros(batch, p.shape[1]), 0) for l in self.layers]
 
-    def features(self, tokens, states: Optional[list] = None, position: int = 0) -> Tuple[torch.Tensor, list]:
-        """tokens [B,T] (``-100``: padding, a zero input), the layers' states, the first token's position -> what the last
-        projection takes [B,T,width], new states"""
+    def features(self, tokens, states: Optional[list] = None, position: Optional[int] = None) -> Tuple[torch.Tensor, list]:
+        """tokens [B,T] (``-100``: padding, a zero input), the layers' states, the first token's position (default: the one after
+        those that the states have seen) -> what the last projection takes [B,T,width], new states"""
         states = self.states(tokens.shape[0]) if states is None else states
         x, new = self.ops.embedding(tokens, self.weight, scale=self.scale), []
         for layer, state in zip(self.layers, states):
@@ -112,7 +114,7 @@ class RecurrentLM(nn.Module):
             new.append(state)
         return self.ops.layer_norm(x, self.norm_weight, self.norm_bias), new
 
-    def forward(self, tokens, states: Optional[list] = None, position: int = 0) -> Tuple[torch.Tensor, list]:
+    def forward(self, tokens, states: Optional[list] = None, position: Optional[int] = None) -> Tuple[torch.Tensor, list]:
         """As ``features``, but with logits [B,T,vocabulary]."""
         x, new = self.features(tokens, states, position)
         return self.head(x), new
@@ -135,12 +137,12 @@ class RecurrentLM(nn.Module):
         """The most probable continuation, token by token, of prompt [B,T]: tokens [B,steps] and their log probabilities."""
         logits, states = self(prompt)
         last, tokens, logprobs = logits[:, -1], [], []
-        for step in range(steps):
+        for _ in range(steps):
             # (the alternatives come with the log probability of any token; 0 stands in for it)
             best = self.ops.token_logprobs(last, torch.zeros_like(prompt[:, 0]), top=1, temperature=temperature)
             tokens.append(best.top_token)
             logprobs.append(best.top_logprob)
-            logits, states = self(best.top_token, states, prompt.shape[1] + step)
+            logits, states = self(best.top_token, states)
             last = logits[:, 0]
         return torch.cat(tokens, 1), torch.cat(logprobs, 1)
 

@@ -7,6 +7,7 @@ import torch
 
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm, runtime
+from flex_rnn_b200.language_model import RecurrentLM, synthetic_text
 from test_block import DTYPES, TINY, UNIT, logprobs_case, logprobs_exact, mlp_case, mlp_check, rand, within
 
 
@@ -204,3 +205,23 @@ def test_rows_in_pieces(dtype):
         want, tol = logprobs_exact(x.detach()[s], w, t[s], [g[s], torch.zeros_like(g[s])], 1.0, -100)
         for got, e, far in zip((r.logprob[s], r.entropy[s], dx[s]), want, tol):
             within(got, e, far)
+
+
+# ---- the language model ---------------------------------------------------------------------------------------------------------------
+
+def test_positions_go_on_with_the_states():
+    """A text read in parts, each from the states of the one before, is the text read at once; a position that is given counts."""
+    torch.manual_seed(1)
+    model = RecurrentLM(97, width=48, layers=2, heads=3, head_width=16, plain=True, hidden=80, turned=12).double()
+    text = synthetic_text(3, 20, 97)
+    whole, _ = model(text)
+    states, parts = None, []
+    for part in text.split([1, 7, 1, 11], 1):
+        logits, states = model(part, states)
+        parts.append(logits)
+    assert torch.allclose(whole, torch.cat(parts, 1), atol=1e-10)
+    _, first = model(text[:, :9])
+    for position in (None, 9):
+        assert torch.allclose(model(text[:, 9:], first, position)[0], whole[:, 9:], atol=1e-10)
+    assert not torch.allclose(model(text[:, 9:], first, 0)[0], whole[:, 9:], atol=1e-3)
+    assert torch.equal(model(text, [s[:2] for s in model.states(3)])[0], whole)
