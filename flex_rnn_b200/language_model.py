@@ -40,11 +40,17 @@ class Layer(nn.Module):
         self.out = nn.Linear(n, width, bias=False)
         self.hidden, self.turned = hidden, turned
         if turned:
-            # (not a buffer: a model that changes its type keeps its frequencies in 64 bits)
+            # (no buffer: a model that changes its type keeps its frequencies in 64 bits; _apply takes them along)
             self.frequencies = lm.rotary_frequencies(turned, base=500.0)
         if hidden:
             self.block_weight, self.block_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
             self.gate, self.up, self.down = nn.Linear(width, hidden, bias=False), nn.Linear(width, hidden, bias=False), nn.Linear(hidden, width, bias=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        if self.turned:                   # (a copy from the host has no place in a call: that may be captured into a graph)
+            self.frequencies = lm.rotary_frequencies(self.turned, base=500.0).to(self.norm_weight.device)
+        return self
 
     def forward(self, x, state, ops, position: Optional[int] = None):
         B, T, _ = x.shape
@@ -60,8 +66,8 @@ class Layer(nn.Module):
         scalar = lambda t: torch.sigmoid(t).view(B, T, H, 1, 1)
         q, k = row(q), row(k)
         if self.turned:
-            self.frequencies = self.frequencies.to(x.device)
-            q, k = ops.rotary(q, position, self.frequencies), ops.rotary(k, position, self.frequencies)
+            f = self.frequencies.to(x.device)      # (there already, unless parameters were replaced one by one)
+            q, k = ops.rotary(q, position, f), ops.rotary(k, position, f)
         # states are kept in 32 bits from call to call; the outputs have their type
         y, state = ops.scan(q, k, v.reshape(B, T, H, M, 1), scalar(g + 3), scalar(beta), state)
         y = ops.layer_norm(y.to(x.dtype), self.head_weight, self.head_bias)

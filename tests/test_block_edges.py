@@ -225,3 +225,28 @@ def test_positions_go_on_with_the_states():
         assert torch.allclose(model(text[:, 9:], first, position)[0], whole[:, 9:], atol=1e-10)
     assert not torch.allclose(model(text[:, 9:], first, 0)[0], whole[:, 9:], atol=1e-3)
     assert torch.equal(model(text, [s[:2] for s in model.states(3)])[0], whole)
+
+
+def test_frequencies_move_with_the_model():
+    for device in ("meta", "cpu"):
+        for dtype in (torch.bfloat16, torch.float64):
+            layer = RecurrentLM(97, width=48, layers=1, heads=3, head_width=16, turned=12).to(device, dtype).layers[0]
+            assert layer.norm_weight.dtype == dtype and layer.frequencies.dtype == torch.float64 and layer.frequencies.device == layer.norm_weight.device
+    layer = RecurrentLM(97, width=48, layers=1, heads=3, head_width=16, turned=12).to("meta").to_empty(device="cpu").layers[0]
+    assert torch.equal(layer.frequencies, lm.rotary_frequencies(12, base=500.0))
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_model_in_a_graph():
+    """A model's first call is captured (the scan has been compiled before, by a model without positions)."""
+    make = lambda turned: RecurrentLM(97, width=48, layers=2, heads=3, head_width=16, hidden=80, turned=turned, keep_logits=False).cuda().bfloat16()
+    text = synthetic_text(4, 33, 97).clamp_min(0).cuda()
+    with torch.no_grad():
+        make(0).score(text)
+        torch.cuda.synchronize()
+        model = make(12)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = model.score(text)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, model.score(text)))
