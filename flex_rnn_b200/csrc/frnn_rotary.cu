@@ -6,7 +6,8 @@
 // the place's sines and cosines once, each a few, into a table in shared memory; a lane then keeps those of its E pairs in
 // registers for all heads that it passes, U of them at a time, whose loads are under way together and before the table is made.
 // Angles: position * frequency in 64 bits, taken modulo a turn there (a position of 10^6 at frequency 1 is 1.6 10^5 turns: in 32 bits
-// 2 % of a turn would be lost), then sine and cosine of the rest in 32 bits.
+// 2 % of a turn would be lost), then sine and cosine of the rest in 32 bits, corrected by what its rounding took off: fp32 results are within 4.5e-8 of
+// 64 bits in norm, without the correction 5.7e-8.  (Sines and cosines in 64 bits: 8 % less, but 1.3 % slower where a place has few heads' pairs to hide them.)
 #include <algorithm>
 
 #include "frnn_lm.cuh"
@@ -45,9 +46,11 @@ __device__ __forceinline__ void turn(double position, double frequency, float sc
     const double angle = position * frequency, whole = rint(angle * 0.15915494309189535);
     // (1 / (2 pi) as the sum of two numbers of 64 bits)
     const double rest = fma(angle, -9.839338337591243e-18, fma(angle, 0.15915494309189535, -whole));
-    sincospif(2.f * (float)rest, &s, &c);
-    c *= scale;
-    s *= scale * direction;
+    const float near = (float)rest, off = 6.2831853f * (float)(rest - near);
+    float c0, s0;
+    sincospif(2.f * near, &s0, &c0);
+    c = fmaf(-off, s0, c0) * scale;
+    s = fmaf(off, c0, s0) * (scale * direction);
 }
 
 template <class T, int E, bool INTERLEAVED> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {

@@ -250,3 +250,16 @@ def test_first_call_of_a_model_in_a_graph():
             got = model.score(text)
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, model.score(text)))
+
+
+# ---- rotary positions -----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start", [0, 10 ** 6])
+def test_rotations_in_fp32(start):
+    """Errors in norm, in units of 2^-24, of which a rounding is 0.42 (half a unit of the last place at most, uniform, over mantissas): the result's, half of
+    one for the product that is rounded, sine and cosine half a unit each: sqrt(0.42^2 (1 + 1 / 2) + 0.5^2) = 0.72.  The angle's rest adds nothing."""
+    x, f = rand(1, 4096, 2, 128), lm.rotary_frequencies(128, device="cuda")
+    for interleaved in (False, True):
+        want = lm.naive_rotary(x.double(), start, f, interleaved)
+        assert float((fr.rotary(x, start, f, interleaved).double() - want).norm()) <= 0.75 * 2.0 ** -24 * float(want.norm())
