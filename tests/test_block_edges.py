@@ -8,7 +8,7 @@ import torch
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm, runtime
 from flex_rnn_b200.language_model import RecurrentLM, synthetic_text
-from test_block import DTYPES, TINY, UNIT, logprobs_case, logprobs_exact, mlp_case, mlp_check, rand, within
+from test_block import DTYPES, TINY, UNIT, logprobs_case, logprobs_exact, mlp_case, mlp_check, near_in_norm, rand, within
 
 
 # ---- log probabilities without logits: upstream gradients ------------------------------------------------------------------------
@@ -263,3 +263,62 @@ def test_rotations_in_fp32(start):
     for interleaved in (False, True):
         want = lm.naive_rotary(x.double(), start, f, interleaved)
         assert float((fr.rotary(x, start, f, interleaved).double() - want).norm()) <= 0.75 * 2.0 ** -24 * float(want.norm())
+
+
+# ---- fp32 ------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,D,F,O,product", [(16, 1024, 2048, 1024, 3e-7), (300, 520, 1300, 520, 1e-6), (1000, 512, 2048, 512, 1e-6), (4096, 256, 3840, 256, 3e-7), (2048, 1024, 4096, 1024, 3e-7)])
+def test_products_of_fp32_in_norm(n, D, F, O, product):
+    """Errors in norm that show each of the six products of planes: without (lo, hi) or (hi, lo) a product is off by 2.4e-6.  An instruction loses two units of
+    the last place at most, 0.72 2^-22 of the part's sum so far, which of terms of either sign grows with the square root: of m instructions 2 / 3 m times
+    that.  Steps of six products have 4 of the largest planes, behind the small ones: 3e-7 (few rows; pairs of blocks; blocks alone, with slices of k);
+    clusters of more rows have parts of 16: 1e-6.  A result has two (y, down's gradient) or three products on its way, and 2^-21 for the activation and roundings."""
+    tensors, dy = mlp_case(n, D, F, O, torch.float32, seed=13)
+    leaves, exact = [v.requires_grad_() for v in tensors], [v.detach().double().requires_grad_() for v in tensors]
+    y, want = fr.gated_mlp(*leaves), lm.naive_gated_mlp(*exact)
+    for a, b, products in zip([y, *torch.autograd.grad(y, leaves, dy)], [want, *torch.autograd.grad(want, exact, dy.double())], (2, 3, 3, 3, 2)):
+        assert float((a.double() - b).norm()) <= (products * product + 2.0 ** -21) * float(b.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,D", [(16, 5003, 1024), (300, 3001, 485), (2000, 9001, 256), (130, 777, 2000)])
+def test_log_probabilities_of_fp32_in_norm(n, V, D):
+    """As above.  Logits of some units (in norm sqrt(2) times a log probability's error at most): one product of either kind; gradients a second one, and p with a
+    logit's error, 2 times its size, in forward and backward."""
+    x, w, t, up = logprobs_case(n, V, D, torch.float32, seed=13)
+    leaves, exact = [v.requires_grad_() for v in (x, w)], [v.detach().double().requires_grad_() for v in (x, w)]
+    r, want = fr.linear_logprobs(*leaves, t), lm.naive_linear_logprobs(*exact, t)
+    for a, b in zip(r, want):
+        assert float((a.double() - b).norm()) <= (1.5e-6 + 2.0 ** -21) * float(b.norm())
+    for a, b in zip(torch.autograd.grad(r, leaves, up), torch.autograd.grad(want, exact, [u.double() for u in up])):
+        assert float((a.double() - b).norm()) <= (1e-6 + 4e-6 + 2.0 ** -21) * float(b.norm())
+
+
+# ---- log probabilities without logits: pieces, planes -----------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n,V,D", [(torch.float32, 1000, 150000, 64), (torch.float32, 2000, 150000, 200), (torch.float16, 600, 600000, 40), (torch.bfloat16, 700, 500000, 40)])
+def test_pieces_of_a_long_vocabulary(dtype, n, V, D):
+    """Few rows against a vocabulary in pieces: x's gradient is added up over pieces and, in each, over slices of it."""
+    x, w, t, up = logprobs_case(n, V, D, dtype)
+    leaves = [v.requires_grad_() for v in (x, w)]
+    got = torch.autograd.grad(fr.linear_logprobs(*leaves, t), leaves, up)
+    want, tol = logprobs_exact(x.detach(), w.detach(), t, up, 1.0, -100)
+    for g, e, far in zip(got, want[2:], tol[2:]):
+        within(g, e, far)
+        near_in_norm(g, e, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,every", [(128, 16), (129, 16), (200, 25), (2000, 100)])
+def test_few_rows_that_count(n, every, dtype):
+    """Most rows ignored: up to 128 rows in two planes of the logits' gradient, above in one, whose rounding is that of the results again."""
+    x, w, t, (g, h) = logprobs_case(n, 3000, 383, dtype, seed=14)
+    ignored = torch.arange(n, device="cuda") % every != 3
+    t[ignored] = -100
+    h[ignored] = 0
+    for got, e, far in zip(logprobs_grads(x, w, t, [g, h]), *(v[2:] for v in logprobs_exact(x, w, t, [g, h], 1.0, -100))):
+        within(got, e, far)
+        near_in_norm(got, e, 1 if n <= 128 else 2)
