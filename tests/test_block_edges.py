@@ -8,7 +8,7 @@ import torch
 import flex_rnn_b200 as fr
 from flex_rnn_b200 import lm, runtime
 from flex_rnn_b200.language_model import RecurrentLM, synthetic_text
-from test_block import DTYPES, TINY, UNIT, logprobs_case, logprobs_exact, mlp_case, mlp_check, near_in_norm, rand, within
+from test_block import DTYPES, TINY, UNIT, logprobs_case, logprobs_exact, mlp_case, mlp_check, mlp_exact, near_in_norm, rand, within
 
 
 # ---- log probabilities without logits: upstream gradients ------------------------------------------------------------------------
@@ -322,3 +322,56 @@ def test_few_rows_that_count(n, every, dtype):
     for got, e, far in zip(logprobs_grads(x, w, t, [g, h]), *(v[2:] for v in logprobs_exact(x, w, t, [g, h], 1.0, -100))):
         within(got, e, far)
         near_in_norm(got, e, 1 if n <= 128 else 2)
+
+
+# ---- large ones -----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,D,F,O", [(20, 9000, 300, 4400), (600, 4500, 1300, 4200), (2100, 4300, 1500, 8300)])
+def test_gated_mlp_of_wide_models(n, D, F, O, dtype):
+    """More than 64 steps of k in the products whose results the activation takes, alone, in clusters and by pairs."""
+    mlp_check(*mlp_case(n, D, F, O, dtype, seed=15))
+
+
+@pytest.mark.gpu
+def test_gated_mlp_offsets_past_31_bits():
+    """2.2 10^9 hidden values; all rows but the last ones are zero, and add nothing to the gradients of the weights."""
+    n, last, (D, F, O) = 131100, 60, (16, 16500, 24)
+    (x, *weights), dy = mlp_case(last, D, F, O, torch.bfloat16, seed=16)
+    wide, far = torch.zeros(n, D, dtype=x.dtype, device="cuda"), torch.zeros(n, O, dtype=x.dtype, device="cuda")
+    wide[-last:], far[-last:] = x, dy
+    leaves = [v.requires_grad_() for v in (wide, *weights)]
+    y = fr.gated_mlp(*leaves)
+    dx, *dw = torch.autograd.grad(y, leaves, far)
+    want, tol = mlp_exact(x, *(v.detach() for v in weights), dy, "silu")
+    assert not y[:-last].any() and not dx[:-last].any()
+    for got, e, t in zip((y[-last:], dx[-last:], *dw), want, tol):
+        within(got, e, t)
+
+
+@pytest.mark.gpu
+def test_linear_logprobs_offsets_past_31_bits():
+    """A weight of 2.5 10^9 elements, of which only the last rows are not zero: the other tokens' logits are 0, and their probabilities equal."""
+    n, V, D, last = 20, 300000, 8192, 3000
+    x, w, _, (g, h) = logprobs_case(n, last, D, torch.float16, seed=17)
+    t = V - 1 - 7 * torch.arange(n, device="cuda")
+    big = torch.zeros(V, D, dtype=w.dtype, device="cuda")
+    big[-last:] = w
+    leaves = [v.requires_grad_() for v in (x, big)]
+    r = fr.linear_logprobs(*leaves, t)
+    dx, dw = torch.autograd.grad(r, leaves, [g, h])
+    z = torch.cat([torch.zeros(n, 1, device="cuda", dtype=torch.float64), x.detach().double() @ w.double().T], 1).requires_grad_()      # (column 0: each of the others)
+    many = torch.ones(last + 1, device="cuda", dtype=torch.float64)
+    many[0] = V - last
+    lse = torch.log((many * z.exp()).sum(-1, True))
+    p = (z - lse).exp()
+    lp, H = (z - lse).gather(1, (t - (V - last) + 1)[:, None])[:, 0], -(many * p * (z - lse)).sum(-1)
+    G, = torch.autograd.grad([lp, H], z, [g.double(), h.double()])
+    G = G / many
+    ez = 2.0 ** -19 * float((x.detach().double().abs() @ w.double().abs().T).max()) + 2.0 ** -20          # (a logit's error in parts of 4 steps; exponentials)
+    assert float((r.logprob.double() - lp.detach()).abs().max()) <= 2 * ez and float((r.entropy.double() - H.detach()).abs().max()) <= 2 * ez * (1 + math.log(V))
+    u = UNIT[w.dtype]
+    for got, e, size in ((dx, G[:, 1:] @ w.double(), G[:, 1:].abs() @ w.double().abs()), (dw[-last:], G[:, 1:].T @ x.detach().double(), G[:, 1:].abs().T @ x.detach().double().abs()),
+                         (dw[:1000], (G[:, :1].T @ x.detach().double()).expand(1000, D), (G[:, :1].abs().T @ x.detach().double().abs()).expand(1000, D))):
+        within(got, e, u * size)
