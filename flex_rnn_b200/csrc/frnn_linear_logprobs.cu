@@ -5,7 +5,7 @@
 //   log p[token] = ln 2 ((u[token] - m) - log2 s),   H = ln 2 (log2 s - t / s)
 // Backward, a piece of the vocabulary at a time: the logits again, their gradient
 //   G = (g (1[v = token] - p) - h p (ln p + H)) / T
-// as a 16-bit operand, dx += G W, dW of the piece = G^T x.  2 n V D operations forward, 6 n V D backward (2 of them for the
+// as a 16-bit operand (in one rounding; up to 128 rows in two planes, see there; fp32 in three), dx += G W, dW of the piece = G^T x.  2 n V D operations forward, 6 n V D backward (2 of them for the
 // logits that were not kept).
 #include "frnn_product.cuh"
 
@@ -169,7 +169,9 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
     const int64_t piece = pieces == 1 ? c->vocab : std::min(most, ((c->vocab + pieces - 1) / pieces + 255) / 256 * 256);
     // Up to 128 rows the gradient is two 16-bit planes, what rounding leaves is the second: few rows' gradients at their own tokens are nearly
     // all of a result, and their rounding did not average out (9 rows, half of them ignored, bf16: 2.7e-3 against 64 bits, where the result's own
-    // rounding is 1.6e-3).  Products of so few rows wait for the weights' copies.
+    // rounding is 1.6e-3).  The limit is one of cost: products of so few rows wait for the weights' copies, and the second plane takes 13 % (3 rows of
+    // 107200 tokens, 6848 wide, 1306 -> 1480 us); of more rows it would take half as long again (12 operations for 8).  So rows that are ignored count,
+    // and a row among 129 has one rounding more than among 128, of at most half a unit of the last place of each gradient.
     const int planes = c->dtype != FRNN_F32 && c->n <= 128 ? 2 : 1;
     const Operand grad = new_operand(s, c->dtype, c->n, piece, planes);
     float* const sum = pieces > 1 ? (float*)s.take((size_t)c->n * padded(c->width) * 4) : nullptr;

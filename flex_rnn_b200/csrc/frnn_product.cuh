@@ -336,16 +336,19 @@ template <int N> __device__ __forceinline__ void glu(int kind, float* a, float* 
 
 // ---- epilogues ---------------------------------------------------------------------------------------------------------------
 
-// The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses about k / 16 halves of its last bit, all in
-// one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096 in 16 bits, 2e-5 at 8192 in fp32, where 32-bit sums rounded to
-// nearest lose some 9e-7).  So sums along k come in parts of `flush` steps, which the epilogue's warps add up in registers, half of a
-// tile's columns a warp; the sums go back to where the last part was, and the epilogue is the same for all.  (One that took them
-// from registers had its loops unrolled, and its code did not fit the instruction cache.)  Results in 16 bits: parts of 64 steps, so that no length of k
-// loses more than those 7e-6 (of positive terms 2.4e-5) beside a rounding of 2e-4 (a vocabulary of 150000 in one part: 2.6e-4).  Log probabilities of 16-bit operands: of 16, 4e-7
-// (up to 128 rows, which wait for weights and not for the epilogue, of 4: 16 rows of 4096 against
-// 65536 tokens 6.3e-7 -> 9e-8 for 104 -> 107 us), and the same in their backward, because a probability is an exponential of the difference between its logits and the forward's log of
-// the sum.  fp32 where a step is six products: parts of one, whose small products come first, while the accumulator is small: 3e-7 (of two steps
-// 1.6e-6 and 4 % faster); fp32 in SPLIT: parts of 4, 6e-7.
+// The tensor cores add to an accumulator with truncation, not rounding: a sum over k loses up to two units of its last bit for each 16
+// values, all in one direction (measured against 64 bits, 2-norm: 7e-6 at k = 4096 in 16 bits, 2e-5 at 8192 in fp32, where 32-bit sums
+// rounded to nearest lose some 9e-7).  So sums along k come in parts of `flush` steps, which the epilogue's warps add up in registers, half
+// of a tile's columns a warp; the sums go back to where the last part was, and the epilogue is the same for all.  (One that took them from
+// registers had its loops unrolled, and its code did not fit the instruction cache.)
+//   results in 16 bits: parts of 64 steps, so that no length of k loses more than 7e-6 (2.4e-5 of positive terms) beside the results'
+//     rounding, 2e-4 in fp16; a k of 100000 in one part leaned by 2e-4.  No cost that shows (mlp_train, in turn: 6.29 and 6.33 ms).
+//   log probabilities of 16-bit operands: parts of 16, 4e-7 (of 4: loss_train a sixth slower).  Up to 128 rows, which wait for weights and not
+//     for the epilogue, of 4: 16 rows of 4096 against 65536 tokens 6.3e-7 -> 9e-8 for 104 -> 107 us.  The same in their backward (2 % of
+//     loss_train), because a probability is an exponential of the difference between its logits and the forward's log of the sum: of
+//     tokens with p = 0.999 at logits of 40, gradients from sums in one part were wrong altogether.
+//   fp32 where a step is six products: parts of one, whose small products come first, while the accumulator is small: 3e-7 (of two steps
+//     1.6e-6 and 4 % faster); in SPLIT: parts of 4, 6e-7.
 
 // 32 columns of accumulators, of the lane's row.  (Waited for apart: the next ones are under way while these are worked on.)
 __device__ __forceinline__ void ask(u32 taddr, float* v) { frnn_tmem_ld<32>(taddr, v); }

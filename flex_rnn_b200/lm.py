@@ -97,9 +97,11 @@ def linear_logprobs(x: th.Tensor, weight: th.Tensor, tokens: th.Tensor, temperat
     (the forward's workspace holds 12 bytes for each row and 64 or 128 of them, of as many rows at once as 256 MB have room for), and
     the backward computes them again, a piece of the vocabulary at a time (its workspace holds 2^28 of their gradients, in
     fp32 2^27, or 256 columns where there are more rows).  In bf16 and fp16 their gradient is rounded to that type before it
-    is multiplied with ``weight`` and ``x`` (up to 128 rows to twice its bits).  Results are fp32 and both differentiable.  Tokens equal to ``ignore_index`` have
-    log probability 0 and no gradient through it; tokens outside the vocabulary have NaN, and the next call on that GPU raises
-    ``FrnnError``."""
+    is multiplied with ``weight`` and ``x`` (up to 128 rows, ignored ones among them, to twice its bits).  In fp16 a power of two, one for the call, brings
+    the largest upstream gradient into range: values of the logits' gradient 2^27 times smaller than that lose bits, below 2^-37 of it they are zero,
+    so that a single row of very large gradients takes them from the others.  (Ignored tokens' gradients and rows that are not finite do not count.)
+    Results are fp32 and both differentiable.  Tokens equal to ``ignore_index`` have log probability 0 and no gradient through it; tokens outside the
+    vocabulary have NaN, and the next call on that GPU raises ``FrnnError``."""
     _operators()
     return LinearLogprobs(*_ops.linear_logprobs.default(x, weight, tokens, temperature, ignore_index, False)[:2])
 
@@ -111,8 +113,10 @@ def gated_mlp(x: th.Tensor, gate: th.Tensor, up: th.Tensor, down: th.Tensor, act
 
     The products run on the tensor cores, with sums in 32 bits (fp32 numbers as sums of three bf16 ones, so that nothing of them
     is lost; an infinity among them gives NaN).  In bf16 and fp16 the hidden vectors and the gradients of the two projections are rounded to
-    that type, as the tensor cores read them.  For the backward a call keeps the hidden vectors and, in 32 bits, their
-    derivatives by the two projections."""
+    that type, as the tensor cores read them: one rounding beside that of the results, and in fp16 an infinity where one of them passes 65504.  For the
+    backward a call keeps the hidden vectors and, in 32 bits, their derivatives by the two projections: 10 bytes a hidden value, in fp32 14.  ``x``
+    and weights whose rows are not runs of consecutive elements (a weight that is another's transpose) or do not begin on 16-byte boundaries, and those in
+    fp32, are copied in each call."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"flex_rnn_b200: gated_mlp: activation has to be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     _operators()

@@ -242,7 +242,8 @@ int frnn_token_logprobs_backward(int dtype, const void* logits, int64_t n, int64
  * The gated feed-forward block: y = (act(x gate^T) * (x up^T)) down^T, x [n, width], gate and up [hidden, width], down
  * [out_width, hidden], all of `dtype`; rows are runs of consecutive elements, `*_stride` elements apart.  The products run on
  * the tensor cores with sums in 32 bits (fp32 operands as sums of three bf16 numbers); for bf16 and fp16 what lies between
- * two products (the hidden vector, and backward its gradients) is rounded to that type, because the tensor cores read it so.
+ * two products (the hidden vector, and backward its gradients) is rounded to that type, because the tensor cores read it so (in fp16
+ * a value above 65504 there is infinite).
  * y and all gradients are contiguous.  What the forward keeps for the backward (all three or none: NULL), on 16-byte boundaries,
  * with H = hidden rounded up to a multiple of 64: `by_gate` and `by_up` fp32 [n, H], the hidden vectors' derivatives by the two
  * projections; `kept` [n, H] of `dtype`, for fp32 [3, n, H] bf16, the hidden vectors.
@@ -268,7 +269,9 @@ int frnn_gated_mlp_backward(const frnn_gated_mlp_call* call, const void* dy, int
  * The forward takes so many rows at once that what its workspace holds of them fits 256 MB.
  * The backward computes the logits again, a piece of the vocabulary at a time (2^28 of their gradients in 16 bits, in fp32 2^27 of
  * three bf16 numbers, or 256 columns where there are more rows), and gives dx and dweight (contiguous; either may be NULL).  The
- * logits' gradient is rounded to `dtype` for its products (fp16: after scaling by a power of two that keeps it in range).
+ * logits' gradient is rounded to `dtype` for its products, up to 128 rows to twice its bits.  In fp16 it is scaled by a power of two that
+ * brings the largest upstream gradient of the call (but those of ignored tokens' log probabilities, and rows that are not finite) into
+ * range: values 2^27 times smaller than that lose bits, below 2^-37 of it they are zero.
  */
 typedef struct frnn_linear_logprobs_call {
     int32_t dtype, token_bytes;
