@@ -109,7 +109,7 @@ int check(const char* what, const frnn_linear_logprobs_call* c) {
     return FRNN_OK;
 }
 
-Product logits(const frnn_linear_logprobs_call* c, const Operand& x, const Operand& w, int64_t first, int* err) {
+Product logits(const frnn_linear_logprobs_call* c, const Operand& x, const Operand& w, int64_t first, bool few, int* err) {
     Product q;
     q.dtype = c->dtype;
     q.m = c->n;
@@ -117,6 +117,7 @@ Product logits(const frnn_linear_logprobs_call* c, const Operand& x, const Opera
     q.k = c->width;
     q.a = x;
     q.b[0] = w;
+    q.few = few;
     q.args.err = err;
     q.args.io = c->dtype;
     q.args.c2 = (float)(1.4426950408889634 / c->temperature);
@@ -132,7 +133,7 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
     const char* what = "linear_logprobs";
     Packs packs = {};
     const Operand x = as_operand(s, packs, c->dtype, c->x, c->n, c->width, c->x_stride), w = as_operand(s, packs, c->dtype, c->weight, c->vocab, c->width, c->weight_stride);
-    // pieces of rows whose partial results, 12 bytes for each row and 64 columns, take 256 MB (of large tiles, for each 128 columns, 128 MB)
+    // pieces of rows whose partial results, 12 bytes for each row and 64 columns, take 256 MB (of large tiles, for each 128 columns, 128 MB), but 256 rows
     const int64_t most = std::max<int64_t>(256, (1ll << 28) / (24 * ((c->vocab + 127) / 128)) / 256 * 256), pieces = (c->n + most - 1) / most;
     const int64_t piece = pieces == 1 ? c->n : ((c->n + pieces - 1) / pieces + 255) / 256 * 256;
     int rc = s.base ? pack(packs, c->dtype, stream) : (int)FRNN_OK;
@@ -142,7 +143,7 @@ int forward(const frnn_linear_logprobs_call* c, float* logprob, float* entropy, 
         frnn_linear_logprobs_call some = *c;
         some.n = std::min(piece, c->n - r);
         some.tokens = (const char*)c->tokens + r * c->token_bytes;
-        Product q = logits(&some, x.from_row(r, some.n), w, 0, err);
+        Product q = logits(&some, x.from_row(r, some.n), w, 0, c->n <= 128, err);
         const ProductPlan plan = plan_product<LOGPROB_STATS, false, false>(q);
         const int64_t blocks = plan.tiles_n * (plan.form == PAIR ? 256 : 128) / plan.columns();
         q.args.partial = (float*)s.take((size_t)blocks * 3 * some.n * 4);
@@ -192,7 +193,7 @@ int backward(const frnn_linear_logprobs_call* c, const float* dlogprob, const fl
         Operand g = grad;
         g.cols = cols;
         {
-            Product q = logits(c, x, part, v, err);
+            Product q = logits(c, x, part, v, c->n <= 128, err);
             q.args.dlogprob = dlogprob;
             q.args.dentropy = dentropy;
             q.args.stats = stats;

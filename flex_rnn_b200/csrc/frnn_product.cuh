@@ -1073,6 +1073,7 @@ struct Product {
     Operand a, b[2];
     int64_t m, n, k;
     int pairs = 1;                                // products that are added up: of a's planes (groups of them) with b[0], b[1]
+    bool few = false;                             // log probabilities of a call of up to 128 rows (forward and backward cut a call into different pieces)
     void* out = nullptr;                          // STORE
     int out_dtype = 0;
     int64_t out_ld = 0;
@@ -1191,7 +1192,7 @@ template <int EPI, bool AT, bool BT> inline int run_product(const char* what, Pr
     const bool thin = is_thin(q, AT, plan.form), fp32 = q.dtype == FRNN_F32, fused = fp32 && (plan.form != SPLIT || thin);
     p.pairs = q.pairs;
     p.segments = q.pairs * (fp32 && !fused ? 6 : 1);
-    p.flush = fused ? 1 : fp32 ? 4 : EPI != LOGPROB_STATS && EPI != LOGPROB_GRAD ? 64 : q.m <= 128 ? 4 : 16;
+    p.flush = fused ? 1 : fp32 ? 4 : EPI != LOGPROB_STATS && EPI != LOGPROB_GRAD ? 64 : q.few ? 4 : 16;
     if ((int64_t)p.ksteps * p.segments >= (1ll << 31) - 64) return frnn_fail(FRNN_E_ARG, "%s: too long", what);
     auto encode = [&](CUtensorMap& map, const Operand& o, bool across, unsigned high) {
         return frnn_tensor_map_swizzled(&map, o.p, o.cols, o.rows, o.planes, (uint64_t)o.ld * 2, (uint64_t)o.plane * 2, 64, across ? 64 : high);

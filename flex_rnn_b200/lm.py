@@ -94,7 +94,7 @@ def linear_logprobs(x: th.Tensor, weight: th.Tensor, tokens: th.Tensor, temperat
     from the vectors ``x`` [..., width] and the last projection's ``weight`` [vocabulary, width], of one type.
 
     The products run on the tensor cores, with sums in 32 bits (of fp32 as in ``gated_mlp``); the logits leave them a tile at a time and are not kept
-    (the forward's workspace holds 12 bytes for each row and 64 or 128 of them, of as many rows at once as 256 MB have room for), and
+    (the forward's workspace holds 12 bytes for each row and 64 or 128 of them, of as many rows at once as 256 MB have room for, but 256), and
     the backward computes them again, a piece of the vocabulary at a time (its workspace holds 2^28 of their gradients, in
     fp32 2^27, or 256 columns where there are more rows).  In bf16 and fp16 their gradient is rounded to that type before it
     is multiplied with ``weight`` and ``x`` (up to 128 rows, ignored ones among them, to twice its bits).  In fp16 a power of two, one for the call, brings

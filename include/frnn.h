@@ -266,7 +266,7 @@ int frnn_gated_mlp_backward(const frnn_gated_mlp_call* call, const void* dy, int
 /*
  * What frnn_token_logprobs_forward gives from logits = x weight^T, x [n, width], weight [vocab, width], without keeping the
  * logits: log probabilities of the tokens and entropies, fp32 [n].  stats (may be NULL): fp32 [n][2] for the backward.
- * The forward takes so many rows at once that what its workspace holds of them fits 256 MB.
+ * The forward takes so many rows at once that what its workspace holds of them fits 256 MB, but at least 256 rows.
  * The backward computes the logits again, a piece of the vocabulary at a time (2^28 of their gradients in 16 bits, in fp32 2^27 of
  * three bf16 numbers, or 256 columns where there are more rows), and gives dx and dweight (contiguous; either may be NULL).  The
  * logits' gradient is rounded to `dtype` for its products, up to 128 rows to twice its bits.  In fp16 it is scaled by a power of two that
